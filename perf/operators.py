@@ -1,0 +1,341 @@
+"""Cases of the operators that decide what a training step keeps between its forward and its backward pass:
+
+* the 8-bit activation tape: a taped activation is kept as one byte a value and one exponent byte per 32 values, and the
+  backward pass reads it in that form (the values themselves, the SoftRectifier derivative recovered from them, the data,
+  weight and bias gradients of a discriminator convolution);
+* the softmax cross entropy of a Dense head with many classes, computed in pieces of the classes without keeping the
+  logits, with the gradients of the features, the kernel and the bias.
+
+`run` is one pass of a case: in elementary torch operations (`own` false) or through the framework's entry points.
+
+Format of the tape: 32 consecutive values share H, the smallest power of two not below the largest magnitude (and not
+below 2^-118); a value v is kept as u = min(255, floor(v 128 / H) + 128) and stands for (u - 127.5) H / 128; a block of
+zeros stands for zeros.
+"""
+import math
+
+import torch
+
+own = False
+
+ALPHA = 20000.0      # SoftRectifier: tanh(v) + v / alpha
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# cases
+# ------------------------------------------------------------------------------------------------------------------
+def listed():
+    return [
+        # one clip's 32-channel activation at 8 x 1500, the smallest stage with taped grow blocks: latency
+        {"name": "keep bf16 8x1500", "op": "keep", "dtype": "bf16", "n": 1, "h": 8, "w": 1500, "c": 32},
+        # a 128-channel float32 activation of the evaluator's fitting batch (64 clips of 4 x 750)
+        {"name": "keep f32 evaluator", "op": "keep", "dtype": "f32", "n": 64, "h": 4, "w": 750, "c": 128},
+        # gradient times the derivative of the from-audio layer (128 channels) at 128 x 24000, a micro-batch of 2
+        {"name": "derivative 128x24000", "op": "derivative", "dtype": "bf16", "n": 2, "h": 128, "w": 24000, "c": 128},
+        # backward of a 3x3 convolution of the smallest grow block, one clip: latency
+        {"name": "conv3 8x1500", "op": "conv", "k": 3, "cin": 32, "act": True, "n": 1, "h": 8, "w": 1500},
+        # the 2x2 convolution at a clip length that is no multiple of any tile
+        {"name": "conv2 ragged", "op": "conv", "k": 2, "cin": 32, "act": True, "n": 3, "h": 37, "w": 1501},
+        # the 3x3 convolution at 64 x 12000, micro-batch of 4: an ordinary training call
+        {"name": "conv3 64x12000", "op": "conv", "k": 3, "cin": 32, "act": True, "n": 4, "h": 64, "w": 12000},
+        # a block's first convolution (128 -> 32 channels) behind the fade-in blend, which has no activation
+        {"name": "conv3 from 128", "op": "conv", "k": 3, "cin": 128, "act": False, "n": 2, "h": 64, "w": 6001},
+        # full resolution, one clip
+        {"name": "conv3 256x48000", "op": "conv", "k": 3, "cin": 32, "act": True, "n": 1, "h": 256, "w": 48000},
+        # one position against a class count that is no multiple of anything: latency, the kernel read once
+        {"name": "xent one row", "op": "xent", "dtype": "f32", "n": 1, "e": 128, "v": 4097, "bias": True},
+        # every position of one clip's 4 x 750 map, 128 features, 8192 classes
+        {"name": "xent one clip", "op": "xent", "dtype": "bf16", "n": 3000, "e": 128, "v": 8192, "bias": True},
+        # float32 features, odd sizes, a wide feature vector, no bias
+        {"name": "xent f32 wide ragged", "op": "xent", "dtype": "f32", "n": 1501, "e": 1000, "v": 10001, "bias": False},
+        # eight clips against one class per 16-bit sample value: the largest
+        {"name": "xent 65536 classes", "op": "xent", "dtype": "bf16", "n": 24000, "e": 128, "v": 65536, "bias": True},
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(("keep", "derivative", "conv", "conv", "xent", "xent", "xent"))
+    if op == "xent":
+        e, v = _log(rng, 16, 1024), _log(rng, 100, 65536)
+        most = min(24000, int(24000 * 128 * 65536 / (e * v)))
+        return {"op": op, "dtype": rng.choice(("f32", "bf16")), "n": _log(rng, 1, most), "e": e, "v": v,
+                "bias": rng.random() < 0.7}
+    n, h = rng.randint(1, 4), _log(rng, 8, 256)
+    if op == "conv":
+        k, cin = rng.choice(((3, 32), (2, 32), (3, 128)))
+        most = 256 * 48000 // (n * h) // (4 if cin == 128 else 1)
+        return {"op": op, "k": k, "cin": cin, "act": rng.random() < 0.6, "n": n, "h": h,
+                "w": _log(rng, 8, min(48000, most))}
+    c = rng.choice((32, 128))
+    most = 2 * 128 * 24000 * 128 // (n * h * c)
+    return {"op": op, "dtype": rng.choice(("f32", "bf16")), "n": n, "h": h, "w": _log(rng, 8, min(48000, most)), "c": c}
+
+
+_TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda")
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(seed)
+
+    def normal(*shape):
+        return torch.randn(shape, generator=gen, device=dev, dtype=torch.float32)
+
+    st = dict(case)
+    if case["op"] == "xent":
+        n, e, v = case["n"], case["e"], case["v"]
+        st["x"] = normal(n, e).to(_TYPES[case["dtype"]])
+        st["kernel"] = normal(e, v) * (2.0 / math.sqrt(e))
+        st["offset"] = normal(v) * 0.2 if case["bias"] else None
+        labels = torch.randint(0, v, (n,), generator=gen, device=dev, dtype=torch.int32)
+        if n > 1:                      # one position in sixteen carries no label
+            labels[torch.rand((n,), generator=gen, device=dev) < 1.0 / 16.0] = -1
+        st["labels"] = labels
+        # the gradient that arrives at each position's loss: a weighted mean
+        st["dloss"] = (0.5 + torch.rand((n,), generator=gen, device=dev)) / n
+        return st
+    # activations of a SoftRectifier layer, tanh(v) + v / alpha
+    shape = (case["n"], case["h"], case["w"], case.get("c", case.get("cin")))
+    pre = normal(*shape).mul_(1.2)
+    y = torch.tanh(pre).add_(pre, alpha=1.0 / ALPHA)
+    del pre
+    st["x"] = y.to(_TYPES[case["dtype"]] if case["op"] == "keep" else torch.bfloat16)
+    del y
+    if case["op"] == "derivative":
+        st["g"] = normal(*shape).mul_(1e-3).to(_TYPES[case["dtype"]])
+    if case["op"] == "conv":
+        k, cin = case["k"], case["cin"]
+        st["g"] = normal(*shape[:3], 32).mul_(1e-3).to(torch.bfloat16)
+        st["kernel"] = normal(k, k, cin, 32) * math.sqrt(2.0 / (k * k * cin))
+    return st
+
+
+def work(case):
+    if case["op"] == "xent":
+        n, e, v = case["n"], case["e"], case["v"]
+        feature = 4 if case["dtype"] == "f32" else 2
+        # features and their gradient, kernel and its gradient, bias and its gradient, labels, loss, arriving gradient
+        byts = 2 * n * e * feature + 2 * e * v * 4 + (8 * v if case["bias"] else 0) + 12 * n
+        return {"bytes": byts, "flops": 3 * 2.0 * n * e * v}     # logits, dx, dw
+    pos = case["n"] * case["h"] * case["w"]
+    tape = 33.0 / 32.0                                           # bytes of a kept value
+    if case["op"] == "conv":
+        cin, taps = case["cin"], case["k"] * case["k"]
+        # x read, tape written and read, g read, dx written; data and weight gradient
+        return {"bytes": pos * (cin * (2 + 2 * tape + 2) + 32 * 2), "flops": 2 * 2.0 * taps * cin * 32 * pos}
+    n = pos * case["c"]
+    size = 4 if case["dtype"] == "f32" else 2
+    if case["op"] == "keep":
+        return {"bytes": n * (2 * size + 2 * tape), "flops": 4.0 * n}
+    return {"bytes": n * (2 + 2 * tape + size + 2), "flops": 8.0 * n}
+
+
+def run(state):
+    if own:
+        return _run_own(state)
+    if state["op"] == "xent":
+        return _plain_xent(state)
+    if state["op"] == "conv":
+        return _plain_conv(state)
+    kept = _plain_kept(state["x"])
+    if state["op"] == "keep":
+        return {"values": kept.to(state["x"].dtype)}
+    return {"grad": (state["g"].float() * _plain_derivative(kept)).to(torch.bfloat16)}
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# the framework's calls
+# ------------------------------------------------------------------------------------------------------------------
+def _run_own(state):
+    from music_generator_amd import ops
+    x = state["x"]
+    if state["op"] == "xent":
+        w, b, labels = state["kernel"], state["offset"], state["labels"]
+        n = x.shape[0]
+        loss, lse = torch.empty((n,), device=x.device), torch.empty((n,), device=x.device)
+        ops.dense_xent_fwd(x, w, b, labels, loss, lse)
+        dx, dw = torch.empty_like(x), torch.empty_like(w)
+        db = torch.empty_like(b) if b is not None else None
+        ops.dense_xent_bwd(x, w, b, labels, lse, state["dloss"], dx, dw, db, accumulate=False)
+        out = {"loss": loss, "dx": dx, "dw": dw}
+        if db is not None:
+            out["db"] = db
+        return out
+    kept = ops.tape8_pack(x)
+    if state["op"] == "keep":
+        return {"values": ops.tape8_unpack(kept)}
+    if state["op"] == "derivative":
+        return {"grad": ops.mul_dact_tape8(state["g"], kept, ALPHA)}
+    if "desc" not in state:                                      # a layer makes its descriptor once per shape
+        k, cin = state["k"], state["cin"]
+        state["desc"] = ops.make_conv_desc(
+            nimg=state["n"], hin=state["h"], win=state["w"], cin=cin, hout=state["h"], wout=state["w"], kh=k, kw=k,
+            pt=(k - 1) // 2, pl=(k - 1) // 2, ngemm=32, cout=32, wsk=32, wsn=1, wtap=cin * 32, nbias=32)
+    dx = torch.empty_like(x)
+    dw = torch.zeros_like(state["kernel"])                       # gradients are added into the caller's buffers
+    db = torch.zeros((32,), device=x.device)
+    ops.conv_bwd_tape8(state["desc"], kept, state["g"], state["kernel"], dw, db, dx, ALPHA if state["act"] else 0.0)
+    return {"dx": dx, "dw": dw, "db": db}
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# plain forms, 32 bits
+# ------------------------------------------------------------------------------------------------------------------
+def _plain_kept(x):
+    """The float32 values that the tape of x stands for."""
+    n = x.numel()
+    flat = x.reshape(-1).float()
+    if n % 32:
+        flat = torch.cat([flat, flat.new_zeros(32 - n % 32)])
+    blocks = flat.view(-1, 32)
+    largest = blocks.abs().amax(dim=1, keepdim=True)
+    bits = largest.view(torch.int32)
+    expo = (bits >> 23) + ((bits & 0x7fffff) != 0)               # 127 + log2 H
+    expo = expo.clamp(min=9)
+    step = ((expo - 7) << 23).view(torch.float32)                # H / 128
+    inv = ((261 - expo) << 23).view(torch.float32)               # 128 / H
+    code = torch.floor(blocks * inv).add_(128.0).clamp_(max=255.0)
+    values = code.sub_(127.5).mul_(step)
+    values.masked_fill_(largest == 0.0, 0.0)
+    return values.view(-1)[:n].view(x.shape)
+
+
+def _plain_derivative(y):
+    return (1.0 + 1.0 / ALPHA - y * y).clamp_(min=1.0 / ALPHA)
+
+
+def _plain_conv(state):
+    k, w, act = state["k"], state["kernel"], state["act"]
+    kept, g = _plain_kept(state["x"]), state["g"].float()
+    n, h, wd, cin = kept.shape
+    p0, p1 = (k - 1) // 2, k - 1 - (k - 1) // 2
+    padded = torch.nn.functional.pad(kept, (0, 0, p0, p1, p0, p1))
+    grows = g.reshape(n * h, wd, 32)
+    dw = torch.empty_like(w)
+    dpad = torch.zeros((n, h + k - 1, wd + k - 1, cin), device=g.device)
+    for a in range(k):
+        for b in range(k):
+            rows = padded[:, a:a + h, b:b + wd].reshape(n * h, wd, cin)
+            dw[a, b] = torch.bmm(rows.transpose(1, 2), grows).sum(dim=0, dtype=torch.float64).float()
+            dpad[:, a:a + h, b:b + wd] += torch.matmul(g.view(-1, 32), w[a, b].t().contiguous()).view(n, h, wd, cin)
+    dx = dpad[:, p0:p0 + h, p0:p0 + wd]
+    if act:
+        dx = dx * _plain_derivative(kept)
+    return {"dx": dx.to(torch.bfloat16).contiguous(), "dw": dw, "db": g.view(-1, 32).sum(dim=0)}
+
+
+def _plain_xent(state):
+    x, w, b = state["x"].float(), state["kernel"], state["offset"]
+    labels, valid = state["labels"].long().clamp(min=0), state["labels"] >= 0
+    z = x @ w
+    if b is not None:
+        z += b
+    m = z.amax(dim=1, keepdim=True)
+    picked = z.gather(1, labels[:, None])
+    p = z.sub_(m).exp_()
+    s = p.sum(dim=1, keepdim=True)
+    loss = torch.where(valid, (m + s.log() - picked)[:, 0], 0.0)
+    p /= s
+    p.scatter_add_(1, labels[:, None], torch.full_like(s, -1.0))
+    p *= torch.where(valid, state["dloss"], 0.0)[:, None]
+    out = {"loss": loss, "dx": (p @ w.t()).to(state["x"].dtype), "dw": x.t() @ p}
+    if b is not None:
+        out["db"] = p.sum(dim=0)
+    return out
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# the definitions in 64 bits
+# ------------------------------------------------------------------------------------------------------------------
+def _exact_kept(x):
+    """(u - 127.5) H / 128 of flat x (whole blocks of 32 and a last ragged one), from frexp in float64."""
+    out = torch.empty(x.numel(), dtype=torch.float64, device=x.device)
+    piece = 1 << 25
+    for i in range(0, x.numel(), piece):
+        v = x[i:i + piece].double()
+        v = torch.nn.functional.pad(v, (0, -v.numel() % 32)).view(-1, 32)
+        m, ex = torch.frexp(v.abs().max(dim=1, keepdim=True).values)
+        ex = torch.where(m == 0.5, ex - 1, ex).clamp(min=-118).long()
+        step = ((ex - 7 + 1023) << 52).view(torch.float64)
+        q = (torch.minimum(torch.floor(v / step), torch.full_like(v, 127.0)) + 0.5) * step
+        q = torch.where(m == 0, torch.zeros_like(q), q)
+        out[i:i + piece] = q.view(-1)[:min(piece, x.numel() - i)]
+    return out
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    if case["op"] == "xent":
+        return _exact_xent(st)
+    x = st["x"].reshape(-1)
+    if case["op"] == "keep":
+        return {"values": _exact_kept(x).view(st["x"].shape)}
+    if case["op"] == "derivative":
+        g, out = st["g"].reshape(-1), torch.empty(x.numel(), dtype=torch.float64, device=x.device)
+        piece = 1 << 25                                          # a multiple of a block
+        for i in range(0, x.numel(), piece):
+            y = _exact_kept(x[i:i + piece])
+            d = torch.maximum(1.0 + 1.0 / ALPHA - y.square(), torch.full_like(y, 1.0 / ALPHA))
+            out[i:i + piece] = d * g[i:i + piece].double()
+        return {"grad": out.view(st["x"].shape)}
+    return _exact_conv(st)
+
+
+def _exact_conv(st):
+    """From the gradient's side: every position of x meets the window of g it was used for."""
+    k, cin = st["k"], st["cin"]
+    n, h, w, _ = st["x"].shape
+    p0 = (k - 1) // 2
+    lead = k - 1 - p0
+    wm = st["kernel"].double().permute(0, 1, 3, 2).reshape(k * k * 32, cin)          # (tap, co) x ci
+    dw = torch.zeros((k * k * 32, cin), dtype=torch.float64, device=wm.device)
+    dx = torch.empty((n, h, w, cin), dtype=torch.float64, device=wm.device)
+    db = torch.zeros((32,), dtype=torch.float64, device=wm.device)
+    kept = _exact_kept(st["x"].reshape(-1)).view(st["x"].shape)
+    rows = max(1, (1 << 18) // w)
+    for i in range(n):
+        padded = torch.nn.functional.pad(st["g"][i], (0, 0, lead, p0, lead, p0))
+        for r in range(0, h, rows):
+            c = min(rows, h - r)
+            # output position of tap (a, b) that read x[q] is q - (a, b) + p0
+            window = torch.stack([padded[r + k - 1 - a:r + k - 1 - a + c, k - 1 - b:k - 1 - b + w].double()
+                                  for a in range(k) for b in range(k)], dim=2).reshape(c * w, k * k * 32)
+            q = kept[i, r:r + c].reshape(c * w, cin)
+            dw += window.t() @ q
+            d = window @ wm
+            if st["act"]:
+                d *= torch.maximum(1.0 + 1.0 / ALPHA - q.square(), torch.full_like(q, 1.0 / ALPHA))
+            dx[i, r:r + c] = d.view(c, w, cin)
+            db += st["g"][i, r:r + c].double().sum(dim=(0, 1))
+    return {"dx": dx, "dw": dw.view(k, k, 32, cin).permute(0, 1, 3, 2).contiguous(), "db": db}
+
+
+def _exact_xent(st):
+    n = st["x"].shape[0]
+    w = st["kernel"].double()
+    e, v = w.shape
+    b = st["offset"].double() if st["offset"] is not None else torch.zeros((v,), dtype=torch.float64, device=w.device)
+    loss = torch.zeros((n,), dtype=torch.float64, device=w.device)
+    dx = torch.zeros((n, e), dtype=torch.float64, device=w.device)
+    dw, db = torch.zeros_like(w), torch.zeros_like(b)
+    piece = max(1, (1 << 27) // v)
+    for i in range(0, n, piece):
+        x, lab = st["x"][i:i + piece].double(), st["labels"][i:i + piece].long()
+        logp = torch.log_softmax(x @ w + b, dim=1)
+        hot = torch.zeros_like(logp)
+        at = (lab >= 0).nonzero()[:, 0]
+        hot[at, lab[at]] = 1.0
+        loss[i:i + piece] = -(hot * logp.clamp(min=-1e300)).sum(dim=1)
+        d = (logp.exp() - hot) * (st["dloss"][i:i + piece].double() * (lab >= 0))[:, None]
+        dx[i:i + piece] = d @ w.t()
+        dw += x.t() @ d
+        db += d.sum(dim=0)
+    out = {"loss": loss, "dx": dx, "dw": dw}
+    if st["offset"] is not None:
+        out["db"] = db
+    return out
