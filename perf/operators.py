@@ -8,9 +8,9 @@
 
 `run` is one pass of a case: in elementary torch operations (`own` false) or through the framework's entry points.
 
-Format of the tape: 32 consecutive values share H, the smallest power of two not below the largest magnitude (and not
-below 2^-118); a value v is kept as u = min(255, floor(v 128 / H) + 128) and stands for (u - 127.5) H / 128; a block of
-zeros stands for zeros.
+Format of the tape: 32 consecutive values share H, the smallest power of two (2^-118 or more) that their largest magnitude
+does not exceed by more than a 256th of H; a value v is kept as u = floor(v 128 / H) + 128, held in 0 .. 255, and stands
+for (u - 127.5) H / 128; a block of zeros stands for zeros.
 """
 import math
 
@@ -195,11 +195,11 @@ def _plain_kept(x):
     blocks = flat.view(-1, 32)
     largest = blocks.abs().amax(dim=1, keepdim=True)
     bits = largest.view(torch.int32)
-    expo = (bits >> 23) + ((bits & 0x7fffff) != 0)               # 127 + log2 H
+    expo = (bits >> 23) + ((bits & 0x7fffff) > 0x8000)           # 127 + log2 H; 0x8000: a 256th of a power of two
     expo = expo.clamp(min=9)
     step = ((expo - 7) << 23).view(torch.float32)                # H / 128
     inv = ((261 - expo) << 23).view(torch.float32)               # 128 / H
-    code = torch.floor(blocks * inv).add_(128.0).clamp_(max=255.0)
+    code = torch.floor(blocks * inv).add_(128.0).clamp_(min=0.0, max=255.0)
     values = code.sub_(127.5).mul_(step)
     values.masked_fill_(largest == 0.0, 0.0)
     return values.view(-1)[:n].view(x.shape)
@@ -260,9 +260,9 @@ def _exact_kept(x):
         v = x[i:i + piece].double()
         v = torch.nn.functional.pad(v, (0, -v.numel() % 32)).view(-1, 32)
         m, ex = torch.frexp(v.abs().max(dim=1, keepdim=True).values)
-        ex = torch.where(m == 0.5, ex - 1, ex).clamp(min=-118).long()
+        ex = torch.where(m <= 0.5 + 0.5 / 256.0, ex - 1, ex).clamp(min=-118).long()
         step = ((ex - 7 + 1023) << 52).view(torch.float64)
-        q = (torch.minimum(torch.floor(v / step), torch.full_like(v, 127.0)) + 0.5) * step
+        q = (torch.floor(v / step).clamp(-128.0, 127.0) + 0.5) * step
         q = torch.where(m == 0, torch.zeros_like(q), q)
         out[i:i + piece] = q.view(-1)[:min(piece, x.numel() - i)]
     return out
