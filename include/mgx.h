@@ -531,6 +531,28 @@ int mgx_mul_dact_bf16(const void* a, int a_is_f32, const void* y, float act_alph
 int mgx_cast_f32_to_bf16(const float* x, void* y, int64_t n, void* stream);
 int mgx_cast_bf16_to_f32(const void* x, float* y, int64_t n, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * 8-bit activation tape: what a taped forward keeps of an activation (tf.GradientTape keeps float32, trainer/models.py:118)
+ * at 33 bytes per 32 values.  32 consecutive values share H, the smallest power of two (2^-118 or more) that
+ * their largest magnitude does not exceed by more than H / 256; a value v is kept as the byte floor(128 v / H) + 128, held in
+ * 0 .. 255, and stands for (byte - 127.5) H / 128, exact in bf16 and half a step (H / 256) off at most (above H: a step).  The block's exponent byte is log2(H) + 126; 0: a block of zeros, which
+ * stands for zeros; 255: a block with an infinity or a NaN, which stands for NaN throughout.  The last block of a tensor
+ * may be shorter; its codes are stored as a whole block.
+ *   codes: 32 * mgx_tape8_blocks(n) bytes, exps: mgx_tape8_blocks(n) bytes.  Tensor pointers and `codes` are 16-byte
+ *   aligned (MGX_ERR_ARG otherwise); n = 0 does nothing.
+ * ---------------------------------------------------------------------------------------- */
+int64_t mgx_tape8_blocks(int64_t n);
+int mgx_tape8_pack(const void* x, int x_is_f32, void* codes, void* exps, int64_t n, void* stream);
+int mgx_tape8_unpack(const void* codes, const void* exps, void* y, int y_is_f32, int64_t n, void* stream);
+/* out (bf16) = a (bf16 or float32) * f'(y): y the kept output of tanh(v) + v / act_alpha, f' = max(1 + 1/act_alpha - y^2,
+ * 1/act_alpha) recovered from it (mgx_mul_dact_bf16 reads a bf16 y). */
+int mgx_mul_dact_tape8(const void* a, int a_is_f32, const void* codes, const void* exps, float act_alpha, void* out,
+                       int64_t n, void* stream);
+/* mgx_conv_bwd_bf16 (same descriptors, workspace and results) with the layer input read from the 8-bit tape. */
+int mgx_conv_bwd_tape8(const mgx_conv_desc* d, const void* codes, const void* exps, const void* g, const float* w,
+                       float* dw, float* dbias, void* dx, float act_alpha, void* workspace, int64_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

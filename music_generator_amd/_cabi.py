@@ -160,6 +160,11 @@ PROTOTYPES = {
     "mgx_mul_dact_bf16": (_I, [_P, _I, _P, _F, _P, _I64, _P]),
     "mgx_cast_f32_to_bf16": (_I, [_P, _P, _I64, _P]),
     "mgx_cast_bf16_to_f32": (_I, [_P, _P, _I64, _P]),
+    "mgx_tape8_blocks": (_I64, [_I64]),
+    "mgx_tape8_pack": (_I, [_P, _I, _P, _P, _I64, _P]),
+    "mgx_tape8_unpack": (_I, [_P, _P, _P, _I, _I64, _P]),
+    "mgx_mul_dact_tape8": (_I, [_P, _I, _P, _P, _F, _P, _I64, _P]),
+    "mgx_conv_bwd_tape8": (_I, [_DESC, _P, _P, _P, _P, _P, _P, _P, _F, _P, _I64, _P]),
 }
 
 _lib = None

@@ -16,7 +16,7 @@
 // placement, so the operand they have in common is fetched from HBM once (speed only).
 // At the end the four waves are added in LDS in fixed order, every workgroup leaves one slab in the
 // workspace, and a second kernel adds the slabs in fixed order into dW / dB (bitwise reproducible).
-#include "bf16.h"
+#include "tape8.h"
 #include <type_traits>
 #include "../../include/mgx.h"
 
@@ -287,8 +287,12 @@ struct FGeo {
 
 __device__ __forceinline__ int sw_off(int p, int c16) { return p * 64 + ((c16 ^ ((p >> 2) & 3)) << 4); }
 
-template <int KH, int KW, bool ACT, int CIN>
-__global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const bf16_t* __restrict__ x,
+// X8: X is the 8-bit tape of the layer input (tape8.h), x its codes and xe its exponent bytes: 33 instead of 64 bytes
+// are read per 32 channels.  A thread loads the eight codes of a 16-byte piece and turns them into the piece when it
+// writes it to LDS; everything behind the staging is the same.
+template <int KH, int KW, bool ACT, int CIN, bool X8>
+__global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const void* __restrict__ x,
+                                                      const unsigned char* __restrict__ xe,
                                                       const bf16_t* __restrict__ g, const float* __restrict__ w,
                                                       bf16_t* __restrict__ dx, float* __restrict__ partial, long ntiles,
                                                       int tiles_h, int tiles_w, float act_alpha) {
@@ -322,7 +326,9 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const bf1
         w0 = (int)(rem - th * tiles_w) * TW;
     };
     const int q4 = tid & 3;
-    u32x4 sg[GITER], sx[XITER];
+    u32x4 sg[GITER], sx[X8 ? 1 : XITER];
+    u32x2 sc[X8 ? XITER : 1];
+    unsigned se[X8 ? XITER : 1];
     auto stage_load = [&](long t) {
         long img; int h0, w0;
         tile_of(t, img, h0, w0);
@@ -341,15 +347,22 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const bf1
         }
         // X tile: 4 NCH 16-byte pieces a position, consecutive threads on consecutive pieces
         const long xband = ((img * H + h0) * (long)W) * CIN;
-        const __amdgpu_buffer_rsrc_t rx =
-            __builtin_amdgcn_make_buffer_rsrc((void*)(x + xband), 0, (unsigned)TH * W * (CIN * 2u), 0x00020000);
+        const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)((const unsigned char*)x + xband * (X8 ? 1 : 2)), 0, (unsigned)TH * W * (CIN * (X8 ? 1u : 2u)), 0x00020000);
+        const __amdgpu_buffer_rsrc_t re =
+            __builtin_amdgcn_make_buffer_rsrc((void*)(X8 ? xe + xband / 32 : nullptr), 0, X8 ? (unsigned)TH * W * NCH : 0u, 0x00020000);
 #pragma unroll
         for (int i = 0; i < XITER; ++i) {
             const int pc = tid + 256 * i, px = pc / (4 * NCH), sub = pc - px * (4 * NCH);
             const int ty = px / TW, tx = px - ty * TW;
             const bool ok = px < XPIX && (unsigned)(ty + h0) < (unsigned)H && (unsigned)(tx + w0) < (unsigned)W;
-            const unsigned off = ok ? (unsigned)(((ty * W + (tx + w0)) * CIN + sub * 8) * 2) : 0xfffffff0u;
-            sx[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 0, 0));
+            const unsigned at = (unsigned)((ty * W + (tx + w0)) * CIN + sub * 8);
+            if constexpr (X8) {      // past the edges: exponent byte 0, a block of zeros
+                sc[i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rx, ok ? at : 0xfffffff0u, 0, 0));
+                se[i] = __builtin_amdgcn_raw_buffer_load_b8(re, ok ? at >> 5 : 0xfffffff0u, 0, 0);
+            } else {
+                sx[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, ok ? at * 2u : 0xfffffff0u, 0, 0));
+            }
         }
     };
     auto stage_write = [&](int b) {
@@ -362,8 +375,11 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const bf1
 #pragma unroll
         for (int i = 0; i < XITER; ++i) {
             const int pc = tid + 256 * i, px = pc / (4 * NCH), sub = pc - px * (4 * NCH);
-            if (256 * (i + 1) <= XPIX * NCH * 4 || px < XPIX)
-                *(u32x4*)(xbuf + (b * NCH + (sub >> 2)) * XPIX * 64 + sw_off(px, sub & 3)) = sx[i];
+            if (256 * (i + 1) <= XPIX * NCH * 4 || px < XPIX) {
+                unsigned char* dst = xbuf + (b * NCH + (sub >> 2)) * XPIX * 64 + sw_off(px, sub & 3);
+                if constexpr (X8) *(u32x4*)dst = tape8_bf16x8(sc[i], se[i]);
+                else *(u32x4*)dst = sx[i];
+            }
         }
     };
 
@@ -469,8 +485,8 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const bf1
                 if constexpr (q < 4) {
                     float v0 = dacc[8 * half + 2 * q], v1 = dacc[8 * half + 2 * q + 1];
                     if constexpr (ACT) {     // x f'(X): the layer before is a SoftRectifier layer and X its stored output
-                        v0 *= dact_from_y(bf_lo(yv[half][q]), inv_alpha, k1);
-                        v1 *= dact_from_y(bf_hi(yv[half][q]), inv_alpha, k1);
+                        v0 *= X8 ? tape8_dact(bf_lo(yv[half][q]), inv_alpha, k1) : dact_from_y(bf_lo(yv[half][q]), inv_alpha, k1);
+                        v1 *= X8 ? tape8_dact(bf_hi(yv[half][q]), inv_alpha, k1) : dact_from_y(bf_hi(yv[half][q]), inv_alpha, k1);
                     }
                     o[half][q] = bf_pack(v0, v1);
                 } else if (oh < H && ow < W) {
@@ -598,20 +614,20 @@ int launch_w(const mgx_conv_desc& d, const bf16_t* x, const bf16_t* g, float* dw
 
 int wgrad_taps(const mgx_conv_desc& d) { return d.kh * d.kw; }
 
-template <int KH, int KW, int CIN>
-int launch_f(const mgx_conv_desc& d, const bf16_t* x, const bf16_t* g, const float* w, float* dw, float* db, bf16_t* dx,
-             float* partial, float act_alpha, hipStream_t st) {
+template <int KH, int KW, int CIN, bool X8 = false>
+int launch_f(const mgx_conv_desc& d, const void* x, const bf16_t* g, const float* w, float* dw, float* db, bf16_t* dx,
+             float* partial, float act_alpha, hipStream_t st, const unsigned char* xe = nullptr) {
     using G = FGeo<KH, KW, CIN>;
     const int tiles_h = (d.hout + G::TH - 1) / G::TH, tiles_w = (d.wout + G::TW - 1) / G::TW;
     const long ntiles = (long)d.nimg * tiles_h * tiles_w;
     if (ntiles <= 0 || ntiles >= (1L << 31)) return MGX_ERR_ARG;
-    const void* fn = act_alpha > 0.f ? (const void*)bbwd_kernel<KH, KW, true, CIN> : (const void*)bbwd_kernel<KH, KW, false, CIN>;
+    const void* fn = act_alpha > 0.f ? (const void*)bbwd_kernel<KH, KW, true, CIN, X8> : (const void*)bbwd_kernel<KH, KW, false, CIN, X8>;
     if (hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS) != hipSuccess) return MGX_ERR_LAUNCH;
     if (act_alpha > 0.f)
-        hipLaunchKernelGGL((bbwd_kernel<KH, KW, true, CIN>), dim3(WGRID), dim3(256), G::LDS, st, d, x, g, w, dx, partial,
+        hipLaunchKernelGGL((bbwd_kernel<KH, KW, true, CIN, X8>), dim3(WGRID), dim3(256), G::LDS, st, d, x, xe, g, w, dx, partial,
                            ntiles, tiles_h, tiles_w, act_alpha);
     else
-        hipLaunchKernelGGL((bbwd_kernel<KH, KW, false, CIN>), dim3(WGRID), dim3(256), G::LDS, st, d, x, g, w, dx, partial,
+        hipLaunchKernelGGL((bbwd_kernel<KH, KW, false, CIN, X8>), dim3(WGRID), dim3(256), G::LDS, st, d, x, xe, g, w, dx, partial,
                            ntiles, tiles_h, tiles_w, act_alpha);
     const long total = (long)G::NCH * G::TAPS * 1024 + (db ? d.ngemm : 0);
     hipLaunchKernelGGL(bwgrad_reduce_kernel, dim3((unsigned)((total + 63) / 64)), dim3(1024), 0, st, d, partial, dw, db,
@@ -678,4 +694,23 @@ extern "C" int mgx_conv_bwd_bf16(const mgx_conv_desc* dp, const void* x, const v
     if (dp->kh == 3)
         return launch_f<3, 3, 32>(*dp, (const bf16_t*)x, (const bf16_t*)g, w, dw, dbias, (bf16_t*)dx, (float*)workspace, act_alpha, st);
     return launch_f<2, 2, 32>(*dp, (const bf16_t*)x, (const bf16_t*)g, w, dw, dbias, (bf16_t*)dx, (float*)workspace, act_alpha, st);
+}
+
+// mgx_conv_bwd_bf16 with the layer input in the 8-bit tape format (mgx_tape8_pack of the NHWC tensor: a block is 32
+// channels of one position).
+extern "C" int mgx_conv_bwd_tape8(const mgx_conv_desc* dp, const void* codes, const void* exps, const void* g, const float* w,
+                                  float* dw, float* dbias, void* dx, float act_alpha, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+    if (!dp || !codes || !exps || !g || !w || !dw || !dx || !workspace || !mgx_conv_bwd_bf16_supported(dp)) return MGX_ERR_ARG;
+    if (workspace_bytes < mgx_conv_bwd_bf16_workspace(dp)) return MGX_ERR_WORKSPACE;
+    if (dbias && dp->nbias != dp->ngemm) return MGX_ERR_ARG;
+    if (!(act_alpha >= 0.f)) return MGX_ERR_ARG;
+    if ((((uintptr_t)codes | (uintptr_t)g | (uintptr_t)w | (uintptr_t)dx) & 15u) != 0) return MGX_ERR_ARG;
+    hipStream_t st = (hipStream_t)stream;
+    const unsigned char* xe = (const unsigned char*)exps;
+    if (dp->cin == 128)
+        return launch_f<3, 3, 128, true>(*dp, codes, (const bf16_t*)g, w, dw, dbias, (bf16_t*)dx, (float*)workspace, act_alpha, st, xe);
+    if (dp->kh == 3)
+        return launch_f<3, 3, 32, true>(*dp, codes, (const bf16_t*)g, w, dw, dbias, (bf16_t*)dx, (float*)workspace, act_alpha, st, xe);
+    return launch_f<2, 2, 32, true>(*dp, codes, (const bf16_t*)g, w, dw, dbias, (bf16_t*)dx, (float*)workspace, act_alpha, st, xe);
 }

@@ -995,3 +995,113 @@ def cast_to_f32(x: torch.Tensor) -> torch.Tensor:
     y = torch.empty(x.shape, dtype=torch.float32, device=x.device)
     check(_lib().mgx_cast_bf16_to_f32(_pb(x), _p(y), x.numel(), K.stream_ptr()), "mgx_cast_bf16_to_f32")
     return y
+
+
+# --------------------------------------------------------------------------------------------
+# 8-bit activation tape
+# --------------------------------------------------------------------------------------------
+class Tape8:
+    """A tensor as the 8-bit tape keeps it: `codes` (uint8, whole blocks of 32 values), `exps` (uint8, one exponent byte
+    a block), and the shape and type it was packed from.  The values it stands for are exact in bfloat16."""
+    __slots__ = ("shape", "dtype", "codes", "exps")
+
+    def __init__(self, shape, dtype, codes, exps):
+        self.shape, self.dtype, self.codes, self.exps = torch.Size(shape), dtype, codes, exps
+
+    def numel(self) -> int:
+        return self.shape.numel()
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.exps.numel()
+
+
+def _on_current(*ts):
+    """Kernels run on the current device's stream: a tensor of another device would be read through a foreign address."""
+    dev = K.device()
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise MgxError("operand on %s, the current device is %s" % (t.device, dev))
+
+
+def _p_act(t):
+    return _p(t) if t.dtype == torch.float32 else _pb(t)
+
+
+def _p8(t: Tape8):
+    n = t.numel()
+    blocks = (n + 31) // 32
+    for b, size in ((t.codes, 32 * blocks), (t.exps, blocks)):
+        if b.dtype != torch.uint8 or not b.is_cuda or not b.is_contiguous() or b.numel() != size:
+            raise MgxError("tape8: codes / exponent bytes do not match a tensor of %d values" % n)
+    return t.codes.data_ptr(), t.exps.data_ptr()
+
+
+def tape8_pack(x: torch.Tensor) -> Tape8:
+    """The 8-bit form of a contiguous float32 or bfloat16 tensor (mgx_tape8_pack; format in include/mgx.h)."""
+    px = _p_act(x)
+    _on_current(x)
+    n = x.numel()
+    blocks = (n + 31) // 32
+    t = Tape8(x.shape, x.dtype, torch.empty((32 * blocks,), dtype=torch.uint8, device=x.device),
+              torch.empty((blocks,), dtype=torch.uint8, device=x.device))
+    e0 = PROFILER.start() if PROFILER is not None else None
+    check(_lib().mgx_tape8_pack(px, int(x.dtype == torch.float32), t.codes.data_ptr(), t.exps.data_ptr(), n,
+                                K.stream_ptr()), "mgx_tape8_pack")
+    if e0 is not None:
+        PROFILER.stop("tape8_pack", 0.0, e0, n * x.element_size() + t.nbytes())
+    return t
+
+
+def tape8_unpack(t: Tape8, dtype=None) -> torch.Tensor:
+    """The values a Tape8 stands for, in the type it was packed from or in `dtype` (float32 or bfloat16)."""
+    dtype = dtype or t.dtype
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise MgxError("tape8_unpack: float32 or bfloat16")
+    pc, pe = _p8(t)
+    _on_current(t.codes, t.exps)
+    y = torch.empty(t.shape, dtype=dtype, device=t.codes.device)
+    e0 = PROFILER.start() if PROFILER is not None else None
+    check(_lib().mgx_tape8_unpack(pc, pe, y.data_ptr(), int(dtype == torch.float32), t.numel(), K.stream_ptr()),
+          "mgx_tape8_unpack")
+    if e0 is not None:
+        PROFILER.stop("tape8_unpack", 0.0, e0, y.numel() * y.element_size() + t.nbytes())
+    return y
+
+
+def mul_dact_tape8(a: torch.Tensor, t: Tape8, act_alpha) -> torch.Tensor:
+    """bf16(a * f'(y)) like mul_dact_bf16, y the activation output kept in `t`."""
+    if a.numel() != t.numel():
+        raise MgxError("mul_dact_tape8: size mismatch")
+    if not act_alpha > 0.0:
+        raise MgxError("mul_dact_tape8: act_alpha must be positive")
+    pa, (pc, pe) = _p_act(a), _p8(t)
+    _on_current(a, t.codes, t.exps)
+    out = torch.empty(t.shape, dtype=torch.bfloat16, device=a.device)
+    e0 = PROFILER.start() if PROFILER is not None else None
+    check(_lib().mgx_mul_dact_tape8(pa, int(a.dtype == torch.float32), pc, pe, float(act_alpha), out.data_ptr(), a.numel(),
+                                    K.stream_ptr()), "mgx_mul_dact_tape8")
+    if e0 is not None:
+        PROFILER.stop("mul_dact_tape8", 0.0, e0, a.numel() * (a.element_size() + 2) + t.nbytes())
+    return out
+
+
+def conv_bwd_tape8(d: ConvDesc, t: Tape8, g, w, dw, dbias, dx, act_alpha=0.0):
+    """conv_bwd_bf16 with the layer input kept in `t` (descriptors of conv_bwd_bf16_supported)."""
+    xe, ye, we = _conv_sizes(d)
+    if t.numel() != xe or g.numel() != ye or dw.numel() < we or w.numel() < we or dx.numel() != xe:
+        raise MgxError("conv_bwd_tape8: operand sizes do not match the descriptor")
+    if dbias is not None and dbias.numel() != d.nbias:
+        raise MgxError("conv_bwd_tape8: bias gradient size mismatch")
+    pc, pe = _p8(t)
+    _on_current(t.codes, t.exps, g, w, dw, dbias, dx)
+    lib = _lib()
+    nbytes = lib.mgx_conv_bwd_bf16_workspace(C.byref(d))
+    if nbytes <= 0:
+        raise MgxError("conv_bwd_tape8: unsupported descriptor")
+    ws = K.workspace(nbytes)
+    e0 = PROFILER.start() if PROFILER is not None else None
+    check(lib.mgx_conv_bwd_tape8(C.byref(d), pc, pe, _pb(g), _p(w), _p(dw), _p(dbias), _pb(dx), float(act_alpha),
+                                 ws.data_ptr(), ws.numel(), K.stream_ptr()), "mgx_conv_bwd_tape8")
+    if e0 is not None:
+        PROFILER.stop("bbwd_kernel<%d,%d,tape8>" % (d.kh, d.kw), 2 * _conv_flops(d), e0,
+                      2.0 * (ye + xe) + t.nbytes() + 4.0 * (we + d.nbias))

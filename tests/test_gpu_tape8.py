@@ -1,0 +1,224 @@
+"""The 8-bit activation tape: format, special blocks, products with the recovered derivative, the fused convolution
+backward that reads it, refusals.  The reference is the definition in float64 on the CPU."""
+import numpy as np
+import pytest
+import torch
+
+import music_generator_amd as M
+from music_generator_amd import ops
+from music_generator_amd._cabi import MgxError
+
+gpu = pytest.mark.gpu
+ALPHA = 20000.0
+
+
+def kept_reference(x):
+    """Values the tape of x stands for, float64, from the definition."""
+    v = x.detach().cpu().double().reshape(-1)
+    n = v.numel()
+    v = torch.nn.functional.pad(v, (0, -n % 32)).view(-1, 32)
+    big = v.abs().max(dim=1, keepdim=True).values
+    m, ex = torch.frexp(torch.where(torch.isfinite(big), big, torch.ones_like(big)))
+    top = torch.ldexp(torch.ones_like(m), torch.where(m <= 0.5 * (1 + 2.0 ** -8), ex - 1, ex).clamp(min=-118))
+    q = ((v * 128.0 / top).floor().clamp(-128.0, 127.0) + 0.5) * top / 128.0
+    q = torch.where(big == 0, torch.zeros_like(q), q)
+    q = torch.where(torch.isfinite(v).all(dim=1, keepdim=True), q, torch.full_like(q, float("nan")))
+    return q.view(-1)[:n].view(x.shape)
+
+
+def derivative(y):
+    return torch.clamp(1.0 + 1.0 / ALPHA - y * y, min=1.0 / ALPHA)
+
+
+def activations(shape, seed, dtype):
+    pre = torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * 1.2
+    return (torch.tanh(pre) + pre / ALPHA).to(dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 7, 31, 32, 33, 256, 1000, 4 * 1501 * 32, 300001])
+def test_kept_values_are_the_definition(n, dtype):
+    x = activations((n,), n, dtype).cuda()
+    t = ops.tape8_pack(x)
+    assert t.nbytes() == 33 * ((n + 31) // 32)
+    want = kept_reference(x)
+    for out in (torch.float32, torch.bfloat16):
+        assert torch.equal(ops.tape8_unpack(t, out).cpu().double(), want)      # eight significant bits: exact in both
+    assert ops.tape8_unpack(t).dtype == dtype
+    # |tanh(v) + v / alpha| <= 1 + |v| / alpha, |v| < 7 here: less than a 256th past 1, so H <= 1; values up to H come back
+    # within H / 256, those above it within H / 128
+    v = x.cpu().double()
+    assert float(v.abs().max()) <= 1 + 2.0 ** -8
+    assert bool(((want - v).abs() <= torch.where(v.abs() <= 1, 2.0 ** -8, 2.0 ** -7)).all())
+
+
+@gpu
+def test_special_blocks():
+    x = torch.zeros((12, 32))
+    x[1] = torch.linspace(-1, 1, 32)                 # both ends of the range
+    x[2, 5] = float("nan")
+    x[3, 9] = float("-inf")
+    x[4] = 1e-42                                     # below the smallest normal number
+    x[5, 3] = 3.3e38                                 # above 2^127
+    x[6] = 2.0 ** torch.arange(-20, 12)
+    x[7, 31] = -2.0 ** -100
+    x[8] = -0.0
+    x[9, 0] = 2.0 ** -118
+    x[10] = torch.nextafter(torch.tensor(1.0), torch.tensor(2.0))
+    x[11] = -1e-7                                    # floor, not rounding towards zero
+    x[11, 0] = 1.0
+    x = torch.cat([x, torch.zeros((3, 32))])
+    x[12, 0], x[12, 1] = -1.0 - 2.0 ** -8, 1.0 + 2.0 ** -8       # the border of the rule for H, both signs
+    x[13, 0] = 1.0 + 2.0 ** -8 + 2.0 ** -23
+    x[14, 0], x[14, 1] = 1.0 + 2.0 ** -7, 0.3
+    for y in (x, x.to(torch.bfloat16)):
+        got = ops.tape8_unpack(ops.tape8_pack(y.cuda()), torch.float32).cpu().double()
+        assert torch.equal(torch.nan_to_num(got, 77.0), torch.nan_to_num(kept_reference(y), 77.0))
+        assert got[2].isnan().all() and got[3].isnan().all()
+        assert (got[0] == 0).all() and (got[8] == 0).all()
+        assert got[1, 0] == -got[1, 31] == -255.0 / 256.0
+        assert got[12, 0] == -got[12, 1] == -255.0 / 256.0 or y.dtype == torch.bfloat16
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [5, 32, 8 * 1500 * 32, 100003])
+def test_product_with_the_recovered_derivative(n, dtype):
+    y = activations((n,), 3, torch.bfloat16).cuda()
+    a = (torch.randn((n,), generator=torch.Generator().manual_seed(4)) * 1e-3).to(dtype).cuda()
+    got = ops.mul_dact_tape8(a, ops.tape8_pack(y), ALPHA).cpu().double()
+    want = a.cpu().double() * derivative(kept_reference(y))
+    # one rounding to bf16 (2^-8 of the value covers it and the float32 steps: 1 + 1/alpha and 1 - y^2 are 2^-24 off
+    # where the derivative is at least 2^-8, the smallest distance of a kept y from 1)
+    assert bool(((got - want).abs() <= 2.0 ** -8 * want.abs() + 1e-30).all())
+
+
+@gpu
+def test_non_finite_blocks_reach_the_gradient():
+    y = torch.zeros((64,), dtype=torch.bfloat16)
+    y[3] = float("inf")
+    got = ops.mul_dact_tape8(torch.ones((64,)).cuda(), ops.tape8_pack(y.cuda()), ALPHA).cpu()
+    assert got[:32].isnan().all() and got[32:].isfinite().all()
+
+
+def conv_case(n, h, w, cin, k, seed):
+    gen = torch.Generator().manual_seed(seed)
+    x = activations((n, h, w, cin), seed, torch.bfloat16)
+    g = torch.randn((n, h, w, 32), generator=gen).to(torch.bfloat16)
+    # kernels that are exact in bf16, so that the data gradient has one rounding only
+    wt = (torch.randn((k, k, cin, 32), generator=gen) / (k * cin ** 0.5)).to(torch.bfloat16).float()
+    p = (k - 1) // 2
+    d = ops.make_conv_desc(nimg=n, hin=h, win=w, cin=cin, hout=h, wout=w, kh=k, kw=k, pt=p, pl=p, ngemm=32, cout=32,
+                           wsk=32, wsn=1, wtap=cin * 32, nbias=32)
+    return d, x, g, wt
+
+
+def conv_reference(x, g, wt, act):
+    """Gradients of the 'same' convolution by autograd in float64 on the kept values."""
+    q = kept_reference(x)
+    k = wt.shape[0]
+    p0, p1 = (k - 1) // 2, k - 1 - (k - 1) // 2
+    xi = q.permute(0, 3, 1, 2).clone().requires_grad_(True)
+    wi = wt.double().permute(3, 2, 0, 1).clone().requires_grad_(True)
+    bi = torch.zeros((32,), dtype=torch.float64, requires_grad=True)
+    y = torch.nn.functional.conv2d(torch.nn.functional.pad(xi, (p0, p1, p0, p1)), wi, bi)
+    dx, dw, db = torch.autograd.grad(y, (xi, wi, bi), g.double().permute(0, 3, 1, 2))
+    dx = dx.permute(0, 2, 3, 1)
+    return dx * derivative(q) if act else dx, dw.permute(2, 3, 1, 0), db
+
+
+@gpu
+@pytest.mark.parametrize("act", [True, False])
+@pytest.mark.parametrize("n,h,w,cin,k", [(1, 8, 64, 32, 3), (1, 1, 1, 32, 3), (2, 9, 65, 32, 3), (3, 13, 131, 32, 2),
+                                         (1, 1, 7, 32, 2), (1, 8, 32, 128, 3), (2, 5, 37, 128, 3), (1, 3, 1501, 32, 3)])
+def test_convolution_backward(n, h, w, cin, k, act):
+    d, x, g, wt = conv_case(n, h, w, cin, k, seed=n * 100 + h + w)
+    t = ops.tape8_pack(x.cuda())
+    dw0 = torch.randn((k, k, cin, 32), generator=torch.Generator().manual_seed(1))
+    dw, db = dw0.cuda(), torch.full((32,), 0.5).cuda()
+    dx = torch.empty((n, h, w, cin), dtype=torch.bfloat16, device="cuda")
+    ops.conv_bwd_tape8(d, t, g.cuda(), wt.cuda(), dw, db, dx, ALPHA if act else 0.0)
+    rx, rw, rb = conv_reference(x, g, wt, act)
+    # dx: one rounding to bf16, and float32 sums of 9 * 32 products of magnitude ~ 1 / (3 sqrt(cin))
+    assert bool(((dx.cpu().double() - rx).abs() <= 2.0 ** -8 * rx.abs() + 288 * 2.0 ** -24).all())
+    # dw, db: exact products, float32 sums of P terms of magnitude ~ 1: P ulp at most, sqrt(P) in practice
+    lim = n * h * w * 2.0 ** -24 * 4 + 2.0 ** -22
+    assert float((dw.cpu().double() - dw0.double() - rw).abs().max()) <= lim
+    assert float((db.cpu().double() - 0.5 - rb).abs().max()) <= lim
+
+
+@gpu
+def test_convolution_backward_equals_the_bf16_kernel_on_the_kept_values():
+    d, x, g, wt = conv_case(2, 17, 200, 32, 3, seed=5)
+    t = ops.tape8_pack(x.cuda())
+    kept = ops.tape8_unpack(t)
+    out = []
+    for f, xin in ((ops.conv_bwd_tape8, t), (ops.conv_bwd_bf16, kept)):
+        dw, db = torch.zeros_like(wt).cuda(), torch.zeros((32,)).cuda()
+        dx = torch.empty_like(kept)
+        f(d, xin, g.cuda(), wt.cuda(), dw, db, dx, ALPHA)
+        out.append((dw, db, dx))
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_captured_pack_and_backward_replay():
+    d, x, g, wt = conv_case(1, 8, 100, 32, 3, seed=6)
+    xd, gd, wd = x.cuda(), g.cuda(), wt.cuda()
+    dw, db, dx = torch.zeros_like(wd), torch.zeros((32,), device="cuda"), torch.empty_like(xd)
+
+    def step():
+        dw.zero_()
+        db.zero_()
+        ops.conv_bwd_tape8(d, ops.tape8_pack(xd), gd, wd, dw, db, dx, ALPHA)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for seed in range(3):
+        xd.copy_(activations(tuple(x.shape), 50 + seed, torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [v.clone() for v in (dw, db, dx)]
+        step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, (dw, db, dx)))
+
+
+@gpu
+def test_empty_tensor():
+    t = ops.tape8_pack(torch.empty((0, 32), device="cuda"))
+    assert t.nbytes() == 0 and tuple(ops.tape8_unpack(t).shape) == (0, 32)
+
+
+@gpu
+def test_refusals():
+    x = torch.zeros((4, 8, 16, 32), dtype=torch.bfloat16, device="cuda")
+    t = ops.tape8_pack(x)
+    d, _, g, wt = conv_case(4, 8, 16, 32, 3, seed=0)
+    g, wt = g.cuda(), wt.cuda()
+    dw, db, dx = torch.zeros_like(wt), torch.zeros((32,), device="cuda"), torch.empty_like(x)
+    for bad in (x.permute(0, 3, 1, 2), x.half(), x.double(), x.cpu()):
+        with pytest.raises(MgxError):
+            ops.tape8_pack(bad)
+    with pytest.raises(MgxError):
+        ops.tape8_pack(x.view(-1)[1:])                                   # not 16-byte aligned
+    with pytest.raises(MgxError):
+        ops.tape8_unpack(t, torch.float16)
+    with pytest.raises(MgxError):
+        ops.tape8_unpack(ops.Tape8((4, 8, 16, 33), t.dtype, t.codes, t.exps))
+    with pytest.raises(MgxError):
+        ops.mul_dact_tape8(x[:2], t, ALPHA)
+    with pytest.raises(MgxError):
+        ops.mul_dact_tape8(x, t, 0.0)
+    with pytest.raises(MgxError):
+        ops.conv_bwd_tape8(d, ops.tape8_pack(x[:2].contiguous()), g, wt, dw, db, dx)
+    with pytest.raises(MgxError):
+        ops.conv_bwd_tape8(d, t, g.float(), wt, dw, db, dx)
+    with pytest.raises(MgxError):
+        ops.conv_bwd_tape8(d, t, g, wt, dw, db, dx, act_alpha=-1.0)
+    with pytest.raises(MgxError):
+        ops.conv_bwd_tape8(d, t, g, wt, dw, torch.zeros((16,), device="cuda"), dx)
