@@ -109,6 +109,12 @@ class Layer:
         """returns (y, saved)"""
         raise NotImplementedError
 
+    def keep8(self, saved, take):
+        """The tape entry `saved` with its tensors replaced by their 8-bit forms (backend.TAPE8): take(0), take(1) give
+        those of the layer's inputs, take(-1) that of the step's output, each packed once per forward.  The default
+        keeps the entry as it is."""
+        return saved
+
     def backward(self, saved, dy: torch.Tensor, need: List[bool], existing: List[Optional[torch.Tensor]],
                  wgrad: bool):
         """returns a list with, per input, None or (tensor, owned)"""
@@ -343,7 +349,7 @@ class Model:
 
     def tape_bytes_estimate(self, n: int) -> int:
         """Bytes a taped forward of `n` samples keeps for its backward, from the plan's symbolic shapes: every
-        step's output (the next step's saved input), in bf16 where the bf16 kernels store it, plus the saved
+        step's output (the next step's saved input), in bf16 where the bf16 kernels store it (8 bits with backend.TAPE8), plus the saved
         activation derivative where one is kept (float32 convolutions; bf16 ones only with
         backend.BF16_SAVE_DERIVATIVE).  An estimate for memory planning, not an accounting."""
         total = 0
@@ -356,6 +362,9 @@ class Model:
             conv = getattr(op.node.layer, "fusable_activation", False) and len(shape) == 4
             half = bf and conv and shape[1] >= K.BF16_MIN_ROWS and shape[-1] in (32, 128)
             copies = 2 if (op.act_node is not None and (not half or K.BF16_SAVE_DERIVATIVE)) else 1
+            if conv and K.TAPE8 and shape[-1] % 32 == 0:
+                total += -(-elems // 32) * 33 * copies
+                continue
             total += elems * (2 if half else 4) * copies
         return int(total) * int(n)
 
@@ -431,6 +440,15 @@ class Model:
         # outputs of from-audio layers not computed yet (tape-free bf16 passes): id -> (layer, alpha, audio).  The
         # fade-in blend re-computes such an input in its epilogue; any other reader gets it computed on first use.
         deferred: Dict[int, tuple] = {}
+        kept: Dict[int, ops.Tape8] = {}       # 8-bit forms by symbolic tensor: one for its producer and all its readers
+
+        def keep8(op, saved, xs, y):
+            def take(j):
+                t, v = (op.output, y) if j < 0 else (op.inputs[j], xs[j])
+                if id(t) not in kept:
+                    kept[id(t)] = ops.tape8_pack(v)
+                return kept[id(t)]
+            return op.node.layer.keep8(saved, take)
 
         def value_of(t):
             pending = deferred.pop(id(t), None)
@@ -519,6 +537,8 @@ class Model:
                     if save:
                         # one launch that also writes the inner outputs; the tape gets every layer's entry
                         vals[id(chain[-1].output)], entries = conv_chain_forward_taped(chain_layers, chain_alphas, xs[0])
+                        if K.TAPE8:
+                            entries = [keep8(o, e, [e.x], e.yact) for o, e in zip(chain, entries)]
                         tape.extend(entries)
                     else:
                         vals[id(chain[-1].output)] = conv_chain_forward(chain_layers, chain_alphas, xs[0])
@@ -560,7 +580,7 @@ class Model:
                 y, saved = op.node.layer.forward(xs, save)
             vals[id(op.output)] = y
             if save:
-                tape.append(saved)
+                tape.append(keep8(op, saved, xs, y) if K.TAPE8 else saved)
             for t in op.inputs:
                 if last_use.get(id(t)) == i and t is not self.output:
                     vals.pop(id(t), None)

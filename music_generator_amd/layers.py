@@ -106,16 +106,34 @@ class _Contraction(Layer):
                       dact=dact, act_alpha=act_alpha)
         return y, ((_CastSaved((x, dact)) if was_bf16 else (x, dact)) if save else None)
 
+    def keep8(self, saved, take):
+        if isinstance(saved, _BSaved):
+            if saved.mode == "conv":          # "audio": the 2-channel float32 input stays as it is
+                saved.x = take(0)
+            if saved.yact is not None:
+                saved.yact = take(-1)
+            return saved
+        if type(saved) not in (tuple, _CastSaved) or len(saved) != 2:
+            return saved
+        x, dact = saved
+        if x.shape[-1] % 32 == 0:
+            x = take(0).view(x.shape)
+        if dact is not None and dact.shape[-1] % 32 == 0:
+            dact = ops.tape8_pack(dact)
+        kept = (x, dact)
+        return kept if type(saved) is tuple else type(saved)(kept)
+
     def backward(self, saved, dy, need, existing, wgrad, outmul=None):
         if isinstance(saved, _BSaved):
             return self._backward_bf16(saved, dy, need, existing, wgrad, outmul)
         x, dact = saved
         was_bf16 = isinstance(saved, _CastSaved)
         n, h, w, _ = x.shape
+        dact = _whole(dact, torch.float32)
         if wgrad and self.trainable:
             if self.kernel.grad is None or self.bias.grad is None:
                 raise RuntimeError("gradient buffers of %s are not bound" % self.name)
-            ops.conv_wgrad(self._desc("f", n, h, w), x, dy, self.kernel.grad, self.bias.grad, dymul=dact)
+            ops.conv_wgrad(self._desc("f", n, h, w), _whole(x, torch.float32), dy, self.kernel.grad, self.bias.grad, dymul=dact)
         if not need[0]:
             return [None]
         if was_bf16:
@@ -158,7 +176,7 @@ class _Contraction(Layer):
         n, h, w, _ = x.shape
         if saved.has_derivative() and not saved.premultiplied:
             # dY (.) f': the kernel upstream could not apply it
-            g = ops.mul_bf16(dy, saved.dact) if saved.dact is not None else ops.mul_dact_bf16(dy, saved.yact, saved.alpha)
+            g = saved.times_derivative(dy)
         else:
             g = dy if dy.dtype == torch.bfloat16 else ops.cast_to_bf16(dy)
         do_w = wgrad and self.trainable
@@ -175,8 +193,10 @@ class _Contraction(Layer):
         fdesc = self._desc("f", n, h, w)
         fuse = do_w and need[0] and existing[0] is None and K.BF16_FUSED_CONV_BACKWARD \
             and (outmul is None or outmul.dact is None) and ops.conv_bwd_bf16_supported(fdesc)
+        eight = isinstance(x, ops.Tape8)
+        xw = _whole(x, torch.bfloat16) if eight and not fuse else x
         if do_w and not fuse:
-            ops.conv_wgrad_bf16(fdesc, x, g, self.kernel.grad, self.bias.grad)
+            ops.conv_wgrad_bf16(fdesc, xw, g, self.kernel.grad, self.bias.grad)
         if not need[0]:
             return [None]
         if existing[0] is not None:
@@ -190,8 +210,9 @@ class _Contraction(Layer):
         if fuse:
             # both gradients read x and g: one pass (x is the producer's stored output the derivative comes from)
             assert ymul is None or ymul is x
-            ops.conv_bwd_bf16(fdesc, x, g, self.kernel.value(), self.kernel.grad, self.bias.grad, dx, mul_alpha)
+            (ops.conv_bwd_tape8 if eight else ops.conv_bwd_bf16)(fdesc, x, g, self.kernel.value(), self.kernel.grad, self.bias.grad, dx, mul_alpha)
         else:
+            ymul = xw if ymul is x else _whole(ymul, torch.bfloat16)
             ops.conv_gemm_bf16(self._desc("d", n, h, w), g, self.kernel.value(), None, dx, ymul=ymul, act_alpha=mul_alpha)
         return [(dx, True)]
 
@@ -218,11 +239,11 @@ def audio_dgrad_backward(conv, saved, audio_conv, audio_saved, dy, existing):
     x = saved.x
     n, h, w, _ = x.shape
     if saved.has_derivative() and not saved.premultiplied:
-        g = ops.mul_bf16(dy, saved.dact) if saved.dact is not None else ops.mul_dact_bf16(dy, saved.yact, saved.alpha)
+        g = saved.times_derivative(dy)
     else:
         g = dy if dy.dtype == torch.bfloat16 else ops.cast_to_bf16(dy)
     dxa = existing if existing is not None else K.empty(tuple(audio_saved.x.shape))
-    ops.conv_dgrad_to_audio_bf16(conv._desc("d", n, h, w), g, conv.kernel.value(), x, audio_saved.alpha,
+    ops.conv_dgrad_to_audio_bf16(conv._desc("d", n, h, w), g, conv.kernel.value(), _whole(x, torch.bfloat16), audio_saved.alpha,
                                  audio_conv.kernel.value(), dxa, existing is not None)
     return dxa
 
@@ -357,6 +378,11 @@ def conv_chain_forward_taped(layers, alphas, x):
     return ys[-1], saved
 
 
+def _whole(t, dtype):
+    """A taped tensor as the kernels without an 8-bit form read it: unpacked into a buffer that lives until they ran."""
+    return ops.tape8_unpack(t, dtype) if isinstance(t, ops.Tape8) else t
+
+
 class _CastSaved(tuple):
     """(x, dact) of a float32 contraction whose input arrived as bf16 and was cast: the data-gradient goes
     back as bf16."""
@@ -367,7 +393,7 @@ class _BSaved:
     saved derivative (`dact`) or the layer's stored output and the activation's alpha the derivative is recovered
     from (`yact`, `alpha`; the output is the next layer's taped input, so it costs no memory); and whether the
     gradient that will arrive has already been multiplied by that derivative (the data-gradient kernel of the
-    consuming layer does it in its epilogue)."""
+    consuming layer does it in its epilogue).  x and yact are ops.Tape8 when the tape is kept in 8 bits."""
     __slots__ = ("mode", "x", "dact", "yact", "alpha", "premultiplied")
 
     def __init__(self, mode, x, dact, yact=None, alpha=0.0):
@@ -375,6 +401,12 @@ class _BSaved:
 
     def has_derivative(self) -> bool:
         return self.dact is not None or self.yact is not None
+
+    def times_derivative(self, dy):
+        """bf16(dy (.) f'), from the saved derivative or the kept output."""
+        if self.dact is not None:
+            return ops.mul_bf16(dy, self.dact)
+        return (ops.mul_dact_tape8 if isinstance(self.yact, ops.Tape8) else ops.mul_dact_bf16)(dy, self.yact, self.alpha)
 
 
 class Conv2D(_Contraction):

@@ -61,8 +61,11 @@ class WeightedSum(Add):
     # epilogue (mgx_conv1x1_blend_bf16) instead of running this layer
     is_weighted_sum = True
 
+    def keep8(self, saved, take):
+        return tuple(take(j) if t.shape[-1] % 32 == 0 else t for j, t in enumerate(saved))
+
     def backward(self, saved, dy, need, existing, wgrad, outmuls=(None, None)):
-        a, b = saved
+        a, b = (ops.tape8_unpack(t) if isinstance(t, ops.Tape8) else t for t in saved)
         dalpha = self.alpha.grad if (wgrad and self.trainable and self.alpha.trainable) else None
         if dalpha is None and wgrad and self.trainable and self.alpha.trainable:
             raise RuntimeError("gradient buffer of %s is not bound" % self.alpha.name)
@@ -75,7 +78,7 @@ class WeightedSum(Add):
             # a producer's activation derivative is applied here instead of in a multiply launch of its own: the
             # saved tensor, or recovered from the producer's stored output, which is this layer's input a / b
             mul, mal = [None, None], [0.0, 0.0]
-            for k, (om, d_, inp) in enumerate(zip(outmuls, (da, db), (a, b))):
+            for k, (om, d_, inp) in enumerate(zip(outmuls, (da, db), saved)):
                 if d_ is None or om is None or not om.has_derivative() or om.premultiplied:
                     continue
                 if om.dact is not None:
@@ -929,7 +932,7 @@ class WGAN:
         # a graph is valid for one batch shape, one set of step-shaping options and one generation of the
         # scratch buffers whose addresses its launches carry
         key = (tuple(real.shape), self.micro_batch, self.generator_chunk, self.reuse_real_logits,
-               FusedGroup.side_budget_bytes, K.precision(), self._overlap(real.shape[0]),
+               FusedGroup.side_budget_bytes, K.precision(), K.TAPE8, self._overlap(real.shape[0]),
                self._merge(real.shape[0]), self.early_generator)
         entry = self._graphs.get(key)
         alpha = self._fade_alpha()

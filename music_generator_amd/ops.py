@@ -1011,6 +1011,15 @@ class Tape8:
     def numel(self) -> int:
         return self.shape.numel()
 
+    def dim(self) -> int:
+        return len(self.shape)
+
+    def view(self, shape) -> "Tape8":
+        """The same bytes as a tensor of another shape (same number of values in the same order)."""
+        if torch.Size(shape).numel() != self.numel():
+            raise MgxError("Tape8.view: another number of values")
+        return self if tuple(shape) == tuple(self.shape) else Tape8(shape, self.dtype, self.codes, self.exps)
+
     def nbytes(self) -> int:
         return self.codes.numel() + self.exps.numel()
 

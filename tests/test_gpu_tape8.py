@@ -222,3 +222,155 @@ def test_refusals():
         ops.conv_bwd_tape8(d, t, g, wt, dw, db, dx, act_alpha=-1.0)
     with pytest.raises(MgxError):
         ops.conv_bwd_tape8(d, t, g, wt, dw, torch.zeros((16,), device="cuda"), dx)
+
+
+# ---- the tape of a model (backend.TAPE8) ----
+@pytest.fixture
+def tape8():
+    M.backend.TAPE8 = True
+    yield
+    M.backend.TAPE8 = False
+    M.backend.set_precision("float32")
+
+
+def discriminator(stage, fade, precision):
+    M.backend.set_precision(precision)
+    M.clear_session()
+    return M.define_discriminator(stage + 1)[stage][int(fade)]
+
+
+def whole_again(tape):
+    """The tape with every 8-bit form replaced by the tensor it stands for (one per Tape8, as a tape shares them)."""
+    seen = {}
+
+    def back(v, dtype=None):
+        if isinstance(v, ops.Tape8):
+            return seen.setdefault((id(v), dtype), ops.tape8_unpack(v, dtype))
+        if isinstance(v, tuple):      # a subclass marks the float32 copy of a bf16 input
+            return tuple(back(u) for u in v) if type(v) is tuple else type(v)([back(u, torch.float32) for u in v])
+        if hasattr(v, "premultiplied"):
+            v.x, v.yact = back(v.x), back(v.yact)
+        return v
+    for i, entry in enumerate(tape):
+        tape[i] = back(entry)
+    return tape
+
+
+def tape_bytes(tape):
+    seen = {}
+
+    def count(v):
+        if isinstance(v, ops.Tape8):
+            seen[v.codes.data_ptr()] = v.nbytes()
+        elif isinstance(v, torch.Tensor):
+            seen[v.data_ptr()] = v.numel() * v.element_size()
+        elif isinstance(v, (tuple, list)):
+            for u in v:
+                count(u)
+        elif hasattr(v, "premultiplied"):
+            for u in (v.x, v.yact, v.dact):
+                count(u)
+    count(list(tape))
+    return sum(seen.values())
+
+
+def gradients(model, tape, dy, **kw):
+    flat = model.bind_grads()
+    flat.zero_()
+    dx = model.backward(tape, dy, **kw)
+    return flat.clone(), dx
+
+
+@gpu
+@pytest.mark.parametrize("precision,fade", [("bfloat16", False), ("bfloat16", True), ("float32", True)])
+def test_model_backward_from_the_8_bit_tape(tape8, precision, fade):
+    """The sweep over the bytes gives the bits of the same sweep over the tensors they stand for, the forward is
+    untouched, and the tape is a half (bf16) or a quarter (float32) of what it was."""
+    d = discriminator(1, fade, precision)
+    x = torch.randn((4, 8, 1500, 2), generator=torch.Generator().manual_seed(2)).cuda()
+    dy = torch.full((4, 1), 0.25).cuda()
+    M.backend.TAPE8 = False
+    y0, full = d.forward(x, save=True)
+    full_bytes, estimate0 = tape_bytes(full), d.tape_bytes_estimate(4)
+    g0, dx0 = gradients(d, full, dy, need_input_grad=True)
+    M.backend.TAPE8 = True
+    y1, tape = d.forward(x, save=True)
+    assert torch.equal(y0, y1)
+    assert tape_bytes(tape) < (0.65 if precision == "bfloat16" else 0.35) * full_bytes
+    assert d.tape_bytes_estimate(4) < 0.65 * estimate0
+    g1, dx1 = gradients(d, tape, dy, need_input_grad=True)
+    g2, dx2 = gradients(d, whole_again(d.forward(x, save=True)[1]), dy, need_input_grad=True)
+    assert torch.equal(g1, g2) and torch.equal(dx1, dx2)
+    # the gradients of activations off by at most 2^-8: a kept value is off by 2^-7 / sqrt(12) = 0.23 % of 1 in the mean
+    # and its derivative by 2 |y| of that; the activations' root mean square is about 0.6, so a layer adds 0.4 % (its
+    # input in the weight gradient) and 0.6 % (derivative), and the 20 layers of the sweep 20 * 0.6 % at most
+    for a, b in ((g1, g0), (dx1, dx0)):
+        assert float((a - b).norm() / b.norm()) < 20 * 0.006
+
+
+@gpu
+def test_sweep_without_weight_gradients(tape8):
+    d = discriminator(1, False, "bfloat16")
+    x = torch.randn((4, 8, 1500, 2), generator=torch.Generator().manual_seed(3)).cuda()
+    dy = torch.full((4, 1), 0.25).cuda()
+    dx = d.backward(d.forward(x, save=True)[1], dy, need_input_grad=True, need_weight_grads=False)
+    want = d.backward(whole_again(d.forward(x, save=True)[1]), dy, need_input_grad=True, need_weight_grads=False)
+    assert torch.equal(dx, want)
+
+
+@gpu
+def test_weight_gradient_against_differences(tape8):
+    """Difference quotient of the last convolution's kernel: its gradient uses the kept input, its derivative and nothing
+    in front of it, so the quotient of the exact forward is met to the rounding of that one layer."""
+    d = discriminator(0, False, "float32")
+    x = torch.randn((4, 4, 750, 2), generator=torch.Generator().manual_seed(4)).cuda()
+    conv = [l for l in d.layers if type(l).__name__ == "Conv2D"][-1]
+    direction = torch.randn((conv.kernel.size,), generator=torch.Generator().manual_seed(5)).cuda()
+    direction /= direction.norm()
+    dy = torch.ones((4, 1)).cuda()
+    _, tape = d.forward(x, save=True)
+    gradients(d, tape, dy)
+    slope = float((conv.kernel.grad.double() * direction.double()).sum())
+    w0, step, ends = conv.kernel.value().clone(), 1e-2, []
+    for s in (step, -step):
+        conv.kernel.value().copy_(w0 + s * direction)
+        ends.append(float(d(x).double().sum()))
+    conv.kernel.value().copy_(w0)
+    quotient = (ends[0] - ends[1]) / (2 * step)
+    norm = float(conv.kernel.grad.double().norm())
+    # 1 % of the gradient's length covers the 0.4 % and 0.6 % of one layer's input and derivative; the quotient's own
+    # float32 noise is 4 outputs of 2^-24 relative over 2 step
+    assert abs(quotient - slope) <= 0.01 * norm + 4 * abs(ends[0]) * 2.0 ** -24 / step
+
+
+@gpu
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_train_step(tape8, use_graph):
+    """Fade-in steps train from the 8-bit tape, eagerly and replayed: finite metrics, other bits than from the ordinary
+    tape, and a graph of its own for each kind of tape."""
+    def build():
+        M.backend.set_precision("bfloat16")
+        M.clear_session()
+        M.layers.set_init_seed(7)
+        d, g = M.define_discriminator(2), M.define_generator(2)
+        gan = M.define_composite(d, g, (1, 100, 2))[1][1]
+        gan.set_train_steps(10)
+        gan.use_graph = use_graph
+        return gan
+    real = torch.randn((4, 8, 1500, 2), generator=torch.Generator().manual_seed(6)).cuda()
+    runs = []
+    for eight in (False, True):
+        M.backend.TAPE8 = eight
+        gan = build()
+        torch.manual_seed(11)
+        out = []
+        for _ in range(4):
+            out.append({k: float(v) for k, v in gan.train_step(real).items()})
+        runs.append(out)
+        assert all(np.isfinite(list(m.values())).all() for m in out)
+    assert runs[0] != runs[1]                       # the gradients are not the same bits
+    if use_graph:
+        M.backend.TAPE8 = False                     # another key: an eager step, then a capture of its own
+        before = len(gan._graphs)
+        gan.train_step(real)
+        assert len(gan._graphs) == before + 1
