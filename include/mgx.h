@@ -553,6 +553,27 @@ int mgx_conv_bwd_tape8(const mgx_conv_desc* d, const void* codes, const void* ex
                        float* dw, float* dbias, void* dx, float act_alpha, void* workspace, int64_t workspace_bytes,
                        void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Softmax cross entropy of a Dense head with many classes (mgx_softmax_xent beside Dense(units, softmax),
+ * trainer/evaluacion.py:97, 160) from the head's input, without keeping the logits z = x W + b:
+ *   forward   lse_i = log sum_j exp(z_ij),  loss_i = lse_i - z_i,label(i)
+ *             hits_i (optional): 1 where no class has a larger logit than the label's
+ *   backward  dz_ij = dloss_i (exp(z_ij - lse_i) - [j = label(i)]);  dx = dz W^T (written, type of x);
+ *             dw = x^T dz, db_j = sum_i dz_ij (float32; written, or added to with accumulate != 0)
+ * x (n, e) float32 or bf16, w (e, v) and b (v, may be NULL) float32, labels (n).  A label outside [0, v) marks a row without
+ * a loss: loss, lse, hits and its gradients are 0 and its features are not used.  A bias of -inf (or the lowest float)
+ * masks a class.  Any of dx, dw, db may be NULL.  n <= 8 000 000, v <= 8 000 000, e <= 65 536; x, w and the workspace
+ * 16-byte aligned; the workspace (mgx_dense_xent_workspace bytes, -1: sizes out of range) is the call's alone while it
+ * runs.  float32 quality throughout: the products are sums of products of fp16 halves of the operands.
+ * ---------------------------------------------------------------------------------------- */
+int64_t mgx_dense_xent_workspace(int64_t n, int64_t e, int64_t v, int x_is_f32, int backward);
+int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, const float* b, const int32_t* labels, float* loss,
+                       float* lse, int32_t* hits, int64_t n, int64_t e, int64_t v, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, const float* b, const int32_t* labels,
+                       const float* lse, const float* dloss, void* dx, float* dw, float* db, int accumulate, int64_t n,
+                       int64_t e, int64_t v, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -160,6 +160,9 @@ PROTOTYPES = {
     "mgx_mul_dact_bf16": (_I, [_P, _I, _P, _F, _P, _I64, _P]),
     "mgx_cast_f32_to_bf16": (_I, [_P, _P, _I64, _P]),
     "mgx_cast_bf16_to_f32": (_I, [_P, _P, _I64, _P]),
+    "mgx_dense_xent_workspace": (_I64, [_I64, _I64, _I64, _I, _I]),
+    "mgx_dense_xent_fwd": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _P]),
+    "mgx_dense_xent_bwd": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _P, _I64, _P]),
     "mgx_tape8_blocks": (_I64, [_I64]),
     "mgx_tape8_pack": (_I, [_P, _I, _P, _P, _I64, _P]),
     "mgx_tape8_unpack": (_I, [_P, _P, _P, _I, _I64, _P]),

@@ -1,0 +1,663 @@
+// Softmax cross entropy of a Dense head with many classes, without keeping the logits (beside mgx_softmax_xent, which
+// takes them as a tensor: the reference's Dense(9, softmax) + categorical_crossentropy, trainer/evaluacion.py:97, 160).
+//     z = x W + b (n x v)     lse_i = log sum_j exp(z_ij)     loss_i = lse_i - z_i,label(i)
+//     dz_ij = dloss_i (exp(z_ij - lse_i) - [j = label(i)])    dx = dz W^T    dW = x^T dz    db_j = sum_i dz_ij
+// x is n x e (float32 or bf16), W e x v and b v (float32, the Keras layout).  The logits exist as 32 x 32 accumulator
+// tiles only: the forward reduces each to a maximum and a sum per row, the backward computes them again, turns them into
+// dz and feeds dz to the two gradient products, a piece of the classes at a time.
+//
+// Arithmetic: all products run on v_mfma_f32_32x32x16_f16 with float32 accumulation, at float32 quality.  A float32
+// operand is the sum of two fp16 planes, hi = fp16(s a) and lo = fp16(s a - hi) with s a power of two that brings the
+// operand's largest magnitude below 2^14: 22 significant bits, and 2^-25 of 2^14 absolute where a value is small.  The
+// product keeps hi hi + hi lo + lo hi (the dropped lo lo is 2^-24 of it).  A bf16 operand is exact in one plane.  This is
+// three (two) of 2.5 PFLOP/s instead of one of the 157 TFLOP/s of the float32 matrix instructions.
+// exp and log are taken in float32 from the float32 logits; maxima, sums, lse and all gradient sums are float32.
+//
+// A row whose label lies outside [0, v) has no loss: loss 0, lse 0, gradient 0 and nothing of its features is read into
+// a product (they may hold anything).  A class may be masked with a bias of -inf or the lowest float.
+#include "bf16.h"
+#include "../../include/mgx.h"
+
+namespace {
+
+typedef _Float16 f16_t;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ f32x16 mfma_f16(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ unsigned f16_pack(float lo, float hi) {
+    f16x2 p = {(f16_t)lo, (f16_t)hi};
+    return __builtin_bit_cast(unsigned, p);
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kLowest = -3.402823466e38f;
+constexpr float kDz = 16384.f;                     // dz planes hold 2^14 dz / (largest |dloss|, rounded up to a power of two)
+constexpr int kMaxParts = 256;
+
+inline int64_t up(int64_t a, int64_t m) { return (a + m - 1) / m * m; }
+
+// ---------------------------------------------------------------- scales
+// Largest finite magnitudes of W, x and dloss as float32 bits: one partial per workgroup and tensor.
+template <bool XF32>
+__global__ __launch_bounds__(256) void xent_max_kernel(const float* __restrict__ w, long nw, const void* __restrict__ x, long nx,
+                                                       const float* __restrict__ dl, long nd, unsigned* __restrict__ part) {
+    __shared__ unsigned red[3][4];
+    const long t = (long)blockIdx.x * 256 + threadIdx.x, stride = (long)gridDim.x * 256;
+    unsigned m[3] = {0u, 0u, 0u};
+    auto take = [](unsigned& a, unsigned b) {
+        b &= 0x7fffffffu;
+        if (b < 0x7f800000u && b > a) a = b;
+    };
+    for (long i = t; i < nw / 4; i += stride) {
+        const u32x4 q = ((const u32x4*)w)[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) take(m[0], q[k]);
+    }
+    for (long i = nw / 4 * 4 + t; i < nw; i += stride) take(m[0], __builtin_bit_cast(unsigned, w[i]));
+    if (XF32) {
+        for (long i = t; i < nx; i += stride) take(m[1], ((const unsigned*)x)[i]);
+    } else {
+        for (long i = t; i < nx; i += stride) take(m[1], (unsigned)((const unsigned short*)x)[i] << 16);
+    }
+    for (long i = t; i < nd; i += stride) take(m[2], __builtin_bit_cast(unsigned, dl[i]));
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) {
+            const unsigned o = (unsigned)__shfl_xor((int)m[k], off, 64);
+            m[k] = m[k] > o ? m[k] : o;
+        }
+        if (lane == 0) red[k][wv] = m[k];
+    }
+    __syncthreads();
+    if (threadIdx.x < 3) {
+        unsigned a = 0u;
+        for (int k = 0; k < 4; ++k) a = a > red[threadIdx.x][k] ? a : red[threadIdx.x][k];
+        part[threadIdx.x * kMaxParts + blockIdx.x] = a;
+    }
+}
+
+// Power of two that brings magnitudes up to the float32 with these bits below 2^14 (its reciprocal stays normal too).
+__device__ __forceinline__ float scale_of(unsigned maxbits) {
+    int e = 14 + 126 - (int)(maxbits >> 23);                  // max < 2^(field - 126)
+    if (maxbits == 0u) e = 0;
+    e = e < -120 ? -120 : (e > 120 ? 120 : e);
+    return __builtin_bit_cast(float, (unsigned)(e + 127) << 23);
+}
+
+// {s_w, s_x, largest |dloss| rounded up to a power of two} into scales[0..2]; part has `parts` partials per tensor.
+__device__ __forceinline__ float scale_from_parts(const unsigned* __restrict__ part, int which, int parts) {
+    unsigned m = 0u;
+    for (int i = threadIdx.x & 63; i < parts; i += 64) {
+        const unsigned o = part[which * kMaxParts + i];
+        m = m > o ? m : o;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const unsigned o = (unsigned)__shfl_xor((int)m, off, 64);
+        m = m > o ? m : o;
+    }
+    if (which == 2) return 16384.f / scale_of(m);
+    return scale_of(m);
+}
+
+// ---------------------------------------------------------------- planes
+__device__ __forceinline__ void split8(const float* v, u32x4& hi, u32x4& lo) {
+    float r[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float h = (float)(f16_t)v[k];
+        r[k] = v[k] - h;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        hi[k] = f16_pack(v[2 * k], v[2 * k + 1]);
+        lo[k] = f16_pack(r[2 * k], r[2 * k + 1]);
+    }
+}
+
+struct XentPrep {
+    const void* x;
+    const float *w, *b, *lse, *dloss;
+    const int* labels;
+    const unsigned* part;
+    int parts;
+    long n, v, np, vp;            // rows, classes, and both padded to 128
+    int e, ep;                    // features, padded to 128
+    f16_t *xh, *xl, *wh, *wl;     // planes: rows x ep, classes x ep
+    float *bias, *scales, *lsep, *dlp;
+    int* lab;
+    long wtiles, xblocks;
+};
+
+// Workgroups 0 .. wtiles-1: a 64 classes x 64 features tile of W, transposed through LDS into the class-major planes;
+// the next xblocks: the planes of x; the rest: padded bias, labels and per-row scalars, and the scales.
+template <bool XF32>
+__global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
+    const int tid = threadIdx.x;
+    if ((long)blockIdx.x < p.wtiles) {
+        __shared__ float t[64][65];
+        const float s = scale_from_parts(p.part, 0, p.parts);
+        const long etiles = p.ep / 64, ct = blockIdx.x / etiles, et = blockIdx.x - ct * etiles;
+        const long c0 = ct * 64, e0 = et * 64;
+        const int cc = tid & 63;
+        for (int k = tid >> 6; k < 64; k += 4) {
+            const bool ok = c0 + cc < p.v && e0 + k < p.e;
+            t[k][cc] = ok ? p.w[(e0 + k) * p.v + c0 + cc] * s : 0.f;
+        }
+        __syncthreads();
+        const int e8 = tid & 7;
+        for (int c = tid >> 3; c < 64; c += 32) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = t[e8 * 8 + k][c];
+            u32x4 hi, lo;
+            split8(v, hi, lo);
+            const long at = (c0 + c) * p.ep + e0 + e8 * 8;
+            *(u32x4*)(p.wh + at) = hi;
+            *(u32x4*)(p.wl + at) = lo;
+        }
+    } else if ((long)blockIdx.x < p.wtiles + p.xblocks) {
+        const float s = scale_from_parts(p.part, 1, p.parts);
+        const int q = p.ep / 8;
+        for (long i = ((long)blockIdx.x - p.wtiles) * 256 + tid; i < p.np * q; i += p.xblocks * 256) {
+            const long row = i / q;
+            const int c = (int)(i - row * q) * 8;
+            const int lab = row < p.n ? p.labels[row] : -1;
+            const bool ok = lab >= 0 && lab < p.v;
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const bool in = ok && c + k < p.e;
+                const long at = row * p.e + c + k;
+                v[k] = in ? (XF32 ? ((const float*)p.x)[at] : (float)((const bf16_t*)p.x)[at]) * s : 0.f;
+            }
+            u32x4 hi, lo;
+            split8(v, hi, lo);
+            *(u32x4*)(p.xh + row * p.ep + c) = hi;
+            if (XF32) *(u32x4*)(p.xl + row * p.ep + c) = lo;
+        }
+    } else {
+        const float sw = scale_from_parts(p.part, 0, p.parts), sx = scale_from_parts(p.part, 1, p.parts),
+                    sd = scale_from_parts(p.part, 2, p.parts);
+        const long first = (long)blockIdx.x - p.wtiles - p.xblocks, nb = gridDim.x - p.wtiles - p.xblocks;
+        if (first == 0 && tid == 0) {
+            p.scales[0] = sw;
+            p.scales[1] = sx;
+            p.scales[2] = sd;
+        }
+        for (long i = first * 256 + tid; i < p.vp; i += nb * 256)
+            p.bias[i] = i < p.v ? (p.b ? p.b[i] : 0.f) : -__builtin_inff();
+        for (long i = first * 256 + tid; i < p.np; i += nb * 256) {
+            int lab = i < p.n ? p.labels[i] : -1;
+            if (lab >= p.v) lab = -1;
+            p.lab[i] = lab < 0 ? -1 : lab;
+            if (p.dlp) {
+                p.dlp[i] = lab < 0 ? 0.f : p.dloss[i] / sd;
+                p.lsep[i] = lab < 0 ? 0.f : p.lse[i];
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- products
+// D (128 x 128 per workgroup) = sum over the kept plane products of A B^T.  An operand is stored either with the
+// contraction index fastest ([row][k], read as 16-byte fragments) or slowest ([k][row], read with ds_read_b64_tr_b16).
+// 4 waves of 64 x 64, 32 of k per step, all planes of a step staged by LDS-DMA into one of two buffers while the other
+// is computed on.  Staged rows are 64 (256) bytes with their 16-byte chunks XOR-swizzled by the row so that both kinds of
+// read spread over all banks.
+constexpr int BK = 32, PLANE = 128 * BK * 2;
+
+struct XentGemm {
+    const f16_t *a[2], *b[2];
+    long lda, ldb;
+    int kiters;
+    // epilogues
+    const float *bias, *scales, *lse, *dl;
+    const int* lab;
+    float2* part;
+    float *zlab, *out, *outb;
+    f16_t *dzh, *dzl;
+    void* dx;
+    long np, n, ldo, class0;           // class0: first class of the piece
+    int e, first, last, dx_f32;
+};
+
+enum { EPI_FWD = 0, EPI_DZ = 1, EPI_DX = 2, EPI_DW = 3 };
+
+__device__ __forceinline__ int swz_row(int row) { return (row >> 2) & 3; }
+__device__ __forceinline__ int swz_k(int k) { return ((k & 3) << 2) | ((k >> 2) & 3); }
+
+template <int NA, int NB, bool AT, bool BT, int EPI>
+__global__ __launch_bounds__(256, 2) void xent_gemm_kernel(XentGemm g) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    constexpr int BUF = (NA + NB) * PLANE;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, h = lane >> 5, wm = wv >> 1, wn = wv & 1;
+    const long m0 = (long)blockIdx.x * 128, n0 = (long)blockIdx.y * 128;
+    // split contraction: part z of gridDim.z takes steps [it0, it1)
+    const int per = (g.kiters + gridDim.z - 1) / gridDim.z;
+    const int it0 = blockIdx.z * per, it1 = it0 + per < g.kiters ? it0 + per : g.kiters;
+
+    auto stage = [&](int buf, int it) {
+        const long k0 = (long)it * BK;
+#pragma unroll
+        for (int pl = 0; pl < NA + NB; ++pl) {
+            const bool isa = pl < NA, tr = isa ? AT : BT;
+            const f16_t* src = isa ? g.a[pl] : g.b[pl - NA];
+            const long ld = isa ? g.lda : g.ldb, o0 = isa ? m0 : n0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int piece = wv * 2 + i;                       // 1 KB: 16 rows of 64 B, or 4 rows of 256 B
+                const f16_t* gp;
+                if (tr) {
+                    const int row = piece * 4 + (lane >> 4), ch = (lane & 15) ^ swz_k(row);
+                    gp = src + (k0 + row) * ld + o0 + ch * 8;
+                } else {
+                    const int row = piece * 16 + (lane >> 2), ch = (lane & 3) ^ swz_row(row);
+                    gp = src + (o0 + row) * ld + k0 + ch * 8;
+                }
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)gp,
+                                                 (__attribute__((address_space(3))) void*)(lds + buf * BUF + pl * PLANE + piece * 1024),
+                                                 16, 0, 0);
+            }
+        }
+    };
+    const int hk = lane >> 5, cb = (lane >> 4) & 1, qq = (lane >> 2) & 3, pp = lane & 3;
+    auto frag = [&](const unsigned char* plane, bool tr, int blk, int ks) -> u32x4 {
+        if (tr) {
+            const int k = 16 * ks + 8 * hk + qq, ch = blk * 4 + 2 * cb + (pp >> 1);
+            const u32x2 a = tr_read(plane + k * 256 + ((ch ^ swz_k(k)) << 4) + 8 * (pp & 1));
+            const u32x2 b = tr_read(plane + (k + 4) * 256 + ((ch ^ swz_k(k + 4)) << 4) + 8 * (pp & 1));
+            return (u32x4){a[0], a[1], b[0], b[1]};
+        }
+        const int row = blk * 32 + r;
+        return *(const u32x4*)(plane + row * 64 + (((2 * ks + h) ^ swz_row(row)) << 4));
+    };
+
+    f32x16 acc[2][2], accb[2];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        acc[0][0][i] = acc[0][1][i] = acc[1][0][i] = acc[1][1][i] = 0.f;
+        accb[0][i] = accb[1][i] = 0.f;
+    }
+    const bool bias_wave = EPI == EPI_DW && blockIdx.x == 0 && wm == 0;       // sums of B's columns: a product with ones
+    const u32x4 ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+
+    if (it0 < it1) stage(0, it0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    int cur = 0;
+    for (int it = it0; it < it1; ++it) {
+        if (it + 1 < it1) stage(cur ^ 1, it + 1);
+        const unsigned char* base = lds + cur * BUF;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            u32x4 fa[NA][2], fb[NB][2];
+#pragma unroll
+            for (int pl = 0; pl < NA; ++pl)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) fa[pl][i] = frag(base + pl * PLANE, AT, wm * 2 + i, ks);
+#pragma unroll
+            for (int pl = 0; pl < NB; ++pl)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) fb[pl][i] = frag(base + (NA + pl) * PLANE, BT, wn * 2 + i, ks);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if (NA > 1) acc[i][j] = mfma_f16(fa[NA - 1][i], fb[0][j], acc[i][j]);
+                    if (NB > 1) acc[i][j] = mfma_f16(fa[0][i], fb[NB - 1][j], acc[i][j]);
+                    acc[i][j] = mfma_f16(fa[0][i], fb[0][j], acc[i][j]);
+                }
+            if (bias_wave) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if (NB > 1) accb[j] = mfma_f16(ones, fb[NB - 1][j], accb[j]);
+                    accb[j] = mfma_f16(ones, fb[0][j], accb[j]);
+                }
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        cur ^= 1;
+    }
+
+    const long mw = m0 + wm * 64, nw = n0 + wn * 64;
+    if constexpr (EPI == EPI_FWD || EPI == EPI_DZ) {
+        // A: classes, B: rows of x
+        const float un = 1.f / g.scales[0], ux = 1.f / g.scales[1];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const long row = nw + j * 32 + r;
+            const int lab = g.lab[row];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 bv = *(const f32x4*)(g.bias + mw + i * 32 + 8 * q + 4 * h);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[i][j][4 * q + k] = acc[i][j][4 * q + k] * un * ux + bv[k];
+                }
+            const long rel = lab - g.class0 - mw;           // the label's place among the wave's 64 classes
+            if constexpr (EPI == EPI_FWD) {
+                float m = kLowest, s = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) m = fmaxf(m, acc[i][j][k]);
+                m = fmaxf(m, __shfl_xor(m, 32, 64));
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) s += __builtin_amdgcn_exp2f((acc[i][j][k] - m) * kLog2e);
+                s += __shfl_xor(s, 32, 64);
+                if (h == 0) g.part[(mw / 64) * g.np + row] = make_float2(m, s);
+                if (lab >= 0 && rel >= 0 && rel < 64) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            if (i * 32 + (k & 3) + 8 * (k >> 2) + 4 * h == (int)rel) g.zlab[row] = acc[i][j][k];
+                }
+            } else {
+                const float lse = g.lse[row], dl = g.dl[row] * kDz;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        float p = __builtin_amdgcn_exp2f((acc[i][j][k] - lse) * kLog2e);
+                        if (i * 32 + (k & 3) + 8 * (k >> 2) + 4 * h == rel) p -= 1.f;           // no label: rel < 0
+                        acc[i][j][k] = dl == 0.f ? 0.f : p * dl;
+                    }
+                    acc_rows_interleaved(acc[i][j]);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        float v[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[k] = acc[i][j][8 * half + k];
+                        u32x4 hi, lo;
+                        split8(v, hi, lo);
+                        const long at = row * g.ldo + mw + i * 32 + 16 * half + 8 * h;
+                        *(u32x4*)(g.dzh + at) = hi;
+                        *(u32x4*)(g.dzl + at) = lo;
+                    }
+                }
+            }
+        }
+    } else if constexpr (EPI == EPI_DX) {
+        // A: rows, B: features
+        const float f = g.scales[2] / kDz / g.scales[0];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const long row = mw + i * 32 + acc_row(k, lane), col = nw + j * 32 + r;
+                    float v = acc[i][j][k];
+                    if (!g.first) v += g.out[row * g.ldo + col];
+                    if (!g.last) g.out[row * g.ldo + col] = v;
+                    else if (row < g.n && col < g.e) {
+                        if (g.dx_f32) ((float*)g.dx)[row * g.e + col] = v * f;
+                        else ((bf16_t*)g.dx)[row * g.e + col] = (bf16_t)(v * f);
+                    }
+                }
+    } else {
+        // A: features, B: classes; slab z of the piece
+        float* out = g.out + (long)blockIdx.z * g.np;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) out[(mw + i * 32 + acc_row(k, lane)) * g.ldo + nw + j * 32 + r] = acc[i][j][k];
+        if (bias_wave && h == 0) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) g.outb[(long)blockIdx.z * g.ldo + nw + j * 32 + r] = accb[j][0];
+        }
+    }
+}
+
+// loss and lse of 32 rows per workgroup from the partial (maximum, sum) of every 64 classes
+__global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict__ part, const float* __restrict__ zlab,
+                                                        const int* __restrict__ lab, float* __restrict__ loss,
+                                                        float* __restrict__ lse, int* __restrict__ hits, long n, long np,
+                                                        long slices) {
+    __shared__ float2 red[8][32];
+    const int rr = threadIdx.x & 31, gr = threadIdx.x >> 5;
+    const long row = (long)blockIdx.x * 32 + rr;
+    float m = kLowest, s = 0.f;
+    for (long i = gr; i < slices; i += 8) {
+        const float2 p = part[i * np + row];
+        const float mm = fmaxf(m, p.x);
+        s = s * __builtin_amdgcn_exp2f((m - mm) * kLog2e) + p.y * __builtin_amdgcn_exp2f((p.x - mm) * kLog2e);
+        m = mm;
+    }
+    red[gr][rr] = make_float2(m, s);
+    __syncthreads();
+    if (gr == 0 && row < n) {
+        for (int q = 1; q < 8; ++q) {
+            const float2 p = red[q][rr];
+            const float mm = fmaxf(m, p.x);
+            s = s * __builtin_amdgcn_exp2f((m - mm) * kLog2e) + p.y * __builtin_amdgcn_exp2f((p.x - mm) * kLog2e);
+            m = mm;
+        }
+        const bool ok = lab[row] >= 0;
+        // (m - z) first: the loss of a row whose label has nearly all the probability is far below an ulp of lse
+        const float ls = __builtin_amdgcn_logf(s) * kLn2;
+        loss[row] = ok ? (m - zlab[row]) + ls : 0.f;
+        lse[row] = ok ? m + ls : 0.f;
+        if (hits) hits[row] = ok && zlab[row] >= m ? 1 : 0;
+    }
+}
+
+// dW and db of a piece of the classes from the slabs of the split contraction, in order
+__global__ __launch_bounds__(256) void xent_dw_reduce_kernel(const float* __restrict__ slabs, const float* __restrict__ slabs_b,
+                                                             const float* __restrict__ scales, float* __restrict__ dw,
+                                                             float* __restrict__ db, int nz, long slab, long ldo, int e,
+                                                             long v, long c0, int accumulate) {
+    const long c = (long)blockIdx.x * 256 + threadIdx.x;
+    const int k = blockIdx.y;
+    if (c >= ldo || c0 + c >= v) return;
+    float s = 0.f;
+    if (k < e) {
+        if (!dw) return;
+        for (int z = 0; z < nz; ++z) s += slabs[z * slab + k * ldo + c];
+        s = s * (scales[2] / kDz) / scales[1];
+        float* d = dw + k * v + c0 + c;
+        *d = accumulate ? *d + s : s;
+    } else if (db) {
+        for (int z = 0; z < nz; ++z) s += slabs_b[z * ldo + c];
+        s *= scales[2] / kDz;
+        float* d = db + c0 + c;
+        *d = accumulate ? *d + s : s;
+    }
+}
+
+__global__ __launch_bounds__(256) void xent_zero_kernel(float* __restrict__ a, long na, float* __restrict__ b, long nb) {
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < na || i < nb; i += (long)gridDim.x * 256) {
+        if (i < na) a[i] = 0.f;
+        if (i < nb) b[i] = 0.f;
+    }
+}
+
+// ---------------------------------------------------------------- host
+struct Layout {
+    int64_t np, vp, ep, vc, nz;
+    int64_t part, bias, scales, lab, zlab, lse, dl, xh, xl, wh, wl, slices, dzh, dzl, dxw, slabs, slabs_b, total;
+};
+
+Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
+    Layout l = {};
+    l.np = up(n, 128);
+    l.vp = up(v, 128);
+    l.ep = up(e, 128);
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t o = at;
+        at += up(bytes, 1024);
+        return o;
+    };
+    l.part = take(3 * kMaxParts * 4);
+    l.scales = take(16);
+    l.bias = take(l.vp * 4);
+    l.lab = take(l.np * 4);
+    l.xh = take(l.np * l.ep * 2);
+    l.xl = xf32 ? take(l.np * l.ep * 2) : 0;
+    l.wh = take(l.vp * l.ep * 2);
+    l.wl = take(l.vp * l.ep * 2);
+    if (!backward) {
+        l.zlab = take(l.np * 4);
+        l.slices = take(l.np * (l.vp / 64) * 8);
+    } else {
+        l.lse = take(l.np * 4);
+        l.dl = take(l.np * 4);
+        // a piece of the classes: dz planes of about 128 MB, which the 256 MB last-level cache holds
+        l.vc = (int64_t)(128 << 20) / (4 * l.np) / 128 * 128;
+        if (l.vc < 128) l.vc = 128;
+        if (l.vc > l.vp) l.vc = l.vp;
+        const int64_t tiles = (l.ep / 128) * (l.vc / 128);
+        l.nz = 512 / tiles;
+        if (l.nz > l.np / 256) l.nz = l.np / 256;
+        if (l.nz < 1) l.nz = 1;
+        l.dzh = take(l.np * l.vc * 2);
+        l.dzl = take(l.np * l.vc * 2);
+        l.dxw = take(l.np * l.ep * 4);
+        l.slabs = take(l.nz * l.ep * l.vc * 4);
+        l.slabs_b = take(l.nz * l.vc * 4);
+    }
+    l.total = at;
+    return l;
+}
+
+bool sizes_ok(int64_t n, int64_t e, int64_t v) {
+    return n >= 0 && e >= 1 && v >= 1 && n <= 8000000 && v <= 8000000 && e <= 65536;      // rows / 128 and classes / 128 are grid dimensions
+}
+
+template <int NA, int NB, bool AT, bool BT, int EPI>
+void launch_gemm(const XentGemm& g, dim3 grid, hipStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    constexpr int bytes = 2 * (NA + NB) * PLANE;
+    mgx_allow_dynamic_lds(xent_gemm_kernel<NA, NB, AT, BT, EPI>, bytes, done);
+    hipLaunchKernelGGL((xent_gemm_kernel<NA, NB, AT, BT, EPI>), grid, dim3(256), bytes, st, g);
+}
+
+void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const float* w, const float* b, const int* labels,
+                 const float* lse, const float* dloss, int64_t n, int64_t e, int64_t v, hipStream_t st) {
+    const int parts = 256;
+    unsigned* part = (unsigned*)(ws + l.part);
+    if (xf32)
+        hipLaunchKernelGGL(xent_max_kernel<true>, dim3(parts), dim3(256), 0, st, w, (long)(e * v), x, (long)(n * e), dloss,
+                           dloss ? (long)n : 0L, part);
+    else
+        hipLaunchKernelGGL(xent_max_kernel<false>, dim3(parts), dim3(256), 0, st, w, (long)(e * v), x, (long)(n * e), dloss,
+                           dloss ? (long)n : 0L, part);
+    XentPrep p = {};
+    p.x = x; p.w = w; p.b = b; p.lse = lse; p.dloss = dloss; p.labels = labels; p.part = part; p.parts = parts;
+    p.n = n; p.v = v; p.np = l.np; p.vp = l.vp; p.e = (int)e; p.ep = (int)l.ep;
+    p.xh = (f16_t*)(ws + l.xh); p.xl = (f16_t*)(ws + l.xl); p.wh = (f16_t*)(ws + l.wh); p.wl = (f16_t*)(ws + l.wl);
+    p.bias = (float*)(ws + l.bias); p.scales = (float*)(ws + l.scales); p.lab = (int*)(ws + l.lab);
+    p.lsep = dloss ? (float*)(ws + l.lse) : nullptr; p.dlp = dloss ? (float*)(ws + l.dl) : nullptr;
+    p.wtiles = (l.vp / 64) * (l.ep / 64);
+    p.xblocks = up(l.np * l.ep / 8, 256) / 256;
+    if (p.xblocks > 2048) p.xblocks = 2048;
+    const dim3 grid((unsigned)(p.wtiles + p.xblocks + 64));
+    if (xf32) hipLaunchKernelGGL(xent_prep_kernel<true>, grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL(xent_prep_kernel<false>, grid, dim3(256), 0, st, p);
+}
+
+}  // namespace
+
+extern "C" int64_t mgx_dense_xent_workspace(int64_t n, int64_t e, int64_t v, int x_is_f32, int backward) {
+    if (!sizes_ok(n, e, v)) return -1;
+    return n == 0 ? 0 : layout(n, e, v, x_is_f32 != 0, backward != 0).total;
+}
+
+extern "C" int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, const float* b, const int32_t* labels,
+                                  float* loss, float* lse, int32_t* hits, int64_t n, int64_t e, int64_t v,
+                                  void* workspace, int64_t workspace_bytes, void* stream) {
+    if (!sizes_ok(n, e, v)) return MGX_ERR_ARG;
+    if (n == 0) return MGX_OK;
+    if (!x || !w || !labels || !loss || !lse || !workspace) return MGX_ERR_ARG;
+    if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)workspace) & 15u) != 0) return MGX_ERR_ARG;
+    const bool xf = x_is_f32 != 0;
+    const Layout l = layout(n, e, v, xf, false);
+    if (workspace_bytes < l.total) return MGX_ERR_WORKSPACE;
+    hipStream_t st = (hipStream_t)stream;
+    char* ws = (char*)workspace;
+    launch_prep(l, ws, x, xf, w, b, labels, nullptr, nullptr, n, e, v, st);
+    XentGemm g = {};
+    g.a[0] = (f16_t*)(ws + l.wh); g.a[1] = (f16_t*)(ws + l.wl); g.b[0] = (f16_t*)(ws + l.xh); g.b[1] = (f16_t*)(ws + l.xl);
+    g.lda = g.ldb = l.ep; g.kiters = (int)(l.ep / BK);
+    g.bias = (float*)(ws + l.bias); g.scales = (float*)(ws + l.scales); g.lab = (int*)(ws + l.lab);
+    g.part = (float2*)(ws + l.slices); g.zlab = (float*)(ws + l.zlab); g.np = l.np;
+    const dim3 grid((unsigned)(l.vp / 128), (unsigned)(l.np / 128));
+    if (xf) launch_gemm<2, 2, false, false, EPI_FWD>(g, grid, st);
+    else launch_gemm<2, 1, false, false, EPI_FWD>(g, grid, st);
+    hipLaunchKernelGGL(xent_join_kernel, dim3((unsigned)(l.np / 32)), dim3(256), 0, st, g.part, g.zlab, g.lab, loss, lse, hits,
+                       (long)n, (long)l.np, (long)(l.vp / 64));
+    return mgx_launch_status();
+}
+
+extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, const float* b, const int32_t* labels,
+                                  const float* lse, const float* dloss, void* dx, float* dw, float* db, int accumulate,
+                                  int64_t n, int64_t e, int64_t v, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (!sizes_ok(n, e, v)) return MGX_ERR_ARG;
+    hipStream_t st = (hipStream_t)stream;
+    if (n == 0) {
+        if (!accumulate && (dw || db))
+            hipLaunchKernelGGL(xent_zero_kernel, dim3(1024), dim3(256), 0, st, dw, dw ? (long)(e * v) : 0L, db, db ? (long)v : 0L);
+        return mgx_launch_status();
+    }
+    if (!x || !w || !labels || !lse || !dloss || !workspace) return MGX_ERR_ARG;
+    if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)workspace) & 15u) != 0) return MGX_ERR_ARG;
+    const bool xf = x_is_f32 != 0;
+    const Layout l = layout(n, e, v, xf, true);
+    if (workspace_bytes < l.total) return MGX_ERR_WORKSPACE;
+    char* ws = (char*)workspace;
+    launch_prep(l, ws, x, xf, w, b, labels, lse, dloss, n, e, v, st);
+    f16_t *xh = (f16_t*)(ws + l.xh), *xl = (f16_t*)(ws + l.xl), *dzh = (f16_t*)(ws + l.dzh), *dzl = (f16_t*)(ws + l.dzl);
+    for (int64_t c0 = 0; c0 < l.vp; c0 += l.vc) {
+        const int64_t cnt = l.vp - c0 < l.vc ? l.vp - c0 : l.vc;
+        f16_t *wh = (f16_t*)(ws + l.wh) + c0 * l.ep, *wl = (f16_t*)(ws + l.wl) + c0 * l.ep;
+        XentGemm g = {};
+        g.scales = (float*)(ws + l.scales);
+        g.a[0] = wh; g.a[1] = wl; g.b[0] = xh; g.b[1] = xl;
+        g.lda = g.ldb = l.ep; g.kiters = (int)(l.ep / BK);
+        g.bias = (float*)(ws + l.bias) + c0; g.lab = (int*)(ws + l.lab); g.lse = (float*)(ws + l.lse); g.dl = (float*)(ws + l.dl);
+        g.dzh = dzh; g.dzl = dzl; g.ldo = l.vc; g.np = l.np; g.class0 = c0;
+        const dim3 grid((unsigned)(cnt / 128), (unsigned)(l.np / 128));
+        if (xf) launch_gemm<2, 2, false, false, EPI_DZ>(g, grid, st);
+        else launch_gemm<2, 1, false, false, EPI_DZ>(g, grid, st);
+        if (dx) {
+            XentGemm q = {};
+            q.scales = g.scales;
+            q.a[0] = dzh; q.a[1] = dzl; q.b[0] = wh; q.b[1] = wl;
+            q.lda = l.vc; q.ldb = l.ep; q.kiters = (int)(cnt / BK);
+            q.out = (float*)(ws + l.dxw); q.ldo = l.ep; q.dx = dx; q.dx_f32 = xf; q.n = n; q.e = (int)e;
+            q.first = c0 == 0; q.last = c0 + cnt >= l.vp;
+            const dim3 gx((unsigned)(l.np / 128), (unsigned)(l.ep / 128));
+            if (xf) launch_gemm<2, 2, false, true, EPI_DX>(q, gx, st);
+            else launch_gemm<1, 1, false, true, EPI_DX>(q, gx, st);
+        }
+        if (dw || db) {
+            XentGemm q = {};
+            q.scales = g.scales;
+            q.a[0] = xh; q.a[1] = xl; q.b[0] = dzh; q.b[1] = dzl;
+            q.lda = l.ep; q.ldb = l.vc; q.kiters = (int)(l.np / BK);
+            q.out = (float*)(ws + l.slabs); q.outb = (float*)(ws + l.slabs_b); q.ldo = l.vc; q.np = l.ep * l.vc;
+            const dim3 gw((unsigned)(l.ep / 128), (unsigned)(cnt / 128), (unsigned)l.nz);
+            if (xf) launch_gemm<2, 2, true, true, EPI_DW>(q, gw, st);
+            else launch_gemm<1, 2, true, true, EPI_DW>(q, gw, st);
+            hipLaunchKernelGGL(xent_dw_reduce_kernel, dim3((unsigned)(up(cnt, 256) / 256), (unsigned)(e + 1)), dim3(256), 0, st,
+                               q.out, q.outb, g.scales, dw, db, (int)l.nz, (long)q.np, (long)l.vc, (int)e, (long)v, (long)c0,
+                               accumulate);
+        }
+    }
+    return mgx_launch_status();
+}

@@ -1114,3 +1114,71 @@ def conv_bwd_tape8(d: ConvDesc, t: Tape8, g, w, dw, dbias, dx, act_alpha=0.0):
     if e0 is not None:
         PROFILER.stop("bbwd_kernel<%d,%d,tape8>" % (d.kh, d.kw), 2 * _conv_flops(d), e0,
                       2.0 * (ye + xe) + t.nbytes() + 4.0 * (we + d.nbias))
+
+
+# --------------------------------------------------------------------------------------------
+# softmax cross entropy of a Dense head with many classes, without the logits
+# --------------------------------------------------------------------------------------------
+def _pi(t: Optional[torch.Tensor]):
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
+        raise MgxError("operand must be a contiguous int32 device tensor")
+    return t.data_ptr()
+
+
+def _dense_xent_sizes(what, x, w, b, labels, rows):
+    """(n, e, v) after checking that x (n, e), w (e * v values), b (v), labels (n) and the per-row tensors agree."""
+    if x.dim() != 2 or x.dtype not in (torch.float32, torch.bfloat16):
+        raise MgxError("%s: x must be a float32 or bfloat16 (rows, features) tensor" % what)
+    n, e = x.shape
+    if e < 1 or w.numel() < e or w.numel() % e:
+        raise MgxError("%s: the kernel must hold (features, classes) values" % what)
+    v = w.numel() // e
+    if (w.dim() == 2 and tuple(w.shape) != (e, v)) or (b is not None and b.numel() != v) or labels.numel() != n \
+            or any(t is not None and t.numel() != n for t in rows):
+        raise MgxError("%s: size mismatch" % what)
+    _on_current(x, w, b, labels, *rows)
+    return n, e, v
+
+
+def _dense_xent_workspace(what, n, e, v, f32, backward):
+    nbytes = int(_lib().mgx_dense_xent_workspace(n, e, v, f32, backward))
+    if nbytes < 0:
+        raise MgxError("%s: %d rows, %d features, %d classes are out of range" % (what, n, e, v))
+    # of its own for every call: two captured graphs never share it
+    return torch.empty((max(nbytes, 16),), dtype=torch.uint8, device=K.device())
+
+
+def dense_xent_fwd(x, w, b, labels, loss, lse, hits=None):
+    """Per-row softmax cross entropy of the logits x W + b, which are never stored (mgx_dense_xent_fwd): x (n, e) float32 or
+    bfloat16, w (e, v) and b (v) float32 (b may be None), labels (n) int32; loss and lse (n) float32 are written, hits (n)
+    int32 too if given.  Rows whose label lies outside [0, v) have loss, lse and hits 0."""
+    n, e, v = _dense_xent_sizes("dense_xent_fwd", x, w, b, labels, (loss, lse, hits))
+    f32 = int(x.dtype == torch.float32)
+    px, pw, pb, pl, po, ps, ph = _p_act(x), _p(w), _p(b), _pi(labels), _p(loss), _p(lse), _pi(hits)
+    ws = _dense_xent_workspace("dense_xent_fwd", n, e, v, f32, 0)
+    e0 = PROFILER.start() if PROFILER is not None else None
+    check(_lib().mgx_dense_xent_fwd(px, f32, pw, pb, pl, po, ps, ph, n, e, v, ws.data_ptr(), ws.numel(), K.stream_ptr()),
+          "mgx_dense_xent_fwd")
+    if e0 is not None:
+        PROFILER.stop("dense_xent_fwd", 2.0 * n * e * v, e0, n * e * x.element_size() + 4.0 * e * v)
+
+
+def dense_xent_bwd(x, w, b, labels, lse, dloss, dx, dw, db, accumulate=False):
+    """Gradients of sum_i dloss_i loss_i: dx (n, e) in the type of x is written, dw (e, v) and db (v) float32 are written or,
+    with `accumulate`, added to; any of them may be None.  lse is the forward's, for the same x, w, b and labels."""
+    n, e, v = _dense_xent_sizes("dense_xent_bwd", x, w, b, labels, (lse, dloss))
+    if (dx is not None and (dx.dtype != x.dtype or dx.numel() != x.numel())) or (dw is not None and dw.numel() != w.numel()) \
+            or (db is not None and db.numel() != v):
+        raise MgxError("dense_xent_bwd: a gradient does not match its operand")
+    _on_current(dx, dw, db)
+    f32 = int(x.dtype == torch.float32)
+    args = (_p_act(x), f32, _p(w), _p(b), _pi(labels), _p(lse), _p(dloss), _p_act(dx) if dx is not None else None, _p(dw),
+            _p(db))
+    ws = _dense_xent_workspace("dense_xent_bwd", n, e, v, f32, 1)
+    e0 = PROFILER.start() if PROFILER is not None else None
+    check(_lib().mgx_dense_xent_bwd(*args, int(accumulate), n, e, v, ws.data_ptr(), ws.numel(), K.stream_ptr()),
+          "mgx_dense_xent_bwd")
+    if e0 is not None:
+        PROFILER.stop("dense_xent_bwd", 6.0 * n * e * v, e0, 2.0 * n * e * x.element_size() + 8.0 * e * v)

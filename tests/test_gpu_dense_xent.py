@@ -1,0 +1,305 @@
+"""Softmax cross entropy of a Dense head without its logits: loss, gradients, masks, refusals, against the definition in
+float64 on the CPU."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import music_generator_amd as M
+from music_generator_amd import ops
+from music_generator_amd._cabi import MgxError
+
+gpu = pytest.mark.gpu
+
+
+def case(n, e, v, dtype, seed=0, bias=True, unlabelled=0.1, spread=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn((n, e), generator=gen).to(dtype)
+    w = torch.randn((e, v), generator=gen) * (spread / math.sqrt(e))
+    b = torch.randn((v,), generator=gen) * 0.3 if bias else None
+    labels = torch.randint(0, v, (n,), generator=gen, dtype=torch.int32)
+    if unlabelled:
+        labels[torch.rand((n,), generator=gen) < unlabelled] = -1
+    dloss = (0.5 + torch.rand((n,), generator=gen)) / max(n, 1)
+    return x, w, b, labels, dloss
+
+
+def reference(x, w, b, labels, dloss):
+    x64, w64 = x.double(), w.double()
+    z = x64 @ w64 + (b.double() if b is not None else 0.0)
+    lse = torch.logsumexp(z, dim=1)
+    ok = (labels >= 0) & (labels < w.shape[1])
+    at = labels.clamp(0, w.shape[1] - 1).long()
+    picked = z.gather(1, at[:, None])[:, 0]
+    loss = torch.where(ok, lse - picked, torch.zeros_like(lse))
+    d = torch.exp(z - lse[:, None])
+    at_label = torch.zeros_like(d)
+    at_label[torch.arange(len(at)), at] = torch.where(ok, d[torch.arange(len(at)), at] * dloss.double().abs(), torch.zeros_like(lse))
+    d[torch.arange(len(at)), at] -= 1.0
+    d = torch.where(ok[:, None], d * dloss.double()[:, None], torch.zeros_like(d))
+    x64 = torch.where(ok[:, None], x64, torch.zeros_like(x64))
+    hits = (ok & (picked >= z.amax(dim=1))).int()
+    slack = {"dx": at_label @ w64.abs().t(), "dw": x64.abs().t() @ at_label, "db": at_label.sum(dim=0)}
+    return {"slack": {k: float(s.norm()) for k, s in slack.items()}, "loss": loss, "lse": torch.where(ok, lse, torch.zeros_like(lse)), "dx": d @ w64.t(), "dw": x64.t() @ d,
+            "db": d.sum(dim=0), "hits": hits}
+
+
+def run(x, w, b, labels, dloss, accumulate=False, dw=None, db=None):
+    dev = [t.cuda() if t is not None else None for t in (x, w, b, labels, dloss)]
+    x, w, b, labels, dloss = dev
+    n, v = x.shape[0], w.shape[1]
+    loss, lse, hits = torch.empty((n,)).cuda(), torch.empty((n,)).cuda(), torch.empty((n,), dtype=torch.int32).cuda()
+    ops.dense_xent_fwd(x, w, b, labels, loss, lse, hits)
+    dx = torch.full_like(x, float("nan"))
+    dw = torch.full_like(w, float("nan")) if dw is None else dw.cuda()
+    db = torch.full((v,), float("nan")).cuda() if db is None else db.cuda()
+    ops.dense_xent_bwd(x, w, b, labels, lse, dloss, dx, dw, db, accumulate=accumulate)
+    return {k: t.cpu() for k, t in (("loss", loss), ("lse", lse), ("dx", dx), ("dw", dw), ("db", db), ("hits", hits))}
+
+
+def check(got, want, dtype, largest_logit):
+    """Logits: operands of 22 bits and float32 sums, so a logit is off by a few 2^-23 of the largest one, and lse, a float32,
+    by its rounding: `unit`.  A loss is off by that and one rounding, a probability by unit relative to itself, and so are
+    the gradients (sums of terms of both signs: compared in the 2-norm) but for the label's term p - 1, which is off by
+    unit p however small it is itself: `slack` is the gradient with p dloss at the labels, the size of that part.  A bf16 dx has one rounding, eps / 2 = 2^-8 of a value at most and so 2^-8 of the 2-norm, and its
+    second product may take both operands to 11 bits (2^-11 of a term each, terms of both signs)."""
+    unit = 2.0 ** -23 * (8 + 2 * largest_logit)
+    assert float((got["loss"].double() - want["loss"]).abs().max()) <= unit + 2.0 ** -23 * float(want["loss"].abs().max())
+    assert float((got["lse"].double() - want["lse"]).abs().max()) <= unit + 2.0 ** -23 * float(want["lse"].abs().max())
+    for k in ("dw", "db", "dx"):
+        norm = float(want[k].norm())
+        off = float((got[k].double() - want[k]).norm())
+        tol = 4 * unit + (2.0 ** -8 + 2.0 ** -10 if k == "dx" and dtype == torch.bfloat16 else 0.0)
+        assert off <= tol * norm + unit * want["slack"][k] + 1e-30, (k, off / max(norm, 1e-300), tol)
+
+
+SIZES = [(1, 1, 1), (1, 128, 4097), (2, 16, 2), (5, 33, 130), (64, 128, 256), (127, 64, 129), (129, 130, 1000), (300, 256, 511),
+         (257, 500, 2049), (1000, 128, 3001), (17, 1000, 10001), (4, 1, 70000), (640, 32, 128)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,e,v", SIZES)
+def test_loss_and_gradients(n, e, v, dtype):
+    args = case(n, e, v, dtype, seed=n + e + v, bias=(n % 2 == 1))
+    want = reference(*args)
+    check(run(*args), want, dtype, float((args[0].double() @ args[1].double()).abs().max()))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_hits(dtype):
+    x, w, b, labels, dloss = case(200, 64, 40, dtype, seed=3)
+    z = x.double() @ w.double() + b.double()
+    top = z.topk(2, dim=1)
+    clear = top.values[:, 0] - top.values[:, 1] > 1e-3          # no tie within the logits' accuracy
+    labels[::2] = top.indices[::2, 0].int()
+    got, want = run(x, w, b, labels, dloss)["hits"], reference(x, w, b, labels, dloss)["hits"]
+    assert torch.equal(got[clear], want[clear]) and int(want.sum()) >= 90
+
+
+@gpu
+@pytest.mark.parametrize("scale_x,scale_w", [(1e-6, 1e-3), (1e4, 1e-6), (3e-3, 2e3), (1e-20, 1e18)])
+def test_magnitudes(scale_x, scale_w):
+    """The planes follow the operands' magnitudes: the result is as exact for small and large ones."""
+    x, w, b, labels, dloss = case(150, 96, 700, torch.float32, seed=8)
+    args = (x * scale_x, w * scale_w, b, labels, dloss * 1e-5)
+    z = args[0].double() @ args[1].double()
+    check(run(*args), reference(*args), torch.float32, float(z.abs().max()) + 1)
+
+
+@gpu
+def test_confident_rows():
+    """Rows whose label has nearly all the probability: dz = p - 1 is small and taken before any rounding to fewer bits, and a
+    small loss keeps its digits (lse - z would lose those below 2^-24 lse)."""
+    x, w, b, labels, dloss = case(128, 64, 300, torch.float32, seed=5, unlabelled=0, spread=1.0)
+    w = w * 0.05
+    for i in range(128):                           # the label's class points along the row
+        labels[i] = i
+        w[:, i] += x[i] * (14.0 / float(x[i].square().sum()))
+    want = reference(x, w, b, labels, dloss)
+    assert float(want["loss"].median()) < 1e-2
+    got = run(x, w, b, labels, dloss)
+    check(got, want, torch.float32, 20.0)
+    # log of 1 + small exponentials: those are off by a few 2^-23 of a logit's 20, and the sum by half a unit, 2^-24, for
+    # each addition behind the 1: at most 32 in a lane's part of the classes, and one for each of the parts joined to it
+    # (300 classes: under 32)
+    assert bool(((got["loss"].double() - want["loss"]).abs() <= 2.0 ** -23 * (1 + 32 + 48 * want["loss"])).all())
+
+
+@gpu
+@pytest.mark.parametrize("mask", [float("-inf"), -3.4028234663852886e38])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_masked_classes(mask, dtype):
+    x, w, b, labels, dloss = case(100, 40, 777, dtype, seed=6)
+    b[torch.rand((777,), generator=torch.Generator().manual_seed(1)) < 0.5] = mask
+    b[256:512] = mask                              # whole tiles
+    b[640:] = mask
+    labels = torch.where(b[labels.clamp(min=0).long()] == mask, torch.full_like(labels, -1), labels)
+    assert int((labels >= 0).sum()) > 5
+    want = reference(x, w, b, labels, dloss)
+    got = run(x, w, b, labels, dloss)
+    check(got, want, dtype, 6.0)
+    assert bool((got["dw"][:, b == mask] == 0).all()) and bool((got["db"][b == mask] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_without_a_label_may_hold_anything(dtype):
+    x, w, b, labels, dloss = case(90, 48, 200, dtype, seed=7, unlabelled=0.3)
+    labels[3], labels[4], labels[5], labels[6] = 200, 2 ** 31 - 1, -2 ** 31, -1       # outside [0, v)
+    want = reference(x, w, b, labels, dloss)
+    bad = (labels < 0) | (labels >= 200)
+    x[bad] = float("nan")
+    x[4] = float("inf")
+    dloss[5] = float("nan")
+    got = run(x, w, b, labels, dloss)
+    check(got, want, dtype, 6.0)
+    assert bool((got["loss"][bad] == 0).all()) and bool((got["dx"][bad] == 0).all())
+
+
+@gpu
+def test_no_row_has_a_label():
+    x, w, b, labels, dloss = case(70, 20, 150, torch.float32, seed=9)
+    got = run(x, w, b, torch.full_like(labels, -1), dloss)
+    for k in ("loss", "lse", "dx", "dw", "db"):
+        assert bool((got[k] == 0).all()), k
+
+
+@gpu
+def test_a_row_that_is_not_finite_stays_in_its_row():
+    x, w, b, labels, dloss = case(130, 24, 90, torch.float32, seed=10, unlabelled=0)
+    want = reference(x, w, b, labels, dloss)
+    x[7, 3] = float("nan")
+    got = run(x, w, b, labels, dloss)
+    others = torch.arange(130) != 7
+    assert bool(got["loss"][7].isnan())
+    assert float((got["loss"][others].double() - want["loss"][others]).abs().max()) < 1e-5
+    assert float((got["dx"][others].double() - want["dx"][others]).norm() / want["dx"][others].norm()) < 1e-5
+
+
+@gpu
+def test_accumulation_and_missing_outputs():
+    x, w, b, labels, dloss = case(100, 130, 300, torch.float32, seed=11)
+    want = reference(x, w, b, labels, dloss)
+    dw0, db0 = torch.ones_like(w), torch.full_like(b, -2.0)
+    got = run(x, w, b, labels, dloss, accumulate=True, dw=dw0, db=db0)
+    # sums near 1 and 2: half a unit of 2^-23 and 2^-22 beside the gradient's own error
+    assert float((got["dw"].double() - 1 - want["dw"]).abs().max()) < 2.0 ** -22
+    assert float((got["db"].double() + 2 - want["db"]).abs().max()) < 2.0 ** -21
+    dev = [t.cuda() for t in (x, w, b, labels)]
+    loss, lse = torch.empty((100,)).cuda(), torch.empty((100,)).cuda()
+    ops.dense_xent_fwd(*dev, loss, lse)
+    whole = run(x, w, b, labels, dloss)
+    for pick in ("dx", "dw", "db"):
+        out = {"dx": None, "dw": None, "db": None}
+        out[pick] = torch.full_like({"dx": dev[0], "dw": dev[1], "db": dev[2]}[pick], 7.0)
+        ops.dense_xent_bwd(*dev, lse, dloss.cuda(), out["dx"], out["dw"], out["db"])
+        assert torch.equal(out[pick].cpu(), whole[pick])
+
+
+@gpu
+def test_same_bits_every_time():
+    args = case(500, 128, 5000, torch.bfloat16, seed=12)
+    a, b = run(*args), run(*args)
+    assert all(torch.equal(a[k], b[k]) for k in a)
+
+
+@gpu
+def test_no_rows():
+    w, b = torch.randn((16, 40)).cuda(), torch.randn((40,)).cuda()
+    x, labels = torch.empty((0, 16)).cuda(), torch.empty((0,), dtype=torch.int32).cuda()
+    none = torch.empty((0,)).cuda()
+    ops.dense_xent_fwd(x, w, b, labels, none, none)
+    dw, db = torch.ones_like(w), torch.ones_like(b)
+    ops.dense_xent_bwd(x, w, b, labels, none, none, torch.empty_like(x), dw, db, accumulate=True)
+    assert bool((dw == 1).all()) and bool((db == 1).all())
+    ops.dense_xent_bwd(x, w, b, labels, none, none, torch.empty_like(x), dw, db)
+    assert bool((dw == 0).all()) and bool((db == 0).all())
+
+
+@gpu
+def test_gradient_against_differences():
+    """Central differences of the float64 definition along a random direction of every operand."""
+    x, w, b, labels, dloss = case(40, 20, 100, torch.float32, seed=13)
+    got = run(x, w, b, labels, dloss)
+    step = 1e-5
+    for k, (name, t) in enumerate((("dx", x), ("dw", w), ("db", b))):
+        direction = torch.randn(t.shape, generator=torch.Generator().manual_seed(k)).double()
+        ends = []
+        for s in (step, -step):
+            moved = [x.double(), w.double(), b.double()]
+            moved[k] = moved[k] + s * direction
+            ends.append(float((reference(moved[0], moved[1], moved[2], labels, dloss)["loss"] * dloss.double()).sum()))
+        quotient = (ends[0] - ends[1]) / (2 * step)
+        slope = float((got[name].double() * direction).sum())
+        # quotient: step^2 relative, and 2^-52 of the loss over the step; slope: float32 gradients
+        assert abs(quotient - slope) <= 1e-5 * float(got[name].double().norm() * direction.norm()) + 1e-9
+
+
+@gpu
+def test_captured_forward_and_backward_replay():
+    args = case(200, 128, 1000, torch.bfloat16, seed=14)
+    x, w, b, labels, dloss = [t.cuda() for t in args]
+    loss, lse = torch.empty((200,)).cuda(), torch.empty((200,)).cuda()
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+
+    def step():
+        ops.dense_xent_fwd(x, w, b, labels, loss, lse)
+        ops.dense_xent_bwd(x, w, b, labels, lse, dloss, dx, dw, db)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for seed in range(3):
+        x.copy_(case(200, 128, 1000, torch.bfloat16, seed=20 + seed)[0])
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (loss, dx, dw, db)]
+        step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, (loss, dx, dw, db)))
+
+
+@gpu
+def test_two_streams_at_once():
+    sets = [[t.cuda() for t in case(300, 128, 2000, torch.float32, seed=30 + k)] for k in range(2)]
+    want = [run(*[t.cpu() for t in s]) for s in sets]
+    outs, streams = [], [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        outs = []
+        for (x, w, b, labels, dloss), st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                loss, lse = torch.empty((300,), device="cuda"), torch.empty((300,), device="cuda")
+                dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+                ops.dense_xent_fwd(x, w, b, labels, loss, lse)
+                ops.dense_xent_bwd(x, w, b, labels, lse, dloss, dx, dw, db)
+                outs.append((loss, dx, dw, db))
+        torch.cuda.synchronize()
+        for got, ref in zip(outs, want):
+            assert all(torch.equal(g.cpu(), ref[k]) for g, k in zip(got, ("loss", "dx", "dw", "db")))
+
+
+@gpu
+def test_refusals():
+    x, w, b, labels, dloss = [t.cuda() for t in case(8, 16, 40, torch.float32)]
+    row = torch.empty((8,), device="cuda")
+    good = dict(x=x, w=w, b=b, labels=labels, loss=row, lse=row)
+    for bad in (dict(x=x.double()), dict(x=x.half()), dict(x=x.t()), dict(x=x[:, :8]), dict(x=x.view(8, 4, 4)), dict(x=x.cpu()),
+                dict(w=w.to(torch.bfloat16)), dict(w=w.t()), dict(w=w[:, :30]), dict(b=b[:39].contiguous()), dict(labels=labels.long()),
+                dict(labels=labels[:7].contiguous()), dict(loss=row[:7].contiguous()), dict(lse=row.double()),
+                dict(hits=row), dict(x=torch.cat([x.view(-1), x.view(-1)])[1:129].view(8, 16))):
+        with pytest.raises(MgxError):
+            ops.dense_xent_fwd(**{**good, **bad})
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+    good = dict(x=x, w=w, b=b, labels=labels, lse=row, dloss=dloss, dx=dx, dw=dw, db=db)
+    for bad in (dict(dx=dx.to(torch.bfloat16)), dict(dx=dx[:7].contiguous()), dict(dw=dw[:15].contiguous()), dict(db=db[:3].contiguous()),
+                dict(dloss=dloss[:3].contiguous()), dict(dw=dw.double()), dict(lse=row[:5].contiguous())):
+        with pytest.raises(MgxError):
+            ops.dense_xent_bwd(**{**good, **bad})
+    with pytest.raises(MgxError):                  # more features than the library serves
+        ops.dense_xent_fwd(torch.empty((1, 70000), device="cuda"), torch.empty((70000, 1), device="cuda"), None,
+                           labels[:1], row[:1], row[:1])
