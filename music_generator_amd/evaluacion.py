@@ -23,17 +23,57 @@ from .layers import Conv2D, Dense, Flatten
 
 
 class SoftmaxDense(Dense):
-    """Dense(units, activation='softmax') on a flattened input (evaluacion.py:97).  With a tape
-    the layer returns its LOGITS: the fitting loop pairs them with the fused softmax +
-    cross-entropy kernel, whose logit gradient is what backward() receives."""
+    """Dense(units, activation='softmax') on a flattened input (evaluacion.py:97) or on every position of a feature map.
+    With a tape the layer returns its LOGITS: the fitting loop pairs them with the fused softmax +
+    cross-entropy kernel, whose logit gradient is what backward() receives.  Fitting on class numbers does not
+    run this layer: `loss` takes its input and never stores the logits."""
 
     def forward(self, xs, save, act_alpha: float = 0.0):
         logits, saved = super().forward(xs, save, 0.0)
         if save:
             return logits, saved
         y = K.empty(logits.shape)
-        ops.softmax_rows(logits.contiguous(), y)
+        ops.softmax_rows(logits.contiguous().view(-1, self.units), y.view(-1, self.units))
         return y, None
+
+    def loss(self, features, labels, backward: bool = True):
+        """(sum of the losses, hits, labelled rows, gradient of the mean loss with respect to `features` or None) of the
+        head on `features` (..., cin) for class numbers `labels` (one per row of features; outside [0, units): no
+        label), as 0-d device tensors.  With `backward` the gradients of the mean are added to the bound views of the
+        head's variables.  The logits are never stored (ops.dense_xent_fwd / _bwd), unless they are no wider than the
+        features beside them (the 9 classes of define_evaluator on 384 000 features): then storing them costs nothing."""
+        x = features.reshape(-1, self.cin)
+        n = x.shape[0]
+        labelled = (labels >= 0) & (labels < self.units)
+        count = labelled.sum().float()
+        if self.units <= self.cin and features.dim() == 2:
+            return self._loss_from_logits(x, labels, labelled, count, backward)
+        w, b = self.kernel.value().view(self.cin, self.units), self.bias.value()
+        loss, lse, hits = K.empty((n,)), K.empty((n,)), K.empty((n,), dtype=torch.int32)
+        ops.dense_xent_fwd(x, w, b, labels, loss, lse, hits)
+        dx = None
+        if backward:
+            if self.kernel.grad is None or self.bias.grad is None:
+                raise RuntimeError("gradient buffers of %s are not bound" % self.name)
+            dx = torch.empty_like(x)
+            ops.dense_xent_bwd(x, w, b, labels, lse, labelled.float() / count.clamp(min=1.0), dx,
+                               self.kernel.grad.view(self.cin, self.units), self.bias.grad, accumulate=True)
+            dx = dx.view(features.shape)
+        return loss.sum(), hits.sum(), count, dx
+
+    def _loss_from_logits(self, x, labels, labelled, count, backward):
+        x = torch.where(labelled[:, None], x, torch.zeros_like(x))       # an unlabelled sample may hold anything
+        logits, saved = super().forward([x], True)
+        hot = torch.zeros_like(logits).scatter_(1, labels.long().clamp(0, self.units - 1)[:, None], 1.0)
+        prob, rows, dlogits = K.empty(logits.shape), K.empty((x.shape[0],)), K.empty(logits.shape)
+        ops.softmax_xent(logits.contiguous(), hot, prob, rows, dlogits)
+        loss = torch.where(labelled, rows, torch.zeros_like(rows)).sum()
+        hits = ((prob.argmax(dim=1) == labels) & labelled).sum()
+        if not backward:
+            return loss, hits, count, None
+        # dlogits is the gradient of the mean over all rows
+        dlogits = torch.where(labelled[:, None], dlogits * (x.shape[0] / count.clamp(min=1.0)), torch.zeros_like(dlogits))
+        return loss, hits, count, super().backward(saved, dlogits, [True], [None], True)[0][0]
 
 
 def _conv(t, ksize, **kw):
@@ -97,9 +137,39 @@ def labels_to_device(y) -> torch.Tensor:
     return t.to(device=K.device(), dtype=torch.float32).contiguous()
 
 
+def _class_numbers(y) -> bool:
+    """Labels are class numbers (an integer type: sparse categorical cross-entropy) rather than one-hot rows."""
+    return not (y.is_floating_point() if isinstance(y, torch.Tensor) else np.issubdtype(np.asarray(y).dtype, np.floating))
+
+
+def class_numbers_to_device(y) -> torch.Tensor:
+    """Class numbers of any shape as a flat int32 device tensor; numbers that int32 does not hold become -1 (no label)."""
+    t = y if isinstance(y, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(y))
+    t = t.to(device=K.device(), dtype=torch.int64).reshape(-1)
+    return torch.where((t >= 0) & (t < 2 ** 31), t, torch.full_like(t, -1)).to(torch.int32)
+
+
+def _split_head(model):
+    """(model of everything in front of the classifier head, head) for a model that ends in a SoftmaxDense."""
+    node = model.output.node
+    if not isinstance(node.layer, SoftmaxDense):
+        raise ValueError("fitting on class numbers needs a model that ends in a SoftmaxDense")
+    return Model(model.input, node.inputs[0]), node.layer
+
+
 def evaluate(model, x, y, batch_size: int = 32) -> Dict[str, float]:
-    """Mean categorical cross-entropy and accuracy over (x, y) - keras' evaluate / validation pass."""
+    """Mean categorical cross-entropy and accuracy over (x, y) - keras' evaluate / validation pass.  y: one-hot rows, or
+    class numbers (one per sample or per position, negative: none), then the mean is over the labelled rows."""
     n = x.shape[0]
+    if _class_numbers(y):
+        trunk, head = _split_head(model)
+        sums = torch.zeros((3,), dtype=torch.float64, device=K.device())
+        for i in range(0, n, batch_size):
+            features, _ = trunk.forward(model._to_device(x[i:i + batch_size]))
+            loss, hits, count, _ = head.loss(features, class_numbers_to_device(y[i:i + batch_size]), backward=False)
+            sums += torch.stack([loss.double(), hits.double(), count.double()])
+        loss, hits, count = sums.tolist()
+        return {"loss": loss / max(count, 1.0), "accuracy": hits / max(count, 1.0)}
     loss, hits = 0.0, 0
     for i in range(0, n, batch_size):
         xb = model._to_device(x[i:i + batch_size])
@@ -116,19 +186,42 @@ def fit_evaluator(model, x, y, epochs: int, batch_size: int, optimizer=None, val
                   shuffle_seed: int = 0, verbose: int = 0) -> Dict[str, List[float]]:
     """model.compile(optimizer="Adam", loss='categorical_crossentropy', metrics=["accuracy"]) +
     model.fit(X, y, epochs, batch_size, validation_data) of evaluacion.py:160-161.  Returns the
-    history: per epoch the sample-weighted mean of the batch losses / accuracies (and val_*)."""
+    history: per epoch the sample-weighted mean of the batch losses / accuracies (and val_*).
+
+    y as an integer array holds class numbers instead of one-hot rows (keras' sparse categorical cross-entropy): one per
+    sample, or one per position for a head without a Flatten in front; negative numbers are positions without a label, and
+    a batch's loss is the mean over its labelled ones.  The logits of that form are never stored, so that it is the one for
+    many classes or many positions; backend.TAPE8 keeps the rest of the tape in 8 bits."""
     from .models import Adam
     opt = optimizer or Adam()                              # keras defaults: 1e-3, 0.9, 0.999, 1e-7
     n = x.shape[0]
     rng = np.random.default_rng(shuffle_seed)
     hist: Dict[str, List[float]] = {"loss": [], "accuracy": []}
-    y = np.ascontiguousarray(y, dtype=np.float32)
+    numbers = _class_numbers(y)
+    if numbers:
+        trunk, head = _split_head(model)
+        y = np.ascontiguousarray(y.cpu().numpy() if isinstance(y, torch.Tensor) else y)
+        if y.shape[0] != n:
+            raise ValueError("one row of class numbers per sample expected")
+    else:
+        y = np.ascontiguousarray(y, dtype=np.float32)
     for epoch in range(epochs):
         order = rng.permutation(n)
         loss_sum = torch.zeros((), dtype=torch.float32, device=K.device())
         hits = torch.zeros((), dtype=torch.int64, device=K.device())
+        counted = torch.zeros((), dtype=torch.float64, device=K.device())
         for i in range(0, n, batch_size):
             idx = order[i:i + batch_size]
+            if numbers:
+                model.bind_grads(0).zero_()
+                features, tape = trunk.forward(model._to_device(x[idx]), save=True)
+                loss, right, count, dx = head.loss(features, class_numbers_to_device(y[idx]))
+                trunk.backward(tape, dx, need_input_grad=False)
+                opt.apply_model_gradients(model)
+                loss_sum += loss
+                hits += right
+                counted += count
+                continue
             xb, yb = model._to_device(x[idx]), labels_to_device(y[idx])
             flat = model.bind_grads(0)
             flat.zero_()
@@ -139,8 +232,9 @@ def fit_evaluator(model, x, y, epochs: int, batch_size: int, optimizer=None, val
             opt.apply_model_gradients(model)
             loss_sum += rows.sum()
             hits += (prob.argmax(dim=1) == yb.argmax(dim=1)).sum()
-        hist["loss"].append(float(loss_sum) / n)
-        hist["accuracy"].append(int(hits) / n)
+        total = max(float(counted), 1.0) if numbers else n
+        hist["loss"].append(float(loss_sum) / total)
+        hist["accuracy"].append(int(hits) / total)
         if validation_data is not None:
             val = evaluate(model, validation_data[0], validation_data[1], batch_size)
             hist.setdefault("val_loss", []).append(val["loss"])

@@ -303,3 +303,128 @@ def test_refusals():
     with pytest.raises(MgxError):                  # more features than the library serves
         ops.dense_xent_fwd(torch.empty((1, 70000), device="cuda"), torch.empty((70000, 1), device="cuda"), None,
                            labels[:1], row[:1], row[:1])
+
+
+# ---- the evaluator's fit on class numbers, with and without the 8-bit tape ----
+def position_classifier(classes, precision="float32"):
+    """A small evaluator-like trunk with a classifier on every position (no Flatten)."""
+    from music_generator_amd.evaluacion import SoftmaxDense
+    from music_generator_amd.graph import Input, Model
+    from music_generator_amd.layers import Conv2D
+    M.backend.set_precision(precision)
+    M.clear_session()
+    M.layers.set_init_seed(5)
+    image = Input(shape=(8, 40, 2))
+    t = Conv2D(128, (1, 1), padding="same", kernel_initializer="he_normal")(image)
+    t = Conv2D(32, (3, 3), padding="same", kernel_initializer="he_normal")(t)
+    t = Conv2D(128, (1, 1), padding="same", kernel_initializer="he_normal")(t)
+    return Model(image, SoftmaxDense(classes)(t))
+
+
+@pytest.fixture
+def restore():
+    yield
+    M.backend.TAPE8 = False
+    M.backend.set_precision("float32")
+
+
+@gpu
+def test_fit_on_class_numbers_equals_one_hot_labels(restore):
+    from music_generator_amd import evaluacion as E
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((12, 4, 750, 2)).astype(np.float32)
+    numbers = rng.integers(0, 9, 12)
+    weights, history = [], []
+    for y in (np.eye(9, dtype=np.float32)[numbers], numbers):
+        M.clear_session()
+        M.layers.set_init_seed(3)
+        model = E.define_evaluator(1)[0]
+        history.append(E.fit_evaluator(model, x, y, 1, 4, validation_data=(x, y)))
+        weights.append(model.get_weights_dict())
+    # three batches; the first two losses come from weights that agree to the rounding of one update, which Adam's division by
+    # the root of the squared gradient turns into 2 lr = 2e-3 for a weight whose gradient is all rounding: compared in the mean
+    assert abs(history[0]["loss"][0] - history[1]["loss"][0]) < 1e-3 * abs(history[0]["loss"][0])
+    for k in weights[0]:
+        moved = np.abs(weights[0][k] - weights[1][k])
+        assert moved.max() <= 6.1e-3 and moved.mean() < 3e-4, k
+
+
+@gpu
+@pytest.mark.parametrize("precision", ["float32", "bfloat16"])
+@pytest.mark.parametrize("tape8", [False, True])
+def test_positions_with_many_classes(restore, precision, tape8):
+    """Loss and gradients of a classifier on every position against the float64 definition behind the same features, and the
+    whole fit running from the 8-bit tape."""
+    from music_generator_amd import evaluacion as E
+    classes = 1500
+    model = position_classifier(classes, precision)
+    M.backend.TAPE8 = tape8
+    gen = torch.Generator().manual_seed(1)
+    x = torch.randn((3, 8, 40, 2), generator=gen)
+    labels = torch.randint(-1, classes, (3, 8, 40), generator=gen)
+    trunk, head = E._split_head(model)
+    model.bind_grads(0).zero_()
+    features, tape = trunk.forward(x.cuda(), save=True)
+    assert features.dtype == (torch.bfloat16 if precision == "bfloat16" else torch.float32)
+    if tape8:
+        assert any(isinstance(v, ops.Tape8) for s in tape for v in (s if isinstance(s, tuple) else (getattr(s, "x", None),)))
+    loss, hits, count, dx = head.loss(features, E.class_numbers_to_device(labels))
+    flat = features.cpu().reshape(-1, 128)
+    lab = labels.reshape(-1).int()
+    dl = (lab >= 0).double() / int((lab >= 0).sum())
+    want = reference(flat, torch.from_numpy(head.kernel.numpy()), torch.from_numpy(head.bias.numpy()), lab, dl)
+    got = {"loss": want["loss"], "lse": want["lse"], "dx": dx.cpu().reshape(-1, 128), "dw": head.kernel.grad.cpu().view(128, classes),
+           "db": head.bias.grad.cpu()}
+    largest = float((flat.double() @ torch.from_numpy(head.kernel.numpy()).double()).abs().max())
+    check(got, want, features.dtype, largest)
+    assert int(count) == int((lab >= 0).sum())
+    # a float32 sum of the losses: half a unit a step at most
+    assert abs(float(loss) - float(want["loss"].sum())) <= 960 * 2.0 ** -24 * float(want["loss"].sum()) + 960 * 2.0 ** -20
+    trunk.backward(tape, dx, need_input_grad=False)
+    assert all(bool(v.grad.isfinite().all()) and float(v.grad.abs().max()) > 0 for v in model.trainable_variables)
+    hist = E.fit_evaluator(model, x.numpy(), labels.numpy(), 2, 2, validation_data=(x.numpy(), labels.numpy()))
+    assert all(np.isfinite(hist[k]).all() for k in hist) and 0 <= hist["accuracy"][-1] <= 1
+
+
+@gpu
+def test_narrow_head_on_class_numbers(restore):
+    """Fewer classes than features: the logits are stored; unlabelled samples, whatever they hold, leave no trace."""
+    from music_generator_amd import evaluacion as E
+    M.clear_session()
+    model = E.define_evaluator(1)[0]
+    _, head = E._split_head(model)
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randn((6, head.cin), generator=gen)
+    labels = torch.tensor([3, -1, 0, 8, 9, 5])
+    w = torch.randn((head.cin, 9), generator=gen) / head.cin ** 0.5
+    head.kernel.assign(w.numpy())
+    lab = torch.where(labels < 9, labels, torch.full_like(labels, -1)).int()
+    dl = (lab >= 0).double() / 4
+    want = reference(x, w, torch.zeros((9,)), lab, dl)
+    x[1], x[4] = float("nan"), 1e30
+    model.bind_grads(0).zero_()
+    loss, hits, count, dx = head.loss(x.cuda(), E.class_numbers_to_device(labels))
+    got = {"loss": want["loss"], "lse": want["lse"], "dx": dx.cpu(), "dw": head.kernel.grad.cpu().view(-1, 9), "db": head.bias.grad.cpu()}
+    # products over 384 000 float32 terms: sqrt(384 000) roundings of 2^-24 relative in the mean
+    check(got, want, torch.float32, 40.0)
+    assert int(count) == 4 and int(hits) == int(want["hits"].sum())
+    assert abs(float(loss) - float(want["loss"].sum())) < 1e-4
+
+
+@gpu
+def test_probabilities_on_every_position(restore):
+    model = position_classifier(30)
+    p = model(torch.randn((2, 8, 40, 2)).cuda())
+    assert tuple(p.shape) == (2, 8, 40, 30) and float((p.sum(dim=-1) - 1).abs().max()) < 1e-5
+
+
+def test_class_numbers_are_told_by_their_type():
+    from music_generator_amd import evaluacion as E
+    assert E._class_numbers(np.array([1, 2])) and E._class_numbers(torch.tensor([1, 2]))
+    assert not E._class_numbers(np.eye(3)) and not E._class_numbers(torch.eye(3))
+
+
+def test_a_model_without_a_classifier_head_is_refused():
+    from music_generator_amd import evaluacion as E
+    with pytest.raises(ValueError):
+        E._split_head(M.define_discriminator(1)[0][0])
