@@ -11,7 +11,8 @@
 // operand's largest magnitude below 2^14: 22 significant bits, and 2^-25 of 2^14 absolute where a value is small.  The
 // product keeps hi hi + hi lo + lo hi (the dropped lo lo is 2^-24 of it).  A bf16 operand is exact in one plane.  This is
 // three (two) of 2.5 PFLOP/s instead of one of the 157 TFLOP/s of the float32 matrix instructions.
-// exp and log are taken in float32 from the float32 logits; maxima, sums, lse and all gradient sums are float32.
+// Logits, maxima, sums, lse and all gradient sums are float32; inside the kernels logits are in units of log 2 (the bias
+// and the reciprocal scales carry the factor), so that an exponential is one v_exp_f32.
 //
 // A row whose label lies outside [0, v) has no loss: loss 0, lse 0, gradient 0 and nothing of its features is read into
 // a product (they may hold anything).  A class may be masked with a bias of -inf or the lowest float.
@@ -190,15 +191,17 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
             p.scales[1] = sx;
             p.scales[2] = sd;
         }
-        for (long i = first * 256 + tid; i < p.vp; i += nb * 256)
-            p.bias[i] = i < p.v ? (p.b ? p.b[i] : 0.f) : -__builtin_inff();
+        for (long i = first * 256 + tid; i < p.vp; i += nb * 256) {
+            const float b = i < p.v ? (p.b ? p.b[i] : 0.f) : -__builtin_inff();
+            p.bias[i] = b < 0.f && b >= kLowest ? fmaxf(b * kLog2e, kLowest) : b * kLog2e;      // the lowest float stays finite
+        }
         for (long i = first * 256 + tid; i < p.np; i += nb * 256) {
             int lab = i < p.n ? p.labels[i] : -1;
             if (lab >= p.v) lab = -1;
             p.lab[i] = lab < 0 ? -1 : lab;
             if (p.dlp) {
                 p.dlp[i] = lab < 0 ? 0.f : p.dloss[i] / sd;
-                p.lsep[i] = lab < 0 ? 0.f : p.lse[i];
+                p.lsep[i] = lab < 0 ? __builtin_inff() : p.lse[i] * kLog2e;      // every exponential of the row is 0
             }
         }
     }
@@ -330,7 +333,7 @@ __global__ __launch_bounds__(256, 2) void xent_gemm_kernel(XentGemm g) {
     const long mw = m0 + wm * 64, nw = n0 + wn * 64;
     if constexpr (EPI == EPI_FWD || EPI == EPI_DZ) {
         // A: classes, B: rows of x
-        const float un = 1.f / g.scales[0], ux = 1.f / g.scales[1];
+        const float un = 1.f / g.scales[0], ux = 1.f / g.scales[1] * kLog2e;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const long row = nw + j * 32 + r;
@@ -354,7 +357,7 @@ __global__ __launch_bounds__(256, 2) void xent_gemm_kernel(XentGemm g) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) s += __builtin_amdgcn_exp2f((acc[i][j][k] - m) * kLog2e);
+                    for (int k = 0; k < 16; ++k) s += __builtin_amdgcn_exp2f(acc[i][j][k] - m);
                 s += __shfl_xor(s, 32, 64);
                 if (h == 0) g.part[(mw / 64) * g.np + row] = make_float2(m, s);
                 if (lab >= 0 && rel >= 0 && rel < 64) {
@@ -370,9 +373,9 @@ __global__ __launch_bounds__(256, 2) void xent_gemm_kernel(XentGemm g) {
                 for (int i = 0; i < 2; ++i) {
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        float p = __builtin_amdgcn_exp2f((acc[i][j][k] - lse) * kLog2e);
+                        float p = __builtin_amdgcn_exp2f(acc[i][j][k] - lse);
                         if (i * 32 + (k & 3) + 8 * (k >> 2) + 4 * h == rel) p -= 1.f;           // no label: rel < 0
-                        acc[i][j][k] = dl == 0.f ? 0.f : p * dl;
+                        acc[i][j][k] = p * dl;
                     }
                     acc_rows_interleaved(acc[i][j]);
 #pragma unroll
@@ -423,7 +426,297 @@ __global__ __launch_bounds__(256, 2) void xent_gemm_kernel(XentGemm g) {
     }
 }
 
-// loss and lse of 32 rows per workgroup from the partial (maximum, sum) of every 64 classes
+// ---------------------------------------------------------------- narrow features
+// Up to EP features (EP = 128) the two products around the exponential run in one kernel and no dz is stored.  One operand is
+// resident: a wave keeps 32 RB of its items (rows of x, or classes) as B fragments in registers.  The other is streamed: tiles of 64 of
+// its items in LDS, double-buffered by LDS-DMA and shared by the four waves.  Per 32 streamed items:
+//     S (32 streamed x 32 RB resident) = sum over plane products                         first product
+//     forward: the lane's running maximum and sum over the streamed classes
+//     backward: P = exp(S - lse) (times dloss where rows are streamed) - label, as fp16 planes: the accumulator registers
+//               8 t .. 8 t + 7 of a lane are the streamed items 16 t + 4 h + {0..3} and 16 t + 8 + 4 h + {0..3}, which is the
+//               B fragment of a product over 16 streamed items taken in that order
+//     D (EP x 32 RB) += streamed^T P, the A fragments read transposed (ds_read_b64_tr_b16) from the same tile in that order
+// MODE FWD and DX: rows resident, classes streamed; DW: classes resident, rows streamed.  gridDim.y parts of the streamed
+// operand leave partial results that are joined in order.
+enum { MODE_FWD = 0, MODE_DX = 1, MODE_DW = 2 };
+constexpr int ST = 64;                              // streamed items of a tile
+
+struct XentStream {
+    const f16_t *r[2], *s[2];
+    const float *scales;
+    const float *bias;                              // classes
+    const float *lse, *dl;                          // rows
+    const int* lab;                                 // rows
+    int tiles;                                      // streamed tiles of 64
+    float2* part;                                   // FWD: (maximum, sum) per part and row
+    float* zlab;                                    // FWD
+    float* out;                                     // DX: part x rows x EP; DW: part x EP x classes
+    float* outb;                                    // DW: part x classes
+    long ld;                                        // rows (FWD, DX) or classes (DW), padded
+};
+
+template <int EP>
+__device__ __forceinline__ int swz_item(int row) {
+    return EP == 64 ? ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) : (((row & 3) << 2) | ((row >> 2) & 3));
+}
+
+template <int EP, int NR, int NS, int RB, int MODE, int OCC>
+__global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    constexpr int KS = EP / 16, EB = EP / 32, ROWB = EP * 2, SPLANE = ST * ROWB, INFO = 3 * ST * 4;
+    constexpr int BUF = NS * SPLANE + 1024;
+    constexpr int NP = MODE == MODE_DW ? 2 : NR;    // planes of P: DX of a bf16 x needs one (its result is rounded to 8 bits)
+    constexpr int NA = MODE == MODE_DW ? NS : NR;   // planes of the streamed operand in the second product
+    static_assert(INFO <= 1024, "");
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, h = lane >> 5;
+    const long item0 = ((long)blockIdx.x * 4 + wv) * (32 * RB);
+    const int per = (g.tiles + gridDim.y - 1) / gridDim.y;
+    const int t0 = blockIdx.y * per, t1 = t0 + per < g.tiles ? t0 + per : g.tiles;
+
+    auto stage = [&](int buf, int t) {
+        unsigned char* dst = lds + buf * BUF;
+        constexpr int RPI = 1024 / ROWB, PIECES = SPLANE / 1024;
+#pragma unroll
+        for (int pl = 0; pl < NS; ++pl)
+#pragma unroll
+            for (int i = 0; i < PIECES / 4; ++i) {
+                const int piece = wv * (PIECES / 4) + i;
+                const int row = piece * RPI + lane / (64 / RPI), ch = (lane & (64 / RPI - 1)) ^ swz_item<EP>(row);
+                const f16_t* gp = g.s[pl] + ((long)t * ST + row) * EP + ch * 8;
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)gp,
+                                                 (__attribute__((address_space(3))) void*)(dst + pl * SPLANE + piece * 1024), 16, 0, 0);
+            }
+        const void* ip = MODE != MODE_DW ? (const void*)g.bias : wv == 0 ? (const void*)g.lse : wv == 1 ? (const void*)g.dl : (const void*)g.lab;
+        if (wv < (MODE == MODE_DW ? 3 : 1))
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((const float*)ip + (long)t * ST + lane),
+                                             (__attribute__((address_space(3))) void*)(dst + NS * SPLANE + wv * 256), 4, 0, 0);
+    };
+
+    if (t0 < t1) stage(0, t0);
+
+    // resident fragments: lane r's item, features 16 ks + 8 h .. + 7
+    u32x4 fb[NR][RB][KS];
+#pragma unroll
+    for (int pl = 0; pl < NR; ++pl)
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                fb[pl][b][ks] = *(const u32x4*)(g.r[pl] + (item0 + 32 * b + r) * EP + 16 * ks + 8 * h);
+    const float unit = kLog2e / g.scales[0] / g.scales[1];
+    float rinfo[RB];                                // DX: lse - 14; DW: bias
+    int rlab[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        const long it = item0 + 32 * b + r;
+        rinfo[b] = MODE == MODE_DW ? g.bias[it] : MODE == MODE_DX ? g.lse[it] - 14.f : 0.f;
+        rlab[b] = MODE == MODE_DW ? 0 : g.lab[it];
+    }
+    // LDS offsets of the lane: fragment ks of its row, and the transposed reads of feature block eb
+    const int cb = (lane >> 4) & 1, qq = (lane >> 2) & 3, pp = lane & 3;
+    int ao[KS], to[EB][2];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) ao[ks] = r * ROWB + (((2 * ks + h) ^ swz_item<EP>(r)) << 4);
+    if constexpr (MODE != MODE_FWD) {
+#pragma unroll
+        for (int eb = 0; eb < EB; ++eb)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int row = 8 * j + 4 * h + qq;
+                to[eb][j] = row * ROWB + (((4 * eb + 2 * cb + (pp >> 1)) ^ swz_item<EP>(row)) << 4) + 8 * (pp & 1);
+            }
+    }
+
+    float m[RB], ssum[RB];
+    f32x16 dacc[MODE == MODE_FWD ? 1 : EB][RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        m[b] = kLowest;
+        ssum[b] = 0.f;
+#pragma unroll
+        for (int eb = 0; eb < (MODE == MODE_FWD ? 1 : EB); ++eb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dacc[eb][b][i] = 0.f;
+    }
+
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    int cur = 0;
+    for (int t = t0; t < t1; ++t) {
+        if (t + 1 < t1) stage(cur ^ 1, t + 1);
+        const unsigned char* base = lds + cur * BUF;
+        const unsigned char* info = base + NS * SPLANE;
+#pragma unroll 1
+        for (int ib = 0; ib < ST / 32; ++ib) {
+            const unsigned char* tile = base + ib * 32 * ROWB;
+            f32x16 acc[RB];
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int pl = NS - 1; pl >= 0; --pl) {
+                    const u32x4 fa = *(const u32x4*)(tile + pl * SPLANE + ao[ks]);
+#pragma unroll
+                    for (int b = 0; b < RB; ++b) {
+                        if (NR > 1 && pl == 0) acc[b] = mfma_f16(fa, fb[NR - 1][b][ks], acc[b]);
+                        acc[b] = mfma_f16(fa, fb[0][b][ks], acc[b]);
+                    }
+                }
+            const long s0 = (long)t * ST + ib * 32;                 // first streamed item of the block
+            if constexpr (MODE != MODE_DW) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 bv = *(const f32x4*)(info + (ib * 32 + 8 * q + 4 * h) * 4);
+#pragma unroll
+                    for (int b = 0; b < RB; ++b)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) acc[b][4 * q + k] = __builtin_fmaf(acc[b][4 * q + k], unit, bv[k]);
+                }
+            }
+            if constexpr (MODE == MODE_FWD) {
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    float mm = m[b];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) mm = fmaxf(mm, acc[b][i]);
+                    float s = ssum[b] * __builtin_amdgcn_exp2f(m[b] - mm);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s += __builtin_amdgcn_exp2f(acc[b][i] - mm);
+                    ssum[b] = s;
+                    m[b] = mm;
+                    const long rel = rlab[b] - s0;
+                    if (rlab[b] >= 0 && rel >= 0 && rel < 32) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if ((i & 3) + 8 * (i >> 2) + 4 * h == rel) g.zlab[item0 + 32 * b + r] = acc[b][i];
+                    }
+                }
+            } else {
+                u32x4 fp[NP][RB][2];
+                if constexpr (MODE == MODE_DX) {
+#pragma unroll
+                    for (int b = 0; b < RB; ++b) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[b][i] = __builtin_amdgcn_exp2f(acc[b][i] - rinfo[b]);
+                        const long rel = rlab[b] - s0;
+                        if (rlab[b] >= 0 && rel >= 0 && rel < 32) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                if ((i & 3) + 8 * (i >> 2) + 4 * h == rel) acc[b][i] -= kDz;
+                        }
+                    }
+                } else {
+                    const int lab32 = *(const int*)(info + 512 + (ib * 32 + r) * 4);
+                    const bool any = __ballot(lab32 >= item0 && lab32 < item0 + 32 * RB) != 0;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const f32x4 ls = *(const f32x4*)(info + (ib * 32 + 8 * q + 4 * h) * 4);
+                        const f32x4 dl = *(const f32x4*)(info + 256 + (ib * 32 + 8 * q + 4 * h) * 4);
+#pragma unroll
+                        for (int b = 0; b < RB; ++b)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                acc[b][4 * q + k] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][4 * q + k], unit, rinfo[b]) - ls[k]);
+                        if (any) {
+                            const u32x4 lb = *(const u32x4*)(info + 512 + (ib * 32 + 8 * q + 4 * h) * 4);
+#pragma unroll
+                            for (int b = 0; b < RB; ++b)
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    if ((int)lb[k] - (int)item0 - 32 * b == r) acc[b][4 * q + k] -= 1.f;
+                        }
+#pragma unroll
+                        for (int b = 0; b < RB; ++b)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                acc[b][4 * q + k] *= dl[k] * kDz;
+                                ssum[b] += acc[b][4 * q + k];
+                            }
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        float v[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[k] = acc[b][8 * x + k];
+                        if constexpr (NP > 1) split8(v, fp[0][b][x], fp[NP - 1][b][x]);
+                        else fp[0][b][x] = (u32x4){f16_pack(v[0], v[1]), f16_pack(v[2], v[3]), f16_pack(v[4], v[5]), f16_pack(v[6], v[7])};
+                    }
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int eb = 0; eb < EB; ++eb)
+#pragma unroll
+                        for (int pl = NA - 1; pl >= 0; --pl) {
+                            const unsigned char* tp = tile + pl * SPLANE + x * 16 * ROWB;
+                            const u32x2 a0 = tr_read(tp + to[eb][0]), a1 = tr_read(tp + to[eb][1]);
+                            const u32x4 fa = {a0[0], a0[1], a1[0], a1[1]};
+#pragma unroll
+                            for (int b = 0; b < RB; ++b) {
+                                if (NP > 1 && pl == 0) dacc[eb][b] = mfma_f16(fa, fp[NP - 1][b][x], dacc[eb][b]);
+                                dacc[eb][b] = mfma_f16(fa, fp[0][b][x], dacc[eb][b]);
+                            }
+                        }
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        cur ^= 1;
+    }
+
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        const long it = item0 + 32 * b + r;
+        if constexpr (MODE == MODE_FWD) {
+            const float mo = __shfl_xor(m[b], 32, 64), so = __shfl_xor(ssum[b], 32, 64);
+            const float mm = fmaxf(m[b], mo);
+            const float s = ssum[b] * __builtin_amdgcn_exp2f(m[b] - mm) + so * __builtin_amdgcn_exp2f(mo - mm);
+            if (h == 0) g.part[(long)blockIdx.y * g.ld + it] = make_float2(mm, s);
+        } else if constexpr (MODE == MODE_DX) {
+            float* o = g.out + ((long)blockIdx.y * g.ld + it) * EP;
+#pragma unroll
+            for (int eb = 0; eb < EB; ++eb)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *(f32x4*)(o + 32 * eb + 8 * q + 4 * h) =
+                        (f32x4){dacc[eb][b][4 * q], dacc[eb][b][4 * q + 1], dacc[eb][b][4 * q + 2], dacc[eb][b][4 * q + 3]};
+        } else {
+            float* o = g.out + (long)blockIdx.y * EP * g.ld + it;
+#pragma unroll
+            for (int eb = 0; eb < EB; ++eb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[(32 * eb + acc_row(i, lane)) * g.ld] = dacc[eb][b][i];
+            const float so = __shfl_xor(ssum[b], 32, 64);
+            if (h == 0) g.outb[(long)blockIdx.y * g.ld + it] = ssum[b] + so;
+        }
+    }
+}
+
+// dx from the parts of the streamed product, in order
+__global__ __launch_bounds__(256) void xent_dx_join_kernel(const float* __restrict__ parts, const float* __restrict__ scales,
+                                                           const float* __restrict__ dl, void* __restrict__ dx, int dx_f32, int np,
+                                                           long part, long n, int e, int ep) {
+    const float f = scales[2] / kDz / scales[0];
+    const long total = n * ep;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+        const long row = i / ep;
+        const int c = (int)(i - row * ep);
+        if (c >= e) continue;
+        float s = 0.f;
+        for (int p = 0; p < np; ++p) s += parts[p * part + i];
+        s *= f * dl[row];
+        if (dx_f32) ((float*)dx)[row * e + c] = s;
+        else ((bf16_t*)dx)[row * e + c] = (bf16_t)s;
+    }
+}
+
+// loss and lse of 32 rows per workgroup from the partial (maximum, sum) of the parts or of every 64 classes
 __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict__ part, const float* __restrict__ zlab,
                                                         const int* __restrict__ lab, float* __restrict__ loss,
                                                         float* __restrict__ lse, int* __restrict__ hits, long n, long np,
@@ -435,7 +728,7 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
     for (long i = gr; i < slices; i += 8) {
         const float2 p = part[i * np + row];
         const float mm = fmaxf(m, p.x);
-        s = s * __builtin_amdgcn_exp2f((m - mm) * kLog2e) + p.y * __builtin_amdgcn_exp2f((p.x - mm) * kLog2e);
+        s = s * __builtin_amdgcn_exp2f(m - mm) + p.y * __builtin_amdgcn_exp2f(p.x - mm);
         m = mm;
     }
     red[gr][rr] = make_float2(m, s);
@@ -444,14 +737,14 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
         for (int q = 1; q < 8; ++q) {
             const float2 p = red[q][rr];
             const float mm = fmaxf(m, p.x);
-            s = s * __builtin_amdgcn_exp2f((m - mm) * kLog2e) + p.y * __builtin_amdgcn_exp2f((p.x - mm) * kLog2e);
+            s = s * __builtin_amdgcn_exp2f(m - mm) + p.y * __builtin_amdgcn_exp2f(p.x - mm);
             m = mm;
         }
         const bool ok = lab[row] >= 0;
         // (m - z) first: the loss of a row whose label has nearly all the probability is far below an ulp of lse
-        const float ls = __builtin_amdgcn_logf(s) * kLn2;
-        loss[row] = ok ? (m - zlab[row]) + ls : 0.f;
-        lse[row] = ok ? m + ls : 0.f;
+        const float ls = __builtin_amdgcn_logf(s);
+        loss[row] = ok ? ((m - zlab[row]) + ls) * kLn2 : 0.f;
+        lse[row] = ok ? (m + ls) * kLn2 : 0.f;
         if (hits) hits[row] = ok && zlab[row] >= m ? 1 : 0;
     }
 }
@@ -488,15 +781,29 @@ __global__ __launch_bounds__(256) void xent_zero_kernel(float* __restrict__ a, l
 
 // ---------------------------------------------------------------- host
 struct Layout {
-    int64_t np, vp, ep, vc, nz;
+    bool narrow;                   // the streamed kernels
+    int rows_wg;                   // resident rows of a workgroup (FWD, DX)
+    int64_t np, vp, ep, vc, nz, nf, nx;      // nf, nx, nz: parts of the streamed operand in FWD, DX, DW (nz: of the rows in general)
     int64_t part, bias, scales, lab, zlab, lse, dl, xh, xl, wh, wl, slices, dzh, dzl, dxw, slabs, slabs_b, total;
 };
 
 Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
     Layout l = {};
-    l.np = up(n, 128);
+    l.narrow = e <= 128;
+    l.rows_wg = l.narrow && !xf32 ? 256 : 128;
+    l.np = up(n, l.rows_wg);
     l.vp = up(v, 128);
     l.ep = up(e, 128);
+    // two workgroups a CU where there is enough to split, four tiles of 64 a part at least
+    auto split = [](int64_t wgs, int64_t tiles) {
+        int64_t p = 512 / wgs;
+        if (p > tiles / 4) p = tiles / 4;
+        return p < 1 ? (int64_t)1 : p;
+    };
+    if (l.narrow) {
+        l.nf = l.nx = split(l.np / l.rows_wg, l.vp / ST);
+        l.nz = split(l.vp / 128, l.np / ST);
+    }
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t o = at;
@@ -513,7 +820,15 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
     l.wl = take(l.vp * l.ep * 2);
     if (!backward) {
         l.zlab = take(l.np * 4);
-        l.slices = take(l.np * (l.vp / 64) * 8);
+        if (!l.narrow) l.nf = l.vp / 64;
+        l.slices = take(l.np * l.nf * 8);
+    } else if (l.narrow) {
+        l.lse = take(l.np * 4);
+        l.dl = take(l.np * 4);
+        l.vc = l.vp;
+        l.dxw = take(l.nx * l.np * l.ep * 4);
+        l.slabs = take(l.nz * l.ep * l.vp * 4);
+        l.slabs_b = take(l.nz * l.vp * 4);
     } else {
         l.lse = take(l.np * 4);
         l.dl = take(l.np * 4);
@@ -545,6 +860,14 @@ void launch_gemm(const XentGemm& g, dim3 grid, hipStream_t st) {
     constexpr int bytes = 2 * (NA + NB) * PLANE;
     mgx_allow_dynamic_lds(xent_gemm_kernel<NA, NB, AT, BT, EPI>, bytes, done);
     hipLaunchKernelGGL((xent_gemm_kernel<NA, NB, AT, BT, EPI>), grid, dim3(256), bytes, st, g);
+}
+
+template <int NR, int NS, int RB, int MODE>
+void launch_stream(const XentStream& g, int64_t wgs, int64_t parts, hipStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    constexpr int bytes = 2 * (NS * ST * 256 + 1024);
+    mgx_allow_dynamic_lds(xent_stream_kernel<128, NR, NS, RB, MODE, 2>, bytes, done);
+    hipLaunchKernelGGL((xent_stream_kernel<128, NR, NS, RB, MODE, 2>), dim3((unsigned)wgs, (unsigned)parts), dim3(256), bytes, st, g);
 }
 
 void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const float* w, const float* b, const int* labels,
@@ -597,10 +920,20 @@ extern "C" int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, c
     g.bias = (float*)(ws + l.bias); g.scales = (float*)(ws + l.scales); g.lab = (int*)(ws + l.lab);
     g.part = (float2*)(ws + l.slices); g.zlab = (float*)(ws + l.zlab); g.np = l.np;
     const dim3 grid((unsigned)(l.vp / 128), (unsigned)(l.np / 128));
-    if (xf) launch_gemm<2, 2, false, false, EPI_FWD>(g, grid, st);
-    else launch_gemm<2, 1, false, false, EPI_FWD>(g, grid, st);
+    if (l.narrow) {
+        XentStream q = {};
+        q.r[0] = g.b[0]; q.r[1] = g.b[1]; q.s[0] = g.a[0]; q.s[1] = g.a[1];
+        q.scales = g.scales; q.bias = g.bias; q.lab = g.lab; q.tiles = (int)(l.vp / ST);
+        q.part = g.part; q.zlab = g.zlab; q.ld = l.np;
+        if (xf) launch_stream<2, 2, 1, MODE_FWD>(q, l.np / l.rows_wg, l.nf, st);
+        else launch_stream<1, 2, 2, MODE_FWD>(q, l.np / l.rows_wg, l.nf, st);
+    } else if (xf) {
+        launch_gemm<2, 2, false, false, EPI_FWD>(g, grid, st);
+    } else {
+        launch_gemm<2, 1, false, false, EPI_FWD>(g, grid, st);
+    }
     hipLaunchKernelGGL(xent_join_kernel, dim3((unsigned)(l.np / 32)), dim3(256), 0, st, g.part, g.zlab, g.lab, loss, lse, hits,
-                       (long)n, (long)l.np, (long)(l.vp / 64));
+                       (long)n, (long)l.np, (long)l.nf);
     return mgx_launch_status();
 }
 
@@ -622,6 +955,31 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
     char* ws = (char*)workspace;
     launch_prep(l, ws, x, xf, w, b, labels, lse, dloss, n, e, v, st);
     f16_t *xh = (f16_t*)(ws + l.xh), *xl = (f16_t*)(ws + l.xl), *dzh = (f16_t*)(ws + l.dzh), *dzl = (f16_t*)(ws + l.dzl);
+    if (l.narrow) {
+        XentStream q = {};
+        q.scales = (float*)(ws + l.scales); q.bias = (float*)(ws + l.bias); q.lab = (int*)(ws + l.lab);
+        q.lse = (float*)(ws + l.lse); q.dl = (float*)(ws + l.dl);
+        f16_t *wh = (f16_t*)(ws + l.wh), *wl = (f16_t*)(ws + l.wl);
+        if (dx) {
+            q.r[0] = xh; q.r[1] = xl; q.s[0] = wh; q.s[1] = wl;
+            q.tiles = (int)(l.vp / ST); q.out = (float*)(ws + l.dxw); q.ld = l.np;
+            if (xf) launch_stream<2, 2, 1, MODE_DX>(q, l.np / l.rows_wg, l.nx, st);
+            else launch_stream<1, 2, 2, MODE_DX>(q, l.np / l.rows_wg, l.nx, st);
+            const int64_t blocks = up(n * l.ep, 256) / 256;
+            hipLaunchKernelGGL(xent_dx_join_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, q.out, q.scales,
+                               q.dl, dx, (int)xf, (int)l.nx, (long)(l.np * l.ep), (long)n, (int)e, (int)l.ep);
+        }
+        if (dw || db) {
+            q.r[0] = wh; q.r[1] = wl; q.s[0] = xh; q.s[1] = xl;
+            q.tiles = (int)(l.np / ST); q.out = (float*)(ws + l.slabs); q.outb = (float*)(ws + l.slabs_b); q.ld = l.vp;
+            if (xf) launch_stream<2, 2, 1, MODE_DW>(q, l.vp / 128, l.nz, st);
+            else launch_stream<2, 1, 1, MODE_DW>(q, l.vp / 128, l.nz, st);
+            hipLaunchKernelGGL(xent_dw_reduce_kernel, dim3((unsigned)(up(l.vp, 256) / 256), (unsigned)(e + 1)), dim3(256), 0, st,
+                               q.out, q.outb, q.scales, dw, db, (int)l.nz, (long)(l.ep * l.vp), (long)l.vp, (int)e, (long)v, 0L,
+                               accumulate);
+        }
+        return mgx_launch_status();
+    }
     for (int64_t c0 = 0; c0 < l.vp; c0 += l.vc) {
         const int64_t cnt = l.vp - c0 < l.vc ? l.vp - c0 : l.vc;
         f16_t *wh = (f16_t*)(ws + l.wh) + c0 * l.ep, *wl = (f16_t*)(ws + l.wl) + c0 * l.ep;
