@@ -11,8 +11,9 @@
 // operand's largest magnitude below 2^14: 22 significant bits, and 2^-25 of 2^14 absolute where a value is small.  The
 // product keeps hi hi + hi lo + lo hi (the dropped lo lo is 2^-24 of it).  A bf16 operand is exact in one plane.  This is
 // three (two) of 2.5 PFLOP/s instead of one of the 157 TFLOP/s of the float32 matrix instructions.
-// Logits, maxima, sums, lse and all gradient sums are float32; inside the kernels logits are in units of log 2 (the bias
-// and the reciprocal scales carry the factor), so that an exponential is one v_exp_f32.
+// Logits, maxima, sums, lse and all gradient sums are float32.  An accumulator starts at the class's bias times both scales
+// (exact, they are powers of two), and log2(e) is in the factor that takes the scales out again: an exponential is one fma
+// and one v_exp_f32.
 //
 // A row whose label lies outside [0, v) has no loss: loss 0, lse 0, gradient 0 and nothing of its features is read into
 // a product (they may hold anything).  A class may be masked with a bias of -inf or the lowest float.
@@ -30,8 +31,7 @@ __device__ __forceinline__ f32x16 mfma_f16(u32x4 a, u32x4 b, f32x16 c) {
 }
 
 __device__ __forceinline__ unsigned f16_pack(float lo, float hi) {
-    f16x2 p = {(f16_t)lo, (f16_t)hi};
-    return __builtin_bit_cast(unsigned, p);
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){lo, hi}, f16x2));
 }
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kLowest = -3.402823466e38f;
@@ -108,16 +108,11 @@ __device__ __forceinline__ float scale_from_parts(const unsigned* __restrict__ p
 
 // ---------------------------------------------------------------- planes
 __device__ __forceinline__ void split8(const float* v, u32x4& hi, u32x4& lo) {
-    float r[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const float h = (float)(f16_t)v[k];
-        r[k] = v[k] - h;
-    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        hi[k] = f16_pack(v[2 * k], v[2 * k + 1]);
-        lo[k] = f16_pack(r[2 * k], r[2 * k + 1]);
+        const f16x2 h2 = __builtin_convertvector((f32x2){v[2 * k], v[2 * k + 1]}, f16x2);
+        hi[k] = __builtin_bit_cast(unsigned, h2);
+        lo[k] = f16_pack(v[2 * k] - (float)h2[0], v[2 * k + 1] - (float)h2[1]);
     }
 }
 
@@ -192,8 +187,8 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
             p.scales[2] = sd;
         }
         for (long i = first * 256 + tid; i < p.vp; i += nb * 256) {
-            const float b = i < p.v ? (p.b ? p.b[i] : 0.f) : -__builtin_inff();
-            p.bias[i] = b < 0.f && b >= kLowest ? fmaxf(b * kLog2e, kLowest) : b * kLog2e;      // the lowest float stays finite
+            const float b = i < p.v ? (p.b ? p.b[i] : 0.f) : -__builtin_inff(), q = b * sw * sx;
+            p.bias[i] = b >= kLowest ? fmaxf(q, kLowest) : q;       // a finite mask stays finite
         }
         for (long i = first * 256 + tid; i < p.np; i += nb * 256) {
             int lab = i < p.n ? p.labels[i] : -1;
@@ -333,7 +328,7 @@ __global__ __launch_bounds__(256, 2) void xent_gemm_kernel(XentGemm g) {
     const long mw = m0 + wm * 64, nw = n0 + wn * 64;
     if constexpr (EPI == EPI_FWD || EPI == EPI_DZ) {
         // A: classes, B: rows of x
-        const float un = 1.f / g.scales[0], ux = 1.f / g.scales[1] * kLog2e;
+        const float unit = kLog2e / g.scales[0] / g.scales[1];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const long row = nw + j * 32 + r;
@@ -344,7 +339,7 @@ __global__ __launch_bounds__(256, 2) void xent_gemm_kernel(XentGemm g) {
                 for (int q = 0; q < 4; ++q) {
                     const f32x4 bv = *(const f32x4*)(g.bias + mw + i * 32 + 8 * q + 4 * h);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[i][j][4 * q + k] = acc[i][j][4 * q + k] * un * ux + bv[k];
+                    for (int k = 0; k < 4; ++k) acc[i][j][4 * q + k] = (acc[i][j][4 * q + k] + bv[k]) * unit;
                 }
             const long rel = lab - g.class0 - mw;           // the label's place among the wave's 64 classes
             if constexpr (EPI == EPI_FWD) {
@@ -505,27 +500,23 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
             for (int ks = 0; ks < KS; ++ks)
                 fb[pl][b][ks] = *(const u32x4*)(g.r[pl] + (item0 + 32 * b + r) * EP + 16 * ks + 8 * h);
     const float unit = kLog2e / g.scales[0] / g.scales[1];
-    float rinfo[RB];                                // DX: lse - 14; DW: bias
+    float rinfo[RB];                                // DX: -(lse - 14); DW: bias
     int rlab[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
         const long it = item0 + 32 * b + r;
-        rinfo[b] = MODE == MODE_DW ? g.bias[it] : MODE == MODE_DX ? g.lse[it] - 14.f : 0.f;
+        rinfo[b] = MODE == MODE_DW ? g.bias[it] : MODE == MODE_DX ? 14.f - g.lse[it] : 0.f;
         rlab[b] = MODE == MODE_DW ? 0 : g.lab[it];
     }
-    // LDS offsets of the lane: fragment ks of its row, and the transposed reads of feature block eb
+    // LDS offsets of the lane: the first fragment of its row, and the first transposed reads.  A row starts at a multiple of
+    // its size and the swizzle is an XOR, so further fragments (feature blocks) are an XOR of 32 ks (64 eb) away.
     const int cb = (lane >> 4) & 1, qq = (lane >> 2) & 3, pp = lane & 3;
-    int ao[KS], to[EB][2];
+    const int ao = r * ROWB + ((h ^ swz_item<EP>(r)) << 4);
+    int to[2];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) ao[ks] = r * ROWB + (((2 * ks + h) ^ swz_item<EP>(r)) << 4);
-    if constexpr (MODE != MODE_FWD) {
-#pragma unroll
-        for (int eb = 0; eb < EB; ++eb)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int row = 8 * j + 4 * h + qq;
-                to[eb][j] = row * ROWB + (((4 * eb + 2 * cb + (pp >> 1)) ^ swz_item<EP>(row)) << 4) + 8 * (pp & 1);
-            }
+    for (int j = 0; j < 2; ++j) {
+        const int row = 8 * j + 4 * h + qq;
+        to[j] = row * ROWB + (((2 * cb + (pp >> 1)) ^ swz_item<EP>(row)) << 4) + 8 * (pp & 1);
     }
 
     float m[RB], ssum[RB];
@@ -550,16 +541,21 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
 #pragma unroll 1
         for (int ib = 0; ib < ST / 32; ++ib) {
             const unsigned char* tile = base + ib * 32 * ROWB;
-            f32x16 acc[RB];
+            f32x16 acc[RB];                                         // starts at the classes' bias
 #pragma unroll
-            for (int b = 0; b < RB; ++b)
+            for (int q = 0; q < 4; ++q) {
+                f32x4 bv;
+                if constexpr (MODE != MODE_DW) bv = *(const f32x4*)(info + (ib * 32 + 8 * q + 4 * h) * 4);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
+                for (int b = 0; b < RB; ++b)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[b][4 * q + k] = MODE == MODE_DW ? rinfo[b] : bv[k];
+            }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int pl = NS - 1; pl >= 0; --pl) {
-                    const u32x4 fa = *(const u32x4*)(tile + pl * SPLANE + ao[ks]);
+                    const u32x4 fa = *(const u32x4*)(tile + pl * SPLANE + (ao ^ (ks << 5)));
 #pragma unroll
                     for (int b = 0; b < RB; ++b) {
                         if (NR > 1 && pl == 0) acc[b] = mfma_f16(fa, fb[NR - 1][b][ks], acc[b]);
@@ -567,32 +563,23 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                     }
                 }
             const long s0 = (long)t * ST + ib * 32;                 // first streamed item of the block
-            if constexpr (MODE != MODE_DW) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const f32x4 bv = *(const f32x4*)(info + (ib * 32 + 8 * q + 4 * h) * 4);
-#pragma unroll
-                    for (int b = 0; b < RB; ++b)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) acc[b][4 * q + k] = __builtin_fmaf(acc[b][4 * q + k], unit, bv[k]);
-                }
-            }
             if constexpr (MODE == MODE_FWD) {
 #pragma unroll
                 for (int b = 0; b < RB; ++b) {
                     float mm = m[b];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) mm = fmaxf(mm, acc[b][i]);
-                    float s = ssum[b] * __builtin_amdgcn_exp2f(m[b] - mm);
+                    float s = ssum[b] * __builtin_amdgcn_exp2f((m[b] - mm) * unit);
+                    const float off = -mm * unit;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s += __builtin_amdgcn_exp2f(acc[b][i] - mm);
+                    for (int i = 0; i < 16; ++i) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][i], unit, off));
                     ssum[b] = s;
                     m[b] = mm;
                     const long rel = rlab[b] - s0;
                     if (rlab[b] >= 0 && rel >= 0 && rel < 32) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            if ((i & 3) + 8 * (i >> 2) + 4 * h == rel) g.zlab[item0 + 32 * b + r] = acc[b][i];
+                            if ((i & 3) + 8 * (i >> 2) + 4 * h == rel) g.zlab[item0 + 32 * b + r] = acc[b][i] * unit;
                     }
                 }
             } else {
@@ -601,7 +588,7 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
 #pragma unroll
                     for (int b = 0; b < RB; ++b) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[b][i] = __builtin_amdgcn_exp2f(acc[b][i] - rinfo[b]);
+                        for (int i = 0; i < 16; ++i) acc[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][i], unit, rinfo[b]));
                         const long rel = rlab[b] - s0;
                         if (rlab[b] >= 0 && rel >= 0 && rel < 32) {
 #pragma unroll
@@ -620,7 +607,7 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                         for (int b = 0; b < RB; ++b)
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
-                                acc[b][4 * q + k] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][4 * q + k], unit, rinfo[b]) - ls[k]);
+                                acc[b][4 * q + k] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][4 * q + k], unit, -ls[k]));
                         if (any) {
                             const u32x4 lb = *(const u32x4*)(info + 512 + (ib * 32 + 8 * q + 4 * h) * 4);
 #pragma unroll
@@ -655,7 +642,7 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
 #pragma unroll
                         for (int pl = NA - 1; pl >= 0; --pl) {
                             const unsigned char* tp = tile + pl * SPLANE + x * 16 * ROWB;
-                            const u32x2 a0 = tr_read(tp + to[eb][0]), a1 = tr_read(tp + to[eb][1]);
+                            const u32x2 a0 = tr_read(tp + (to[0] ^ (eb << 6))), a1 = tr_read(tp + (to[1] ^ (eb << 6)));
                             const u32x4 fa = {a0[0], a0[1], a1[0], a1[1]};
 #pragma unroll
                             for (int b = 0; b < RB; ++b) {
@@ -676,8 +663,8 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
         if constexpr (MODE == MODE_FWD) {
             const float mo = __shfl_xor(m[b], 32, 64), so = __shfl_xor(ssum[b], 32, 64);
             const float mm = fmaxf(m[b], mo);
-            const float s = ssum[b] * __builtin_amdgcn_exp2f(m[b] - mm) + so * __builtin_amdgcn_exp2f(mo - mm);
-            if (h == 0) g.part[(long)blockIdx.y * g.ld + it] = make_float2(mm, s);
+            const float s = ssum[b] * __builtin_amdgcn_exp2f((m[b] - mm) * unit) + so * __builtin_amdgcn_exp2f((mo - mm) * unit);
+            if (h == 0) g.part[(long)blockIdx.y * g.ld + it] = make_float2(mm * unit, s);
         } else if constexpr (MODE == MODE_DX) {
             float* o = g.out + ((long)blockIdx.y * g.ld + it) * EP;
 #pragma unroll
