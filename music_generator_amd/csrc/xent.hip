@@ -18,6 +18,7 @@
 // A row whose label lies outside [0, v) has no loss: loss 0, lse 0, gradient 0 and nothing of its features is read into
 // a product (they may hold anything).  A class may be masked with a bias of -inf or the lowest float.
 #include "bf16.h"
+#include <type_traits>
 #include "../../include/mgx.h"
 
 namespace {
@@ -125,7 +126,8 @@ struct XentPrep {
     long n, v, np, vp;            // rows, classes, and both padded to 128
     int e, ep;                    // features, padded to 128
     f16_t *xh, *xl, *wh, *wl;     // planes: rows x ep, classes x ep
-    float *bias, *scales, *lsep, *dlp;
+    float *bias, *scales;
+    float2* row;                  // lse (log 2 units), 2^14 dloss / scales[2]
     int* lab;
     long wtiles, xblocks;
 };
@@ -194,10 +196,8 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
             int lab = i < p.n ? p.labels[i] : -1;
             if (lab >= p.v) lab = -1;
             p.lab[i] = lab < 0 ? -1 : lab;
-            if (p.dlp) {
-                p.dlp[i] = lab < 0 ? 0.f : p.dloss[i] / sd;
-                p.lsep[i] = lab < 0 ? __builtin_inff() : p.lse[i] * kLog2e;      // every exponential of the row is 0
-            }
+            if (p.row)                                       // no label: every exponential of the row is 0
+                p.row[i] = lab < 0 ? make_float2(__builtin_inff(), 0.f) : make_float2(p.lse[i] * kLog2e, p.dloss[i] / sd * kDz);
         }
     }
 }
@@ -215,7 +215,8 @@ struct XentGemm {
     long lda, ldb;
     int kiters;
     // epilogues
-    const float *bias, *scales, *lse, *dl;
+    const float *bias, *scales;
+    const float2* row;
     const int* lab;
     float2* part;
     float *zlab, *out, *outb;
@@ -363,7 +364,7 @@ __global__ __launch_bounds__(256, 2) void xent_gemm_kernel(XentGemm g) {
                             if (i * 32 + (k & 3) + 8 * (k >> 2) + 4 * h == (int)rel) g.zlab[row] = acc[i][j][k];
                 }
             } else {
-                const float lse = g.lse[row], dl = g.dl[row] * kDz;
+                const float lse = g.row[row].x, dl = g.row[row].y;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -423,32 +424,49 @@ __global__ __launch_bounds__(256, 2) void xent_gemm_kernel(XentGemm g) {
 
 // ---------------------------------------------------------------- narrow features
 // Up to EP features (EP = 128) the two products around the exponential run in one kernel and no dz is stored.  One operand is
-// resident: a wave keeps 32 RB of its items (rows of x, or classes) as B fragments in registers.  The other is streamed: tiles of 64 of
-// its items in LDS, double-buffered by LDS-DMA and shared by the four waves.  Per 32 streamed items:
-//     S (32 streamed x 32 RB resident) = sum over plane products                         first product
+// resident: a wave keeps 32 RB of its items (rows of x, or classes) as B fragments in registers.  The other is streamed: tiles of
+// 32 of its items in LDS, a ring of four filled by LDS-DMA and shared by the four waves.  Per streamed tile:
+//     S (32 streamed x 32 RB resident) = bias + sum over plane products                  first product
 //     forward: the lane's running maximum and sum over the streamed classes
 //     backward: P = exp(S - lse) (times dloss where rows are streamed) - label, as fp16 planes: the accumulator registers
 //               8 t .. 8 t + 7 of a lane are the streamed items 16 t + 4 h + {0..3} and 16 t + 8 + 4 h + {0..3}, which is the
 //               B fragment of a product over 16 streamed items taken in that order
 //     D (EP x 32 RB) += streamed^T P, the A fragments read transposed (ds_read_b64_tr_b16) from the same tile in that order
+// The three run as a pipeline, one step a tile: S of tile i + 1, the exponentials of tile i and D of tile i - 1 do not depend on
+// each other.  A step is a fixed sequence of units, each the matrix instructions of one A fragment (read from LDS two units
+// ahead) with a piece of the exponentials, pinned by scheduling barriers: left to itself the compiler moves all LDS reads of a step to
+// its front and spills the resident fragments.  The labels of a tile are few and are put in behind its step: P is formed
+// again with the comparisons (a branch around two whole copies of the step costs 100 registers of copies where they meet).
 // MODE FWD and DX: rows resident, classes streamed; DW: classes resident, rows streamed.  gridDim.y parts of the streamed
 // operand leave partial results that are joined in order.
+// DX of a bf16 x (NR = 1), whose result is rounded to 8 bits, takes one plane of W in both products and one of P: a logit is then
+// 2^-12 of its terms off and a probability that much of itself.  Only the label's p - 1 could be smaller than that; it is
+// formed from the whole logit, a dot product of a lane with the two planes of its label's class in front of the loop.
 enum { MODE_FWD = 0, MODE_DX = 1, MODE_DW = 2 };
-constexpr int ST = 64;                              // streamed items of a tile
+constexpr int ST = 32;                              // streamed items of a tile
 
 struct XentStream {
     const f16_t *r[2], *s[2];
     const float *scales;
     const float *bias;                              // classes
-    const float *lse, *dl;                          // rows
+    const float2* row;                              // rows: lse, scaled dloss
     const int* lab;                                 // rows
-    int tiles;                                      // streamed tiles of 64
+    int tiles;                                      // streamed tiles
     float2* part;                                   // FWD: (maximum, sum) per part and row
     float* zlab;                                    // FWD
     float* out;                                     // DX: part x rows x EP; DW: part x EP x classes
     float* outb;                                    // DW: part x classes
     long ld;                                        // rows (FWD, DX) or classes (DW), padded
 };
+
+// compile-time unrolled loop: f(integral_constant<int, I>) for I in [I0, N)
+template <int I, int N, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        static_for<I + 1, N>(f);
+    }
+}
 
 template <int EP>
 __device__ __forceinline__ int swz_item(int row) {
@@ -458,37 +476,45 @@ __device__ __forceinline__ int swz_item(int row) {
 template <int EP, int NR, int NS, int RB, int MODE, int OCC>
 __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
-    constexpr int KS = EP / 16, EB = EP / 32, ROWB = EP * 2, SPLANE = ST * ROWB, INFO = 3 * ST * 4;
+    constexpr int KS = EP / 16, EB = EP / 32, ROWB = EP * 2, SPLANE = ST * ROWB;
     constexpr int BUF = NS * SPLANE + 1024;
     constexpr int NP = MODE == MODE_DW ? 2 : NR;    // planes of P: DX of a bf16 x needs one (its result is rounded to 8 bits)
     constexpr int NA = MODE == MODE_DW ? NS : NR;   // planes of the streamed operand in the second product
-    static_assert(INFO <= 1024, "");
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, h = lane >> 5;
-    const long item0 = ((long)blockIdx.x * 4 + wv) * (32 * RB);
+    const int item0 = (int)(blockIdx.x * 4 + wv) * (32 * RB);
     const int per = (g.tiles + gridDim.y - 1) / gridDim.y;
     const int t0 = blockIdx.y * per, t1 = t0 + per < g.tiles ? t0 + per : g.tiles;
 
-    auto stage = [&](int buf, int t) {
-        unsigned char* dst = lds + buf * BUF;
-        constexpr int RPI = 1024 / ROWB, PIECES = SPLANE / 1024;
+    // LDS-DMA of tile t: a wave fills 1 KB pieces (4 rows of 256 B), lane l the 16-byte place l of the piece with the chunk that
+    // belongs there.  A plane is under 4 GB: uniform offset of the piece plus the lane's.
+    static_assert(ROWB == 256, "a piece is four rows");
+    const __amdgpu_buffer_rsrc_t rs0 = __builtin_amdgcn_make_buffer_rsrc((void*)g.s[0], 0, 0xffffffffu, 0x00020000);
+    [[maybe_unused]] const __amdgpu_buffer_rsrc_t rs1 = __builtin_amdgcn_make_buffer_rsrc((void*)g.s[NS - 1], 0, 0xffffffffu, 0x00020000);
+    // beside the planes: FWD and DX the biases, DW (lse, dloss) and the labels of the tile's items
+    const void* ip = MODE != MODE_DW ? (const void*)g.bias : wv == 0 ? (const void*)g.row : (const void*)g.lab;
+    const __amdgpu_buffer_rsrc_t ri = __builtin_amdgcn_make_buffer_rsrc((void*)ip, 0, 0xffffffffu, 0x00020000);
+    const int lo0 = (lane >> 4) * ROWB + (((lane & 15) ^ ((lane >> 4) << 2)) << 4);
+    auto stage = [&](int t) {
+        unsigned char* dst = lds + (t & 3) * BUF;
+        constexpr int PIECES = SPLANE / 1024;
 #pragma unroll
         for (int pl = 0; pl < NS; ++pl)
 #pragma unroll
             for (int i = 0; i < PIECES / 4; ++i) {
-                const int piece = wv * (PIECES / 4) + i;
-                const int row = piece * RPI + lane / (64 / RPI), ch = (lane & (64 / RPI - 1)) ^ swz_item<EP>(row);
-                const f16_t* gp = g.s[pl] + ((long)t * ST + row) * EP + ch * 8;
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)gp,
-                                                 (__attribute__((address_space(3))) void*)(dst + pl * SPLANE + piece * 1024), 16, 0, 0);
+                const int piece = wv * (PIECES / 4) + i;                       // rows 4 piece ..: bits 2-3 of the row are piece & 3
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(pl == 0 ? rs0 : rs1, (__attribute__((address_space(3))) void*)(dst + pl * SPLANE + piece * 1024),
+                                                         16, lo0 ^ ((piece & 3) << 4), t * SPLANE + piece * 1024, 0, 0);
             }
-        const void* ip = MODE != MODE_DW ? (const void*)g.bias : wv == 0 ? (const void*)g.lse : wv == 1 ? (const void*)g.dl : (const void*)g.lab;
-        if (wv < (MODE == MODE_DW ? 3 : 1))
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((const float*)ip + (long)t * ST + lane),
-                                             (__attribute__((address_space(3))) void*)(dst + NS * SPLANE + wv * 256), 4, 0, 0);
+        if (wv < (MODE == MODE_DW ? 2 : 1)) {        // 64 floats, or 32 twice
+            const bool two = MODE == MODE_DW && wv == 0;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ri, (__attribute__((address_space(3))) void*)(dst + NS * SPLANE + wv * 256), 4,
+                                                     two ? lane * 4 : r * 4, t * (two ? ST * 8 : ST * 4), 0, 0);
+        }
     };
 
-    if (t0 < t1) stage(0, t0);
+    if (t0 < t1) stage(t0);
+    if (t0 + 1 < t1) stage(t0 + 1);
 
     // resident fragments: lane r's item, features 16 ks + 8 h .. + 7
     u32x4 fb[NR][RB][KS];
@@ -498,20 +524,34 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
         for (int b = 0; b < RB; ++b)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
-                fb[pl][b][ks] = *(const u32x4*)(g.r[pl] + (item0 + 32 * b + r) * EP + 16 * ks + 8 * h);
+                fb[pl][b][ks] = *(const u32x4*)(g.r[pl] + ((long)item0 + 32 * b + r) * EP + 16 * ks + 8 * h);
     const float unit = kLog2e / g.scales[0] / g.scales[1];
     float rinfo[RB];                                // DX: -(lse - 14); DW: bias
+    float plab[RB];                                 // DX, NR = 1: 2^14 (p - 1) of the label
     int rlab[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
         const long it = item0 + 32 * b + r;
-        rinfo[b] = MODE == MODE_DW ? g.bias[it] : MODE == MODE_DX ? 14.f - g.lse[it] : 0.f;
+        rinfo[b] = MODE == MODE_DW ? g.bias[it] : MODE == MODE_DX ? 14.f - g.row[it].x : 0.f;
         rlab[b] = MODE == MODE_DW ? 0 : g.lab[it];
+        if constexpr (MODE == MODE_DX && NR == 1) {
+            const long c = rlab[b] < 0 ? 0 : rlab[b];
+            float z = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const f16x8 xv = __builtin_bit_cast(f16x8, fb[0][b][ks]);
+                const f16x8 wh = *(const f16x8*)(g.s[0] + c * EP + 16 * ks + 8 * h), wl = *(const f16x8*)(g.s[1] + c * EP + 16 * ks + 8 * h);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) z = __builtin_fmaf((float)xv[k], (float)wl[k], __builtin_fmaf((float)xv[k], (float)wh[k], z));
+            }
+            z += __shfl_xor(z, 32, 64);
+            plab[b] = (__builtin_amdgcn_exp2f(__builtin_fmaf(z + g.bias[c], unit, rinfo[b] - 14.f)) - 1.f) * kDz;
+        }
     }
     // LDS offsets of the lane: the first fragment of its row, and the first transposed reads.  A row starts at a multiple of
     // its size and the swizzle is an XOR, so further fragments (feature blocks) are an XOR of 32 ks (64 eb) away.
     const int cb = (lane >> 4) & 1, qq = (lane >> 2) & 3, pp = lane & 3;
-    const int ao = r * ROWB + ((h ^ swz_item<EP>(r)) << 4);
+    int ao = r * ROWB + ((h ^ swz_item<EP>(r)) << 4);
     int to[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -531,130 +571,194 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
             for (int i = 0; i < 16; ++i) dacc[eb][b][i] = 0.f;
     }
 
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    int cur = 0;
-    for (int t = t0; t < t1; ++t) {
-        if (t + 1 < t1) stage(cur ^ 1, t + 1);
-        const unsigned char* base = lds + cur * BUF;
-        const unsigned char* info = base + NS * SPLANE;
-#pragma unroll 1
-        for (int ib = 0; ib < ST / 32; ++ib) {
-            const unsigned char* tile = base + ib * 32 * ROWB;
-            f32x16 acc[RB];                                         // starts at the classes' bias
+    // whether tile t holds a label of this wave's resident items (rows resident: a lane's own label; classes: the rows' labels)
+    auto labels_in = [&](int t) -> bool {
+        bool in = false;
+        if constexpr (MODE == MODE_DW) {
+            const int lb = *(const int*)(lds + (t & 3) * BUF + NS * SPLANE + 256 + r * 4);
+            in = lb >= item0 && lb < item0 + 32 * RB;
+        } else {
+#pragma unroll
+            for (int b = 0; b < RB; ++b) in = in || (unsigned)(rlab[b] - t * ST) < (unsigned)ST;
+        }
+        return __ballot(in) != 0;
+    };
+    // one barrier a step: tile i + 1 has landed for every wave, and none reads tile i - 2 any more, whose place tile i + 2 takes
+    auto arrive = [&](int i) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (i + 2 < t1) stage(i + 2);
+    };
+    // units of a step: NSU fragments of S (feature step, plane) and NGU of D (16 items, feature block, plane), evenly mixed with D first
+    constexpr int NSU = KS * NS, NGU = MODE == MODE_FWD ? 0 : 2 * EB * NA, NU = NSU + NGU;
+    constexpr int PB = MODE == MODE_FWD ? 9 : 8, NPIECE = PB * RB;         // pieces: pairs of values (FWD: the maximum first)
+    // PART 1: S only (in front of the first tile); 2: S and the exponentials; 3: all; 4: D only (behind the last tile)
+    auto step = [&](int i, f32x16 (&cur)[RB], f32x16 (&nxt)[RB], u32x4 (&fcur)[NP][RB][2], u32x4 (&fprev)[NP][RB][2], auto part) {
+        constexpr int PART = decltype(part)::value;
+        constexpr bool DO_S = PART != 4, DO_E = PART == 2 || PART == 3, DO_G = PART >= 3;
+        const unsigned char* ts = lds + ((i + 1) & 3) * BUF;
+        const unsigned char* te = lds + (i & 3) * BUF + NS * SPLANE;
+        const unsigned char* tg = lds + ((i - 1) & 3) * BUF;
+        asm volatile("" : "+v"(ao), "+v"(to[0]), "+v"(to[1]));      // keeps the 16 addresses derived from them out of registers
+        const int s0 = i * ST;
+        u32x4 fr[3];
+        f32x4 ri2[2];
+        float tsum[RB];                              // DW: the tile's sum of P, added to the running one once a tile
+#pragma unroll
+        for (int b = 0; b < RB; ++b) tsum[b] = 0.f;
+        auto load = [&](auto U_) {
+            constexpr int u = decltype(U_)::value;
+            if constexpr (u < NU) {
+                constexpr int gc = (u * NGU + NU - 1) / NU;
+                if constexpr (((u + 1) * NGU + NU - 1) / NU > gc) {
+                    constexpr int x = gc / (EB * NA), eb = gc % (EB * NA) / NA, pl = NA - 1 - gc % NA;
+                    if constexpr (DO_G) {
+                        const unsigned char* tp = tg + pl * SPLANE + x * 16 * ROWB;
+                        const u32x2 a0 = tr_read(tp + (to[0] ^ (eb << 6))), a1 = tr_read(tp + (to[1] ^ (eb << 6)));
+                        fr[u % 3] = (u32x4){a0[0], a0[1], a1[0], a1[1]};
+                    }
+                } else if constexpr (DO_S) {
+                    constexpr int si = u - gc, ks = si / NS, pl = NS - 1 - si % NS;
+                    fr[u % 3] = *(const u32x4*)(ts + pl * SPLANE + (ao ^ (ks << 5)));
+                }
+            }
+        };
+        auto products = [&](auto U_) {
+            constexpr int u = decltype(U_)::value, gc = (u * NGU + NU - 1) / NU;
+            if constexpr (((u + 1) * NGU + NU - 1) / NU > gc) {
+                constexpr int x = gc / (EB * NA), eb = gc % (EB * NA) / NA, pl = NA - 1 - gc % NA;
+                if constexpr (DO_G) {
+#pragma unroll
+                    for (int b = 0; b < RB; ++b) {
+                        if constexpr (NP > 1 && pl == 0) dacc[eb][b] = mfma_f16(fr[u % 3], fprev[NP - 1][b][x], dacc[eb][b]);
+                        dacc[eb][b] = mfma_f16(fr[u % 3], fprev[0][b][x], dacc[eb][b]);
+                    }
+                }
+            } else if constexpr (DO_S) {
+                constexpr int si = u - gc, ks = si / NS, pl = NS - 1 - si % NS;
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    if constexpr (NR > 1 && pl == 0) nxt[b] = mfma_f16(fr[u % 3], fb[NR - 1][b][ks], nxt[b]);
+                    nxt[b] = mfma_f16(fr[u % 3], fb[0][b][ks], nxt[b]);
+                }
+            }
+        };
+        // pair j of P as fp16 planes
+        auto put = [&](auto P_, float v0, float v1) {
+            constexpr int p = decltype(P_)::value, b = p / 8, j = p % 8;
+            const f16x2 h2 = __builtin_convertvector((f32x2){v0, v1}, f16x2);
+            fcur[0][b][j >> 2][j & 3] = __builtin_bit_cast(unsigned, h2);
+            if constexpr (NP > 1) fcur[NP - 1][b][j >> 2][j & 3] = f16_pack(v0 - (float)h2[0], v1 - (float)h2[1]);
+        };
+        // (lse, dloss) of the two streamed rows of pair j
+        auto row2 = [&](int j) { return *(const f32x4*)(te + (8 * (j >> 1) + 4 * h + 2 * (j & 1)) * 8); };
+        auto piece = [&](auto P_) {
+            constexpr int p = decltype(P_)::value, b = p / PB, j = p % PB - (PB - 8);
+            if constexpr (MODE == MODE_FWD && j < 0) {
+                float mm = m[b];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) mm = fmaxf(mm, cur[b][k]);
+                ssum[b] *= __builtin_amdgcn_exp2f((m[b] - mm) * unit);
+                m[b] = mm;
+            } else if constexpr (MODE == MODE_FWD) {
+                const float off = -m[b] * unit;
+#pragma unroll
+                for (int k = 2 * j; k < 2 * j + 2; ++k) ssum[b] += __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k], unit, off));
+            } else if constexpr (MODE == MODE_DX) {
+                put(P_, __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j], unit, rinfo[b])),
+                    __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j + 1], unit, rinfo[b])));
+            } else {
+                const f32x4 q = ri2[j & 1];
+                const float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j], unit, -q[0])) * q[1];
+                const float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j + 1], unit, -q[2])) * q[3];
+                tsum[b] += v0 + v1;
+                if constexpr (b == RB - 1 && j + 2 < 8) ri2[j & 1] = row2(j + 2);
+                put(P_, v0, v1);
+            }
+        };
+        // the labels of tile i: FWD keeps their logits, DX and DW form P again
+        auto label_piece = [&](auto P_) {
+            constexpr int p = decltype(P_)::value, b = p / 8, j = p % 8, k = 2 * j, c0 = (k & 3) + 8 * (k >> 2);
+            if constexpr (MODE == MODE_FWD) {
+                const int rel = rlab[b] - s0 - 4 * h;
+                if (rel == c0) g.zlab[item0 + 32 * b + r] = cur[b][k] * unit;
+                if (rel == c0 + 1) g.zlab[item0 + 32 * b + r] = cur[b][k + 1] * unit;
+            } else if constexpr (MODE == MODE_DX) {
+                const int rel = rlab[b] - s0 - 4 * h;
+                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k], unit, rinfo[b]));
+                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k + 1], unit, rinfo[b]));
+                put(P_, rel == c0 ? (NR == 1 ? plab[b] : e0 - kDz) : e0, rel == c0 + 1 ? (NR == 1 ? plab[b] : e1 - kDz) : e1);
+            } else {
+                const f32x4 q = row2(j);
+                const u32x2 lb = *(const u32x2*)(te + 256 + (c0 + 4 * h) * 4);
+                const float d0 = (int)lb[0] - item0 - 32 * b == r ? q[1] : 0.f, d1 = (int)lb[1] - item0 - 32 * b == r ? q[3] : 0.f;
+                tsum[b] -= d0 + d1;
+                // (p - 1) dloss, as one fma each: p dloss would have lost the digits of a p next to 1
+                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k], unit, -q[0]));
+                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k + 1], unit, -q[2]));
+                put(P_, __builtin_fmaf(e0, q[1], -d0), __builtin_fmaf(e1, q[3], -d1));
+            }
+        };
+        if constexpr (DO_S) {                        // S starts at the biases
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 f32x4 bv;
-                if constexpr (MODE != MODE_DW) bv = *(const f32x4*)(info + (ib * 32 + 8 * q + 4 * h) * 4);
+                if constexpr (MODE != MODE_DW) bv = *(const f32x4*)(ts + NS * SPLANE + (8 * q + 4 * h) * 4);
 #pragma unroll
                 for (int b = 0; b < RB; ++b)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[b][4 * q + k] = MODE == MODE_DW ? rinfo[b] : bv[k];
-            }
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                for (int pl = NS - 1; pl >= 0; --pl) {
-                    const u32x4 fa = *(const u32x4*)(tile + pl * SPLANE + (ao ^ (ks << 5)));
-#pragma unroll
-                    for (int b = 0; b < RB; ++b) {
-                        if (NR > 1 && pl == 0) acc[b] = mfma_f16(fa, fb[NR - 1][b][ks], acc[b]);
-                        acc[b] = mfma_f16(fa, fb[0][b][ks], acc[b]);
-                    }
-                }
-            const long s0 = (long)t * ST + ib * 32;                 // first streamed item of the block
-            if constexpr (MODE == MODE_FWD) {
-#pragma unroll
-                for (int b = 0; b < RB; ++b) {
-                    float mm = m[b];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) mm = fmaxf(mm, acc[b][i]);
-                    float s = ssum[b] * __builtin_amdgcn_exp2f((m[b] - mm) * unit);
-                    const float off = -mm * unit;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][i], unit, off));
-                    ssum[b] = s;
-                    m[b] = mm;
-                    const long rel = rlab[b] - s0;
-                    if (rlab[b] >= 0 && rel >= 0 && rel < 32) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if ((i & 3) + 8 * (i >> 2) + 4 * h == rel) g.zlab[item0 + 32 * b + r] = acc[b][i] * unit;
-                    }
-                }
-            } else {
-                u32x4 fp[NP][RB][2];
-                if constexpr (MODE == MODE_DX) {
-#pragma unroll
-                    for (int b = 0; b < RB; ++b) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][i], unit, rinfo[b]));
-                        const long rel = rlab[b] - s0;
-                        if (rlab[b] >= 0 && rel >= 0 && rel < 32) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if ((i & 3) + 8 * (i >> 2) + 4 * h == rel) acc[b][i] -= kDz;
-                        }
-                    }
-                } else {
-                    const int lab32 = *(const int*)(info + 512 + (ib * 32 + r) * 4);
-                    const bool any = __ballot(lab32 >= item0 && lab32 < item0 + 32 * RB) != 0;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const f32x4 ls = *(const f32x4*)(info + (ib * 32 + 8 * q + 4 * h) * 4);
-                        const f32x4 dl = *(const f32x4*)(info + 256 + (ib * 32 + 8 * q + 4 * h) * 4);
-#pragma unroll
-                        for (int b = 0; b < RB; ++b)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                acc[b][4 * q + k] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[b][4 * q + k], unit, -ls[k]));
-                        if (any) {
-                            const u32x4 lb = *(const u32x4*)(info + 512 + (ib * 32 + 8 * q + 4 * h) * 4);
-#pragma unroll
-                            for (int b = 0; b < RB; ++b)
-#pragma unroll
-                                for (int k = 0; k < 4; ++k)
-                                    if ((int)lb[k] - (int)item0 - 32 * b == r) acc[b][4 * q + k] -= 1.f;
-                        }
-#pragma unroll
-                        for (int b = 0; b < RB; ++b)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                acc[b][4 * q + k] *= dl[k] * kDz;
-                                ssum[b] += acc[b][4 * q + k];
-                            }
-                    }
-                }
-#pragma unroll
-                for (int b = 0; b < RB; ++b)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        float v[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) v[k] = acc[b][8 * x + k];
-                        if constexpr (NP > 1) split8(v, fp[0][b][x], fp[NP - 1][b][x]);
-                        else fp[0][b][x] = (u32x4){f16_pack(v[0], v[1]), f16_pack(v[2], v[3]), f16_pack(v[4], v[5]), f16_pack(v[6], v[7])};
-                    }
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int eb = 0; eb < EB; ++eb)
-#pragma unroll
-                        for (int pl = NA - 1; pl >= 0; --pl) {
-                            const unsigned char* tp = tile + pl * SPLANE + x * 16 * ROWB;
-                            const u32x2 a0 = tr_read(tp + (to[0] ^ (eb << 6))), a1 = tr_read(tp + (to[1] ^ (eb << 6)));
-                            const u32x4 fa = {a0[0], a0[1], a1[0], a1[1]};
-#pragma unroll
-                            for (int b = 0; b < RB; ++b) {
-                                if (NP > 1 && pl == 0) dacc[eb][b] = mfma_f16(fa, fp[NP - 1][b][x], dacc[eb][b]);
-                                dacc[eb][b] = mfma_f16(fa, fp[0][b][x], dacc[eb][b]);
-                            }
-                        }
+                    for (int k = 0; k < 4; ++k) nxt[b][4 * q + k] = MODE == MODE_DW ? rinfo[b] : bv[k];
             }
         }
+        if constexpr (DO_E && MODE == MODE_DW) {
+            ri2[0] = row2(0);
+            ri2[1] = row2(1);
+        }
+        load(std::integral_constant<int, 0>{});
+        load(std::integral_constant<int, 1>{});
+        static_for<0, NU>([&](auto U_) {
+            constexpr int u = decltype(U_)::value;
+            load(std::integral_constant<int, u + 2>{});
+            products(U_);
+            if constexpr (DO_E) static_for<u * NPIECE / NU, (u + 1) * NPIECE / NU>(piece);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        if constexpr (DO_E) {
+            if (labels_in(i)) static_for<0, 8 * RB>(label_piece);
+            if constexpr (MODE == MODE_DW) {
+#pragma unroll
+                for (int b = 0; b < RB; ++b) ssum[b] += tsum[b];
+            }
+        }
+    };
+    using P1 = std::integral_constant<int, 1>;
+    using P2 = std::integral_constant<int, 2>;
+    using P3 = std::integral_constant<int, 3>;
+    using P4 = std::integral_constant<int, 4>;
+
+    if (t0 < t1) {
+        f32x16 a0[RB], a1[RB];
+        u32x4 p0[NP][RB][2], p1[NP][RB][2];
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        cur ^= 1;
+        step(t0 - 1, a1, a0, p1, p0, P1{});
+        // the S of a step past the last tile works on a stale buffer and is not used
+        auto full = [&](int i, f32x16 (&cur)[RB], f32x16 (&nxt)[RB], u32x4 (&fcur)[NP][RB][2], u32x4 (&fprev)[NP][RB][2], auto part) {
+            arrive(i);
+            step(i, cur, nxt, fcur, fprev, part);
+        };
+        full(t0, a0, a1, p0, p1, P2{});
+        int i = t0 + 1;
+        for (; i + 1 < t1; i += 2) {
+            full(i, a1, a0, p1, p0, P3{});
+            full(i + 1, a0, a1, p0, p1, P3{});
+        }
+        if (i < t1) {
+            full(i, a1, a0, p1, p0, P3{});
+            step(i + 1, a0, a1, p0, p1, P4{});
+        } else {
+            step(i, a1, a0, p1, p0, P4{});
+        }
     }
 
 #pragma unroll
@@ -687,9 +791,9 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
 
 // dx from the parts of the streamed product, in order
 __global__ __launch_bounds__(256) void xent_dx_join_kernel(const float* __restrict__ parts, const float* __restrict__ scales,
-                                                           const float* __restrict__ dl, void* __restrict__ dx, int dx_f32, int np,
+                                                           const float2* __restrict__ rowinfo, void* __restrict__ dx, int dx_f32, int np,
                                                            long part, long n, int e, int ep) {
-    const float f = scales[2] / kDz / scales[0];
+    const float f = scales[2] / kDz / scales[0];             // dl holds 2^14 dloss / scales[2], the product 2^14 dz / dloss
     const long total = n * ep;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
         const long row = i / ep;
@@ -697,7 +801,7 @@ __global__ __launch_bounds__(256) void xent_dx_join_kernel(const float* __restri
         if (c >= e) continue;
         float s = 0.f;
         for (int p = 0; p < np; ++p) s += parts[p * part + i];
-        s *= f * dl[row];
+        s *= f * (rowinfo[row].y / kDz);
         if (dx_f32) ((float*)dx)[row * e + c] = s;
         else ((bf16_t*)dx)[row * e + c] = (bf16_t)s;
     }
@@ -771,7 +875,7 @@ struct Layout {
     bool narrow;                   // the streamed kernels
     int rows_wg;                   // resident rows of a workgroup (FWD, DX)
     int64_t np, vp, ep, vc, nz, nf, nx;      // nf, nx, nz: parts of the streamed operand in FWD, DX, DW (nz: of the rows in general)
-    int64_t part, bias, scales, lab, zlab, lse, dl, xh, xl, wh, wl, slices, dzh, dzl, dxw, slabs, slabs_b, total;
+    int64_t part, bias, scales, lab, zlab, row, xh, xl, wh, wl, slices, dzh, dzl, dxw, slabs, slabs_b, total;
 };
 
 Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
@@ -781,15 +885,24 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
     l.np = up(n, l.rows_wg);
     l.vp = up(v, 128);
     l.ep = up(e, 128);
-    // two workgroups a CU where there is enough to split, four tiles of 64 a part at least
-    auto split = [](int64_t wgs, int64_t tiles) {
-        int64_t p = 512 / wgs;
-        if (p > tiles / 4) p = tiles / 4;
-        return p < 1 ? (int64_t)1 : p;
+    // Parts of the streamed operand: the number that wastes least of the last round of workgroups (`slots` run at once), with
+    // eight tiles a part at least and 2 % for each part's start and its share of the join.
+    auto split = [](int64_t wgs, int64_t tiles, int64_t slots) {
+        int64_t best = 1;
+        double least = 1e30;
+        for (int64_t p = 1; p <= 32 && (p == 1 || tiles / p >= 8); ++p) {
+            const double t = (double)((wgs * p + slots - 1) / slots) / (double)p * (1.0 + 0.02 * (double)p);
+            if (t < least) {
+                least = t;
+                best = p;
+            }
+        }
+        return best;
     };
     if (l.narrow) {
-        l.nf = l.nx = split(l.np / l.rows_wg, l.vp / ST);
-        l.nz = split(l.vp / 128, l.np / ST);
+        l.nf = split(l.np / l.rows_wg, l.vp / ST, 512);
+        l.nx = split(l.np / l.rows_wg, l.vp / ST, xf32 ? 512 : 256);
+        l.nz = split(l.vp / 128, l.np / ST, 512);
     }
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -810,15 +923,13 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
         if (!l.narrow) l.nf = l.vp / 64;
         l.slices = take(l.np * l.nf * 8);
     } else if (l.narrow) {
-        l.lse = take(l.np * 4);
-        l.dl = take(l.np * 4);
+        l.row = take(l.np * 8);
         l.vc = l.vp;
         l.dxw = take(l.nx * l.np * l.ep * 4);
         l.slabs = take(l.nz * l.ep * l.vp * 4);
         l.slabs_b = take(l.nz * l.vp * 4);
     } else {
-        l.lse = take(l.np * 4);
-        l.dl = take(l.np * 4);
+        l.row = take(l.np * 8);
         // a piece of the classes: dz planes of about 128 MB, which the 256 MB last-level cache holds
         l.vc = (int64_t)(128 << 20) / (4 * l.np) / 128 * 128;
         if (l.vc < 128) l.vc = 128;
@@ -849,12 +960,12 @@ void launch_gemm(const XentGemm& g, dim3 grid, hipStream_t st) {
     hipLaunchKernelGGL((xent_gemm_kernel<NA, NB, AT, BT, EPI>), grid, dim3(256), bytes, st, g);
 }
 
-template <int NR, int NS, int RB, int MODE>
+template <int NR, int NS, int RB, int MODE, int OCC>
 void launch_stream(const XentStream& g, int64_t wgs, int64_t parts, hipStream_t st) {
     static std::atomic<uint64_t> done{0};
-    constexpr int bytes = 2 * (NS * ST * 256 + 1024);
-    mgx_allow_dynamic_lds(xent_stream_kernel<128, NR, NS, RB, MODE, 2>, bytes, done);
-    hipLaunchKernelGGL((xent_stream_kernel<128, NR, NS, RB, MODE, 2>), dim3((unsigned)wgs, (unsigned)parts), dim3(256), bytes, st, g);
+    constexpr int bytes = 4 * (NS * ST * 256 + 1024);
+    mgx_allow_dynamic_lds(xent_stream_kernel<128, NR, NS, RB, MODE, OCC>, bytes, done);
+    hipLaunchKernelGGL((xent_stream_kernel<128, NR, NS, RB, MODE, OCC>), dim3((unsigned)wgs, (unsigned)parts), dim3(256), bytes, st, g);
 }
 
 void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const float* w, const float* b, const int* labels,
@@ -872,7 +983,7 @@ void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const floa
     p.n = n; p.v = v; p.np = l.np; p.vp = l.vp; p.e = (int)e; p.ep = (int)l.ep;
     p.xh = (f16_t*)(ws + l.xh); p.xl = (f16_t*)(ws + l.xl); p.wh = (f16_t*)(ws + l.wh); p.wl = (f16_t*)(ws + l.wl);
     p.bias = (float*)(ws + l.bias); p.scales = (float*)(ws + l.scales); p.lab = (int*)(ws + l.lab);
-    p.lsep = dloss ? (float*)(ws + l.lse) : nullptr; p.dlp = dloss ? (float*)(ws + l.dl) : nullptr;
+    p.row = dloss ? (float2*)(ws + l.row) : nullptr;
     p.wtiles = (l.vp / 64) * (l.ep / 64);
     p.xblocks = up(l.np * l.ep / 8, 256) / 256;
     if (p.xblocks > 2048) p.xblocks = 2048;
@@ -912,8 +1023,8 @@ extern "C" int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, c
         q.r[0] = g.b[0]; q.r[1] = g.b[1]; q.s[0] = g.a[0]; q.s[1] = g.a[1];
         q.scales = g.scales; q.bias = g.bias; q.lab = g.lab; q.tiles = (int)(l.vp / ST);
         q.part = g.part; q.zlab = g.zlab; q.ld = l.np;
-        if (xf) launch_stream<2, 2, 1, MODE_FWD>(q, l.np / l.rows_wg, l.nf, st);
-        else launch_stream<1, 2, 2, MODE_FWD>(q, l.np / l.rows_wg, l.nf, st);
+        if (xf) launch_stream<2, 2, 1, MODE_FWD, 2>(q, l.np / l.rows_wg, l.nf, st);
+        else launch_stream<1, 2, 2, MODE_FWD, 2>(q, l.np / l.rows_wg, l.nf, st);
     } else if (xf) {
         launch_gemm<2, 2, false, false, EPI_FWD>(g, grid, st);
     } else {
@@ -945,22 +1056,22 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
     if (l.narrow) {
         XentStream q = {};
         q.scales = (float*)(ws + l.scales); q.bias = (float*)(ws + l.bias); q.lab = (int*)(ws + l.lab);
-        q.lse = (float*)(ws + l.lse); q.dl = (float*)(ws + l.dl);
+        q.row = (float2*)(ws + l.row);
         f16_t *wh = (f16_t*)(ws + l.wh), *wl = (f16_t*)(ws + l.wl);
         if (dx) {
             q.r[0] = xh; q.r[1] = xl; q.s[0] = wh; q.s[1] = wl;
             q.tiles = (int)(l.vp / ST); q.out = (float*)(ws + l.dxw); q.ld = l.np;
-            if (xf) launch_stream<2, 2, 1, MODE_DX>(q, l.np / l.rows_wg, l.nx, st);
-            else launch_stream<1, 2, 2, MODE_DX>(q, l.np / l.rows_wg, l.nx, st);
+            if (xf) launch_stream<2, 2, 1, MODE_DX, 2>(q, l.np / l.rows_wg, l.nx, st);
+            else launch_stream<1, 1, 2, MODE_DX, 1>(q, l.np / l.rows_wg, l.nx, st);
             const int64_t blocks = up(n * l.ep, 256) / 256;
             hipLaunchKernelGGL(xent_dx_join_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, q.out, q.scales,
-                               q.dl, dx, (int)xf, (int)l.nx, (long)(l.np * l.ep), (long)n, (int)e, (int)l.ep);
+                               q.row, dx, (int)xf, (int)l.nx, (long)(l.np * l.ep), (long)n, (int)e, (int)l.ep);
         }
         if (dw || db) {
             q.r[0] = wh; q.r[1] = wl; q.s[0] = xh; q.s[1] = xl;
             q.tiles = (int)(l.np / ST); q.out = (float*)(ws + l.slabs); q.outb = (float*)(ws + l.slabs_b); q.ld = l.vp;
-            if (xf) launch_stream<2, 2, 1, MODE_DW>(q, l.vp / 128, l.nz, st);
-            else launch_stream<2, 1, 1, MODE_DW>(q, l.vp / 128, l.nz, st);
+            if (xf) launch_stream<2, 2, 1, MODE_DW, 2>(q, l.vp / 128, l.nz, st);
+            else launch_stream<2, 1, 1, MODE_DW, 2>(q, l.vp / 128, l.nz, st);
             hipLaunchKernelGGL(xent_dw_reduce_kernel, dim3((unsigned)(up(l.vp, 256) / 256), (unsigned)(e + 1)), dim3(256), 0, st,
                                q.out, q.outb, q.scales, dw, db, (int)l.nz, (long)(l.ep * l.vp), (long)l.vp, (int)e, (long)v, 0L,
                                accumulate);
@@ -974,7 +1085,7 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
         g.scales = (float*)(ws + l.scales);
         g.a[0] = wh; g.a[1] = wl; g.b[0] = xh; g.b[1] = xl;
         g.lda = g.ldb = l.ep; g.kiters = (int)(l.ep / BK);
-        g.bias = (float*)(ws + l.bias) + c0; g.lab = (int*)(ws + l.lab); g.lse = (float*)(ws + l.lse); g.dl = (float*)(ws + l.dl);
+        g.bias = (float*)(ws + l.bias) + c0; g.lab = (int*)(ws + l.lab); g.row = (float2*)(ws + l.row);
         g.dzh = dzh; g.dzl = dzl; g.ldo = l.vc; g.np = l.np; g.class0 = c0;
         const dim3 grid((unsigned)(cnt / 128), (unsigned)(l.np / 128));
         if (xf) launch_gemm<2, 2, false, false, EPI_DZ>(g, grid, st);
