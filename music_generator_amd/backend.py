@@ -55,7 +55,7 @@ def device() -> torch.device:
 
 
 def stream_ptr() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())      # current_stream().cuda_stream without the objects
 
 
 class Variable:

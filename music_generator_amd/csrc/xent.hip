@@ -863,6 +863,206 @@ __global__ __launch_bounds__(256) void xent_dw_reduce_kernel(const float* __rest
     }
 }
 
+// ---------------------------------------------------------------- few rows
+// Up to 16 rows the kernel W is what the call reads and dW what it writes: float32 on the vector ALU, no planes, two launches a
+// direction.  A workgroup takes 64 classes (a lane each, so a wave reads 256 consecutive bytes of a row of W), its four
+// waves a quarter of the features each.  RT: rows rounded up, accumulators of a lane.
+constexpr int FEW = 16, RC = 256;                   // RC: features staged at a time
+
+struct XentRows {
+    const void* x;
+    const float *w, *b, *lse, *dloss;
+    const int* labels;
+    float2* part;                                   // forward: (maximum, sum) per 64 classes and row
+    float* zlab;
+    float *dxp, *dw, *db;                           // backward: dx per 64 classes, row and feature; gradients
+    long v;
+    int n, e, accumulate;
+};
+
+// xs[RT][RC]: features e0 .. of the rows that have a label, zeros elsewhere
+template <int RT, bool XF32>
+__device__ __forceinline__ void xent_rows_stage(const XentRows& g, float* xs, int e0, int cnt) {
+    for (int k = threadIdx.x; k < RT * RC; k += 256) {
+        const int i = k / RC, c = k - i * RC;
+        float v = 0.f;
+        if (i < g.n && c < cnt) {
+            const int lab = g.labels[i];
+            const long at = (long)i * g.e + e0 + c;
+            if (lab >= 0 && lab < g.v) v = XF32 ? ((const float*)g.x)[at] : (float)((const bf16_t*)g.x)[at];
+        }
+        xs[k] = v;
+    }
+}
+
+// zs[RT][64]: the logits of the workgroup's classes in units of log 2
+template <int RT, bool XF32>
+__device__ __forceinline__ void xent_rows_logits(const XentRows& g, float* xs, float* red, float* zs) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const long c = (long)blockIdx.x * 64 + lane;
+    const bool ok = c < g.v;
+    float z[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) z[i] = 0.f;
+    for (int e0 = 0; e0 < g.e; e0 += RC) {
+        const int cnt = g.e - e0 < RC ? g.e - e0 : RC;
+        __syncthreads();
+        xent_rows_stage<RT, XF32>(g, xs, e0, cnt);
+        __syncthreads();
+        const int per = (cnt + 3) / 4, k1 = (wv + 1) * per < cnt ? (wv + 1) * per : cnt;
+        for (int k = wv * per; k < k1; k += 16) {
+            float w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = ok && k + j < k1 ? g.w[(long)(e0 + k + j) * g.v + c] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int at = k + j < RC ? k + j : RC - 1;
+#pragma unroll
+                for (int i = 0; i < RT; ++i) z[i] = __builtin_fmaf(w[j], xs[i * RC + at], z[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) red[(wv * RT + i) * 64 + lane] = z[i];
+    __syncthreads();
+    const float b = ok ? (g.b ? g.b[c] : 0.f) : -__builtin_inff();
+    for (int i = wv; i < RT; i += 4) {
+        const float s = (red[i * 64 + lane] + red[(RT + i) * 64 + lane]) + (red[(2 * RT + i) * 64 + lane] + red[(3 * RT + i) * 64 + lane]);
+        const float t = (s + b) * kLog2e;
+        zs[i * 64 + lane] = s + b >= kLowest ? fmaxf(t, kLowest) : t;
+    }
+}
+
+template <int RT, bool XF32>
+__global__ __launch_bounds__(256) void xent_rows_fwd_kernel(XentRows g) {
+    __shared__ float xs[RT * RC], red[4 * RT * 64], zs[RT * 64];
+    xent_rows_logits<RT, XF32>(g, xs, red, zs);
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    for (int i = wv; i < g.n; i += 4) {             // the wave that wrote row i of zs
+        const float z = zs[i * 64 + lane];
+        float m = fmaxf(z, kLowest);
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+        float s = __builtin_amdgcn_exp2f(z - m);
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+        if (lane == 0) g.part[(long)blockIdx.x * g.n + i] = make_float2(m, s);
+        if ((long)blockIdx.x * 64 + lane == g.labels[i] && g.labels[i] < g.v) g.zlab[i] = z;
+    }
+}
+
+// one row per workgroup of 64: its parts, a lane every 64th, then across the lanes
+__global__ __launch_bounds__(64) void xent_rows_join_kernel(XentRows g, float* __restrict__ loss, float* __restrict__ lse,
+                                                            int* __restrict__ hits, long parts) {
+    const int i = blockIdx.x, lane = threadIdx.x;
+    float m = kLowest, s = 0.f;
+    auto join = [&](float pm, float ps) {
+        const float mm = fmaxf(m, pm);
+        s = s * __builtin_amdgcn_exp2f(m - mm) + ps * __builtin_amdgcn_exp2f(pm - mm);
+        m = mm;
+    };
+    for (long p = lane; p < parts; p += 64) {
+        const float2 q = g.part[p * g.n + i];
+        join(q.x, q.y);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) join(__shfl_xor(m, off, 64), __shfl_xor(s, off, 64));
+    if (lane == 0) {
+        const int lab = g.labels[i];
+        const bool ok = lab >= 0 && lab < g.v;
+        const float z = ok ? g.zlab[i] : 0.f, ls = __builtin_amdgcn_logf(s);
+        loss[i] = ok ? ((m - z) + ls) * kLn2 : 0.f;
+        lse[i] = ok ? (m + ls) * kLn2 : 0.f;
+        if (hits) hits[i] = ok && z >= m ? 1 : 0;
+    }
+}
+
+template <int RT, bool XF32>
+__global__ __launch_bounds__(256) void xent_rows_bwd_kernel(XentRows g) {
+    __shared__ float xs[RT * RC], red[4 * RT * 64], zs[RT * 64], wt[64][65];
+    xent_rows_logits<RT, XF32>(g, xs, red, zs);
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const long c = (long)blockIdx.x * 64 + lane;
+    __syncthreads();
+    for (int k = tid; k < RT * 64; k += 256) {      // zs becomes dz
+        const int i = k >> 6;
+        const int lab = i < g.n ? g.labels[i] : -1;
+        float d = 0.f;
+        if (lab >= 0 && lab < g.v) {
+            const float p = __builtin_amdgcn_exp2f(zs[k] - g.lse[i] * kLog2e);
+            d = ((long)blockIdx.x * 64 + (k & 63) == lab ? p - 1.f : p) * g.dloss[i];
+        }
+        zs[k] = d;
+    }
+    __syncthreads();
+    if (g.db && wv == 0 && c < g.v) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) s += zs[i * 64 + lane];
+        g.db[c] = g.accumulate ? g.db[c] + s : s;
+    }
+    for (int e0 = 0; e0 < g.e; e0 += RC) {
+        const int cnt = g.e - e0 < RC ? g.e - e0 : RC;
+        if (g.e > RC) {                             // otherwise the stage of the logits is still there
+            __syncthreads();
+            xent_rows_stage<RT, XF32>(g, xs, e0, cnt);
+            __syncthreads();
+        }
+        if (g.dw && c < g.v) {
+            for (int k = wv; k < cnt; k += 4) {
+                float s = 0.f;
+#pragma unroll
+                for (int i = 0; i < RT; ++i) s = __builtin_fmaf(xs[i * RC + k], zs[i * 64 + lane], s);
+                float* d = g.dw + (long)(e0 + k) * g.v + c;
+                *d = g.accumulate ? *d + s : s;
+            }
+        }
+        if (g.dxp) {
+            for (int k0 = 0; k0 < cnt; k0 += 64) {
+                __syncthreads();
+                for (int k = wv; k < 64; k += 4)
+                    wt[k][lane] = k0 + k < cnt && c < g.v ? g.w[(long)(e0 + k0 + k) * g.v + c] : 0.f;
+                __syncthreads();
+                const int k = tid >> 2, q = tid & 3;
+                float s[RT];
+#pragma unroll
+                for (int i = 0; i < RT; ++i) s[i] = 0.f;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float w = wt[k][4 * j + q];
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) s[i] = __builtin_fmaf(w, zs[i * 64 + 4 * j + q], s[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    s[i] += __shfl_xor(s[i], 1, 64);
+                    s[i] += __shfl_xor(s[i], 2, 64);
+                    if (q == 0 && i < g.n && k0 + k < cnt) g.dxp[((long)blockIdx.x * g.n + i) * g.e + e0 + k0 + k] = s[i];
+                }
+            }
+        }
+    }
+}
+
+// dx of 64 consecutive values per workgroup: 16 groups of parts, then the groups in order
+__global__ __launch_bounds__(1024) void xent_rows_dx_kernel(const float* __restrict__ dxp, void* __restrict__ dx, int dx_f32, long total,
+                                                            long parts) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
+    const long i = (long)blockIdx.x * 64 + lane;
+    float s = 0.f;
+    if (i < total)
+        for (long p = q; p < parts; p += 16) s += dxp[p * total + i];
+    red[q][lane] = s;
+    __syncthreads();
+    if (q == 0 && i < total) {
+#pragma unroll
+        for (int k = 1; k < 16; ++k) s += red[k][lane];
+        if (dx_f32) ((float*)dx)[i] = s;
+        else ((bf16_t*)dx)[i] = (bf16_t)s;
+    }
+}
+
 __global__ __launch_bounds__(256) void xent_zero_kernel(float* __restrict__ a, long na, float* __restrict__ b, long nb) {
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < na || i < nb; i += (long)gridDim.x * 256) {
         if (i < na) a[i] = 0.f;
@@ -871,6 +1071,35 @@ __global__ __launch_bounds__(256) void xent_zero_kernel(float* __restrict__ a, l
 }
 
 // ---------------------------------------------------------------- host
+template <bool XF32>
+int few_forward(const XentRows& g, float* loss, float* lse, int* hits, hipStream_t st) {
+    const dim3 grid((unsigned)(up(g.v, 64) / 64)), block(256);
+    if (g.n == 1) hipLaunchKernelGGL((xent_rows_fwd_kernel<1, XF32>), grid, block, 0, st, g);
+    else if (g.n <= 4) hipLaunchKernelGGL((xent_rows_fwd_kernel<4, XF32>), grid, block, 0, st, g);
+    else hipLaunchKernelGGL((xent_rows_fwd_kernel<16, XF32>), grid, block, 0, st, g);
+    hipLaunchKernelGGL(xent_rows_join_kernel, dim3((unsigned)g.n), dim3(64), 0, st, g, loss, lse, hits, (long)grid.x);
+    return mgx_launch_status();
+}
+
+template <bool XF32>
+int few_backward(const XentRows& g, void* dx, hipStream_t st) {
+    const dim3 grid((unsigned)(up(g.v, 64) / 64)), block(256);
+    if (g.n == 1) hipLaunchKernelGGL((xent_rows_bwd_kernel<1, XF32>), grid, block, 0, st, g);
+    else if (g.n <= 4) hipLaunchKernelGGL((xent_rows_bwd_kernel<4, XF32>), grid, block, 0, st, g);
+    else hipLaunchKernelGGL((xent_rows_bwd_kernel<16, XF32>), grid, block, 0, st, g);
+    const long total = (long)g.n * g.e;
+    if (dx)
+        hipLaunchKernelGGL(xent_rows_dx_kernel, dim3((unsigned)(up(total, 64) / 64)), dim3(1024), 0, st, g.dxp, dx, (int)XF32, total,
+                           (long)grid.x);
+    return mgx_launch_status();
+}
+
+// workspace of the few-rows form: parts and label logits, or the parts of dx
+int64_t few_bytes(int64_t n, int64_t e, int64_t v, bool backward) {
+    const int64_t parts = up(v, 64) / 64;
+    return backward ? parts * n * e * 4 : up(parts * n * 8, 16) + n * 4;
+}
+
 struct Layout {
     bool narrow;                   // the streamed kernels
     int rows_wg;                   // resident rows of a workgroup (FWD, DX)
@@ -996,6 +1225,7 @@ void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const floa
 
 extern "C" int64_t mgx_dense_xent_workspace(int64_t n, int64_t e, int64_t v, int x_is_f32, int backward) {
     if (!sizes_ok(n, e, v)) return -1;
+    if (n > 0 && n <= FEW) return few_bytes(n, e, v, backward != 0);
     return n == 0 ? 0 : layout(n, e, v, x_is_f32 != 0, backward != 0).total;
 }
 
@@ -1007,9 +1237,17 @@ extern "C" int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, c
     if (!x || !w || !labels || !loss || !lse || !workspace) return MGX_ERR_ARG;
     if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)workspace) & 15u) != 0) return MGX_ERR_ARG;
     const bool xf = x_is_f32 != 0;
+    hipStream_t st = (hipStream_t)stream;
+    if (n <= FEW) {
+        if (workspace_bytes < few_bytes(n, e, v, false)) return MGX_ERR_WORKSPACE;
+        XentRows g = {};
+        g.x = x; g.w = w; g.b = b; g.labels = labels; g.n = (int)n; g.e = (int)e; g.v = v;
+        g.part = (float2*)workspace;
+        g.zlab = (float*)((char*)workspace + up(up(v, 64) / 64 * n * 8, 16));
+        return xf ? few_forward<true>(g, loss, lse, hits, st) : few_forward<false>(g, loss, lse, hits, st);
+    }
     const Layout l = layout(n, e, v, xf, false);
     if (workspace_bytes < l.total) return MGX_ERR_WORKSPACE;
-    hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
     launch_prep(l, ws, x, xf, w, b, labels, nullptr, nullptr, n, e, v, st);
     XentGemm g = {};
@@ -1048,6 +1286,14 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
     if (!x || !w || !labels || !lse || !dloss || !workspace) return MGX_ERR_ARG;
     if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)workspace) & 15u) != 0) return MGX_ERR_ARG;
     const bool xf = x_is_f32 != 0;
+    if (n <= FEW) {
+        if (workspace_bytes < few_bytes(n, e, v, true)) return MGX_ERR_WORKSPACE;
+        XentRows g = {};
+        g.x = x; g.w = w; g.b = b; g.lse = lse; g.dloss = dloss; g.labels = labels; g.n = (int)n; g.e = (int)e; g.v = v;
+        g.dxp = dx ? (float*)workspace : nullptr;
+        g.dw = dw; g.db = db; g.accumulate = accumulate;
+        return xf ? few_backward<true>(g, dx, st) : few_backward<false>(g, dx, st);
+    }
     const Layout l = layout(n, e, v, xf, true);
     if (workspace_bytes < l.total) return MGX_ERR_WORKSPACE;
     char* ws = (char*)workspace;

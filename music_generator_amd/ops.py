@@ -1026,10 +1026,10 @@ class Tape8:
 
 def _on_current(*ts):
     """Kernels run on the current device's stream: a tensor of another device would be read through a foreign address."""
-    dev = K.device()
+    dev = torch.cuda.current_device()
     for t in ts:
-        if t is not None and t.device != dev:
-            raise MgxError("operand on %s, the current device is %s" % (t.device, dev))
+        if t is not None and t.get_device() != dev:
+            raise MgxError("operand on %s, the current device is cuda:%d" % (t.device, dev))
 
 
 def _p_act(t):
