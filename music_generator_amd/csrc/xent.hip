@@ -37,7 +37,7 @@ __device__ __forceinline__ unsigned f16_pack(float lo, float hi) {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kLowest = -3.402823466e38f;
 constexpr float kDz = 16384.f;                     // dz planes hold 2^14 dz / (largest |dloss|, rounded up to a power of two)
-constexpr int kMaxParts = 256;
+constexpr int kMaxParts = 1024;
 
 inline int64_t up(int64_t a, int64_t m) { return (a + m - 1) / m * m; }
 
@@ -53,10 +53,14 @@ __global__ __launch_bounds__(256) void xent_max_kernel(const float* __restrict__
         b &= 0x7fffffffu;
         if (b < 0x7f800000u && b > a) a = b;
     };
-    for (long i = t; i < nw / 4; i += stride) {
-        const u32x4 q = ((const u32x4*)w)[i];
+    for (long i = t; i < nw / 4; i += 4 * stride) {          // four loads in flight
+        u32x4 q[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) take(m[0], q[k]);
+        for (int j = 0; j < 4; ++j) q[j] = i + j * stride < nw / 4 ? ((const u32x4*)w)[i + j * stride] : (u32x4){0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) take(m[0], q[j][k]);
     }
     for (long i = nw / 4 * 4 + t; i < nw; i += stride) take(m[0], __builtin_bit_cast(unsigned, w[i]));
     if (XF32) {
@@ -221,9 +225,7 @@ struct XentGemm {
     float2* part;
     float *zlab, *out, *outb;
     f16_t *dzh, *dzl;
-    void* dx;
-    long np, n, ldo, class0;           // class0: first class of the piece
-    int e, first, last, dx_f32;
+    long np, ldo, class0;              // class0: first class of the piece
 };
 
 enum { EPI_FWD = 0, EPI_DZ = 1, EPI_DX = 2, EPI_DW = 3 };
@@ -389,22 +391,16 @@ __global__ __launch_bounds__(256, 2) void xent_gemm_kernel(XentGemm g) {
             }
         }
     } else if constexpr (EPI == EPI_DX) {
-        // A: rows, B: features
-        const float f = g.scales[2] / kDz / g.scales[0];
+        // A: rows, B: features; slab z, which the pieces of the classes add to one after the other
+        float* out = g.out + (long)blockIdx.z * g.np * g.ldo;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    const long row = mw + i * 32 + acc_row(k, lane), col = nw + j * 32 + r;
-                    float v = acc[i][j][k];
-                    if (!g.first) v += g.out[row * g.ldo + col];
-                    if (!g.last) g.out[row * g.ldo + col] = v;
-                    else if (row < g.n && col < g.e) {
-                        if (g.dx_f32) ((float*)g.dx)[row * g.e + col] = v * f;
-                        else ((bf16_t*)g.dx)[row * g.e + col] = (bf16_t)(v * f);
-                    }
+                    float* o = out + (mw + i * 32 + acc_row(k, lane)) * g.ldo + nw + j * 32 + r;
+                    *o = g.class0 == 0 ? acc[i][j][k] : *o + acc[i][j][k];
                 }
     } else {
         // A: features, B: classes; slab z of the piece
@@ -789,11 +785,11 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
     }
 }
 
-// dx from the parts of the streamed product, in order
+// dx from its parts, in order
 __global__ __launch_bounds__(256) void xent_dx_join_kernel(const float* __restrict__ parts, const float* __restrict__ scales,
                                                            const float2* __restrict__ rowinfo, void* __restrict__ dx, int dx_f32, int np,
                                                            long part, long n, int e, int ep) {
-    const float f = scales[2] / kDz / scales[0];             // dl holds 2^14 dloss / scales[2], the product 2^14 dz / dloss
+    const float f = scales[2] / kDz / scales[0];             // streamed: the parts hold 2^14 dz / dloss, the rows 2^14 dloss / scales[2]
     const long total = n * ep;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
         const long row = i / ep;
@@ -801,7 +797,7 @@ __global__ __launch_bounds__(256) void xent_dx_join_kernel(const float* __restri
         if (c >= e) continue;
         float s = 0.f;
         for (int p = 0; p < np; ++p) s += parts[p * part + i];
-        s *= f * (rowinfo[row].y / kDz);
+        s *= rowinfo ? f * (rowinfo[row].y / kDz) : f;
         if (dx_f32) ((float*)dx)[row * e + c] = s;
         else ((bf16_t*)dx)[row * e + c] = (bf16_t)s;
     }
@@ -1114,13 +1110,14 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
     l.np = up(n, l.rows_wg);
     l.vp = up(v, 128);
     l.ep = up(e, 128);
-    // Parts of the streamed operand: the number that wastes least of the last round of workgroups (`slots` run at once), with
-    // eight tiles a part at least and 2 % for each part's start and its share of the join.
-    auto split = [](int64_t wgs, int64_t tiles, int64_t slots) {
+    // Parts of a contraction of `tiles` steps by `wgs` workgroups, `slots` of which run at once: a step takes step_us, and each part
+    // costs a start of half a step's latency (1 us) and `bytes` written and read once more for the join at 4 TB/s.
+    auto split = [](int64_t wgs, int64_t tiles, int64_t slots, double step_us, double bytes) {
         int64_t best = 1;
         double least = 1e30;
-        for (int64_t p = 1; p <= 32 && (p == 1 || tiles / p >= 8); ++p) {
-            const double t = (double)((wgs * p + slots - 1) / slots) / (double)p * (1.0 + 0.02 * (double)p);
+        for (int64_t p = 1; p <= 32 && (p == 1 || tiles / p >= 4); ++p) {
+            const double rounds = (double)((wgs * p + slots - 1) / slots);
+            const double t = rounds * ((double)((tiles + p - 1) / p) * step_us + 1.0) + (double)p * bytes * 2.0 / 4e6;
             if (t < least) {
                 least = t;
                 best = p;
@@ -1128,10 +1125,10 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
         }
         return best;
     };
-    if (l.narrow) {
-        l.nf = split(l.np / l.rows_wg, l.vp / ST, 512);
-        l.nx = split(l.np / l.rows_wg, l.vp / ST, xf32 ? 512 : 256);
-        l.nz = split(l.vp / 128, l.np / ST, 512);
+    if (l.narrow) {      // step times: 128 (256) resident items x 32 streamed x 128 features at 1 PFLOP/s over the slots
+        l.nf = split(l.np / l.rows_wg, l.vp / ST, 512, xf32 ? 1.6 : 2.1, 8.0 * (double)l.np);
+        l.nx = split(l.np / l.rows_wg, l.vp / ST, xf32 ? 512 : 256, xf32 ? 3.2 : 1.1, 4.0 * (double)(l.np * l.ep));
+        l.nz = split(l.vp / 128, l.np / ST, 512, xf32 ? 3.2 : 2.1, 4.0 * (double)(l.ep * l.vp));
     }
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -1163,13 +1160,12 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
         l.vc = (int64_t)(128 << 20) / (4 * l.np) / 128 * 128;
         if (l.vc < 128) l.vc = 128;
         if (l.vc > l.vp) l.vc = l.vp;
-        const int64_t tiles = (l.ep / 128) * (l.vc / 128);
-        l.nz = 512 / tiles;
-        if (l.nz > l.np / 256) l.nz = l.np / 256;
-        if (l.nz < 1) l.nz = 1;
+        // a step: 128 x 128 x 32 with two or three plane products at 0.8 PFLOP/s over the slots
+        l.nx = split((l.np / 128) * (l.ep / 128), l.vc / BK, 512, xf32 ? 2.0 : 0.7, 4.0 * (double)(l.np * l.ep));
+        l.nz = split((l.ep / 128) * (l.vc / 128), l.np / BK, 512, xf32 ? 2.0 : 1.4, 4.0 * (double)(l.ep * l.vc));
         l.dzh = take(l.np * l.vc * 2);
         l.dzl = take(l.np * l.vc * 2);
-        l.dxw = take(l.np * l.ep * 4);
+        l.dxw = take(l.nx * l.np * l.ep * 4);
         l.slabs = take(l.nz * l.ep * l.vc * 4);
         l.slabs_b = take(l.nz * l.vc * 4);
     }
@@ -1199,16 +1195,17 @@ void launch_stream(const XentStream& g, int64_t wgs, int64_t parts, hipStream_t 
 
 void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const float* w, const float* b, const int* labels,
                  const float* lse, const float* dloss, int64_t n, int64_t e, int64_t v, hipStream_t st) {
-    const int parts = 256;
+    int64_t parts = up(e * v / 16 + n * e / 16, 256) / 256;         // sixteen values a thread, up to four workgroups a CU
+    parts = parts < 64 ? 64 : (parts > kMaxParts ? kMaxParts : parts);
     unsigned* part = (unsigned*)(ws + l.part);
     if (xf32)
-        hipLaunchKernelGGL(xent_max_kernel<true>, dim3(parts), dim3(256), 0, st, w, (long)(e * v), x, (long)(n * e), dloss,
+        hipLaunchKernelGGL(xent_max_kernel<true>, dim3((unsigned)parts), dim3(256), 0, st, w, (long)(e * v), x, (long)(n * e), dloss,
                            dloss ? (long)n : 0L, part);
     else
-        hipLaunchKernelGGL(xent_max_kernel<false>, dim3(parts), dim3(256), 0, st, w, (long)(e * v), x, (long)(n * e), dloss,
+        hipLaunchKernelGGL(xent_max_kernel<false>, dim3((unsigned)parts), dim3(256), 0, st, w, (long)(e * v), x, (long)(n * e), dloss,
                            dloss ? (long)n : 0L, part);
     XentPrep p = {};
-    p.x = x; p.w = w; p.b = b; p.lse = lse; p.dloss = dloss; p.labels = labels; p.part = part; p.parts = parts;
+    p.x = x; p.w = w; p.b = b; p.lse = lse; p.dloss = dloss; p.labels = labels; p.part = part; p.parts = (int)parts;
     p.n = n; p.v = v; p.np = l.np; p.vp = l.vp; p.e = (int)e; p.ep = (int)l.ep;
     p.xh = (f16_t*)(ws + l.xh); p.xl = (f16_t*)(ws + l.xl); p.wh = (f16_t*)(ws + l.wh); p.wl = (f16_t*)(ws + l.wl);
     p.bias = (float*)(ws + l.bias); p.scales = (float*)(ws + l.scales); p.lab = (int*)(ws + l.lab);
@@ -1219,6 +1216,13 @@ void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const floa
     const dim3 grid((unsigned)(p.wtiles + p.xblocks + 64));
     if (xf32) hipLaunchKernelGGL(xent_prep_kernel<true>, grid, dim3(256), 0, st, p);
     else hipLaunchKernelGGL(xent_prep_kernel<false>, grid, dim3(256), 0, st, p);
+}
+
+void launch_dx_join(const Layout& l, char* ws, const float2* row, void* dx, bool xf32, int64_t n, int64_t e, hipStream_t st) {
+    const int64_t blocks = up(n * l.ep, 256) / 256;
+    hipLaunchKernelGGL(xent_dx_join_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st,
+                       (const float*)(ws + l.dxw), (const float*)(ws + l.scales), row, dx, (int)xf32, (int)l.nx, (long)(l.np * l.ep),
+                       (long)n, (int)e, (int)l.ep);
 }
 
 }  // namespace
@@ -1309,9 +1313,7 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
             q.tiles = (int)(l.vp / ST); q.out = (float*)(ws + l.dxw); q.ld = l.np;
             if (xf) launch_stream<2, 2, 1, MODE_DX, 2>(q, l.np / l.rows_wg, l.nx, st);
             else launch_stream<1, 1, 2, MODE_DX, 1>(q, l.np / l.rows_wg, l.nx, st);
-            const int64_t blocks = up(n * l.ep, 256) / 256;
-            hipLaunchKernelGGL(xent_dx_join_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, q.out, q.scales,
-                               q.row, dx, (int)xf, (int)l.nx, (long)(l.np * l.ep), (long)n, (int)e, (int)l.ep);
+            launch_dx_join(l, ws, q.row, dx, xf, n, e, st);
         }
         if (dw || db) {
             q.r[0] = wh; q.r[1] = wl; q.s[0] = xh; q.s[1] = xl;
@@ -1341,9 +1343,8 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
             q.scales = g.scales;
             q.a[0] = dzh; q.a[1] = dzl; q.b[0] = wh; q.b[1] = wl;
             q.lda = l.vc; q.ldb = l.ep; q.kiters = (int)(cnt / BK);
-            q.out = (float*)(ws + l.dxw); q.ldo = l.ep; q.dx = dx; q.dx_f32 = xf; q.n = n; q.e = (int)e;
-            q.first = c0 == 0; q.last = c0 + cnt >= l.vp;
-            const dim3 gx((unsigned)(l.np / 128), (unsigned)(l.ep / 128));
+            q.out = (float*)(ws + l.dxw); q.ldo = l.ep; q.np = l.np; q.class0 = c0;
+            const dim3 gx((unsigned)(l.np / 128), (unsigned)(l.ep / 128), (unsigned)l.nx);
             if (xf) launch_gemm<2, 2, false, true, EPI_DX>(q, gx, st);
             else launch_gemm<1, 1, false, true, EPI_DX>(q, gx, st);
         }
@@ -1361,5 +1362,6 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
                                accumulate);
         }
     }
+    if (dx) launch_dx_join(l, ws, nullptr, dx, xf, n, e, st);
     return mgx_launch_status();
 }
