@@ -905,17 +905,19 @@ __device__ __forceinline__ void xent_rows_logits(const XentRows& g, float* xs, f
         __syncthreads();
         xent_rows_stage<RT, XF32>(g, xs, e0, cnt);
         __syncthreads();
-        const int per = (cnt + 3) / 4, k1 = (wv + 1) * per < cnt ? (wv + 1) * per : cnt;
-        for (int k = wv * per; k < k1; k += 16) {
+        const int per = (cnt + 63) / 64 * 16, k1 = (wv + 1) * per < cnt ? (wv + 1) * per : cnt;
+        for (int k = wv * per; k < k1; k += 16) {                  // 16 loads in flight; k + 15 < RC
             float w[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) w[j] = ok && k + j < k1 ? g.w[(long)(e0 + k + j) * g.v + c] : 0.f;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int at = k + j < RC ? k + j : RC - 1;
+            for (int j = 0; j < 16; j += 4)
 #pragma unroll
-                for (int i = 0; i < RT; ++i) z[i] = __builtin_fmaf(w[j], xs[i * RC + at], z[i]);
-            }
+                for (int i = 0; i < RT; ++i) {
+                    const f32x4 xv = *(const f32x4*)(xs + i * RC + k + j);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) z[i] = __builtin_fmaf(w[j + t], xv[t], z[i]);
+                }
         }
     }
 #pragma unroll
@@ -931,7 +933,7 @@ __device__ __forceinline__ void xent_rows_logits(const XentRows& g, float* xs, f
 
 template <int RT, bool XF32>
 __global__ __launch_bounds__(256) void xent_rows_fwd_kernel(XentRows g) {
-    __shared__ float xs[RT * RC], red[4 * RT * 64], zs[RT * 64];
+    __shared__ __attribute__((aligned(16))) float xs[RT * RC], red[4 * RT * 64], zs[RT * 64];
     xent_rows_logits<RT, XF32>(g, xs, red, zs);
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     for (int i = wv; i < g.n; i += 4) {             // the wave that wrote row i of zs
@@ -975,8 +977,9 @@ __global__ __launch_bounds__(64) void xent_rows_join_kernel(XentRows g, float* _
 
 template <int RT, bool XF32>
 __global__ __launch_bounds__(256) void xent_rows_bwd_kernel(XentRows g) {
-    __shared__ float xs[RT * RC], red[4 * RT * 64], zs[RT * 64], wt[64][65];
+    __shared__ __attribute__((aligned(16))) float xs[RT * RC], red[4 * RT * 64], zs[RT * 64], wt[64][65];
     xent_rows_logits<RT, XF32>(g, xs, red, zs);
+    float* dzt = red;                               // dz as [class][row], for reads of all rows of a class
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const long c = (long)blockIdx.x * 64 + lane;
     __syncthreads();
@@ -989,12 +992,16 @@ __global__ __launch_bounds__(256) void xent_rows_bwd_kernel(XentRows g) {
             d = ((long)blockIdx.x * 64 + (k & 63) == lab ? p - 1.f : p) * g.dloss[i];
         }
         zs[k] = d;
+        dzt[(k & 63) * RT + i] = d;
     }
     __syncthreads();
+    float dz[RT];                                   // of the lane's class
+#pragma unroll
+    for (int i = 0; i < RT; ++i) dz[i] = zs[i * 64 + lane];
     if (g.db && wv == 0 && c < g.v) {
         float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < RT; ++i) s += zs[i * 64 + lane];
+        for (int i = 0; i < RT; ++i) s += dz[i];
         g.db[c] = g.accumulate ? g.db[c] + s : s;
     }
     for (int e0 = 0; e0 < g.e; e0 += RC) {
@@ -1005,29 +1012,44 @@ __global__ __launch_bounds__(256) void xent_rows_bwd_kernel(XentRows g) {
             __syncthreads();
         }
         if (g.dw && c < g.v) {
-            for (int k = wv; k < cnt; k += 4) {
-                float s = 0.f;
+            for (int k = 4 * wv; k < cnt; k += 16) {
+                f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < RT; ++i) s = __builtin_fmaf(xs[i * RC + k], zs[i * 64 + lane], s);
-                float* d = g.dw + (long)(e0 + k) * g.v + c;
-                *d = g.accumulate ? *d + s : s;
+                for (int i = 0; i < RT; ++i) {
+                    const f32x4 xv = *(const f32x4*)(xs + i * RC + k);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) s[t] = __builtin_fmaf(xv[t], dz[i], s[t]);
+                }
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    if (k + t < cnt) {
+                        float* d = g.dw + (long)(e0 + k + t) * g.v + c;
+                        *d = g.accumulate ? *d + s[t] : s[t];
+                    }
+                }
             }
         }
         if (g.dxp) {
             for (int k0 = 0; k0 < cnt; k0 += 64) {
+                float w[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int k = k0 + wv + 4 * j;
+                    w[j] = k < cnt && c < g.v ? g.w[(long)(e0 + k) * g.v + c] : 0.f;
+                }
                 __syncthreads();
-                for (int k = wv; k < 64; k += 4)
-                    wt[k][lane] = k0 + k < cnt && c < g.v ? g.w[(long)(e0 + k0 + k) * g.v + c] : 0.f;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) wt[wv + 4 * j][lane] = w[j];
                 __syncthreads();
                 const int k = tid >> 2, q = tid & 3;
                 float s[RT];
 #pragma unroll
                 for (int i = 0; i < RT; ++i) s[i] = 0.f;
-#pragma unroll
+#pragma unroll 4
                 for (int j = 0; j < 16; ++j) {
-                    const float w = wt[k][4 * j + q];
+                    const float w1 = wt[k][4 * j + q];
 #pragma unroll
-                    for (int i = 0; i < RT; ++i) s[i] = __builtin_fmaf(w, zs[i * 64 + 4 * j + q], s[i]);
+                    for (int i = 0; i < RT; ++i) s[i] = __builtin_fmaf(w1, dzt[(4 * j + q) * RT + i], s[i]);
                 }
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
