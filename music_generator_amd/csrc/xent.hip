@@ -35,6 +35,19 @@ __device__ __forceinline__ unsigned f16_pack(float lo, float hi) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){lo, hi}, f16x2));
 }
 
+__device__ __forceinline__ unsigned lds_byte(const unsigned char* p) {
+    return (unsigned)(size_t)(__attribute__((address_space(3))) const void*)p;
+}
+
+// One LDS-DMA instruction: lane l moves 16 (4) bytes from byte `off` of the uniform address `base` to LDS byte dst + 16 l (4 l),
+// dst uniform.  Complete when the issuing wave has waited for vmcnt.
+__device__ __forceinline__ void lds_dma16(const void* base, int off, unsigned dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void lds_dma4(const void* base, int off, unsigned dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
+}
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kLowest = -3.402823466e38f;
 constexpr float kDz = 16384.f;                     // dz planes hold 2^14 dz / (largest |dloss|, rounded up to a power of two)
 constexpr int kMaxParts = 1024;
@@ -483,29 +496,25 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
     const int t0 = blockIdx.y * per, t1 = t0 + per < g.tiles ? t0 + per : g.tiles;
 
     // LDS-DMA of tile t: a wave fills 1 KB pieces (4 rows of 256 B), lane l the 16-byte place l of the piece with the chunk that
-    // belongs there.  A plane is under 4 GB: uniform offset of the piece plus the lane's.
+    // belongs there.  In assembly: in front of a transposed LDS read the compiler waits for every LDS-DMA it knows of, the
+    // one just issued for a later tile included.
     static_assert(ROWB == 256, "a piece is four rows");
-    const __amdgpu_buffer_rsrc_t rs0 = __builtin_amdgcn_make_buffer_rsrc((void*)g.s[0], 0, 0xffffffffu, 0x00020000);
-    [[maybe_unused]] const __amdgpu_buffer_rsrc_t rs1 = __builtin_amdgcn_make_buffer_rsrc((void*)g.s[NS - 1], 0, 0xffffffffu, 0x00020000);
     // beside the planes: FWD and DX the biases, DW (lse, dloss) and the labels of the tile's items
     const void* ip = MODE != MODE_DW ? (const void*)g.bias : wv == 0 ? (const void*)g.row : (const void*)g.lab;
-    const __amdgpu_buffer_rsrc_t ri = __builtin_amdgcn_make_buffer_rsrc((void*)ip, 0, 0xffffffffu, 0x00020000);
     const int lo0 = (lane >> 4) * ROWB + (((lane & 15) ^ ((lane >> 4) << 2)) << 4);
     auto stage = [&](int t) {
-        unsigned char* dst = lds + (t & 3) * BUF;
+        const unsigned dst = lds_byte(lds) + (t & 3) * BUF;
         constexpr int PIECES = SPLANE / 1024;
 #pragma unroll
         for (int pl = 0; pl < NS; ++pl)
 #pragma unroll
             for (int i = 0; i < PIECES / 4; ++i) {
                 const int piece = wv * (PIECES / 4) + i;                       // rows 4 piece ..: bits 2-3 of the row are piece & 3
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(pl == 0 ? rs0 : rs1, (__attribute__((address_space(3))) void*)(dst + pl * SPLANE + piece * 1024),
-                                                         16, lo0 ^ ((piece & 3) << 4), t * SPLANE + piece * 1024, 0, 0);
+                lds_dma16(g.s[pl] + ((long)t * SPLANE + piece * 1024) / 2, lo0 ^ ((piece & 3) << 4), dst + pl * SPLANE + piece * 1024);
             }
         if (wv < (MODE == MODE_DW ? 2 : 1)) {        // 64 floats, or 32 twice
             const bool two = MODE == MODE_DW && wv == 0;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ri, (__attribute__((address_space(3))) void*)(dst + NS * SPLANE + wv * 256), 4,
-                                                     two ? lane * 4 : r * 4, t * (two ? ST * 8 : ST * 4), 0, 0);
+            lds_dma4((const float*)ip + (long)t * (two ? 2 * ST : ST), two ? lane * 4 : r * 4, dst + NS * SPLANE + wv * 256);
         }
     };
 
@@ -696,6 +705,10 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
             }
         };
         if constexpr (DO_S) {                        // S starts at the biases
+            if constexpr (MODE == MODE_DW) {         // or the compiler keeps 16 copies of the lane's
+#pragma unroll
+                for (int b = 0; b < RB; ++b) asm volatile("" : "+v"(rinfo[b]));
+            }
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 f32x4 bv;
