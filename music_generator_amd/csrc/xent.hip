@@ -50,7 +50,7 @@ __device__ __forceinline__ void lds_dma4(const void* base, int off, unsigned dst
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kLowest = -3.402823466e38f;
 constexpr float kDz = 16384.f;                     // dz planes hold 2^14 dz / (largest |dloss|, rounded up to a power of two)
-constexpr int kMaxParts = 1024;
+constexpr int kMaxParts = 512;
 
 inline int64_t up(int64_t a, int64_t m) { return (a + m - 1) / m * m; }
 
@@ -110,15 +110,18 @@ __device__ __forceinline__ float scale_of(unsigned maxbits) {
 
 // {s_w, s_x, largest |dloss| rounded up to a power of two} into scales[0..2]; part has `parts` partials per tensor.
 __device__ __forceinline__ float scale_from_parts(const unsigned* __restrict__ part, int which, int parts) {
-    unsigned m = 0u;
-    for (int i = threadIdx.x & 63; i < parts; i += 64) {
-        const unsigned o = part[which * kMaxParts + i];
-        m = m > o ? m : o;
+    unsigned m = 0u, o[kMaxParts / 64];
+#pragma unroll
+    for (int k = 0; k < kMaxParts / 64; ++k) {                   // all loads in flight at once
+        const int i = (threadIdx.x & 63) + 64 * k;
+        o[k] = i < parts ? part[which * kMaxParts + i] : 0u;
     }
 #pragma unroll
+    for (int k = 0; k < kMaxParts / 64; ++k) m = m > o[k] ? m : o[k];
+#pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
-        const unsigned o = (unsigned)__shfl_xor((int)m, off, 64);
-        m = m > o ? m : o;
+        const unsigned q = (unsigned)__shfl_xor((int)m, off, 64);
+        m = m > q ? m : q;
     }
     if (which == 2) return 16384.f / scale_of(m);
     return scale_of(m);
@@ -156,14 +159,18 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
     const int tid = threadIdx.x;
     if ((long)blockIdx.x < p.wtiles) {
         __shared__ float t[64][65];
-        const float s = scale_from_parts(p.part, 0, p.parts);
         const long etiles = p.ep / 64, ct = blockIdx.x / etiles, et = blockIdx.x - ct * etiles;
         const long c0 = ct * 64, e0 = et * 64;
-        const int cc = tid & 63;
-        for (int k = tid >> 6; k < 64; k += 4) {
-            const bool ok = c0 + cc < p.v && e0 + k < p.e;
-            t[k][cc] = ok ? p.w[(e0 + k) * p.v + c0 + cc] * s : 0.f;
+        const int cc = tid & 63, k0 = tid >> 6;
+        float in[16];                                          // in flight while the scale is found
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int k = k0 + 4 * j;
+            in[j] = c0 + cc < p.v && e0 + k < p.e ? p.w[(e0 + k) * p.v + c0 + cc] : 0.f;
         }
+        const float s = scale_from_parts(p.part, 0, p.parts);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) t[k0 + 4 * j][cc] = in[j] * s;
         __syncthreads();
         const int e8 = tid & 7;
         for (int c = tid >> 3; c < 64; c += 32) {
@@ -184,13 +191,27 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
             const int c = (int)(i - row * q) * 8;
             const int lab = row < p.n ? p.labels[row] : -1;
             const bool ok = lab >= 0 && lab < p.v;
-            float v[8];
+            const long at = row * p.e + c;
+            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (ok && (p.e & 7) == 0) {                        // rows of whole 16-byte pieces
+                if (c < p.e) {
+                    if (XF32) {
+                        const f32x4 a = *(const f32x4*)((const float*)p.x + at), b = *(const f32x4*)((const float*)p.x + at + 4);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const bool in = ok && c + k < p.e;
-                const long at = row * p.e + c + k;
-                v[k] = in ? (XF32 ? ((const float*)p.x)[at] : (float)((const bf16_t*)p.x)[at]) * s : 0.f;
+                        for (int k = 0; k < 4; ++k) { v[k] = a[k]; v[4 + k] = b[k]; }
+                    } else {
+                        const u32x4 a = *(const u32x4*)((const bf16_t*)p.x + at);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) { v[2 * k] = bf_lo(a[k]); v[2 * k + 1] = bf_hi(a[k]); }
+                    }
+                }
+            } else if (ok) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (c + k < p.e) v[k] = XF32 ? ((const float*)p.x)[at + k] : (float)((const bf16_t*)p.x)[at + k];
             }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] *= s;
             u32x4 hi, lo;
             split8(v, hi, lo);
             *(u32x4*)(p.xh + row * p.ep + c) = hi;
@@ -798,6 +819,19 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
     }
 }
 
+// p[0] + p[stride] + ... of n parts, in order, eight loads in flight
+__device__ __forceinline__ float sum_parts(const float* __restrict__ p, int n, long stride) {
+    float s = 0.f;
+    for (int z = 0; z < n; z += 8) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = z + k < n ? p[(z + k) * stride] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += v[k];
+    }
+    return s;
+}
+
 // dx from its parts, in order
 __global__ __launch_bounds__(256) void xent_dx_join_kernel(const float* __restrict__ parts, const float* __restrict__ scales,
                                                            const float2* __restrict__ rowinfo, void* __restrict__ dx, int dx_f32, int np,
@@ -808,8 +842,7 @@ __global__ __launch_bounds__(256) void xent_dx_join_kernel(const float* __restri
         const long row = i / ep;
         const int c = (int)(i - row * ep);
         if (c >= e) continue;
-        float s = 0.f;
-        for (int p = 0; p < np; ++p) s += parts[p * part + i];
+        float s = sum_parts(parts + i, np, part);
         s *= rowinfo ? f * (rowinfo[row].y / kDz) : f;
         if (dx_f32) ((float*)dx)[row * e + c] = s;
         else ((bf16_t*)dx)[row * e + c] = (bf16_t)s;
@@ -825,11 +858,16 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
     const int rr = threadIdx.x & 31, gr = threadIdx.x >> 5;
     const long row = (long)blockIdx.x * 32 + rr;
     float m = kLowest, s = 0.f;
-    for (long i = gr; i < slices; i += 8) {
-        const float2 p = part[i * np + row];
-        const float mm = fmaxf(m, p.x);
-        s = s * __builtin_amdgcn_exp2f(m - mm) + p.y * __builtin_amdgcn_exp2f(p.x - mm);
-        m = mm;
+    for (long i = gr; i < slices; i += 32) {                     // four loads in flight
+        float2 p[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) p[k] = i + 8 * k < slices ? part[(i + 8 * k) * np + row] : make_float2(kLowest, 0.f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float mm = fmaxf(m, p[k].x);
+            s = s * __builtin_amdgcn_exp2f(m - mm) + p[k].y * __builtin_amdgcn_exp2f(p[k].x - mm);
+            m = mm;
+        }
     }
     red[gr][rr] = make_float2(m, s);
     __syncthreads();
@@ -860,12 +898,12 @@ __global__ __launch_bounds__(256) void xent_dw_reduce_kernel(const float* __rest
     float s = 0.f;
     if (k < e) {
         if (!dw) return;
-        for (int z = 0; z < nz; ++z) s += slabs[z * slab + k * ldo + c];
+        s = sum_parts(slabs + k * ldo + c, nz, slab);
         s = s * (scales[2] / kDz) / scales[1];
         float* d = dw + k * v + c0 + c;
         *d = accumulate ? *d + s : s;
     } else if (db) {
-        for (int z = 0; z < nz; ++z) s += slabs_b[z * ldo + c];
+        s = sum_parts(slabs_b + c, nz, ldo);
         s *= scales[2] / kDz;
         float* d = db + c0 + c;
         *d = accumulate ? *d + s : s;
