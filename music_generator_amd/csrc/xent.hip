@@ -241,12 +241,12 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
 }
 
 // ---------------------------------------------------------------- products
-// D (128 x 128 per workgroup) = sum over the kept plane products of A B^T.  An operand is stored either with the
-// contraction index fastest ([row][k], read as 16-byte fragments) or slowest ([k][row], read with ds_read_b64_tr_b16).
-// 4 waves of 64 x 64, 32 of k per step, all planes of a step staged by LDS-DMA into one of two buffers while the other
-// is computed on.  Staged rows are 64 (256) bytes with their 16-byte chunks XOR-swizzled by the row so that both kinds of
-// read spread over all banks.
-constexpr int BK = 32, PLANE = 128 * BK * 2;
+// D (64 WM x 64 WN per workgroup of WM x WN = 8 waves) = sum over the kept plane products of A B^T.  An operand is stored either
+// with the contraction index fastest ([row][k], read as 16-byte fragments) or slowest ([k][row], read with
+// ds_read_b64_tr_b16).  32 of k per step; all planes of a step are staged by LDS-DMA, two steps ahead, into a ring of three: a step is
+// 0.4 us of matrix instructions, less than what a load takes under load.  Staged rows have their 16-byte chunks
+// XOR-swizzled by the row so that both kinds of read spread over all banks.
+constexpr int BK = 32;
 
 struct XentGemm {
     const f16_t *a[2], *b[2];
@@ -267,47 +267,50 @@ enum { EPI_FWD = 0, EPI_DZ = 1, EPI_DX = 2, EPI_DW = 3 };
 __device__ __forceinline__ int swz_row(int row) { return (row >> 2) & 3; }
 __device__ __forceinline__ int swz_k(int k) { return ((k & 3) << 2) | ((k >> 2) & 3); }
 
-template <int NA, int NB, bool AT, bool BT, int EPI>
-__global__ __launch_bounds__(256, 2) void xent_gemm_kernel(XentGemm g) {
+template <int NA, int NB, bool AT, bool BT, int EPI, int WM>
+__global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
-    constexpr int BUF = (NA + NB) * PLANE;
+    constexpr int WN = 8 / WM, TM = 64 * WM, TN = 64 * WN, PA = TM * BK * 2, PB = TN * BK * 2, BUF = NA * PA + NB * PB;
+    constexpr int PIECES = (NA * PA + NB * PB) / 8192;              // LDS-DMA instructions of a wave and step
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = lane & 31, h = lane >> 5, wm = wv >> 1, wn = wv & 1;
-    const long m0 = (long)blockIdx.x * 128, n0 = (long)blockIdx.y * 128;
+    const int r = lane & 31, h = lane >> 5, wm = wv / WN, wn = wv % WN;
+    const long m0 = (long)blockIdx.x * TM, n0 = (long)blockIdx.y * TN;
     // split contraction: part z of gridDim.z takes steps [it0, it1)
     const int per = (g.kiters + gridDim.z - 1) / gridDim.z;
     const int it0 = blockIdx.z * per, it1 = it0 + per < g.kiters ? it0 + per : g.kiters;
 
-    auto stage = [&](int buf, int it) {
-        const long k0 = (long)it * BK;
+    // one plane (T rows) of step it: pieces of 1 KB, 16 rows of 64 B or 2 (4) rows of 512 (256) B
+    auto stage_plane = [&](unsigned dst, const f16_t* src, long ld, long o0, int it, auto tr_, auto T_) {
+        constexpr bool tr = decltype(tr_)::value;
+        constexpr int T = decltype(T_)::value, PER = T * BK * 2 / 8192;
 #pragma unroll
-        for (int pl = 0; pl < NA + NB; ++pl) {
-            const bool isa = pl < NA, tr = isa ? AT : BT;
-            const f16_t* src = isa ? g.a[pl] : g.b[pl - NA];
-            const long ld = isa ? g.lda : g.ldb, o0 = isa ? m0 : n0;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int piece = wv * 2 + i;                       // 1 KB: 16 rows of 64 B, or 4 rows of 256 B
-                const f16_t* gp;
-                if (tr) {
-                    const int row = piece * 4 + (lane >> 4), ch = (lane & 15) ^ swz_k(row);
-                    gp = src + (k0 + row) * ld + o0 + ch * 8;
-                } else {
-                    const int row = piece * 16 + (lane >> 2), ch = (lane & 3) ^ swz_row(row);
-                    gp = src + (o0 + row) * ld + k0 + ch * 8;
-                }
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)gp,
-                                                 (__attribute__((address_space(3))) void*)(lds + buf * BUF + pl * PLANE + piece * 1024),
-                                                 16, 0, 0);
+        for (int i = 0; i < PER; ++i) {
+            const int piece = wv * PER + i;
+            if constexpr (tr) {
+                constexpr int RPP = 512 / T, LPR = 64 / RPP;            // rows of a piece, lanes of a row
+                const int row = piece * RPP + lane / LPR, ch = (lane % LPR) ^ swz_k(row);
+                lds_dma16(src + ((long)it * BK + piece * RPP) * ld + o0, (int)(lane / LPR * ld * 2) + ch * 16, dst + piece * 1024);
+            } else {
+                const int ch = (lane & 3) ^ ((lane >> 4) & 3);          // swz_row of row 16 piece + lane / 4
+                lds_dma16(src + (o0 + piece * 16) * ld + (long)it * BK, (int)((lane >> 2) * ld * 2) + ch * 16, dst + piece * 1024);
             }
         }
     };
+    auto stage = [&](int it) {
+        const unsigned dst = lds_byte(lds) + (it - it0) % 3 * BUF;
+#pragma unroll
+        for (int pl = 0; pl < NA; ++pl)
+            stage_plane(dst + pl * PA, g.a[pl], g.lda, m0, it, std::integral_constant<bool, AT>{}, std::integral_constant<int, TM>{});
+#pragma unroll
+        for (int pl = 0; pl < NB; ++pl)
+            stage_plane(dst + NA * PA + pl * PB, g.b[pl], g.ldb, n0, it, std::integral_constant<bool, BT>{}, std::integral_constant<int, TN>{});
+    };
     const int hk = lane >> 5, cb = (lane >> 4) & 1, qq = (lane >> 2) & 3, pp = lane & 3;
-    auto frag = [&](const unsigned char* plane, bool tr, int blk, int ks) -> u32x4 {
+    auto frag = [&](const unsigned char* plane, bool tr, int rowb, int blk, int ks) -> u32x4 {
         if (tr) {
             const int k = 16 * ks + 8 * hk + qq, ch = blk * 4 + 2 * cb + (pp >> 1);
-            const u32x2 a = tr_read(plane + k * 256 + ((ch ^ swz_k(k)) << 4) + 8 * (pp & 1));
-            const u32x2 b = tr_read(plane + (k + 4) * 256 + ((ch ^ swz_k(k + 4)) << 4) + 8 * (pp & 1));
+            const u32x2 a = tr_read(plane + k * rowb + ((ch ^ swz_k(k)) << 4) + 8 * (pp & 1));
+            const u32x2 b = tr_read(plane + (k + 4) * rowb + ((ch ^ swz_k(k + 4)) << 4) + 8 * (pp & 1));
             return (u32x4){a[0], a[1], b[0], b[1]};
         }
         const int row = blk * 32 + r;
@@ -323,24 +326,26 @@ __global__ __launch_bounds__(256, 2) void xent_gemm_kernel(XentGemm g) {
     const bool bias_wave = EPI == EPI_DW && blockIdx.x == 0 && wm == 0;       // sums of B's columns: a product with ones
     const u32x4 ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 
-    if (it0 < it1) stage(0, it0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    int cur = 0;
+    if (it0 < it1) stage(it0);
+    if (it0 + 1 < it1) stage(it0 + 1);
     for (int it = it0; it < it1; ++it) {
-        if (it + 1 < it1) stage(cur ^ 1, it + 1);
-        const unsigned char* base = lds + cur * BUF;
+        // step it has landed (the one behind it may be on its way), and no wave reads step it - 1 any more
+        if (it + 1 < it1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (it + 2 < it1) stage(it + 2);
+        const unsigned char* base = lds + (it - it0) % 3 * BUF;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             u32x4 fa[NA][2], fb[NB][2];
 #pragma unroll
             for (int pl = 0; pl < NA; ++pl)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) fa[pl][i] = frag(base + pl * PLANE, AT, wm * 2 + i, ks);
+                for (int i = 0; i < 2; ++i) fa[pl][i] = frag(base + pl * PA, AT, TM * 2, wm * 2 + i, ks);
 #pragma unroll
             for (int pl = 0; pl < NB; ++pl)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) fb[pl][i] = frag(base + (NA + pl) * PLANE, BT, wn * 2 + i, ks);
+                for (int i = 0; i < 2; ++i) fb[pl][i] = frag(base + NA * PA + pl * PB, BT, TN * 2, wn * 2 + i, ks);
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -357,9 +362,6 @@ __global__ __launch_bounds__(256, 2) void xent_gemm_kernel(XentGemm g) {
                 }
             }
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        cur ^= 1;
     }
 
     const long mw = m0 + wm * 64, nw = n0 + wn * 64;
@@ -1179,9 +1181,9 @@ struct Layout {
 Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
     Layout l = {};
     l.narrow = e <= 128;
-    l.rows_wg = l.narrow && !xf32 ? 256 : 128;
+    l.rows_wg = l.narrow && xf32 ? 128 : 256;
     l.np = up(n, l.rows_wg);
-    l.vp = up(v, 128);
+    l.vp = up(v, l.narrow ? 128 : 256);
     l.ep = up(e, 128);
     // Parts of a contraction of `tiles` steps by `wgs` workgroups, `slots` of which run at once: a step takes step_us, and each part
     // costs a start of half a step's latency (1 us) and `bytes` written and read once more for the join at 4 TB/s.
@@ -1230,12 +1232,12 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
     } else {
         l.row = take(l.np * 8);
         // a piece of the classes: dz planes of about 128 MB, which the 256 MB last-level cache holds
-        l.vc = (int64_t)(128 << 20) / (4 * l.np) / 128 * 128;
-        if (l.vc < 128) l.vc = 128;
+        l.vc = (int64_t)(128 << 20) / (4 * l.np) / 256 * 256;
+        if (l.vc < 256) l.vc = 256;
         if (l.vc > l.vp) l.vc = l.vp;
-        // a step: 128 x 128 x 32 with two or three plane products at 0.8 PFLOP/s over the slots
-        l.nx = split((l.np / 128) * (l.ep / 128), l.vc / BK, 512, xf32 ? 2.0 : 0.7, 4.0 * (double)(l.np * l.ep));
-        l.nz = split((l.ep / 128) * (l.vc / 128), l.np / BK, 512, xf32 ? 2.0 : 1.4, 4.0 * (double)(l.ep * l.vc));
+        // a step: 256 x 128 x 32 with one to three plane products at 1 PFLOP/s over the slots
+        l.nx = split((l.np / 256) * (l.ep / 128), l.vc / BK, 256, xf32 ? 1.6 : 0.55, 4.0 * (double)(l.np * l.ep));
+        l.nz = split((l.ep / 128) * (l.vc / 256), l.np / BK, 256, xf32 ? 1.6 : 1.1, 4.0 * (double)(l.ep * l.vc));
         l.dzh = take(l.np * l.vc * 2);
         l.dzl = take(l.np * l.vc * 2);
         l.dxw = take(l.nx * l.np * l.ep * 4);
@@ -1250,12 +1252,14 @@ bool sizes_ok(int64_t n, int64_t e, int64_t v) {
     return n >= 0 && e >= 1 && v >= 1 && n <= 8000000 && v <= 8000000 && e <= 65536;      // rows / 128 and classes / 128 are grid dimensions
 }
 
-template <int NA, int NB, bool AT, bool BT, int EPI>
-void launch_gemm(const XentGemm& g, dim3 grid, hipStream_t st) {
+// m x n results in `parts` parts of the contraction; WM waves of 64 along m, 8 / WM along n
+template <int NA, int NB, bool AT, bool BT, int EPI, int WM>
+void launch_gemm(const XentGemm& g, int64_t m, int64_t n, int64_t parts, hipStream_t st) {
     static std::atomic<uint64_t> done{0};
-    constexpr int bytes = 2 * (NA + NB) * PLANE;
-    mgx_allow_dynamic_lds(xent_gemm_kernel<NA, NB, AT, BT, EPI>, bytes, done);
-    hipLaunchKernelGGL((xent_gemm_kernel<NA, NB, AT, BT, EPI>), grid, dim3(256), bytes, st, g);
+    constexpr int bytes = 3 * (NA * 64 * WM + NB * 512 / WM) * BK * 2;
+    mgx_allow_dynamic_lds(xent_gemm_kernel<NA, NB, AT, BT, EPI, WM>, bytes, done);
+    hipLaunchKernelGGL((xent_gemm_kernel<NA, NB, AT, BT, EPI, WM>), dim3((unsigned)(m / (64 * WM)), (unsigned)(n / (512 / WM)), (unsigned)parts),
+                       dim3(512), bytes, st, g);
 }
 
 template <int NR, int NS, int RB, int MODE, int OCC>
@@ -1332,7 +1336,6 @@ extern "C" int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, c
     g.lda = g.ldb = l.ep; g.kiters = (int)(l.ep / BK);
     g.bias = (float*)(ws + l.bias); g.scales = (float*)(ws + l.scales); g.lab = (int*)(ws + l.lab);
     g.part = (float2*)(ws + l.slices); g.zlab = (float*)(ws + l.zlab); g.np = l.np;
-    const dim3 grid((unsigned)(l.vp / 128), (unsigned)(l.np / 128));
     if (l.narrow) {
         XentStream q = {};
         q.r[0] = g.b[0]; q.r[1] = g.b[1]; q.s[0] = g.a[0]; q.s[1] = g.a[1];
@@ -1341,9 +1344,9 @@ extern "C" int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, c
         if (xf) launch_stream<2, 2, 1, MODE_FWD, 2>(q, l.np / l.rows_wg, l.nf, st);
         else launch_stream<1, 2, 2, MODE_FWD, 2>(q, l.np / l.rows_wg, l.nf, st);
     } else if (xf) {
-        launch_gemm<2, 2, false, false, EPI_FWD>(g, grid, st);
+        launch_gemm<2, 2, false, false, EPI_FWD, 4>(g, l.vp, l.np, 1, st);
     } else {
-        launch_gemm<2, 1, false, false, EPI_FWD>(g, grid, st);
+        launch_gemm<2, 1, false, false, EPI_FWD, 4>(g, l.vp, l.np, 1, st);
     }
     hipLaunchKernelGGL(xent_join_kernel, dim3((unsigned)(l.np / 32)), dim3(256), 0, st, g.part, g.zlab, g.lab, loss, lse, hits,
                        (long)n, (long)l.np, (long)l.nf);
@@ -1408,18 +1411,16 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
         g.lda = g.ldb = l.ep; g.kiters = (int)(l.ep / BK);
         g.bias = (float*)(ws + l.bias) + c0; g.lab = (int*)(ws + l.lab); g.row = (float2*)(ws + l.row);
         g.dzh = dzh; g.dzl = dzl; g.ldo = l.vc; g.np = l.np; g.class0 = c0;
-        const dim3 grid((unsigned)(cnt / 128), (unsigned)(l.np / 128));
-        if (xf) launch_gemm<2, 2, false, false, EPI_DZ>(g, grid, st);
-        else launch_gemm<2, 1, false, false, EPI_DZ>(g, grid, st);
+        if (xf) launch_gemm<2, 2, false, false, EPI_DZ, 4>(g, cnt, l.np, 1, st);
+        else launch_gemm<2, 1, false, false, EPI_DZ, 4>(g, cnt, l.np, 1, st);
         if (dx) {
             XentGemm q = {};
             q.scales = g.scales;
             q.a[0] = dzh; q.a[1] = dzl; q.b[0] = wh; q.b[1] = wl;
             q.lda = l.vc; q.ldb = l.ep; q.kiters = (int)(cnt / BK);
             q.out = (float*)(ws + l.dxw); q.ldo = l.ep; q.np = l.np; q.class0 = c0;
-            const dim3 gx((unsigned)(l.np / 128), (unsigned)(l.ep / 128), (unsigned)l.nx);
-            if (xf) launch_gemm<2, 2, false, true, EPI_DX>(q, gx, st);
-            else launch_gemm<1, 1, false, true, EPI_DX>(q, gx, st);
+            if (xf) launch_gemm<2, 2, false, true, EPI_DX, 4>(q, l.np, l.ep, l.nx, st);
+            else launch_gemm<1, 1, false, true, EPI_DX, 4>(q, l.np, l.ep, l.nx, st);
         }
         if (dw || db) {
             XentGemm q = {};
@@ -1427,9 +1428,8 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
             q.a[0] = xh; q.a[1] = xl; q.b[0] = dzh; q.b[1] = dzl;
             q.lda = l.ep; q.ldb = l.vc; q.kiters = (int)(l.np / BK);
             q.out = (float*)(ws + l.slabs); q.outb = (float*)(ws + l.slabs_b); q.ldo = l.vc; q.np = l.ep * l.vc;
-            const dim3 gw((unsigned)(l.ep / 128), (unsigned)(cnt / 128), (unsigned)l.nz);
-            if (xf) launch_gemm<2, 2, true, true, EPI_DW>(q, gw, st);
-            else launch_gemm<1, 2, true, true, EPI_DW>(q, gw, st);
+            if (xf) launch_gemm<2, 2, true, true, EPI_DW, 2>(q, l.ep, cnt, l.nz, st);
+            else launch_gemm<1, 2, true, true, EPI_DW, 2>(q, l.ep, cnt, l.nz, st);
             hipLaunchKernelGGL(xent_dw_reduce_kernel, dim3((unsigned)(up(cnt, 256) / 256), (unsigned)(e + 1)), dim3(256), 0, st,
                                q.out, q.outb, g.scales, dw, db, (int)l.nz, (long)q.np, (long)l.vc, (int)e, (long)v, (long)c0,
                                accumulate);
