@@ -49,6 +49,13 @@ __device__ __forceinline__ void lds_dma4(const void* base, int off, unsigned dst
 }
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kLowest = -3.402823466e38f;
+// Where the results of the dW products go when the contraction is not split: the gradients themselves (slabs otherwise).
+struct XentOut {
+    float *dw, *db;               // of the piece's first class
+    long v, cnt;                  // classes of W, valid classes of the piece
+    int e, accumulate, direct;
+};
+
 constexpr float kDz = 16384.f;                     // dz planes hold 2^14 dz / (largest |dloss|, rounded up to a power of two)
 constexpr int kMaxParts = 512;
 
@@ -260,6 +267,7 @@ struct XentGemm {
     float *zlab, *out, *outb;
     f16_t *dzh, *dzl;
     long np, ldo, class0;              // class0: first class of the piece
+    XentOut o;                         // DW
 };
 
 enum { EPI_FWD = 0, EPI_DZ = 1, EPI_DX = 2, EPI_DW = 3 };
@@ -439,7 +447,30 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
                     *o = g.class0 == 0 ? acc[i][j][k] : *o + acc[i][j][k];
                 }
     } else {
-        // A: features, B: classes; slab z of the piece
+        // A: features, B: classes; the gradients, or slab z of the piece
+        if (g.o.direct) {
+            const float fb = g.scales[2] / kDz, fw = fb / g.scales[1];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const long c = nw + j * 32 + r;
+                if (c >= g.o.cnt) continue;
+                if (g.o.dw) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const long f = mw + i * 32 + acc_row(k, lane);
+                            if (f < g.o.e) {
+                                float* d = g.o.dw + f * g.o.v + c;
+                                const float q = acc[i][j][k] * fw;
+                                *d = g.o.accumulate ? *d + q : q;
+                            }
+                        }
+                }
+                if (bias_wave && h == 0 && g.o.db) g.o.db[c] = g.o.accumulate ? g.o.db[c] + accb[j][0] * fb : accb[j][0] * fb;
+            }
+            return;
+        }
         float* out = g.out + (long)blockIdx.z * g.np;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -489,6 +520,7 @@ struct XentStream {
     float* out;                                     // DX: part x rows x EP; DW: part x EP x classes
     float* outb;                                    // DW: part x classes
     long ld;                                        // rows (FWD, DX) or classes (DW), padded
+    XentOut o;                                      // DW
 };
 
 // compile-time unrolled loop: f(integral_constant<int, I>) for I in [I0, N)
@@ -810,12 +842,34 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                     *(f32x4*)(o + 32 * eb + 8 * q + 4 * h) =
                         (f32x4){dacc[eb][b][4 * q], dacc[eb][b][4 * q + 1], dacc[eb][b][4 * q + 2], dacc[eb][b][4 * q + 3]};
         } else {
+            const float so = __shfl_xor(ssum[b], 32, 64);
+            if (g.o.direct) {
+                if (it >= g.o.cnt) continue;
+                const float fb_ = g.scales[2] / kDz, fw = fb_ / g.scales[1];
+                if (g.o.dw) {
+#pragma unroll
+                    for (int eb = 0; eb < EB; ++eb)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int f = 32 * eb + acc_row(i, lane);
+                            if (f < g.o.e) {
+                                float* d = g.o.dw + f * g.o.v + it;
+                                const float q = dacc[eb][b][i] * fw;
+                                *d = g.o.accumulate ? *d + q : q;
+                            }
+                        }
+                }
+                if (h == 0 && g.o.db) {
+                    const float q = (ssum[b] + so) * fb_;
+                    g.o.db[it] = g.o.accumulate ? g.o.db[it] + q : q;
+                }
+                continue;
+            }
             float* o = g.out + (long)blockIdx.y * EP * g.ld + it;
 #pragma unroll
             for (int eb = 0; eb < EB; ++eb)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[(32 * eb + acc_row(i, lane)) * g.ld] = dacc[eb][b][i];
-            const float so = __shfl_xor(ssum[b], 32, 64);
             if (h == 0) g.outb[(long)blockIdx.y * g.ld + it] = ssum[b] + so;
         }
     }
@@ -1186,13 +1240,13 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
     l.vp = up(v, l.narrow ? 128 : 256);
     l.ep = up(e, 128);
     // Parts of a contraction of `tiles` steps by `wgs` workgroups, `slots` of which run at once: a step takes step_us, and each part
-    // costs a start of half a step's latency (1 us) and `bytes` written and read once more for the join at 4 TB/s.
-    auto split = [](int64_t wgs, int64_t tiles, int64_t slots, double step_us, double bytes) {
+    // costs a start of half a step's latency (1 us) and `bytes` written and read once more for the join at 4 TB/s (one part of dW goes to the gradient itself).
+    auto split = [](int64_t wgs, int64_t tiles, int64_t slots, double step_us, double bytes, bool direct = false) {
         int64_t best = 1;
         double least = 1e30;
         for (int64_t p = 1; p <= 32 && (p == 1 || tiles / p >= 4); ++p) {
             const double rounds = (double)((wgs * p + slots - 1) / slots);
-            const double t = rounds * ((double)((tiles + p - 1) / p) * step_us + 1.0) + (double)p * bytes * 2.0 / 4e6;
+            const double t = rounds * ((double)((tiles + p - 1) / p) * step_us + 1.0) + (direct && p == 1 ? 0.0 : 4.0 + (double)p * bytes * 2.0 / 4e6);
             if (t < least) {
                 least = t;
                 best = p;
@@ -1203,7 +1257,7 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
     if (l.narrow) {      // step times: 128 (256) resident items x 32 streamed x 128 features at 1 PFLOP/s over the slots
         l.nf = split(l.np / l.rows_wg, l.vp / ST, 512, xf32 ? 1.6 : 2.1, 8.0 * (double)l.np);
         l.nx = split(l.np / l.rows_wg, l.vp / ST, xf32 ? 512 : 256, xf32 ? 3.2 : 1.1, 4.0 * (double)(l.np * l.ep));
-        l.nz = split(l.vp / 128, l.np / ST, 512, xf32 ? 3.2 : 2.1, 4.0 * (double)(l.ep * l.vp));
+        l.nz = split(l.vp / 128, l.np / ST, 512, xf32 ? 3.2 : 2.1, 4.0 * (double)(l.ep * l.vp), true);
     }
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -1227,8 +1281,8 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
         l.row = take(l.np * 8);
         l.vc = l.vp;
         l.dxw = take(l.nx * l.np * l.ep * 4);
-        l.slabs = take(l.nz * l.ep * l.vp * 4);
-        l.slabs_b = take(l.nz * l.vp * 4);
+        l.slabs = l.nz > 1 ? take(l.nz * l.ep * l.vp * 4) : 0;
+        l.slabs_b = l.nz > 1 ? take(l.nz * l.vp * 4) : 0;
     } else {
         l.row = take(l.np * 8);
         // a piece of the classes: dz planes of about 128 MB, which the 256 MB last-level cache holds
@@ -1237,12 +1291,12 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
         if (l.vc > l.vp) l.vc = l.vp;
         // a step: 256 x 128 x 32 with one to three plane products at 1 PFLOP/s over the slots
         l.nx = split((l.np / 256) * (l.ep / 128), l.vc / BK, 256, xf32 ? 1.6 : 0.55, 4.0 * (double)(l.np * l.ep));
-        l.nz = split((l.ep / 128) * (l.vc / 256), l.np / BK, 256, xf32 ? 1.6 : 1.1, 4.0 * (double)(l.ep * l.vc));
+        l.nz = split((l.ep / 128) * (l.vc / 256), l.np / BK, 256, xf32 ? 1.6 : 1.1, 4.0 * (double)(l.ep * l.vc), true);
         l.dzh = take(l.np * l.vc * 2);
         l.dzl = take(l.np * l.vc * 2);
         l.dxw = take(l.nx * l.np * l.ep * 4);
-        l.slabs = take(l.nz * l.ep * l.vc * 4);
-        l.slabs_b = take(l.nz * l.vc * 4);
+        l.slabs = l.nz > 1 ? take(l.nz * l.ep * l.vc * 4) : 0;
+        l.slabs_b = l.nz > 1 ? take(l.nz * l.vc * 4) : 0;
     }
     l.total = at;
     return l;
@@ -1394,9 +1448,10 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
         if (dw || db) {
             q.r[0] = wh; q.r[1] = wl; q.s[0] = xh; q.s[1] = xl;
             q.tiles = (int)(l.np / ST); q.out = (float*)(ws + l.slabs); q.outb = (float*)(ws + l.slabs_b); q.ld = l.vp;
+            q.o = {dw, db, (long)v, (long)v, (int)e, accumulate, l.nz == 1};
             if (xf) launch_stream<2, 2, 1, MODE_DW, 2>(q, l.vp / 128, l.nz, st);
             else launch_stream<2, 1, 1, MODE_DW, 2>(q, l.vp / 128, l.nz, st);
-            hipLaunchKernelGGL(xent_dw_reduce_kernel, dim3((unsigned)(up(l.vp, 256) / 256), (unsigned)(e + 1)), dim3(256), 0, st,
+            if (l.nz > 1) hipLaunchKernelGGL(xent_dw_reduce_kernel, dim3((unsigned)(up(l.vp, 256) / 256), (unsigned)(e + 1)), dim3(256), 0, st,
                                q.out, q.outb, q.scales, dw, db, (int)l.nz, (long)(l.ep * l.vp), (long)l.vp, (int)e, (long)v, 0L,
                                accumulate);
         }
@@ -1428,9 +1483,11 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
             q.a[0] = xh; q.a[1] = xl; q.b[0] = dzh; q.b[1] = dzl;
             q.lda = l.ep; q.ldb = l.vc; q.kiters = (int)(l.np / BK);
             q.out = (float*)(ws + l.slabs); q.outb = (float*)(ws + l.slabs_b); q.ldo = l.vc; q.np = l.ep * l.vc;
+            const int64_t valid = v - c0 < cnt ? v - c0 : cnt;
+            q.o = {dw ? dw + c0 : nullptr, db ? db + c0 : nullptr, (long)v, (long)valid, (int)e, accumulate, l.nz == 1};
             if (xf) launch_gemm<2, 2, true, true, EPI_DW, 2>(q, l.ep, cnt, l.nz, st);
             else launch_gemm<1, 2, true, true, EPI_DW, 2>(q, l.ep, cnt, l.nz, st);
-            hipLaunchKernelGGL(xent_dw_reduce_kernel, dim3((unsigned)(up(cnt, 256) / 256), (unsigned)(e + 1)), dim3(256), 0, st,
+            if (l.nz > 1) hipLaunchKernelGGL(xent_dw_reduce_kernel, dim3((unsigned)(up(cnt, 256) / 256), (unsigned)(e + 1)), dim3(256), 0, st,
                                q.out, q.outb, g.scales, dw, db, (int)l.nz, (long)q.np, (long)l.vc, (int)e, (long)v, (long)c0,
                                accumulate);
         }
