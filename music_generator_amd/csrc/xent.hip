@@ -486,7 +486,7 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
 }
 
 // ---------------------------------------------------------------- narrow features
-// Up to EP features (EP = 128) the two products around the exponential run in one kernel and no dz is stored.  One operand is
+// Up to EP features (EP = 64 or 128) the two products around the exponential run in one kernel and no dz is stored.  One operand is
 // resident: a wave keeps 32 RB of its items (rows of x, or classes) as B fragments in registers.  The other is streamed: tiles of
 // 32 of its items in LDS, a ring of four filled by LDS-DMA and shared by the four waves.  Per streamed tile:
 //     S (32 streamed x 32 RB resident) = bias + sum over plane products                  first product
@@ -550,13 +550,13 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
     const int per = (g.tiles + gridDim.y - 1) / gridDim.y;
     const int t0 = blockIdx.y * per, t1 = t0 + per < g.tiles ? t0 + per : g.tiles;
 
-    // LDS-DMA of tile t: a wave fills 1 KB pieces (4 rows of 256 B), lane l the 16-byte place l of the piece with the chunk that
-    // belongs there.  In assembly: in front of a transposed LDS read the compiler waits for every LDS-DMA it knows of, the
+    // LDS-DMA of tile t: a wave fills 1 KB pieces (4 rows of 256 B or 8 of 128 B), lane l the 16-byte place l of the piece with
+    // the chunk that belongs there: the swizzle of the lane's row in the first piece, and a bit that is uniform in later ones.  In assembly: in front of a transposed LDS read the compiler waits for every LDS-DMA it knows of, the
     // one just issued for a later tile included.
-    static_assert(ROWB == 256, "a piece is four rows");
     // beside the planes: FWD and DX the biases, DW (lse, dloss) and the labels of the tile's items
     const void* ip = MODE != MODE_DW ? (const void*)g.bias : wv == 0 ? (const void*)g.row : (const void*)g.lab;
-    const int lo0 = (lane >> 4) * ROWB + (((lane & 15) ^ ((lane >> 4) << 2)) << 4);
+    const int lrow = EP == 128 ? lane >> 4 : lane >> 3;
+    const int lo0 = lrow * ROWB + (((lane & (EP / 8 - 1)) ^ swz_item<EP>(lrow)) << 4);
     auto stage = [&](int t) {
         const unsigned dst = lds_byte(lds) + (t & 3) * BUF;
         constexpr int PIECES = SPLANE / 1024;
@@ -564,8 +564,8 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
         for (int pl = 0; pl < NS; ++pl)
 #pragma unroll
             for (int i = 0; i < PIECES / 4; ++i) {
-                const int piece = wv * (PIECES / 4) + i;                       // rows 4 piece ..: bits 2-3 of the row are piece & 3
-                lds_dma16(g.s[pl] + ((long)t * SPLANE + piece * 1024) / 2, lo0 ^ ((piece & 3) << 4), dst + pl * SPLANE + piece * 1024);
+                const int piece = wv * (PIECES / 4) + i, flip = EP == 128 ? (piece & 3) << 4 : (piece & 1) << 5;
+                lds_dma16(g.s[pl] + ((long)t * SPLANE + piece * 1024) / 2, lo0 ^ flip, dst + pl * SPLANE + piece * 1024);
             }
         if (wv < (MODE == MODE_DW ? 2 : 1)) {        // 64 floats, or 32 twice
             const bool two = MODE == MODE_DW && wv == 0;
@@ -888,20 +888,33 @@ __device__ __forceinline__ float sum_parts(const float* __restrict__ p, int n, l
     return s;
 }
 
-// dx from its parts, in order
-__global__ __launch_bounds__(256) void xent_dx_join_kernel(const float* __restrict__ parts, const float* __restrict__ scales,
-                                                           const float2* __restrict__ rowinfo, void* __restrict__ dx, int dx_f32, int np,
-                                                           long part, long n, int e, int ep) {
+// dx from its parts in G groups of consecutive parts, then the groups in order: one group where the outputs fill the chip, sixteen
+// where they are few and the parts many
+template <int G>
+__global__ __launch_bounds__(G == 1 ? 256 : 1024) void xent_dx_join_kernel(const float* __restrict__ parts, const float* __restrict__ scales,
+                                                                           const float2* __restrict__ rowinfo, void* __restrict__ dx,
+                                                                           int dx_f32, int np, long part, long n, int e, int ep) {
+    constexpr int W = G == 1 ? 256 : 64;
+    __shared__ float red[G][G == 1 ? 1 : 64];
     const float f = scales[2] / kDz / scales[0];             // streamed: the parts hold 2^14 dz / dloss, the rows 2^14 dloss / scales[2]
-    const long total = n * ep;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+    const int lane = threadIdx.x % W, q = threadIdx.x / W;
+    const int per = (np + G - 1) / G, p0 = q * per, cnt = np - p0 < per ? np - p0 : per;
+    for (long i = (long)blockIdx.x * W + lane; i - lane < n * ep; i += (long)gridDim.x * W) {
+        float s = i < n * ep && cnt > 0 ? sum_parts(parts + p0 * part + i, cnt, part) : 0.f;
+        if constexpr (G > 1) {
+            __syncthreads();
+            red[q][lane] = s;
+            __syncthreads();
+            if (q == 0)
+                for (int k = 1; k < G; ++k) s += red[k][lane];
+        }
         const long row = i / ep;
         const int c = (int)(i - row * ep);
-        if (c >= e) continue;
-        float s = sum_parts(parts + i, np, part);
-        s *= rowinfo ? f * (rowinfo[row].y / kDz) : f;
-        if (dx_f32) ((float*)dx)[row * e + c] = s;
-        else ((bf16_t*)dx)[row * e + c] = (bf16_t)s;
+        if (q == 0 && row < n && c < e) {
+            s *= rowinfo ? f * (rowinfo[row].y / kDz) : f;
+            if (dx_f32) ((float*)dx)[row * e + c] = s;
+            else ((bf16_t*)dx)[row * e + c] = (bf16_t)s;
+        }
     }
 }
 
@@ -1238,15 +1251,15 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
     l.rows_wg = l.narrow && xf32 ? 128 : 256;
     l.np = up(n, l.rows_wg);
     l.vp = up(v, l.narrow ? 128 : 256);
-    l.ep = up(e, 128);
+    l.ep = e <= 64 ? 64 : up(e, 128);
     // Parts of a contraction of `tiles` steps by `wgs` workgroups, `slots` of which run at once: a step takes step_us, and each part
     // costs a start of half a step's latency (1 us) and `bytes` written and read once more for the join at 4 TB/s (one part of dW goes to the gradient itself).
     auto split = [](int64_t wgs, int64_t tiles, int64_t slots, double step_us, double bytes, bool direct = false) {
         int64_t best = 1;
         double least = 1e30;
-        for (int64_t p = 1; p <= 32 && (p == 1 || tiles / p >= 4); ++p) {
+        for (int64_t p = 1; p <= 128 && (p == 1 || tiles / p >= 4); ++p) {
             const double rounds = (double)((wgs * p + slots - 1) / slots);
-            const double t = rounds * ((double)((tiles + p - 1) / p) * step_us + 1.0) + (direct && p == 1 ? 0.0 : 4.0 + (double)p * bytes * 2.0 / 4e6);
+            const double t = rounds * ((double)((tiles + p - 1) / p) * step_us + 1.0) + (direct && p == 1 ? 0.0 : 4.0 + (double)p * (bytes * 2.0 / 4e6 + 0.05));
             if (t < least) {
                 least = t;
                 best = p;
@@ -1254,10 +1267,12 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
         }
         return best;
     };
-    if (l.narrow) {      // step times: 128 (256) resident items x 32 streamed x 128 features at 1 PFLOP/s over the slots
-        l.nf = split(l.np / l.rows_wg, l.vp / ST, 512, xf32 ? 1.6 : 2.1, 8.0 * (double)l.np);
-        l.nx = split(l.np / l.rows_wg, l.vp / ST, xf32 ? 512 : 256, xf32 ? 3.2 : 1.1, 4.0 * (double)(l.np * l.ep));
-        l.nz = split(l.vp / 128, l.np / ST, 512, xf32 ? 3.2 : 2.1, 4.0 * (double)(l.ep * l.vp), true);
+    if (l.narrow) {      // step times: 128 (256) resident items x 32 streamed x 128 (64) features at 1 PFLOP/s over the slots
+        const double f = l.ep == 64 ? 0.6 : 1.0;
+        l.nf = split(l.np / l.rows_wg, l.vp / ST, 512, f * (xf32 ? 1.6 : 2.1), 8.0 * (double)l.np);
+        l.nx = split(l.np / l.rows_wg, l.vp / ST, xf32 || l.ep == 64 ? 512 : 256, f * (xf32 ? 3.2 : l.ep == 64 ? 2.2 : 1.1),
+                     4.0 * (double)(l.np * l.ep));
+        l.nz = split(l.vp / 128, l.np / ST, 512, f * (xf32 ? 3.2 : 2.1), 4.0 * (double)(l.ep * l.vp), true);
     }
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -1316,12 +1331,18 @@ void launch_gemm(const XentGemm& g, int64_t m, int64_t n, int64_t parts, hipStre
                        dim3(512), bytes, st, g);
 }
 
-template <int NR, int NS, int RB, int MODE, int OCC>
-void launch_stream(const XentStream& g, int64_t wgs, int64_t parts, hipStream_t st) {
+template <int EP, int NR, int NS, int RB, int MODE, int OCC>
+void launch_stream_ep(const XentStream& g, int64_t wgs, int64_t parts, hipStream_t st) {
     static std::atomic<uint64_t> done{0};
-    constexpr int bytes = 4 * (NS * ST * 256 + 1024);
-    mgx_allow_dynamic_lds(xent_stream_kernel<128, NR, NS, RB, MODE, OCC>, bytes, done);
-    hipLaunchKernelGGL((xent_stream_kernel<128, NR, NS, RB, MODE, OCC>), dim3((unsigned)wgs, (unsigned)parts), dim3(256), bytes, st, g);
+    constexpr int bytes = 4 * (NS * ST * EP * 2 + 1024);
+    mgx_allow_dynamic_lds(xent_stream_kernel<EP, NR, NS, RB, MODE, OCC>, bytes, done);
+    hipLaunchKernelGGL((xent_stream_kernel<EP, NR, NS, RB, MODE, OCC>), dim3((unsigned)wgs, (unsigned)parts), dim3(256), bytes, st, g);
+}
+
+template <int NR, int NS, int RB, int MODE, int OCC>
+void launch_stream(const Layout& l, const XentStream& g, int64_t wgs, int64_t parts, hipStream_t st) {
+    if (l.ep == 64) launch_stream_ep<64, NR, NS, RB, MODE, 2>(g, wgs, parts, st);
+    else launch_stream_ep<128, NR, NS, RB, MODE, OCC>(g, wgs, parts, st);
 }
 
 void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const float* w, const float* b, const int* labels,
@@ -1350,10 +1371,16 @@ void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const floa
 }
 
 void launch_dx_join(const Layout& l, char* ws, const float2* row, void* dx, bool xf32, int64_t n, int64_t e, hipStream_t st) {
-    const int64_t blocks = up(n * l.ep, 256) / 256;
-    hipLaunchKernelGGL(xent_dx_join_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st,
-                       (const float*)(ws + l.dxw), (const float*)(ws + l.scales), row, dx, (int)xf32, (int)l.nx, (long)(l.np * l.ep),
-                       (long)n, (int)e, (int)l.ep);
+    const float *parts = (const float*)(ws + l.dxw), *scales = (const float*)(ws + l.scales);
+    const long part = (long)(l.np * l.ep);
+    if (l.nx >= 16 && n * l.ep <= 1 << 18) {
+        hipLaunchKernelGGL(xent_dx_join_kernel<16>, dim3((unsigned)(up(n * l.ep, 64) / 64)), dim3(1024), 0, st, parts, scales, row, dx,
+                           (int)xf32, (int)l.nx, part, (long)n, (int)e, (int)l.ep);
+    } else {
+        const int64_t blocks = up(n * l.ep, 256) / 256;
+        hipLaunchKernelGGL(xent_dx_join_kernel<1>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, parts, scales, row, dx,
+                           (int)xf32, (int)l.nx, part, (long)n, (int)e, (int)l.ep);
+    }
 }
 
 }  // namespace
@@ -1395,8 +1422,8 @@ extern "C" int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, c
         q.r[0] = g.b[0]; q.r[1] = g.b[1]; q.s[0] = g.a[0]; q.s[1] = g.a[1];
         q.scales = g.scales; q.bias = g.bias; q.lab = g.lab; q.tiles = (int)(l.vp / ST);
         q.part = g.part; q.zlab = g.zlab; q.ld = l.np;
-        if (xf) launch_stream<2, 2, 1, MODE_FWD, 2>(q, l.np / l.rows_wg, l.nf, st);
-        else launch_stream<1, 2, 2, MODE_FWD, 2>(q, l.np / l.rows_wg, l.nf, st);
+        if (xf) launch_stream<2, 2, 1, MODE_FWD, 2>(l, q, l.np / l.rows_wg, l.nf, st);
+        else launch_stream<1, 2, 2, MODE_FWD, 2>(l, q, l.np / l.rows_wg, l.nf, st);
     } else if (xf) {
         launch_gemm<2, 2, false, false, EPI_FWD, 4>(g, l.vp, l.np, 1, st);
     } else {
@@ -1441,16 +1468,16 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
         if (dx) {
             q.r[0] = xh; q.r[1] = xl; q.s[0] = wh; q.s[1] = wl;
             q.tiles = (int)(l.vp / ST); q.out = (float*)(ws + l.dxw); q.ld = l.np;
-            if (xf) launch_stream<2, 2, 1, MODE_DX, 2>(q, l.np / l.rows_wg, l.nx, st);
-            else launch_stream<1, 1, 2, MODE_DX, 1>(q, l.np / l.rows_wg, l.nx, st);
+            if (xf) launch_stream<2, 2, 1, MODE_DX, 2>(l, q, l.np / l.rows_wg, l.nx, st);
+            else launch_stream<1, 1, 2, MODE_DX, 1>(l, q, l.np / l.rows_wg, l.nx, st);
             launch_dx_join(l, ws, q.row, dx, xf, n, e, st);
         }
         if (dw || db) {
             q.r[0] = wh; q.r[1] = wl; q.s[0] = xh; q.s[1] = xl;
             q.tiles = (int)(l.np / ST); q.out = (float*)(ws + l.slabs); q.outb = (float*)(ws + l.slabs_b); q.ld = l.vp;
             q.o = {dw, db, (long)v, (long)v, (int)e, accumulate, l.nz == 1};
-            if (xf) launch_stream<2, 2, 1, MODE_DW, 2>(q, l.vp / 128, l.nz, st);
-            else launch_stream<2, 1, 1, MODE_DW, 2>(q, l.vp / 128, l.nz, st);
+            if (xf) launch_stream<2, 2, 1, MODE_DW, 2>(l, q, l.vp / 128, l.nz, st);
+            else launch_stream<2, 1, 1, MODE_DW, 2>(l, q, l.vp / 128, l.nz, st);
             if (l.nz > 1) hipLaunchKernelGGL(xent_dw_reduce_kernel, dim3((unsigned)(up(l.vp, 256) / 256), (unsigned)(e + 1)), dim3(256), 0, st,
                                q.out, q.outb, q.scales, dw, db, (int)l.nz, (long)(l.ep * l.vp), (long)l.vp, (int)e, (long)v, 0L,
                                accumulate);
