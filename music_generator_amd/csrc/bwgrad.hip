@@ -288,8 +288,8 @@ struct FGeo {
 __device__ __forceinline__ int sw_off(int p, int c16) { return p * 64 + ((c16 ^ ((p >> 2) & 3)) << 4); }
 
 // X8: X is the 8-bit tape of the layer input (tape8.h), x its codes and xe its exponent bytes: 33 instead of 64 bytes
-// are read per 32 channels.  A thread loads the eight codes of a 16-byte piece and turns them into the piece when it
-// writes it to LDS; everything behind the staging is the same.
+// are read per 32 channels.  A thread loads the eight codes of a 16-byte piece and turns them into the piece between the
+// MFMAs of the tile before; everything behind the staging is the same.
 template <int KH, int KW, bool ACT, int CIN, bool X8>
 __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const void* __restrict__ x,
                                                       const unsigned char* __restrict__ xe,
@@ -329,9 +329,7 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const voi
     u32x4 sg[GITER], sx[X8 ? 1 : XITER];
     u32x2 sc[X8 ? XITER : 1];
     unsigned se[X8 ? XITER : 1];
-    auto stage_load = [&](long t) {
-        long img; int h0, w0;
-        tile_of(t, img, h0, w0);
+    auto load_g = [&](long img, int h0, int w0) {
         const int hb = h0 - gy0, wb = w0 - gx0;
         const long gband = ((img * H + hb) * (long)W) * 32;
         const __amdgpu_buffer_rsrc_t rg =
@@ -345,6 +343,8 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const voi
             const unsigned off = ok ? (unsigned)(((ty * W + (tx + wb)) * 32 + q4 * 8) * 2) : 0xfffffff0u;
             sg[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rg, off, 0, 0));
         }
+    };
+    auto load_x = [&](long img, int h0, int w0) {
         // X tile: 4 NCH 16-byte pieces a position, consecutive threads on consecutive pieces
         const long xband = ((img * H + h0) * (long)W) * CIN;
         const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
@@ -365,20 +365,50 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const voi
             }
         }
     };
-    auto stage_write = [&](int b) {
+    auto stage_load = [&](long t) {
+        long img; int h0, w0;
+        tile_of(t, img, h0, w0);
+        if constexpr (X8) {          // the codes are turned into bf16 before the gradients are written: in front
+            load_x(img, h0, w0);
+            load_g(img, h0, w0);
+        } else {
+            load_g(img, h0, w0);
+            load_x(img, h0, w0);
+        }
+    };
+    // X8: chunk q (two of eight values, the LDS write with the last) of piece i
+    u32x4 xo;
+    float xstep = 0.f, xoff = 0.f;
+    auto x8_chunk = [&](auto I_, int b) {
+        constexpr int i = decltype(I_)::value / 4, q = decltype(I_)::value % 4;
+        if constexpr (q == 0) {
+            xstep = tape8_step(se[X8 ? i : 0]);
+            xoff = -127.5f * xstep;
+        }
+        const unsigned c = sc[X8 ? i : 0][q >> 1] >> (16 * (q & 1));
+        xo[q] = tape8_bf16_pair(__builtin_fmaf((float)(c & 0xffu), xstep, xoff), __builtin_fmaf((float)((c >> 8) & 0xffu), xstep, xoff));
+        if constexpr (q == 3) {
+            const int pc = tid + 256 * i, px = pc / (4 * NCH), sub = pc - px * (4 * NCH);
+            if (256 * (i + 1) <= XPIX * NCH * 4 || px < XPIX)
+                *(u32x4*)(xbuf + (b * NCH + (sub >> 2)) * XPIX * 64 + sw_off(px, sub & 3)) = xo;
+        }
+    };
+    auto stage_write = [&](int b, auto with_x) {
 #pragma unroll
         for (int i = 0; i < GITER; ++i) {
             const int px = (tid >> 2) + 64 * i;
             const int ty = px / GW, tx = px - ty * GW;
             if (64 * (i + 1) <= GPIX || px < GPIX) *(u32x4*)(gbuf + b * GPIX * 64 + ty * ROWB + sw_off(tx, q4)) = sg[i];
         }
+        if constexpr (X8) {
+            if constexpr (decltype(with_x)::value) static_for<0, 4 * XITER>([&](auto I_) { x8_chunk(I_, b); });
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < XITER; ++i) {
             const int pc = tid + 256 * i, px = pc / (4 * NCH), sub = pc - px * (4 * NCH);
             if (256 * (i + 1) <= XPIX * NCH * 4 || px < XPIX) {
-                unsigned char* dst = xbuf + (b * NCH + (sub >> 2)) * XPIX * 64 + sw_off(px, sub & 3);
-                if constexpr (X8) *(u32x4*)dst = tape8_bf16x8(sc[i], se[i]);
-                else *(u32x4*)dst = sx[i];
+                *(u32x4*)(xbuf + (b * NCH + (sub >> 2)) * XPIX * 64 + sw_off(px, sub & 3)) = sx[X8 ? 0 : i];
             }
         }
     };
@@ -429,13 +459,13 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const voi
     int cur = 0;
     if (t < ntiles) {
         stage_load(t);
-        stage_write(0);
+        stage_write(0, std::true_type{});
     }
     __syncthreads();
     while (t < ntiles) {
         const long tn = t + nslots;
         const bool has_next = tn < ntiles;
-        if (has_next) stage_load(tn);
+        if (X8 || has_next) stage_load(has_next ? tn : t);       // X8: the last tile again, which keeps its blocks free of branches
         long img; int h0, w0;
         tile_of(t, img, h0, w0);
         // One 32-position block at a time (row wr, columns col0 .. col0 + 31), its MFMAs in stages of one kernel row:
@@ -497,8 +527,11 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const voi
         };
         // MFMA M of stage S (the centre tap's second one sums the unshifted window for the bias gradient), with the
         // reads and epilogue pieces that go around it
-        auto step = [&](auto S_, auto M_) {
-            constexpr int S = decltype(S_)::value, m = decltype(M_)::value;
+        // X8: the blocks 2 and 3 of a tile, when the next tile's codes have arrived, turn them into bf16 between the MFMAs of
+        // their data gradients (chunk by chunk, evenly)
+        constexpr int ND = KH * NJ;
+        auto step = [&](auto IT_, auto S_, auto M_) {
+            constexpr int S = decltype(S_)::value, m = decltype(M_)::value, IT = decltype(IT_)::value;
             constexpr bool dstage = S < KH;
             constexpr int st = dstage ? 0 : S - KH, ks = st / KH, ta = dstage ? S : st - ks * KH;
             constexpr int nm = dstage ? NJ : KW + (ta == PT ? 1 : 0);
@@ -515,6 +548,11 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const voi
                 else acc[ta * KW + tb] = mfma_bf16(af[ks & 1], wq[st & 1][tb], acc[ta * KW + tb]);
             }
             __builtin_amdgcn_sched_barrier(0);
+            if constexpr (X8 && dstage && IT >= 2) {
+                constexpr int at = (IT - 2) * ND + S * NJ + m, nc = 4 * XITER;
+                static_for<at * nc / (2 * ND), (at + 1) * nc / (2 * ND)>([&](auto I_) { x8_chunk(I_, cur ^ 1); });
+                __builtin_amdgcn_sched_barrier(0);
+            }
             if constexpr (!dstage) {
                 constexpr int wm = ks * (TAPS + 1) + ta * KW + (ta > PT ? 1 : 0) + m;     // weight-gradient MFMAs of the block so far
                 if constexpr (wm >= WM0) {
@@ -525,8 +563,7 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const voi
             }
         };
         static_for<0, NJ>([&](auto I_) { prep(std::integral_constant<int, NSTAGE>{}, I_); });
-#pragma unroll 1
-        for (int it = 0; it < 4; ++it) {
+        auto block = [&](int it, auto IT_) {
             const int wr = CIN == 128 ? it : 2 * wvs + (it >> 1), col0 = CIN == 128 ? 0 : 32 * (it & 1);
             const int itn = (it + 1) & 3;                                      // the last block prepares the first again: unused, in range
             ug = ugb + wr * ROWB + col0 * 64;
@@ -539,10 +576,16 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const voi
             static_for<0, NSTAGE>([&](auto S_) {
                 constexpr int S = decltype(S_)::value;
                 constexpr int nm = S < KH ? NJ : KW + ((S - KH) % KH == PT ? 1 : 0);
-                static_for<0, nm>([&](auto M_) { step(S_, M_); });
+                static_for<0, nm>([&](auto M_) { step(IT_, S_, M_); });
             });
+        };
+        if constexpr (X8) {
+            static_for<0, 4>([&](auto IT_) { block(decltype(IT_)::value, IT_); });
+        } else {
+#pragma unroll 1
+            for (int it = 0; it < 4; ++it) block(it, std::integral_constant<int, 0>{});
         }
-        if (has_next) stage_write(cur ^ 1);
+        if (has_next) stage_write(cur ^ 1, std::false_type{});
         __syncthreads();
         cur ^= 1;
         t = tn;

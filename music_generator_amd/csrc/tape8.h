@@ -73,16 +73,6 @@ __device__ __forceinline__ unsigned tape8_bf16_pair(float lo, float hi) {
     return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, hi), __builtin_bit_cast(unsigned, lo), 0x07060302u);
 }
 
-// eight codes of one block -> eight bf16
-__device__ __forceinline__ u32x4 tape8_bf16x8(u32x2 c, unsigned e) {
-    const float step = tape8_step(e), off = -127.5f * step;
-    float v[8];
-    tape8_value4(c[0], step, off, v);
-    tape8_value4(c[1], step, off, v + 4);
-    return (u32x4){tape8_bf16_pair(v[0], v[1]), tape8_bf16_pair(v[2], v[3]), tape8_bf16_pair(v[4], v[5]),
-                   tape8_bf16_pair(v[6], v[7])};
-}
-
 // dact_from_y (bf16.h) that lets a NaN through, so that a non-finite block reaches the gradients.
 __device__ __forceinline__ float tape8_dact(float y, float inv_alpha, float k1) {
     const float d = __builtin_fmaf(-y, y, k1);
