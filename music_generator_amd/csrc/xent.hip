@@ -134,6 +134,11 @@ __device__ __forceinline__ float scale_from_parts(const unsigned* __restrict__ p
     return scale_of(m);
 }
 
+// The power of two above a magnitude (2^-100 at least, so that reciprocals and ratios stay normal).
+__device__ __forceinline__ float row_scale(float d) {
+    return 16384.f / scale_of(__builtin_bit_cast(unsigned, fmaxf(fabsf(d), 7.9e-31f)));
+}
+
 // ---------------------------------------------------------------- planes
 __device__ __forceinline__ void split8(const float* v, u32x4& hi, u32x4& lo) {
 #pragma unroll
@@ -154,7 +159,12 @@ struct XentPrep {
     int e, ep;                    // features, padded to 128
     f16_t *xh, *xl, *wh, *wl;     // planes: rows x ep, classes x ep
     float *bias, *scales;
-    float2* row;                  // lse (log 2 units), 2^14 dloss / scales[2]
+    // per row: lse (log 2 units) and the factor of its dz.  Streamed: 2^14 dloss / scales[2].  Wide features, where dz is stored:
+    // 2^14 dloss / rs, rs the power of two above |dloss|, so that the dz of a row of small weight keeps its digits; rs goes into
+    // dx, and rs / scales[2] into the planes of x that dW is made of (xsh, xsl) and into the weights of db (ones).
+    float2* row;
+    float* rs;
+    f16_t *xsh, *xsl, *ones;
     int* lab;
     long wtiles, xblocks;
 };
@@ -191,7 +201,7 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
             *(u32x4*)(p.wl + at) = lo;
         }
     } else if ((long)blockIdx.x < p.wtiles + p.xblocks) {
-        const float s = scale_from_parts(p.part, 1, p.parts);
+        const float s = scale_from_parts(p.part, 1, p.parts), sd = p.xsh ? scale_from_parts(p.part, 2, p.parts) : 1.f;
         const int q = p.ep / 8;
         for (long i = ((long)blockIdx.x - p.wtiles) * 256 + tid; i < p.np * q; i += p.xblocks * 256) {
             const long row = i / q;
@@ -223,6 +233,14 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
             split8(v, hi, lo);
             *(u32x4*)(p.xh + row * p.ep + c) = hi;
             if (XF32) *(u32x4*)(p.xl + row * p.ep + c) = lo;
+            if (p.xsh) {
+                const float rel = ok ? row_scale(p.dloss[row]) / sd : 0.f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] *= rel;
+                split8(v, hi, lo);
+                *(u32x4*)(p.xsh + row * p.ep + c) = hi;
+                if (XF32) *(u32x4*)(p.xsl + row * p.ep + c) = lo;
+            }
         }
     } else {
         const float sw = scale_from_parts(p.part, 0, p.parts), sx = scale_from_parts(p.part, 1, p.parts),
@@ -241,8 +259,14 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
             int lab = i < p.n ? p.labels[i] : -1;
             if (lab >= p.v) lab = -1;
             p.lab[i] = lab < 0 ? -1 : lab;
-            if (p.row)                                       // no label: every exponential of the row is 0
-                p.row[i] = lab < 0 ? make_float2(__builtin_inff(), 0.f) : make_float2(p.lse[i] * kLog2e, p.dloss[i] / sd * kDz);
+            if (p.row) {                                     // no label: every exponential of the row is 0
+                const float rs = p.rs && lab >= 0 ? row_scale(p.dloss[i]) : sd;
+                p.row[i] = lab < 0 ? make_float2(__builtin_inff(), 0.f) : make_float2(p.lse[i] * kLog2e, p.dloss[i] / rs * kDz);
+                if (p.rs) {
+                    p.rs[i] = lab < 0 ? 0.f : rs;
+                    p.ones[i] = (f16_t)(lab < 0 ? 0.f : rs / sd);
+                }
+            }
         }
     }
 }
@@ -268,6 +292,7 @@ struct XentGemm {
     f16_t *dzh, *dzl;
     long np, ldo, class0;              // class0: first class of the piece
     XentOut o;                         // DW
+    const f16_t* ones;                 // DW: what the rows' dz weigh in db
 };
 
 enum { EPI_FWD = 0, EPI_DZ = 1, EPI_DX = 2, EPI_DW = 3 };
@@ -331,8 +356,7 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
         acc[0][0][i] = acc[0][1][i] = acc[1][0][i] = acc[1][1][i] = 0.f;
         accb[0][i] = accb[1][i] = 0.f;
     }
-    const bool bias_wave = EPI == EPI_DW && blockIdx.x == 0 && wm == 0;       // sums of B's columns: a product with ones
-    const u32x4 ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+    const bool bias_wave = EPI == EPI_DW && blockIdx.x == 0 && wm == 0;       // sums of B's columns: a product with the rows' weights
 
     if (it0 < it1) stage(it0);
     if (it0 + 1 < it1) stage(it0 + 1);
@@ -363,6 +387,7 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
                     acc[i][j] = mfma_f16(fa[0][i], fb[0][j], acc[i][j]);
                 }
             if (bias_wave) {
+                const u32x4 ones = *(const u32x4*)(g.ones + (long)it * BK + 16 * ks + 8 * h);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     if (NB > 1) accb[j] = mfma_f16(ones, fb[NB - 1][j], accb[j]);
@@ -892,11 +917,13 @@ __device__ __forceinline__ float sum_parts(const float* __restrict__ p, int n, l
 // where they are few and the parts many
 template <int G>
 __global__ __launch_bounds__(G == 1 ? 256 : 1024) void xent_dx_join_kernel(const float* __restrict__ parts, const float* __restrict__ scales,
-                                                                           const float2* __restrict__ rowinfo, void* __restrict__ dx,
+                                                                           const float2* __restrict__ rowinfo, const float* __restrict__ rs,
+                                                                           void* __restrict__ dx,
                                                                            int dx_f32, int np, long part, long n, int e, int ep) {
     constexpr int W = G == 1 ? 256 : 64;
     __shared__ float red[G][G == 1 ? 1 : 64];
-    const float f = scales[2] / kDz / scales[0];             // streamed: the parts hold 2^14 dz / dloss, the rows 2^14 dloss / scales[2]
+    // streamed: the parts hold 2^14 dz / dloss, the rows 2^14 dloss / scales[2]; wide: 2^14 dz / rs
+    const float f = (rs ? 1.f : scales[2] / kDz) / kDz / scales[0];
     const int lane = threadIdx.x % W, q = threadIdx.x / W;
     const int per = (np + G - 1) / G, p0 = q * per, cnt = np - p0 < per ? np - p0 : per;
     for (long i = (long)blockIdx.x * W + lane; i - lane < n * ep; i += (long)gridDim.x * W) {
@@ -911,7 +938,7 @@ __global__ __launch_bounds__(G == 1 ? 256 : 1024) void xent_dx_join_kernel(const
         const long row = i / ep;
         const int c = (int)(i - row * ep);
         if (q == 0 && row < n && c < e) {
-            s *= rowinfo ? f * (rowinfo[row].y / kDz) : f;
+            s *= f * (rs ? rs[row] : rowinfo[row].y);
             if (dx_f32) ((float*)dx)[row * e + c] = s;
             else ((bf16_t*)dx)[row * e + c] = (bf16_t)s;
         }
@@ -1242,7 +1269,7 @@ struct Layout {
     bool narrow;                   // the streamed kernels
     int rows_wg;                   // resident rows of a workgroup (FWD, DX)
     int64_t np, vp, ep, vc, nz, nf, nx;      // nf, nx, nz: parts of the streamed operand in FWD, DX, DW (nz: of the rows in general)
-    int64_t part, bias, scales, lab, zlab, row, xh, xl, wh, wl, slices, dzh, dzl, dxw, slabs, slabs_b, total;
+    int64_t part, bias, scales, lab, zlab, row, rs, ones, xh, xl, xsh, xsl, wh, wl, slices, dzh, dzl, dxw, slabs, slabs_b, total;
 };
 
 Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
@@ -1300,6 +1327,10 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
         l.slabs_b = l.nz > 1 ? take(l.nz * l.vp * 4) : 0;
     } else {
         l.row = take(l.np * 8);
+        l.rs = take(l.np * 4);
+        l.ones = take(l.np * 2);
+        l.xsh = take(l.np * l.ep * 2);
+        l.xsl = xf32 ? take(l.np * l.ep * 2) : 0;
         // a piece of the classes: dz planes of about 128 MB, which the 256 MB last-level cache holds
         l.vc = (int64_t)(128 << 20) / (4 * l.np) / 256 * 256;
         if (l.vc < 256) l.vc = 256;
@@ -1318,7 +1349,7 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
 }
 
 bool sizes_ok(int64_t n, int64_t e, int64_t v) {
-    return n >= 0 && e >= 1 && v >= 1 && n <= 8000000 && v <= 8000000 && e <= 65536;      // rows / 128 and classes / 128 are grid dimensions
+    return n >= 0 && e >= 1 && v >= 1 && n <= 8000000 && v <= 8000000 && e <= 65000;      // rows / 128, classes / 128 and e + 1 are grid dimensions
 }
 
 // m x n results in `parts` parts of the contraction; WM waves of 64 along m, 8 / WM along n
@@ -1362,6 +1393,9 @@ void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const floa
     p.xh = (f16_t*)(ws + l.xh); p.xl = (f16_t*)(ws + l.xl); p.wh = (f16_t*)(ws + l.wh); p.wl = (f16_t*)(ws + l.wl);
     p.bias = (float*)(ws + l.bias); p.scales = (float*)(ws + l.scales); p.lab = (int*)(ws + l.lab);
     p.row = dloss ? (float2*)(ws + l.row) : nullptr;
+    if (dloss && !l.narrow) {
+        p.rs = (float*)(ws + l.rs); p.ones = (f16_t*)(ws + l.ones); p.xsh = (f16_t*)(ws + l.xsh); p.xsl = (f16_t*)(ws + l.xsl);
+    }
     p.wtiles = (l.vp / 64) * (l.ep / 64);
     p.xblocks = up(l.np * l.ep / 8, 256) / 256;
     if (p.xblocks > 2048) p.xblocks = 2048;
@@ -1370,15 +1404,17 @@ void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const floa
     else hipLaunchKernelGGL(xent_prep_kernel<false>, grid, dim3(256), 0, st, p);
 }
 
-void launch_dx_join(const Layout& l, char* ws, const float2* row, void* dx, bool xf32, int64_t n, int64_t e, hipStream_t st) {
+void launch_dx_join(const Layout& l, char* ws, void* dx, bool xf32, int64_t n, int64_t e, hipStream_t st) {
     const float *parts = (const float*)(ws + l.dxw), *scales = (const float*)(ws + l.scales);
     const long part = (long)(l.np * l.ep);
+    const float* rs = l.narrow ? nullptr : (const float*)(ws + l.rs);
+    const float2* row = (const float2*)(ws + l.row);
     if (l.nx >= 16 && n * l.ep <= 1 << 18) {
-        hipLaunchKernelGGL(xent_dx_join_kernel<16>, dim3((unsigned)(up(n * l.ep, 64) / 64)), dim3(1024), 0, st, parts, scales, row, dx,
+        hipLaunchKernelGGL(xent_dx_join_kernel<16>, dim3((unsigned)(up(n * l.ep, 64) / 64)), dim3(1024), 0, st, parts, scales, row, rs, dx,
                            (int)xf32, (int)l.nx, part, (long)n, (int)e, (int)l.ep);
     } else {
         const int64_t blocks = up(n * l.ep, 256) / 256;
-        hipLaunchKernelGGL(xent_dx_join_kernel<1>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, parts, scales, row, dx,
+        hipLaunchKernelGGL(xent_dx_join_kernel<1>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, parts, scales, row, rs, dx,
                            (int)xf32, (int)l.nx, part, (long)n, (int)e, (int)l.ep);
     }
 }
@@ -1470,7 +1506,7 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
             q.tiles = (int)(l.vp / ST); q.out = (float*)(ws + l.dxw); q.ld = l.np;
             if (xf) launch_stream<2, 2, 1, MODE_DX, 2>(l, q, l.np / l.rows_wg, l.nx, st);
             else launch_stream<1, 1, 2, MODE_DX, 1>(l, q, l.np / l.rows_wg, l.nx, st);
-            launch_dx_join(l, ws, q.row, dx, xf, n, e, st);
+            launch_dx_join(l, ws, dx, xf, n, e, st);
         }
         if (dw || db) {
             q.r[0] = wh; q.r[1] = wl; q.s[0] = xh; q.s[1] = xl;
@@ -1507,7 +1543,7 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
         if (dw || db) {
             XentGemm q = {};
             q.scales = g.scales;
-            q.a[0] = xh; q.a[1] = xl; q.b[0] = dzh; q.b[1] = dzl;
+            q.a[0] = (f16_t*)(ws + l.xsh); q.a[1] = (f16_t*)(ws + l.xsl); q.b[0] = dzh; q.b[1] = dzl; q.ones = (f16_t*)(ws + l.ones);
             q.lda = l.ep; q.ldb = l.vc; q.kiters = (int)(l.np / BK);
             q.out = (float*)(ws + l.slabs); q.outb = (float*)(ws + l.slabs_b); q.ldo = l.vc; q.np = l.ep * l.vc;
             const int64_t valid = v - c0 < cnt ? v - c0 : cnt;
@@ -1519,6 +1555,6 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
                                accumulate);
         }
     }
-    if (dx) launch_dx_join(l, ws, nullptr, dx, xf, n, e, st);
+    if (dx) launch_dx_join(l, ws, dx, xf, n, e, st);
     return mgx_launch_status();
 }

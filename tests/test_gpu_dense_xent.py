@@ -428,3 +428,23 @@ def test_a_model_without_a_classifier_head_is_refused():
     from music_generator_amd import evaluacion as E
     with pytest.raises(ValueError):
         E._split_head(M.define_discriminator(1)[0][0])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,e,v", [(9, 20, 300), (90, 40, 700), (200, 128, 900), (150, 300, 1000)])
+def test_weights_of_very_different_size(n, e, v, dtype):
+    """dloss from 1e-7 to 1, of both signs, and zeros: the gradient of every single row is as exact as if it stood alone."""
+    x, w, b, labels, dloss = case(n, e, v, dtype, seed=40 + e, unlabelled=0)
+    gen = torch.Generator().manual_seed(41)
+    dloss = torch.sign(torch.randn((n,), generator=gen)) * 10.0 ** (-7 * torch.rand((n,), generator=gen))
+    dloss[::5] = 0.0
+    want, got = reference(x, w, b, labels, dloss), run(x, w, b, labels, dloss)
+    check(got, want, dtype, float((x.double() @ w.double()).abs().max()))
+    unit = 2.0 ** -23 * (8 + 2 * float((x.double() @ w.double()).abs().max()))
+    # one row: the bound of check() on that row; the label's term of a row is at most |dloss| |W[:, label]|
+    slack = unit * dloss.double().abs() * w.double().norm(dim=0)[labels.long()]
+    tol = 4 * unit + (2.0 ** -8 + 2.0 ** -10 if dtype == torch.bfloat16 else 0.0)
+    off = (got["dx"].double() - want["dx"]).norm(dim=1)
+    assert bool((off <= tol * want["dx"].norm(dim=1) + slack + 1e-30).all()), float((off / want["dx"].norm(dim=1).clamp(min=1e-30)).max())
+    assert bool((got["dx"][dloss == 0] == 0).all())
