@@ -312,6 +312,9 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
     const int per = (g.kiters + gridDim.z - 1) / gridDim.z;
     const int it0 = blockIdx.z * per, it1 = it0 + per < g.kiters ? it0 + per : g.kiters;
 
+    // sums of B's columns: a product with the rows' weights
+    const bool with_bias = EPI == EPI_DW && blockIdx.x == 0, bias_wave = with_bias && wm == 0;
+
     // one plane (T rows) of step it: pieces of 1 KB, 16 rows of 64 B or 2 (4) rows of 512 (256) B
     auto stage_plane = [&](unsigned dst, const f16_t* src, long ld, long o0, int it, auto tr_, auto T_) {
         constexpr bool tr = decltype(tr_)::value;
@@ -337,6 +340,8 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
 #pragma unroll
         for (int pl = 0; pl < NB; ++pl)
             stage_plane(dst + NA * PA + pl * PB, g.b[pl], g.ldb, n0, it, std::integral_constant<bool, BT>{}, std::integral_constant<int, TN>{});
+        // the rows' weights in db, 64 B behind the ring: every wave writes the same, so that each counts its own loads only
+        if (with_bias && lane < 16) lds_dma4(g.ones + (long)it * BK, lane * 4, lds_byte(lds) + 3 * BUF + (it - it0) % 3 * 64);
     };
     const int hk = lane >> 5, cb = (lane >> 4) & 1, qq = (lane >> 2) & 3, pp = lane & 3;
     auto frag = [&](const unsigned char* plane, bool tr, int rowb, int blk, int ks) -> u32x4 {
@@ -356,13 +361,14 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
         acc[0][0][i] = acc[0][1][i] = acc[1][0][i] = acc[1][1][i] = 0.f;
         accb[0][i] = accb[1][i] = 0.f;
     }
-    const bool bias_wave = EPI == EPI_DW && blockIdx.x == 0 && wm == 0;       // sums of B's columns: a product with the rows' weights
-
     if (it0 < it1) stage(it0);
     if (it0 + 1 < it1) stage(it0 + 1);
     for (int it = it0; it < it1; ++it) {
         // step it has landed (the one behind it may be on its way), and no wave reads step it - 1 any more
-        if (it + 1 < it1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");
+        if (it + 1 < it1) {
+            if (with_bias) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES + 1) : "memory");
+            else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");
+        }
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (it + 2 < it1) stage(it + 2);
@@ -387,7 +393,7 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
                     acc[i][j] = mfma_f16(fa[0][i], fb[0][j], acc[i][j]);
                 }
             if (bias_wave) {
-                const u32x4 ones = *(const u32x4*)(g.ones + (long)it * BK + 16 * ks + 8 * h);
+                const u32x4 ones = *(const u32x4*)(lds + 3 * BUF + (it - it0) % 3 * 64 + 32 * ks + 16 * h);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     if (NB > 1) accb[j] = mfma_f16(ones, fb[NB - 1][j], accb[j]);
@@ -1356,7 +1362,7 @@ bool sizes_ok(int64_t n, int64_t e, int64_t v) {
 template <int NA, int NB, bool AT, bool BT, int EPI, int WM>
 void launch_gemm(const XentGemm& g, int64_t m, int64_t n, int64_t parts, hipStream_t st) {
     static std::atomic<uint64_t> done{0};
-    constexpr int bytes = 3 * (NA * 64 * WM + NB * 512 / WM) * BK * 2;
+    constexpr int bytes = 3 * (NA * 64 * WM + NB * 512 / WM) * BK * 2 + (EPI == EPI_DW ? 3 * 64 : 0);
     mgx_allow_dynamic_lds(xent_gemm_kernel<NA, NB, AT, BT, EPI, WM>, bytes, done);
     hipLaunchKernelGGL((xent_gemm_kernel<NA, NB, AT, BT, EPI, WM>), dim3((unsigned)(m / (64 * WM)), (unsigned)(n / (512 / WM)), (unsigned)parts),
                        dim3(512), bytes, st, g);
