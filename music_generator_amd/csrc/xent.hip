@@ -1275,6 +1275,7 @@ struct Layout {
     bool narrow;                   // the streamed kernels
     int rows_wg;                   // resident rows of a workgroup (FWD, DX)
     int64_t np, vp, ep, vc, nz, nf, nx;      // nf, nx, nz: parts of the streamed operand in FWD, DX, DW (nz: of the rows in general)
+    int64_t vm;                    // classes of a piece whose dW is not split, before the ones whose dW has nz parts
     int64_t part, bias, scales, lab, zlab, row, rs, ones, xh, xl, xsh, xsl, wh, wl, slices, dzh, dzl, dxw, slabs, slabs_b, total;
 };
 
@@ -1287,7 +1288,7 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
     l.ep = e <= 64 ? 64 : up(e, 128);
     // Parts of a contraction of `tiles` steps by `wgs` workgroups, `slots` of which run at once: a step takes step_us, and each part
     // costs a start of half a step's latency (1 us) and `bytes` written and read once more for the join at 4 TB/s (one part of dW goes to the gradient itself).
-    auto split = [](int64_t wgs, int64_t tiles, int64_t slots, double step_us, double bytes, bool direct = false) {
+    auto split = [](int64_t wgs, int64_t tiles, int64_t slots, double step_us, double bytes, bool direct = false, double* time = nullptr) {
         int64_t best = 1;
         double least = 1e30;
         for (int64_t p = 1; p <= 128 && (p == 1 || tiles / p >= 4); ++p) {
@@ -1298,6 +1299,7 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
                 best = p;
             }
         }
+        if (time) *time = least;
         return best;
     };
     if (l.narrow) {      // step times: 128 (256) resident items x 32 streamed x 128 (64) features at 1 PFLOP/s over the slots
@@ -1343,12 +1345,26 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
         if (l.vc > l.vp) l.vc = l.vp;
         // a step: 256 x 128 x 32 with one to three plane products at 1 PFLOP/s over the slots
         l.nx = split((l.np / 256) * (l.ep / 128), l.vc / BK, 256, xf32 ? 1.6 : 0.55, 4.0 * (double)(l.np * l.ep));
-        l.nz = split((l.ep / 128) * (l.vc / 256), l.np / BK, 256, xf32 ? 1.6 : 1.1, 4.0 * (double)(l.ep * l.vc), true);
+        // dW: the classes of a piece that fill whole rounds of the 256 CUs are not split, a part round behind them is
+        // (1501 x 1000 x 10001 float32, 320 tiles: dW and its join 127 us, 155 us as two rounds)
+        const double step = xf32 ? 1.6 : 1.1;
+        const int64_t gx = l.ep / 128, gy = l.vc / 256, gm = gx * gy / 256 * 256 / gx;
+        double whole, tail = 0.0;
+        l.nz = split(gx * gy, l.np / BK, 256, step, 4.0 * (double)(l.ep * l.vc), true, &whole);
+        if (gm > 0 && gm < gy) {
+            const int64_t nt = split(gx * (gy - gm), l.np / BK, 256, step, 4.0 * (double)(l.ep * 256 * (gy - gm)), true, &tail);
+            const double rounds = (double)((gx * gm + 255) / 256);
+            if (rounds * ((double)(l.np / BK) * step + 1.0) + 3.0 + tail < whole) {
+                l.nz = nt;
+                l.vm = 256 * gm;
+            }
+        }
+        const int64_t vs = l.vc - l.vm;
         l.dzh = take(l.np * l.vc * 2);
         l.dzl = take(l.np * l.vc * 2);
         l.dxw = take(l.nx * l.np * l.ep * 4);
-        l.slabs = l.nz > 1 ? take(l.nz * l.ep * l.vc * 4) : 0;
-        l.slabs_b = l.nz > 1 ? take(l.nz * l.vc * 4) : 0;
+        l.slabs = l.nz > 1 ? take(l.nz * l.ep * vs * 4) : 0;
+        l.slabs_b = l.nz > 1 ? take(l.nz * vs * 4) : 0;
     }
     l.total = at;
     return l;
@@ -1547,18 +1563,27 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
             else launch_gemm<1, 1, false, true, EPI_DX, 4>(q, l.np, l.ep, l.nx, st);
         }
         if (dw || db) {
-            XentGemm q = {};
-            q.scales = g.scales;
-            q.a[0] = (f16_t*)(ws + l.xsh); q.a[1] = (f16_t*)(ws + l.xsl); q.b[0] = dzh; q.b[1] = dzl; q.ones = (f16_t*)(ws + l.ones);
-            q.lda = l.ep; q.ldb = l.vc; q.kiters = (int)(l.np / BK);
-            q.out = (float*)(ws + l.slabs); q.outb = (float*)(ws + l.slabs_b); q.ldo = l.vc; q.np = l.ep * l.vc;
-            const int64_t valid = v - c0 < cnt ? v - c0 : cnt;
-            q.o = {dw ? dw + c0 : nullptr, db ? db + c0 : nullptr, (long)v, (long)valid, (int)e, accumulate, l.nz == 1};
-            if (xf) launch_gemm<2, 2, true, true, EPI_DW, 2>(q, l.ep, cnt, l.nz, st);
-            else launch_gemm<1, 2, true, true, EPI_DW, 2>(q, l.ep, cnt, l.nz, st);
-            if (l.nz > 1) hipLaunchKernelGGL(xent_dw_reduce_kernel, dim3((unsigned)(up(cnt, 256) / 256), (unsigned)(e + 1)), dim3(256), 0, st,
-                               q.out, q.outb, g.scales, dw, db, (int)l.nz, (long)q.np, (long)l.vc, (int)e, (long)v, (long)c0,
-                               accumulate);
+            // classes [a0, a1) of the piece in nz parts
+            auto weights = [&](int64_t a0, int64_t a1, int64_t nz) {
+                if (a0 >= a1) return;
+                const int64_t vs = l.vc - l.vm, first = c0 + a0;
+                XentGemm q = {};
+                q.scales = g.scales;
+                q.a[0] = (f16_t*)(ws + l.xsh); q.a[1] = (f16_t*)(ws + l.xsl); q.b[0] = dzh + a0; q.b[1] = dzl + a0;
+                q.ones = (f16_t*)(ws + l.ones);
+                q.lda = l.ep; q.ldb = l.vc; q.kiters = (int)(l.np / BK);
+                q.out = (float*)(ws + l.slabs); q.outb = (float*)(ws + l.slabs_b); q.ldo = vs; q.np = l.ep * vs;
+                const int64_t valid = v - first < a1 - a0 ? v - first : a1 - a0;
+                q.o = {dw ? dw + first : nullptr, db ? db + first : nullptr, (long)v, (long)valid, (int)e, accumulate, nz == 1};
+                if (xf) launch_gemm<2, 2, true, true, EPI_DW, 2>(q, l.ep, a1 - a0, nz, st);
+                else launch_gemm<1, 2, true, true, EPI_DW, 2>(q, l.ep, a1 - a0, nz, st);
+                if (nz > 1) hipLaunchKernelGGL(xent_dw_reduce_kernel, dim3((unsigned)(up(a1 - a0, 256) / 256), (unsigned)(e + 1)), dim3(256), 0, st,
+                                   q.out, q.outb, g.scales, dw, db, (int)nz, (long)q.np, (long)vs, (int)e, (long)v, (long)first,
+                                   accumulate);
+            };
+            const int64_t vm = l.vm < cnt ? l.vm : cnt;
+            weights(0, vm, 1);
+            weights(vm, cnt, l.nz);
         }
     }
     if (dx) launch_dx_join(l, ws, dx, xf, n, e, st);

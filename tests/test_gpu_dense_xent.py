@@ -448,3 +448,23 @@ def test_weights_of_very_different_size(n, e, v, dtype):
     off = (got["dx"].double() - want["dx"]).norm(dim=1)
     assert bool((off <= tol * want["dx"].norm(dim=1) + slack + 1e-30).all()), float((off / want["dx"].norm(dim=1).clamp(min=1e-30)).max())
     assert bool((got["dx"][dloss == 0] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("n,e,v", [(3000, 130, 12000), (300, 1000, 9000), (17, 700, 20000), (2000, 100, 9000), (2000, 33, 9000), (20, 128, 30000),
+                                   (16, 600, 3000), (17, 600, 3000)])
+def test_parts_and_pieces(n, e, v, dtype, accumulate):
+    """Sizes whose classes come in several pieces (the first) or whose products are split, with labels at every end."""
+    x, w, b, labels, dloss = case(n, e, v, dtype, seed=50 + e)
+    labels[0], labels[1], labels[2] = 0, v - 1, v // 2
+    want = reference(x, w, b, labels, dloss)
+    if accumulate:
+        gen = torch.Generator().manual_seed(51)
+        dw, db = torch.randn(w.shape, generator=gen) * 1e-3, torch.randn(b.shape, generator=gen) * 1e-3
+        want["dw"], want["db"] = want["dw"] + dw.double(), want["db"] + db.double()
+        got = run(x, w, b, labels, dloss, accumulate=True, dw=dw, db=db)
+    else:
+        got = run(x, w, b, labels, dloss)
+    check(got, want, dtype, float((x.double() @ w.double()).abs().max()))
