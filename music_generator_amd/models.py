@@ -10,6 +10,7 @@ this file only wires layer objects and sequences kernel launches.
 """
 from __future__ import annotations
 
+import gc
 import math
 from typing import Dict, List, Optional, Sequence
 
@@ -947,6 +948,7 @@ class WGAN:
         if entry["graph"] is not None and entry["generation"] != K.buffer_generation():
             # a scratch buffer moved since the capture (a larger shape, another model, clear_session): the
             # old graph would write through stale addresses, so it is dropped and this shape captured again
+            torch.cuda.synchronize()             # its last replay may still be running
             entry["graph"] = None
         if entry["graph"] is None:
             if "real" not in entry:
@@ -962,9 +964,14 @@ class WGAN:
             graph = torch.cuda.CUDAGraph()
             if self._rng is not None:
                 graph.register_generator_state(self._rng)
+            # Dropped models hold their graphs, events and pinned buffers in reference cycles.  The cyclic collector must
+            # not run inside the capture: it would destroy other graphs, free their memory and record events there.
+            collecting = gc.isenabled()
+            gc.collect()
             torch.cuda.synchronize()
             self._scalars = entry["scal"]
             generation = K.buffer_generation()
+            gc.disable()
             try:
                 with torch.cuda.graph(graph):
                     if alpha is not None:
@@ -976,6 +983,8 @@ class WGAN:
                     K.join_all()
             finally:
                 self._scalars = None
+                if collecting:
+                    gc.enable()
             if K.buffer_generation() != generation:
                 raise RuntimeError("a scratch buffer was reallocated while the step was being captured; the "
                                    "eager step before the capture must see the same shapes")
