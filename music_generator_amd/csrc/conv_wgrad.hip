@@ -450,6 +450,11 @@ __global__ __launch_bounds__(256) void pointwise2_wgrad_kernel(const float* __re
     }
 }
 
+__global__ __launch_bounds__(256) void wgrad_zero_kernel(float* __restrict__ p, long n) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) p[i] = 0.f;
+}
+
 // A block of 1024 threads covers 16 consecutive sums x 64 groups of partial blocks (group g adds blocks g,
 // g+64, ... in order); the 64 group sums are then added in a fixed order, so the result does not depend on
 // scheduling.  (One thread per sum walks ~10^3 dependent loads: 230 us for a 128-channel layer.)
@@ -541,7 +546,8 @@ extern "C" int mgx_conv_wgrad_f32(const mgx_conv_desc* dp, const float* x, const
         // positions in the place of taps) -> dw += G^T dU G
         float* du = partial + p.partial_floats + p.bias_floats;
         if (mgx_wwgrad_launch(d, x, dy, dymul, partial, bpartial, st) != MGX_OK) return MGX_ERR_LAUNCH;
-        if (hipMemsetAsync(du, 0, p.du_floats * sizeof(float), st) != hipSuccess) return MGX_ERR_LAUNCH;
+        // a kernel and no memset: a memset node of a captured graph is not safe to replay here
+        hipLaunchKernelGGL(wgrad_zero_kernel, dim3((unsigned)((p.du_floats + 255) / 256)), dim3(256), 0, st, du, (long)p.du_floats);
         mgx_conv_desc du_desc = d;
         du_desc.kh = du_desc.kw = 4;
         du_desc.wtap = (int64_t)d.cin * 32;
