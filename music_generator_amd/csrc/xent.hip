@@ -62,10 +62,12 @@ constexpr int kMaxParts = 512;
 inline int64_t up(int64_t a, int64_t m) { return (a + m - 1) / m * m; }
 
 // ---------------------------------------------------------------- scales
-// Largest finite magnitudes of W, x and dloss as float32 bits: one partial per workgroup and tensor.
-template <bool XF32>
-__global__ __launch_bounds__(256) void xent_max_kernel(const float* __restrict__ w, long nw, const void* __restrict__ x, long nx,
-                                                       const float* __restrict__ dl, long nd, unsigned* __restrict__ part) {
+// Largest finite magnitudes of W and of the labelled rows of x and dloss (the others may hold anything) as float32 bits: one
+// partial per workgroup and tensor.  2^lsh lanes walk a row of x, in pieces of 16 bytes where rows consist of them (VEC).
+template <bool XF32, bool VEC>
+__global__ __launch_bounds__(256) void xent_max_kernel(const float* __restrict__ w, long nw, const void* __restrict__ x, long n, int e,
+                                                       const int* __restrict__ labels, long v, int lsh, const float* __restrict__ dl,
+                                                       unsigned* __restrict__ part) {
     __shared__ unsigned red[3][4];
     const long t = (long)blockIdx.x * 256 + threadIdx.x, stride = (long)gridDim.x * 256;
     unsigned m[3] = {0u, 0u, 0u};
@@ -83,12 +85,37 @@ __global__ __launch_bounds__(256) void xent_max_kernel(const float* __restrict__
             for (int k = 0; k < 4; ++k) take(m[0], q[j][k]);
     }
     for (long i = nw / 4 * 4 + t; i < nw; i += stride) take(m[0], __builtin_bit_cast(unsigned, w[i]));
-    if (XF32) {
-        for (long i = t; i < nx; i += stride) take(m[1], ((const unsigned*)x)[i]);
-    } else {
-        for (long i = t; i < nx; i += stride) take(m[1], (unsigned)((const unsigned short*)x)[i] << 16);
+    constexpr int PER = VEC ? (XF32 ? 4 : 8) : 1;
+    const int lanes = 1 << lsh, cols = e / PER;
+    for (long row = t >> lsh; row < n; row += stride >> lsh) {
+        const int lab = labels[row];
+        if (lab < 0 || lab >= v) continue;
+        if (dl && (threadIdx.x & (lanes - 1)) == 0) take(m[2], __builtin_bit_cast(unsigned, dl[row]));
+        for (int c = threadIdx.x & (lanes - 1); c < cols; c += 4 * lanes) {
+            if constexpr (VEC) {
+                u32x4 q[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    q[j] = c + j * lanes < cols ? ((const u32x4*)x)[row * cols + c + j * lanes] : (u32x4){0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        take(m[1], XF32 ? q[j][k] : q[j][k] & 0xffff0000u);
+                        if (!XF32) take(m[1], q[j][k] << 16);
+                    }
+            } else {
+                unsigned q[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const long at = row * e + c + j * lanes;
+                    q[j] = c + j * lanes >= cols ? 0u : XF32 ? ((const unsigned*)x)[at] : (unsigned)((const unsigned short*)x)[at] << 16;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) take(m[1], q[j]);
+            }
+        }
     }
-    for (long i = t; i < nd; i += stride) take(m[2], __builtin_bit_cast(unsigned, dl[i]));
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
@@ -1403,12 +1430,18 @@ void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const floa
     int64_t parts = up(e * v / 16 + n * e / 16, 256) / 256;         // sixteen values a thread, up to four workgroups a CU
     parts = parts < 64 ? 64 : (parts > kMaxParts ? kMaxParts : parts);
     unsigned* part = (unsigned*)(ws + l.part);
-    if (xf32)
-        hipLaunchKernelGGL(xent_max_kernel<true>, dim3((unsigned)parts), dim3(256), 0, st, w, (long)(e * v), x, (long)(n * e), dloss,
-                           dloss ? (long)n : 0L, part);
-    else
-        hipLaunchKernelGGL(xent_max_kernel<false>, dim3((unsigned)parts), dim3(256), 0, st, w, (long)(e * v), x, (long)(n * e), dloss,
-                           dloss ? (long)n : 0L, part);
+    const bool vec = e % (xf32 ? 4 : 8) == 0;
+    const int64_t cols = vec ? e / (xf32 ? 4 : 8) : e;
+    int lsh = 0;                                                    // lanes of a row: up to 64, few enough for four loads each
+    while (lsh < 6 && (4 << lsh) < cols) ++lsh;
+    auto largest = [&](auto f32_, auto vec_) {
+        hipLaunchKernelGGL((xent_max_kernel<decltype(f32_)::value, decltype(vec_)::value>), dim3((unsigned)parts), dim3(256), 0, st, w,
+                           (long)(e * v), x, (long)n, (int)e, labels, (long)v, lsh, dloss, part);
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    if (xf32) vec ? largest(yes, yes) : largest(yes, no);
+    else vec ? largest(no, yes) : largest(no, no);
     XentPrep p = {};
     p.x = x; p.w = w; p.b = b; p.lse = lse; p.dloss = dloss; p.labels = labels; p.part = part; p.parts = (int)parts;
     p.n = n; p.v = v; p.np = l.np; p.vp = l.vp; p.e = (int)e; p.ep = (int)l.ep;

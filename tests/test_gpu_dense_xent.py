@@ -468,3 +468,20 @@ def test_parts_and_pieces(n, e, v, dtype, accumulate):
     else:
         got = run(x, w, b, labels, dloss)
     check(got, want, dtype, float((x.double() @ w.double()).abs().max()))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,e,v", [(9, 40, 300), (90, 40, 700), (90, 33, 700), (200, 128, 900), (150, 300, 1000), (150, 301, 1000)])
+def test_unlabelled_rows_may_hold_large_values(n, e, v, dtype):
+    """Rows without a label (below 0 or above the classes) change no bit of the others, whatever finite values they hold: they
+    have no part in the scales of the planes either."""
+    x, w, b, labels, dloss = case(n, e, v, dtype, seed=60 + e, unlabelled=0)
+    off = torch.arange(n) % 3 == 1
+    labels[off] = torch.where(torch.arange(n) % 2 == 0, -7, v)[off].int()
+    clean_x, clean_d = x.clone(), dloss.clone()
+    clean_x[off], clean_d[off] = 0.0, 0.0
+    x[off], dloss[off] = 3e30, -2e30
+    got, want = run(x, w, b, labels, dloss), run(clean_x, w, b, labels, clean_d)
+    assert all(torch.equal(got[k], want[k]) for k in want)
+    check(got, reference(clean_x, w, b, labels, clean_d), dtype, float((clean_x.double() @ w.double()).abs().max()))
