@@ -562,9 +562,11 @@ int mgx_conv_bwd_tape8(const mgx_conv_desc* d, const void* codes, const void* ex
  *             dw = x^T dz, db_j = sum_i dz_ij (float32; written, or added to with accumulate != 0)
  * x (n, e) float32 or bf16, w (e, v) and b (v, may be NULL) float32, labels (n).  A label outside [0, v) marks a row without
  * a loss: loss, lse, hits and its gradients are 0 and its features are not used.  A bias of -inf (or the lowest float)
- * masks a class.  Any of dx, dw, db may be NULL.  n <= 8 000 000, v <= 8 000 000, e <= 65 000; x, w and the workspace
+ * masks a class: its probability is 0 and its column of w is not used (one class at least is not masked; a row whose label is
+ * masked has the loss of that bias).  Any of dx, dw, db may be NULL.  n <= 8 000 000, v <= 8 000 000, e <= 65 000; x, w and the workspace
  * 16-byte aligned; the workspace (mgx_dense_xent_workspace bytes, -1: sizes out of range) is the call's alone while it
- * runs.  float32 quality throughout: the products are sums of products of fp16 halves of the operands.
+ * runs.  float32 quality throughout: the products are sums of products of fp16 halves of the operands (22 bits, counted from an
+ * operand's largest magnitude down to 2^-14 of it; n <= 16: float32).
  * ---------------------------------------------------------------------------------------- */
 int64_t mgx_dense_xent_workspace(int64_t n, int64_t e, int64_t v, int x_is_f32, int backward);
 int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, const float* b, const int32_t* labels, float* loss,

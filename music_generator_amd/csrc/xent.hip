@@ -16,7 +16,8 @@
 // and one v_exp_f32.
 //
 // A row whose label lies outside [0, v) has no loss: loss 0, lse 0, gradient 0 and nothing of its features is read into
-// a product (they may hold anything).  A class may be masked with a bias of -inf or the lowest float.
+// a product (they may hold anything).  A class masked with a bias of -inf or the lowest float has a probability of 0, and its column
+// of W is not used either; one class at least is not masked.
 #include "bf16.h"
 #include <type_traits>
 #include "../../include/mgx.h"
@@ -62,12 +63,15 @@ constexpr int kMaxParts = 512;
 inline int64_t up(int64_t a, int64_t m) { return (a + m - 1) / m * m; }
 
 // ---------------------------------------------------------------- scales
-// Largest finite magnitudes of W and of the labelled rows of x and dloss (the others may hold anything) as float32 bits: one
-// partial per workgroup and tensor.  2^lsh lanes walk a row of x, in pieces of 16 bytes where rows consist of them (VEC).
-template <bool XF32, bool VEC>
-__global__ __launch_bounds__(256) void xent_max_kernel(const float* __restrict__ w, long nw, const void* __restrict__ x, long n, int e,
-                                                       const int* __restrict__ labels, long v, int lsh, const float* __restrict__ dl,
-                                                       unsigned* __restrict__ part) {
+// Largest finite magnitudes of the unmasked classes of W and of the labelled rows of x and dloss (the others may hold anything) as
+// float32 bits: one partial per workgroup and tensor.  A thread takes 4 features of 4 classes of W (WVEC, rows of whole 16-byte
+// pieces) or 16 features of one; 2^lsh lanes walk a row of x, in pieces of 16 bytes where rows consist of them (VEC).
+__device__ __forceinline__ bool masked(float b) { return b <= kLowest; }
+
+template <bool XF32, bool VEC, bool WVEC>
+__global__ __launch_bounds__(256) void xent_max_kernel(const float* __restrict__ w, const float* __restrict__ b,
+                                                       const void* __restrict__ x, long n, int e, const int* __restrict__ labels,
+                                                       long v, int lsh, const float* __restrict__ dl, unsigned* __restrict__ part) {
     __shared__ unsigned red[3][4];
     const long t = (long)blockIdx.x * 256 + threadIdx.x, stride = (long)gridDim.x * 256;
     unsigned m[3] = {0u, 0u, 0u};
@@ -75,16 +79,27 @@ __global__ __launch_bounds__(256) void xent_max_kernel(const float* __restrict__
         b &= 0x7fffffffu;
         if (b < 0x7f800000u && b > a) a = b;
     };
-    for (long i = t; i < nw / 4; i += 4 * stride) {          // four loads in flight
-        u32x4 q[4];
+    constexpr int CL = WVEC ? 4 : 1, FE = 16 / CL;
+    const long groups = v / CL, items = groups * ((e + FE - 1) / FE);
+    for (long i = t; i < items; i += stride) {
+        const long k0 = i / groups * FE, c = (i - i / groups * groups) * CL;
+        u32x4 q[4];                                          // all loads in flight
+        float bv[CL];
+        if constexpr (WVEC) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = i + j * stride < nw / 4 ? ((const u32x4*)w)[i + j * stride] : (u32x4){0u, 0u, 0u, 0u};
+            for (int j = 0; j < 4; ++j) q[j] = *(const u32x4*)(w + (k0 + j < e ? k0 + j : e - 1) * v + c);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 16; ++j) q[j >> 2][j & 3] = __builtin_bit_cast(unsigned, w[(k0 + j < e ? k0 + j : e - 1) * v + c]);
+        }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) take(m[0], q[j][k]);
+        for (int k = 0; k < CL; ++k) bv[k] = b ? b[c + k] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (!masked(bv[WVEC ? k : 0]))
+#pragma unroll
+                for (int j = 0; j < 4; ++j) take(m[0], q[j][k]);
     }
-    for (long i = nw / 4 * 4 + t; i < nw; i += stride) take(m[0], __builtin_bit_cast(unsigned, w[i]));
     constexpr int PER = VEC ? (XF32 ? 4 : 8) : 1;
     const int lanes = 1 << lsh, cols = e / PER;
     for (long row = t >> lsh; row < n; row += stride >> lsh) {
@@ -206,6 +221,7 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
         const long etiles = p.ep / 64, ct = blockIdx.x / etiles, et = blockIdx.x - ct * etiles;
         const long c0 = ct * 64, e0 = et * 64;
         const int cc = tid & 63, k0 = tid >> 6;
+        const float bc = p.b && c0 + cc < p.v ? p.b[c0 + cc] : 0.f;
         float in[16];                                          // in flight while the scale is found
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
@@ -214,7 +230,7 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
         }
         const float s = scale_from_parts(p.part, 0, p.parts);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) t[k0 + 4 * j][cc] = in[j] * s;
+        for (int j = 0; j < 16; ++j) t[k0 + 4 * j][cc] = masked(bc) ? 0.f : in[j] * s;
         __syncthreads();
         const int e8 = tid & 7;
         for (int c = tid >> 3; c < 64; c += 32) {
@@ -1105,7 +1121,8 @@ __device__ __forceinline__ void xent_rows_logits(const XentRows& g, float* xs, f
     __syncthreads();
     const float b = ok ? (g.b ? g.b[c] : 0.f) : -__builtin_inff();
     for (int i = wv; i < RT; i += 4) {
-        const float s = (red[i * 64 + lane] + red[(RT + i) * 64 + lane]) + (red[(2 * RT + i) * 64 + lane] + red[(3 * RT + i) * 64 + lane]);
+        const float all = (red[i * 64 + lane] + red[(RT + i) * 64 + lane]) + (red[(2 * RT + i) * 64 + lane] + red[(3 * RT + i) * 64 + lane]);
+        const float s = masked(b) ? 0.f : all;
         const float t = (s + b) * kLog2e;
         zs[i * 64 + lane] = s + b >= kLowest ? fmaxf(t, kLowest) : t;
     }
@@ -1175,6 +1192,7 @@ __global__ __launch_bounds__(256) void xent_rows_bwd_kernel(XentRows g) {
         dzt[(k & 63) * RT + i] = d;
     }
     __syncthreads();
+    const bool used = c < g.v && !(g.b && masked(g.b[c]));
     float dz[RT];                                   // of the lane's class
 #pragma unroll
     for (int i = 0; i < RT; ++i) dz[i] = zs[i * 64 + lane];
@@ -1215,7 +1233,7 @@ __global__ __launch_bounds__(256) void xent_rows_bwd_kernel(XentRows g) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                     const int k = k0 + wv + 4 * j;
-                    w[j] = k < cnt && c < g.v ? g.w[(long)(e0 + k) * g.v + c] : 0.f;
+                    w[j] = k < cnt && used ? g.w[(long)(e0 + k) * g.v + c] : 0.f;
                 }
                 __syncthreads();
 #pragma unroll
@@ -1434,14 +1452,15 @@ void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const floa
     const int64_t cols = vec ? e / (xf32 ? 4 : 8) : e;
     int lsh = 0;                                                    // lanes of a row: up to 64, few enough for four loads each
     while (lsh < 6 && (4 << lsh) < cols) ++lsh;
-    auto largest = [&](auto f32_, auto vec_) {
-        hipLaunchKernelGGL((xent_max_kernel<decltype(f32_)::value, decltype(vec_)::value>), dim3((unsigned)parts), dim3(256), 0, st, w,
-                           (long)(e * v), x, (long)n, (int)e, labels, (long)v, lsh, dloss, part);
+    auto largest = [&](auto f32_, auto vec_, auto wvec_) {
+        hipLaunchKernelGGL((xent_max_kernel<decltype(f32_)::value, decltype(vec_)::value, decltype(wvec_)::value>), dim3((unsigned)parts),
+                           dim3(256), 0, st, w, b, x, (long)n, (int)e, labels, (long)v, lsh, dloss, part);
     };
     const std::true_type yes;
     const std::false_type no;
-    if (xf32) vec ? largest(yes, yes) : largest(yes, no);
-    else vec ? largest(no, yes) : largest(no, no);
+    auto by_w = [&](auto f32_, auto vec_) { v % 4 == 0 ? largest(f32_, vec_, yes) : largest(f32_, vec_, no); };
+    if (xf32) vec ? by_w(yes, yes) : by_w(yes, no);
+    else vec ? by_w(no, yes) : by_w(no, no);
     XentPrep p = {};
     p.x = x; p.w = w; p.b = b; p.lse = lse; p.dloss = dloss; p.labels = labels; p.part = part; p.parts = (int)parts;
     p.n = n; p.v = v; p.np = l.np; p.vp = l.vp; p.e = (int)e; p.ep = (int)l.ep;

@@ -485,3 +485,23 @@ def test_unlabelled_rows_may_hold_large_values(n, e, v, dtype):
     got, want = run(x, w, b, labels, dloss), run(clean_x, w, b, labels, clean_d)
     assert all(torch.equal(got[k], want[k]) for k in want)
     check(got, reference(clean_x, w, b, labels, clean_d), dtype, float((clean_x.double() @ w.double()).abs().max()))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mask", [float("-inf"), -3.4028234663852886e38])
+@pytest.mark.parametrize("n,e,v", [(1, 40, 301), (9, 300, 300), (90, 40, 700), (90, 33, 701), (200, 128, 900), (150, 300, 1001), (150, 301, 1000)])
+def test_masked_classes_may_hold_anything(n, e, v, mask, dtype):
+    """A masked class changes no bit of the rest, whatever its column of W holds: NaN, infinities, large finite values."""
+    x, w, b, labels, dloss = case(n, e, v, dtype, seed=70 + e, unlabelled=0)
+    off = torch.arange(v) % 4 == 1
+    b[off] = mask
+    labels = torch.where(off[labels.long()], labels - 1, labels)
+    clean = w.clone()
+    clean[:, off] = 0.0
+    for fill in (3e30, float("inf"), float("nan")):
+        w[:, off] = fill
+        got, want = run(x, w, b, labels, dloss), run(x, clean, b, labels, dloss)
+        assert all(torch.equal(got[k], want[k]) for k in want), fill
+    check(got, reference(x, clean, b, labels, dloss), dtype, float((x.double() @ clean.double()).abs().max()))
+    assert bool((got["dw"][:, off] == 0).all()) and bool((got["db"][off] == 0).all())
