@@ -1,6 +1,8 @@
 // bf16 storage helpers for the gfx950 kernels that keep activations in bfloat16 and accumulate in
 // float32 (v_mfma_f32_32x32x16_bf16).
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 typedef __bf16 bf16_t;
@@ -116,3 +118,11 @@ __device__ __forceinline__ u32x2 tr_read(const unsigned char* p) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((mgx_lds_s16x4_ptr)p));
 }
 
+// compile-time unrolled loop: f(integral_constant<int, I>) for I in [I0, N)
+template <int I, int N, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        static_for<I + 1, N>(f);
+    }
+}

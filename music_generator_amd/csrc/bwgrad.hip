@@ -264,15 +264,6 @@ __global__ __launch_bounds__(1024) void bwgrad_reduce_kernel(mgx_conv_desc d, co
 // Staged positions are 64 B with their four 16-byte chunks XOR-swizzled by bits 2-3 of the position index, which
 // keeps both kinds of read conflict-free.
 // ------------------------------------------------------------------------------------------
-// compile-time unrolled loop: f(integral_constant<int, I>) for I in [I0, N)
-template <int I, int N, typename F>
-__device__ __forceinline__ void static_for(F&& f) {
-    if constexpr (I < N) {
-        f(std::integral_constant<int, I>{});
-        static_for<I + 1, N>(f);
-    }
-}
-
 // CIN = 128 (the block's first 3x3 convolution, 128 -> 32): the tile is 4 rows x 32 columns, X is staged as four
 // planes of 32 channels, and wave c owns input-channel chunk c for the WHOLE tile: its 32 of the 128 data-gradient
 // channels and its own weight-gradient tiles (no sum over the waves at the end), the G window shared by all four.

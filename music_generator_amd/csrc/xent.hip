@@ -15,11 +15,21 @@
 // (exact, they are powers of two), and log2(e) is in the factor that takes the scales out again: an exponential is one fma
 // and one v_exp_f32.
 //
+// Three forms.  What each is bound by, and forward + backward times (us, features float32 / bf16):
+//   up to 16 rows: HBM (W read twice, dW written), float32 on the vector ALU.  1 x 1000 x 65536 float32: 48 + 261 us, 5.5 and 3.0 of the
+//     4.75 TB/s that a large copy reaches.  16 rows against 17 (e x v: few rows + matrix form): 128 x 4096 15 + 23 against
+//     21 + 45, 1000 x 10001 57 + 184 against 76 + 139, 1000 x 65536 79 + 494 against 332 + 696.
+//   e <= 128: the matrix pipe, streamed, dz never stored.  24000 x 128 x 65536 bf16: 725 + 2090 us (the three products 0.78, 0.92
+//     and 1.45 ms, 1.0 to 1.1 PFLOP/s of fp16 products; a large library product reaches 1.22).  The form below takes 1400 + 6116 us for
+//     it, and 1720 + 7494 against 1049 + 3722 us for float32 features; at 3000 x 128 x 8192 bf16 40 + 103 against 41 + 89 us.
+//   e > 128: the matrix pipe, tiled products with dz in planes of 128 MB a piece.  1501 x 1000 x 10001 float32: 470 us, of which
+//     the four products (0.97 PFLOP/s) take 415.
+// Up to 64 features the streamed kernels have a form of 64 (24000 x 32 x 65536 bf16: 420 + 1135 against 622 + 1770 us).
+//
 // A row whose label lies outside [0, v) has no loss: loss 0, lse 0, gradient 0 and nothing of its features is read into
 // a product (they may hold anything).  A class masked with a bias of -inf or the lowest float has a probability of 0, and its column
 // of W is not used either; one class at least is not masked.
 #include "bf16.h"
-#include <type_traits>
 #include "../../include/mgx.h"
 
 namespace {
@@ -597,15 +607,6 @@ struct XentStream {
     XentOut o;                                      // DW
 };
 
-// compile-time unrolled loop: f(integral_constant<int, I>) for I in [I0, N)
-template <int I, int N, typename F>
-__device__ __forceinline__ void static_for(F&& f) {
-    if constexpr (I < N) {
-        f(std::integral_constant<int, I>{});
-        static_for<I + 1, N>(f);
-    }
-}
-
 template <int EP>
 __device__ __forceinline__ int swz_item(int row) {
     return EP == 64 ? ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) : (((row & 3) << 2) | ((row >> 2) & 3));
@@ -1058,7 +1059,8 @@ __global__ __launch_bounds__(256) void xent_dw_reduce_kernel(const float* __rest
 // ---------------------------------------------------------------- few rows
 // Up to 16 rows the kernel W is what the call reads and dW what it writes: float32 on the vector ALU, no planes, two launches a
 // direction.  A workgroup takes 64 classes (a lane each, so a wave reads 256 consecutive bytes of a row of W), its four
-// waves a quarter of the features each.  RT: rows rounded up, accumulators of a lane.
+// waves a quarter of the features each.  RT: rows rounded up (1, 4, 16), accumulators of a lane: 4 x 128 x 65536 takes 15 + 42 us
+// with 4 and 18 + 65 with 16, 1 x 1000 x 65536 48 + 261 with 1 and 62 + 397 with 16.
 constexpr int FEW = 16, RC = 256;                   // RC: features staged at a time
 
 struct XentRows {
@@ -1483,7 +1485,9 @@ void launch_dx_join(const Layout& l, char* ws, void* dx, bool xf32, int64_t n, i
     const long part = (long)(l.np * l.ep);
     const float* rs = l.narrow ? nullptr : (const float*)(ws + l.rs);
     const float2* row = (const float2*)(ws + l.row);
-    if (l.nx >= 16 && n * l.ep <= 1 << 18) {
+    // sixteen groups of parts: 200 x 128 x 65536 94.8 us a backward against 101.3 with one, 53 x 75 x 25145 56.4 against 61.3; with the
+    // outputs of 3000 x 32 x 8192 one group fills the chip (75.2 against 83.3)
+    if (l.nx >= 16 && n * l.ep <= 1 << 16) {
         hipLaunchKernelGGL(xent_dx_join_kernel<16>, dim3((unsigned)(up(n * l.ep, 64) / 64)), dim3(1024), 0, st, parts, scales, row, rs, dx,
                            (int)xf32, (int)l.nx, part, (long)n, (int)e, (int)l.ep);
     } else {
