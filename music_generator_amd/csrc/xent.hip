@@ -15,14 +15,15 @@
 // (exact, they are powers of two), and log2(e) is in the factor that takes the scales out again: an exponential is one fma
 // and one v_exp_f32.
 //
-// Three forms.  What each is bound by, and forward + backward times (us, features float32 / bf16):
-//   up to 16 rows: HBM (W read twice, dW written), float32 on the vector ALU.  1 x 1000 x 65536 float32: 48 + 261 us, 5.5 and 3.0 of the
-//     4.75 TB/s that a large copy reaches.  16 rows against 17 (e x v: few rows + matrix form): 128 x 4096 15 + 23 against
-//     21 + 45, 1000 x 10001 57 + 184 against 76 + 139, 1000 x 65536 79 + 494 against 332 + 696.
-//   e <= 128: the matrix pipe, streamed, dz never stored.  24000 x 128 x 65536 bf16: 725 + 2090 us (the three products 0.78, 0.92
-//     and 1.45 ms, 1.0 to 1.1 PFLOP/s of fp16 products; a large library product reaches 1.22).  The form below takes 1400 + 6116 us for
-//     it, and 1720 + 7494 against 1049 + 3722 us for float32 features; at 3000 x 128 x 8192 bf16 40 + 103 against 41 + 89 us.
-//   e > 128: the matrix pipe, tiled products with dz in planes of 128 MB a piece.  1501 x 1000 x 10001 float32: 470 us, of which
+// Four forms.  What each is bound by, and forward + backward times (us; n x e x v):
+//   few rows (up to 4, up to 16 of a small W): launches and HBM (W read twice, dW written), float32 on the vector ALU.
+//     1 x 128 x 4097 15 + 17, 4 x 128 x 65536 15 + 42.
+//   a block of rows (up to 64, 128 of a large W): HBM up to 32 rows (a kernel each for the logits, dx and dW, 4.4 to 4.9 TB/s at 32 x
+//     1000 x 65536; a large copy reaches 4.75), the float32 matrix instructions beyond (64 x 1000 x 65536 96 + 265).
+//   e <= 128: the matrix pipe, streamed, dz never stored.  24000 x 128 x 65536 bf16: 725 + 2090 (the three products 0.78, 0.92
+//     and 1.45 ms, 1.0 to 1.1 PFLOP/s of fp16 products; a large library product reaches 1.22).  The form below takes 1400 + 6116 for
+//     it, and 1720 + 7494 against 1049 + 3722 for float32 features; at 3000 x 128 x 8192 bf16 40 + 103 against 41 + 89.
+//   e > 128: the matrix pipe, tiled products with dz in planes of 128 MB a piece.  1501 x 1000 x 10001 float32: 470 in all, of which
 //     the four products (0.97 PFLOP/s) take 415.
 // Up to 64 features the streamed kernels have a form of 64 (24000 x 32 x 65536 bf16: 420 + 1135 against 622 + 1770 us).
 //
@@ -973,7 +974,7 @@ __global__ __launch_bounds__(G == 1 ? 256 : 1024) void xent_dx_join_kernel(const
     constexpr int W = G == 1 ? 256 : 64;
     __shared__ float red[G][G == 1 ? 1 : 64];
     // streamed: the parts hold 2^14 dz / dloss, the rows 2^14 dloss / scales[2]; wide: 2^14 dz / rs
-    const float f = (rs ? 1.f : scales[2] / kDz) / kDz / scales[0];
+    const float f = !scales ? 1.f : (rs ? 1.f : scales[2] / kDz) / kDz / scales[0];
     const int lane = threadIdx.x % W, q = threadIdx.x / W;
     const int per = (np + G - 1) / G, p0 = q * per, cnt = np - p0 < per ? np - p0 : per;
     for (long i = (long)blockIdx.x * W + lane; i - lane < n * ep; i += (long)gridDim.x * W) {
@@ -988,7 +989,7 @@ __global__ __launch_bounds__(G == 1 ? 256 : 1024) void xent_dx_join_kernel(const
         const long row = i / ep;
         const int c = (int)(i - row * ep);
         if (q == 0 && row < n && c < e) {
-            s *= f * (rs ? rs[row] : rowinfo[row].y);
+            if (scales) s *= f * (rs ? rs[row] : rowinfo[row].y);
             if (dx_f32) ((float*)dx)[row * e + c] = s;
             else ((bf16_t*)dx)[row * e + c] = (bf16_t)s;
         }
@@ -1057,10 +1058,10 @@ __global__ __launch_bounds__(256) void xent_dw_reduce_kernel(const float* __rest
 }
 
 // ---------------------------------------------------------------- few rows
-// Up to 16 rows the kernel W is what the call reads and dW what it writes: float32 on the vector ALU, no planes, two launches a
+// Few rows: the kernel W is what the call reads and dW what it writes: float32 on the vector ALU, no planes, two launches a
 // direction.  A workgroup takes 64 classes (a lane each, so a wave reads 256 consecutive bytes of a row of W), its four
 // waves a quarter of the features each.  RT: rows rounded up (1, 4, 16), accumulators of a lane: 4 x 128 x 65536 takes 15 + 42 us
-// with 4 and 18 + 65 with 16, 1 x 1000 x 65536 48 + 261 with 1 and 62 + 397 with 16.
+// with 4 and 18 + 65 with 16, 1 x 128 x 4097 15 + 17 with 1 and 16 + 20 with 16.
 constexpr int FEW = 16, RC = 256;                   // RC: features staged at a time
 
 struct XentRows {
@@ -1281,6 +1282,445 @@ __global__ __launch_bounds__(1024) void xent_rows_dx_kernel(const float* __restr
     }
 }
 
+// ---------------------------------------------------------------- a block of rows
+// Up to 128 rows (RB blocks of 32) W and dW are still what a call moves, but the products belong on the matrix pipe: float32
+// instructions on W as it lies in memory, no scales and no planes.  A block of rows needs 64 cycles of a SIMD for every 64 values
+// of W and product: with one block the four SIMDs of a CU would take 16 bytes of W a cycle, 8 TB/s over the chip.
+//   logits: a workgroup takes 32 classes, its waves a quarter of the features each; W goes from memory to the A fragments (a lane a
+//       class), x comes transposed from the cache.  Forward: (maximum, sum) per row; backward: dz (rows x classes) and db.
+//   dx: 128 features a workgroup over a part of the classes, tiles of W and dz by LDS-DMA (a ring of three).
+//   dW: a wave keeps dz of 32 classes and multiplies it with the features, 32 at a time.
+struct XentShort {
+    const void* x;
+    const float *w, *b, *lse, *dloss;
+    const int* labels;
+    float *xt, *xz;                   // x with zeros for rows without a label, features x rows and rows x features
+    float* bias;                      // classes padded with -inf
+    float2* row;                      // lse in units of log 2 and dloss; (inf, 0) without a label
+    int* lab;
+    float2* part;                     // forward: (maximum, sum) per 32 classes and row
+    float *zlab, *dz, *dxp, *dw, *db;
+    long v, vp;                       // classes, padded to 128
+    int n, e, ep, np, accumulate;     // features padded to 128, rows to 32
+};
+
+template <bool XF32>
+__global__ __launch_bounds__(256) void xent_short_prep_kernel(XentShort g, int tiles) {
+    __shared__ float t[64][33];
+    const int tid = threadIdx.x;
+    if ((int)blockIdx.x < tiles) {                    // 32 rows x 64 features
+        const int rbs = g.np / 32, r0 = (int)blockIdx.x % rbs * 32, k0 = (int)blockIdx.x / rbs * 64, k = k0 + (tid & 63);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int rr = (tid >> 6) + 4 * i, row = r0 + rr;
+            float a = 0.f;
+            if (row < g.n && k < g.e) {
+                const int lab = g.labels[row];
+                const long at = (long)row * g.e + k;
+                if (lab >= 0 && lab < g.v) a = XF32 ? ((const float*)g.x)[at] : (float)((const bf16_t*)g.x)[at];
+            }
+            if (g.xz) g.xz[(long)row * g.ep + k] = a;
+            t[tid & 63][rr] = a;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int kk = (tid >> 5) + 8 * i;
+            g.xt[(long)(k0 + kk) * g.np + r0 + (tid & 31)] = t[kk][tid & 31];
+        }
+    } else {
+        const long first = (long)(blockIdx.x - tiles) * 256 + tid, stride = (long)(gridDim.x - tiles) * 256;
+        for (long c = first; c < g.vp; c += stride) g.bias[c] = c < g.v ? (g.b ? g.b[c] : 0.f) : -__builtin_inff();
+        for (long i = first; i < g.np; i += stride) {
+            int lab = i < g.n ? g.labels[i] : -1;
+            if (lab < 0 || lab >= g.v) lab = -1;
+            g.lab[i] = lab;
+            if (g.row) g.row[i] = lab < 0 ? make_float2(__builtin_inff(), 0.f) : make_float2(g.lse[i] * kLog2e, g.dloss[i]);
+        }
+    }
+}
+
+template <int RB, bool BWD>
+__global__ __launch_bounds__(256) void xent_short_logits_kernel(XentShort g) {
+    __shared__ float red[4 * 16 * 64], zs[32 * RB * 33];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, r = lane & 31, h = lane >> 5;
+    const long c0 = (long)blockIdx.x * 32, c = c0 + r < g.v ? c0 + r : g.v - 1;
+    const int span = (g.e + 63) / 64 * 16, kb = wv * span, end = (g.e + 15) / 16 * 16, ke = kb + span < end ? kb + span : end;
+    f32x16 acc[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
+    // 16 features: the lane's class and row, features k + h, k + h + 2, ...
+    auto fetch = [&](int k, float (&a)[8], float (&x)[RB][8]) {
+        const float* wp = g.w + (long)(k + h) * g.v + c;
+        if (k + 16 <= g.e) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a[j] = wp[2 * j * g.v];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a[j] = k + 2 * j + h < g.e ? wp[2 * j * g.v] : 0.f;
+        }
+        const float* xp = g.xt + (long)(k + h) * g.np + r;
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[b][j] = xp[2 * j * g.np + 32 * b];
+    };
+    auto products = [&](const float (&a)[8], const float (&x)[RB][8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int b = 0; b < RB; ++b) acc[b] = mfma32(a[j], x[b][j], acc[b]);
+    };
+    if (kb < ke) {
+        float a0[8], a1[8], x0[RB][8], x1[RB][8];
+        fetch(kb, a0, x0);
+        for (int k = kb; k < ke; k += 32) {
+            if (k + 16 < ke) fetch(k + 16, a1, x1);
+            products(a0, x0);
+            if (k + 16 < ke) {
+                if (k + 32 < ke) fetch(k + 32, a0, x0);
+                products(a1, x1);
+            }
+        }
+    }
+    // the waves' sums in order; wave wv finishes the classes 8 wv + 4 h + {0 .. 3}
+    float bv[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) bv[t] = g.bias[c0 + 8 * wv + 4 * h + t];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) red[(wv * 16 + i) * 64 + lane] = acc[b][i];
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const float* q = red + (4 * wv + t) * 64 + lane;
+            const float all = (q[0] + q[16 * 64]) + (q[32 * 64] + q[48 * 64]);
+            const float z = (masked(bv[t]) ? 0.f : all) + bv[t], u = z * kLog2e;
+            zs[(32 * b + r) * 33 + 8 * wv + 4 * h + t] = z >= kLowest ? fmaxf(u, kLowest) : u;
+        }
+        __syncthreads();
+    }
+    const int q = tid & 7;                              // eight lanes a row, four classes each
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        const int row = 32 * b + (tid >> 3);
+        const long rel = g.lab[row] - c0;               // the label's place, if it is one of the 32
+        float* zr = zs + row * 33 + 4 * q;
+        if constexpr (!BWD) {
+            float m = kLowest, s = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = fmaxf(m, zr[i]);
+#pragma unroll
+            for (int off = 1; off < 8; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f(zr[i] - m);
+#pragma unroll
+            for (int off = 1; off < 8; off <<= 1) s += __shfl_xor(s, off, 64);
+            if (q == 0) g.part[(long)row * gridDim.x + blockIdx.x] = make_float2(m, s);
+            if (rel >= 4 * q && rel < 4 * q + 4 && g.lab[row] >= 0) g.zlab[row] = zr[rel - 4 * q];
+        } else {
+            const float2 info = g.row[row];
+            f32x4 d;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = __builtin_amdgcn_exp2f(zr[i] - info.x);
+                d[i] = (g.lab[row] >= 0 && rel == 4 * q + i ? p - 1.f : p) * info.y;
+                zr[i] = d[i];
+            }
+            *(f32x4*)(g.dz + (long)row * g.vp + c0 + 4 * q) = d;
+        }
+    }
+    if (BWD && g.db) {
+        const int cl = tid & 31, part = tid >> 5;
+        __syncthreads();
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4 * RB; ++i) s += zs[(part * 4 * RB + i) * 33 + cl];
+        red[part * 32 + cl] = s;
+        __syncthreads();
+        if (tid < 32 && c0 + cl < g.v) {
+            s = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += red[i * 32 + cl];
+            g.db[c0 + cl] = g.accumulate ? g.db[c0 + cl] + s : s;
+        }
+    }
+}
+
+// The same for many classes: a workgroup takes 128 of them (a wave 32) and walks the features 32 at a time, tiles of W and of x by
+// LDS-DMA (a ring of three), so that x is read a quarter as often.  W16: rows of W consist of 16-byte pieces.
+template <int RB, bool BWD, bool W16>
+__global__ __launch_bounds__(256) void xent_short_tiled_kernel(XentShort g) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    constexpr int WB = 32 * 512, XB = RB * 4096, BUF = WB + XB, PIECES = (W16 ? 4 : 16) + RB;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
+    const long c0 = (long)blockIdx.x * 128;
+    const int steps = (g.e + 31) / 32;
+    // step it; features past the last meet zeros of x, classes past the last are the last ones and get their own place masked
+    auto stage = [&](int it) {
+        const unsigned dst = lds_byte(lds) + it % 3 * BUF;
+        constexpr int PER = W16 ? 4 : 16;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int piece = wv * PER + i;
+            if constexpr (W16) {                          // 2 rows of 512 B
+                const int k = it * 32 + piece * 2, ka = k < g.e ? k : g.e - 1, kr = k + h < g.e ? k + h : g.e - 1;
+                const long c = c0 + 4 * r < g.v ? 4 * r : g.v - 4 - c0;
+                lds_dma16(g.w + ka * g.v + c0, (int)(((kr - ka) * g.v + c) * 4), dst + piece * 1024);
+            } else {                                      // half a row
+                const int k = it * 32 + piece / 2, ka = k < g.e ? k : g.e - 1, cl = piece % 2 * 64 + lane;
+                const long c = c0 + cl < g.v ? cl : g.v - 1 - c0;
+                lds_dma4(g.w + ka * g.v + c0, (int)(c * 4), dst + piece * 256);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {                    // 32 features x np rows as they lie in xt
+            const int piece = wv * RB + i;
+            lds_dma16(g.xt + (long)it * 32 * g.np + piece * 256, lane * 16, dst + WB + piece * 1024);
+        }
+    };
+    f32x16 acc[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
+    stage(0);
+    if (steps > 1) stage(1);
+    for (int it = 0; it < steps; ++it) {
+        if (it + 1 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (it + 2 < steps) stage(it + 2);
+        const unsigned char* buf = lds + it % 3 * BUF;
+        const float *wt = (const float*)buf + h * 128 + 32 * wv + r, *xt = (const float*)(buf + WB) + h * 32 * RB + r;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float a = wt[2 * j * 128];
+#pragma unroll
+            for (int b = 0; b < RB; ++b) acc[b] = mfma32(a, xt[2 * j * 32 * RB + 32 * b], acc[b]);
+        }
+    }
+    // lane: row 32 b + r, classes 8 q + 4 h + {0 .. 3} of the wave's
+    const long cw = c0 + 32 * wv;
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 bv = *(const f32x4*)(g.bias + cw + 8 * q + 4 * h);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float z = (masked(bv[k]) ? 0.f : acc[b][4 * q + k]) + bv[k], u = z * kLog2e;
+                acc[b][4 * q + k] = z >= kLowest ? fmaxf(u, kLowest) : u;
+            }
+        }
+    float db[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) db[i] = 0.f;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        const int row = 32 * b + r, lab = g.lab[row];
+        const long rel = lab < 0 ? -1 : lab - cw - 4 * h;
+        if constexpr (!BWD) {
+            float m = kLowest, s = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = fmaxf(m, acc[b][i]);
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s += __builtin_amdgcn_exp2f(acc[b][i] - m);
+            s += __shfl_xor(s, 32, 64);
+            if (h == 0) g.part[((long)row * gridDim.x + blockIdx.x) * 4 + wv] = make_float2(m, s);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (rel == (i & 3) + 8 * (i >> 2)) g.zlab[row] = acc[b][i];
+        } else {
+            const float2 info = g.row[row];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                f32x4 d;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float p = __builtin_amdgcn_exp2f(acc[b][4 * q + k] - info.x);
+                    d[k] = (rel == 8 * q + k ? p - 1.f : p) * info.y;
+                    db[4 * q + k] += d[k];
+                }
+                *(f32x4*)(g.dz + (long)row * g.vp + cw + 8 * q + 4 * h) = d;
+            }
+        }
+    }
+    if (BWD && g.db) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) db[i] += __shfl_xor(db[i], off, 64);
+            const long c = cw + acc_row(i, lane);
+            if (r == i && c < g.v) g.db[c] = g.accumulate ? g.db[c] + db[i] : db[i];
+        }
+    }
+}
+
+// loss and lse of a row: a thread every 256th part, then across the threads
+__global__ __launch_bounds__(256) void xent_short_join_kernel(XentShort g, float* __restrict__ loss, float* __restrict__ lse,
+                                                              int* __restrict__ hits, int parts) {
+    __shared__ float2 red[4];
+    const int row = blockIdx.x, lane = threadIdx.x & 63;
+    float m = kLowest, s = 0.f;
+    auto join = [&](float pm, float ps) {
+        const float mm = fmaxf(m, pm);
+        s = s * __builtin_amdgcn_exp2f(m - mm) + ps * __builtin_amdgcn_exp2f(pm - mm);
+        m = mm;
+    };
+    for (int p = threadIdx.x; p < parts; p += 1024) {           // four loads in flight
+        float2 q[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[k] = p + 256 * k < parts ? g.part[(long)row * parts + p + 256 * k] : make_float2(kLowest, 0.f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) join(q[k].x, q[k].y);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const float pm = __shfl_xor(m, off, 64), ps = __shfl_xor(s, off, 64);
+        join(pm, ps);
+    }
+    if (lane == 0) red[threadIdx.x >> 6] = make_float2(m, s);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int k = 1; k < 4; ++k) join(red[k].x, red[k].y);
+        const int lab = g.lab[row];
+        const float z = lab >= 0 ? g.zlab[row] : 0.f, ls = __builtin_amdgcn_logf(s);
+        loss[row] = lab >= 0 ? ((m - z) + ls) * kLn2 : 0.f;
+        lse[row] = lab >= 0 ? (m + ls) * kLn2 : 0.f;
+        if (hits) hits[row] = lab >= 0 && z >= m ? 1 : 0;
+    }
+}
+
+// W16: rows of W consist of 16-byte pieces.  Staged rows are 32 classes (128 B); 16-byte chunks are XOR-swizzled by the row so that
+// the 16 rows of a read cover all banks.
+template <int RB, bool W16>
+__global__ __launch_bounds__(256) void xent_short_dx_kernel(XentShort g) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    constexpr int WB = 128 * 128, DB = RB * 4096, BUF = WB + DB + 128, PIECES = (W16 ? 4 : 16) + RB + 1;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
+    const int k0 = blockIdx.x * 128, tiles = (int)((g.v + 31) / 32), per = (tiles + gridDim.y - 1) / gridDim.y;
+    const int t0 = blockIdx.y * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+    // tile t: features past the last and classes past the last are those themselves; the former are not stored, the latter masked
+    auto stage = [&](int t) {
+        const unsigned dst = lds_byte(lds) + (t - t0) % 3 * BUF;
+        const long c0 = (long)t * 32;
+        constexpr int ROWS = W16 ? 8 : 2, PER = W16 ? 4 : 16;          // rows of an instruction, instructions of a wave
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int piece = wv * PER + i, row = piece * ROWS + lane / (64 / ROWS);
+            const int kf = k0 + piece * ROWS < g.e ? k0 + piece * ROWS : g.e - 1, kr = k0 + row < g.e ? k0 + row : g.e - 1;
+            const int s = (row >> 1) & 7;
+            long c = W16 ? c0 + 4 * ((lane & 7) ^ s) : c0 + 4 * (((lane & 31) >> 2) ^ s) + (lane & 3);
+            c = c < g.v ? c : g.v - (W16 ? 4 : 1);
+            const int off = (int)(((kr - kf) * g.v + c - c0) * 4);
+            if constexpr (W16) lds_dma16(g.w + kf * g.v + c0, off, dst + piece * 1024);
+            else lds_dma4(g.w + kf * g.v + c0, off, dst + piece * 256);
+        }
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
+            const int piece = wv * RB + i, row = lane >> 3;
+            const int off = (int)(row * g.vp * 4) + (((lane & 7) ^ (((piece * 8 + row) >> 1) & 7)) << 4);
+            lds_dma16(g.dz + piece * 8 * g.vp + c0, off, dst + WB + piece * 1024);
+        }
+        if (lane < 32) lds_dma4(g.bias + c0, lane * 4, dst + WB + DB);      // every wave the same: each counts its own loads only
+    };
+    f32x16 acc[RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[b][i] = 0.f;
+    if (t0 < t1) stage(t0);
+    if (t0 + 1 < t1) stage(t0 + 1);
+    const int sw = (r >> 1) & 7;
+    for (int t = t0; t < t1; ++t) {
+        if (t + 1 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (t + 2 < t1) stage(t + 2);
+        const unsigned char* buf = lds + (t - t0) % 3 * BUF;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {                   // classes 8 q + 4 h + {0 .. 3}
+            const int at = ((2 * q + h) ^ sw) << 4;
+            const f32x4 bias = *(const f32x4*)(buf + WB + DB + (8 * q + 4 * h) * 4);
+            f32x4 a = *(const f32x4*)(buf + (32 * wv + r) * 128 + at), d[RB];
+#pragma unroll
+            for (int b = 0; b < RB; ++b) d[b] = *(const f32x4*)(buf + WB + (32 * b + r) * 128 + at);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float w = masked(bias[j]) ? 0.f : a[j];
+#pragma unroll
+                for (int b = 0; b < RB; ++b) acc[b] = mfma32(w, d[b][j], acc[b]);
+            }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        float* o = g.dxp + ((long)blockIdx.y * g.np + 32 * b + r) * g.ep + k0 + 32 * wv + 4 * h;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *(f32x4*)(o + 8 * q) = (f32x4){acc[b][4 * q], acc[b][4 * q + 1], acc[b][4 * q + 2], acc[b][4 * q + 3]};
+    }
+}
+
+// kg blocks of 32 features a workgroup.  The stores of a step are never skipped (an offset past the end of the buffer drops them), so
+// that a wait can count them: behind the DMA of a step come the stores of two steps and the DMA of one.
+template <int RB>
+__global__ __launch_bounds__(256) void xent_short_dw_kernel(XentShort g, int kg) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    constexpr int BUF = RB * 4096;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
+    const long c = (long)blockIdx.x * 128 + wv * 32 + r;
+    const int blocks = (g.e + 31) / 32, t0 = blockIdx.y * kg, t1 = t0 + kg < blocks ? t0 + kg : blocks;
+    auto stage = [&](int t) {                            // np rows x 32 features
+        const unsigned dst = lds_byte(lds) + (t - t0) % 3 * BUF;
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
+            const int piece = wv * RB + i;               // 8 rows of 128 B
+            lds_dma16(g.xz + (long)piece * 8 * g.ep + t * 32, ((lane >> 3) * g.ep + (lane & 7) * 4) * 4, dst + piece * 1024);
+        }
+    };
+    float d[16 * RB];
+#pragma unroll
+    for (int j = 0; j < 16 * RB; ++j) d[j] = g.dz[(2 * j + h) * g.vp + c];
+#pragma unroll
+    for (int j = 0; j < 16 * RB; ++j) asm volatile("" : "+v"(d[j]));          // here already: or every step waits for them by count
+    stage(t0);
+    if (t0 + 1 < t1) stage(t0 + 1);
+    for (int t = t0; t < t1; ++t) {
+        if (t + 1 >= t1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        else if (t < t0 + 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(RB) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(RB + 32) : "memory");
+        __syncthreads();
+        if (t + 2 < t1) stage(t + 2);
+        const float* xt = (const float*)(lds + (t - t0) % 3 * BUF) + h * 32 + r;
+        f32x16 acc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16 * RB; ++j) acc = mfma32(xt[2 * j * 32], d[j], acc);
+        float* rows = g.dw + (long)t * 32 * g.v;
+        const int left = g.e - t * 32 < 32 ? g.e - t * 32 : 32;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(rows, 0, (unsigned)(left * g.v * 4), 0x00020000);
+        auto at = [&](int i) { return c < g.v ? (unsigned)(acc_row(i, lane) * g.v + c) * 4u : 0xfffffff0u; };
+        float old[16];
+        if (g.accumulate) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) old[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, at(i), 0, 0));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[i] += old[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float q = acc[i];
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, q), rs, at(i), 0, 0);
+        }
+    }
+}
+
 __global__ __launch_bounds__(256) void xent_zero_kernel(float* __restrict__ a, long na, float* __restrict__ b, long nb) {
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < na || i < nb; i += (long)gridDim.x * 256) {
         if (i < na) a[i] = 0.f;
@@ -1480,29 +1920,155 @@ void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const floa
     else hipLaunchKernelGGL(xent_prep_kernel<false>, grid, dim3(256), 0, st, p);
 }
 
-void launch_dx_join(const Layout& l, char* ws, void* dx, bool xf32, int64_t n, int64_t e, hipStream_t st) {
-    const float *parts = (const float*)(ws + l.dxw), *scales = (const float*)(ws + l.scales);
-    const long part = (long)(l.np * l.ep);
-    const float* rs = l.narrow ? nullptr : (const float*)(ws + l.rs);
-    const float2* row = (const float2*)(ws + l.row);
+// dx from `nx` parts of `part` values; scales NULL: they are dx, not the streamed or the wide products' planes
+void launch_dx_join(const float* parts, const float* scales, const float2* row, const float* rs, void* dx, bool xf32, int64_t nx, int64_t part,
+                    int64_t n, int64_t e, int64_t ep, hipStream_t st) {
     // sixteen groups of parts: 200 x 128 x 65536 94.8 us a backward against 101.3 with one, 53 x 75 x 25145 56.4 against 61.3; with the
     // outputs of 3000 x 32 x 8192 one group fills the chip (75.2 against 83.3)
-    if (l.nx >= 16 && n * l.ep <= 1 << 16) {
-        hipLaunchKernelGGL(xent_dx_join_kernel<16>, dim3((unsigned)(up(n * l.ep, 64) / 64)), dim3(1024), 0, st, parts, scales, row, rs, dx,
-                           (int)xf32, (int)l.nx, part, (long)n, (int)e, (int)l.ep);
+    if (nx >= 16 && n * ep <= 1 << 16) {
+        hipLaunchKernelGGL(xent_dx_join_kernel<16>, dim3((unsigned)(up(n * ep, 64) / 64)), dim3(1024), 0, st, parts, scales, row, rs, dx,
+                           (int)xf32, (int)nx, (long)part, (long)n, (int)e, (int)ep);
     } else {
-        const int64_t blocks = up(n * l.ep, 256) / 256;
+        const int64_t blocks = up(n * ep, 256) / 256;
         hipLaunchKernelGGL(xent_dx_join_kernel<1>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, parts, scales, row, rs, dx,
-                           (int)xf32, (int)l.nx, part, (long)n, (int)e, (int)l.ep);
+                           (int)xf32, (int)nx, (long)part, (long)n, (int)e, (int)ep);
     }
+}
+
+// ------------------------------------------------ a block of rows
+struct ShortLayout {
+    int64_t np, ep, vp, parts;
+    int64_t lab, row, bias, xt, xz, part, zlab, dz, dxp, total;
+};
+
+ShortLayout short_layout(int64_t n, int64_t e, int64_t v, bool backward) {
+    ShortLayout l = {};
+    l.np = up(n, 32);
+    l.ep = up(e, 128);
+    l.vp = up(v, 128);
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t o = at;
+        at += up(bytes, 1024);
+        return o;
+    };
+    l.lab = take(l.np * 4);
+    l.bias = take(l.vp * 4);
+    l.xt = take(l.ep * l.np * 4);
+    if (backward) {
+        l.row = take(l.np * 8);
+        l.xz = take(l.ep * l.np * 4);
+        l.dz = take(l.np * l.vp * 4);
+        // dx: two workgroups a CU, eight tiles of classes each at least
+        const int64_t wgs = l.ep / 128, tiles = up(v, 32) / 32;
+        l.parts = 512 / wgs < tiles / 8 ? 512 / wgs : tiles / 8;
+        if (l.parts < 1) l.parts = 1;
+        l.dxp = take(l.parts * l.np * l.ep * 4);
+    } else {
+        l.part = take(up(v, 128) / 32 * l.np * 8);
+        l.zlab = take(l.np * 4);
+    }
+    l.total = at;
+    return l;
+}
+
+// Logits by tiles of 128 classes where these fill the chip, otherwise 32 classes a workgroup (forward + backward of 64 rows and 1000
+// features: 59 + 156 us at 32768 classes, 81 + 168 the other way; 58 + 118 at 16384, 44 + 98 the other way).
+inline bool short_tiled(int64_t v) { return v >= 32768; }
+inline int64_t short_slices(int64_t v) { return short_tiled(v) ? up(v, 128) / 32 : up(v, 32) / 32; }
+
+template <int RB, bool BWD, bool W16>
+void launch_short_tiled(const XentShort& g, hipStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    constexpr int bytes = 3 * (32 * 512 + RB * 4096);
+    mgx_allow_dynamic_lds(xent_short_tiled_kernel<RB, BWD, W16>, bytes, done);
+    hipLaunchKernelGGL((xent_short_tiled_kernel<RB, BWD, W16>), dim3((unsigned)(up(g.v, 128) / 128)), dim3(256), bytes, st, g);
+}
+
+template <int RB, bool BWD>
+void launch_short_logits(const XentShort& g, hipStream_t st) {
+    if (!short_tiled(g.v))
+        hipLaunchKernelGGL((xent_short_logits_kernel<RB, BWD>), dim3((unsigned)(up(g.v, 32) / 32)), dim3(256), 0, st, g);
+    else if (g.v % 4 == 0) launch_short_tiled<RB, BWD, true>(g, st);
+    else launch_short_tiled<RB, BWD, false>(g, st);
+}
+
+template <int RB, bool W16>
+void launch_short_dx(const XentShort& g, int64_t parts, hipStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    constexpr int bytes = 3 * (128 * 128 + RB * 4096 + 128);
+    mgx_allow_dynamic_lds(xent_short_dx_kernel<RB, W16>, bytes, done);
+    hipLaunchKernelGGL((xent_short_dx_kernel<RB, W16>), dim3((unsigned)(g.ep / 128), (unsigned)parts), dim3(256), bytes, st, g);
+}
+
+template <int RB>
+void short_backward(const XentShort& g, void* dx, bool xf32, int64_t parts, hipStream_t st) {
+    launch_short_logits<RB, true>(g, st);
+    if (dx) {
+        if (g.v % 4 == 0) launch_short_dx<RB, true>(g, parts, st);
+        else launch_short_dx<RB, false>(g, parts, st);
+        launch_dx_join(g.dxp, nullptr, nullptr, nullptr, dx, xf32, parts, (int64_t)g.np * g.ep, g.n, g.e, g.ep, st);
+    }
+    if (g.dw) {
+        const int64_t cols = up(g.v, 128) / 128, blocks = up(g.e, 32) / 32;
+        int64_t kg = cols * blocks / 1024;               // four workgroups a CU where there is enough, up to 16 blocks each
+        kg = kg < 1 ? 1 : (kg > 16 ? 16 : kg);
+        hipLaunchKernelGGL(xent_short_dw_kernel<RB>, dim3((unsigned)cols, (unsigned)(up(blocks, kg) / kg)), dim3(256), 3 * RB * 4096, st, g, (int)kg);
+    }
+}
+
+int short_call(XentShort g, bool xf32, const ShortLayout& l, char* ws, float* loss, float* lse, int* hits, void* dx, bool backward,
+               hipStream_t st) {
+    g.np = (int)l.np; g.ep = (int)l.ep; g.vp = l.vp;
+    g.lab = (int*)(ws + l.lab); g.bias = (float*)(ws + l.bias); g.xt = (float*)(ws + l.xt);
+    if (backward) {
+        g.row = (float2*)(ws + l.row); g.xz = (float*)(ws + l.xz); g.dz = (float*)(ws + l.dz); g.dxp = (float*)(ws + l.dxp);
+    } else {
+        g.part = (float2*)(ws + l.part); g.zlab = (float*)(ws + l.zlab);
+    }
+    const int tiles = (int)(l.np / 32 * (l.ep / 64));
+    const dim3 grid((unsigned)(tiles + 64));
+    if (xf32) hipLaunchKernelGGL(xent_short_prep_kernel<true>, grid, dim3(256), 0, st, g, tiles);
+    else hipLaunchKernelGGL(xent_short_prep_kernel<false>, grid, dim3(256), 0, st, g, tiles);
+    const int rb = g.np / 32;
+    if (backward) {
+        if (rb == 1) short_backward<1>(g, dx, xf32, l.parts, st);
+        else if (rb == 2) short_backward<2>(g, dx, xf32, l.parts, st);
+        else if (rb == 3) short_backward<3>(g, dx, xf32, l.parts, st);
+        else short_backward<4>(g, dx, xf32, l.parts, st);
+    } else {
+        if (rb == 1) launch_short_logits<1, false>(g, st);
+        else if (rb == 2) launch_short_logits<2, false>(g, st);
+        else if (rb == 3) launch_short_logits<3, false>(g, st);
+        else launch_short_logits<4, false>(g, st);
+        hipLaunchKernelGGL(xent_short_join_kernel, dim3((unsigned)g.n), dim3(256), 0, st, g, loss, lse, hits, (int)short_slices(g.v));
+    }
+    return mgx_launch_status();
+}
+
+// Which form a call takes (both sides measured, forward + backward in us, float32):
+//   few rows | a block of rows   1 x 128 x 4097 15 + 17 | 18 + 30; 4 x 128 x 65536 15 + 42 | 19 + 45; 4 x 1000 x 10001 32 + 97 | 27 + 64;
+//                                16 x 128 x 4097 16 + 24 | 18 + 31; 8 x 32 x 65536 16 + 44 | 18 + 35; 8 x 300 x 1000 19 + 46 | 18 + 31;
+//                                16 x 1000 x 65536 80 + 486 | 62 + 200
+//   a block of rows | matrix     17 x 1000 x 65536 62 + 201 | 300 + 603; 64 x 1000 x 10001 43 + 98 | 72 + 138; 64 x 128 x 4097 18 + 37 | 22 + 37;
+//                                64 x 32 x 65536 18 + 47 | 35 + 52; 128 x 1000 x 65536 172 + 495 | 328 + 648;
+//                                128 x 128 x 65536 38 + 109 | 51 + 80; 128 x 1000 x 10001 74 + 174 | 73 + 146
+enum { FORM_FEW, FORM_SHORT, FORM_MATRIX };
+int form_of(int64_t n, int64_t e, int64_t v) {
+    if (n <= 4 && e * v <= 1 << 23) return FORM_FEW;
+    if (n <= FEW && e <= RC && e * v <= 1 << 20) return FORM_FEW;
+    return n <= 64 || (n <= 128 && e > 128 && v >= 32768) ? FORM_SHORT : FORM_MATRIX;
 }
 
 }  // namespace
 
 extern "C" int64_t mgx_dense_xent_workspace(int64_t n, int64_t e, int64_t v, int x_is_f32, int backward) {
     if (!sizes_ok(n, e, v)) return -1;
-    if (n > 0 && n <= FEW) return few_bytes(n, e, v, backward != 0);
-    return n == 0 ? 0 : layout(n, e, v, x_is_f32 != 0, backward != 0).total;
+    if (n == 0) return 0;
+    const int form = form_of(n, e, v);
+    if (form == FORM_FEW) return few_bytes(n, e, v, backward != 0);
+    if (form == FORM_SHORT) return short_layout(n, e, v, backward != 0).total;
+    return layout(n, e, v, x_is_f32 != 0, backward != 0).total;
 }
 
 extern "C" int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, const float* b, const int32_t* labels,
@@ -1514,13 +2080,21 @@ extern "C" int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, c
     if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)workspace) & 15u) != 0) return MGX_ERR_ARG;
     const bool xf = x_is_f32 != 0;
     hipStream_t st = (hipStream_t)stream;
-    if (n <= FEW) {
+    const int form = form_of(n, e, v);
+    if (form == FORM_FEW) {
         if (workspace_bytes < few_bytes(n, e, v, false)) return MGX_ERR_WORKSPACE;
         XentRows g = {};
         g.x = x; g.w = w; g.b = b; g.labels = labels; g.n = (int)n; g.e = (int)e; g.v = v;
         g.part = (float2*)workspace;
         g.zlab = (float*)((char*)workspace + up(up(v, 64) / 64 * n * 8, 16));
         return xf ? few_forward<true>(g, loss, lse, hits, st) : few_forward<false>(g, loss, lse, hits, st);
+    }
+    if (form == FORM_SHORT) {
+        const ShortLayout l = short_layout(n, e, v, false);
+        if (workspace_bytes < l.total) return MGX_ERR_WORKSPACE;
+        XentShort g = {};
+        g.x = x; g.w = w; g.b = b; g.labels = labels; g.n = (int)n; g.e = (int)e; g.v = v;
+        return short_call(g, xf, l, (char*)workspace, loss, lse, hits, nullptr, false, st);
     }
     const Layout l = layout(n, e, v, xf, false);
     if (workspace_bytes < l.total) return MGX_ERR_WORKSPACE;
@@ -1561,13 +2135,22 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
     if (!x || !w || !labels || !lse || !dloss || !workspace) return MGX_ERR_ARG;
     if ((((uintptr_t)x | (uintptr_t)w | (uintptr_t)workspace) & 15u) != 0) return MGX_ERR_ARG;
     const bool xf = x_is_f32 != 0;
-    if (n <= FEW) {
+    const int form = form_of(n, e, v);
+    if (form == FORM_FEW) {
         if (workspace_bytes < few_bytes(n, e, v, true)) return MGX_ERR_WORKSPACE;
         XentRows g = {};
         g.x = x; g.w = w; g.b = b; g.lse = lse; g.dloss = dloss; g.labels = labels; g.n = (int)n; g.e = (int)e; g.v = v;
         g.dxp = dx ? (float*)workspace : nullptr;
         g.dw = dw; g.db = db; g.accumulate = accumulate;
         return xf ? few_backward<true>(g, dx, st) : few_backward<false>(g, dx, st);
+    }
+    if (form == FORM_SHORT) {
+        const ShortLayout l = short_layout(n, e, v, true);
+        if (workspace_bytes < l.total) return MGX_ERR_WORKSPACE;
+        XentShort g = {};
+        g.x = x; g.w = w; g.b = b; g.lse = lse; g.dloss = dloss; g.labels = labels; g.n = (int)n; g.e = (int)e; g.v = v;
+        g.dw = dw; g.db = db; g.accumulate = accumulate;
+        return short_call(g, xf, l, (char*)workspace, nullptr, nullptr, nullptr, dx, true, st);
     }
     const Layout l = layout(n, e, v, xf, true);
     if (workspace_bytes < l.total) return MGX_ERR_WORKSPACE;
@@ -1584,7 +2167,7 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
             q.tiles = (int)(l.vp / ST); q.out = (float*)(ws + l.dxw); q.ld = l.np;
             if (xf) launch_stream<2, 2, 1, MODE_DX, 2>(l, q, l.np / l.rows_wg, l.nx, st);
             else launch_stream<1, 1, 2, MODE_DX, 1>(l, q, l.np / l.rows_wg, l.nx, st);
-            launch_dx_join(l, ws, dx, xf, n, e, st);
+            launch_dx_join((float*)(ws + l.dxw), q.scales, q.row, nullptr, dx, xf, l.nx, l.np * l.ep, n, e, l.ep, st);
         }
         if (dw || db) {
             q.r[0] = wh; q.r[1] = wl; q.s[0] = xh; q.s[1] = xl;
@@ -1642,6 +2225,7 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
             weights(vm, cnt, l.nz);
         }
     }
-    if (dx) launch_dx_join(l, ws, dx, xf, n, e, st);
+    if (dx)
+        launch_dx_join((float*)(ws + l.dxw), (float*)(ws + l.scales), nullptr, (float*)(ws + l.rs), dx, xf, l.nx, l.np * l.ep, n, e, l.ep, st);
     return mgx_launch_status();
 }

@@ -505,3 +505,25 @@ def test_masked_classes_may_hold_anything(n, e, v, mask, dtype):
         assert all(torch.equal(got[k], want[k]) for k in want), fill
     check(got, reference(x, clean, b, labels, dloss), dtype, float((x.double() @ clean.double()).abs().max()))
     assert bool((got["dw"][:, off] == 0).all()) and bool((got["db"][off] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("n,e,v", [(17, 1, 1), (17, 16, 33), (32, 15, 4097), (33, 63, 300), (64, 129, 1000), (65, 300, 2049), (96, 128, 130),
+                                   (97, 1000, 4001), (128, 257, 31), (100, 17, 40000), (128, 1000, 5000),
+                                   (20, 70, 40003), (60, 130, 32770), (70, 40, 32768), (128, 20, 33001)])
+def test_blocks_of_rows(n, e, v, dtype, accumulate):
+    """17 to 128 rows: every count of row blocks, features and classes that end inside a tile, rows of W with and without whole
+    16-byte pieces."""
+    x, w, b, labels, dloss = case(n, e, v, dtype, seed=80 + e)
+    labels[0], labels[1], labels[2] = 0, v - 1, v // 2
+    want = reference(x, w, b, labels, dloss)
+    largest = float((x.double() @ w.double()).abs().max())
+    if accumulate:
+        gen = torch.Generator().manual_seed(81)
+        dw, db = torch.randn(w.shape, generator=gen) * 1e-3, torch.randn(b.shape, generator=gen) * 1e-3
+        want["dw"], want["db"] = want["dw"] + dw.double(), want["db"] + db.double()
+        check(run(x, w, b, labels, dloss, accumulate=True, dw=dw, db=db), want, dtype, largest)
+    else:
+        check(run(x, w, b, labels, dloss), want, dtype, largest)
