@@ -1107,7 +1107,7 @@ def conv_bwd_tape8(d: ConvDesc, t: Tape8, g, w, dw, dbias, dx, act_alpha=0.0):
     nbytes = lib.mgx_conv_bwd_bf16_workspace(C.byref(d))
     if nbytes <= 0:
         raise MgxError("conv_bwd_tape8: unsupported descriptor")
-    ws = K.workspace(nbytes)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=g.device)      # of its own: two captured graphs never share it
     e0 = PROFILER.start() if PROFILER is not None else None
     check(lib.mgx_conv_bwd_tape8(C.byref(d), pc, pe, _pb(g), _p(w), _p(dw), _p(dbias), _pb(dx), float(act_alpha),
                                  ws.data_ptr(), ws.numel(), K.stream_ptr()), "mgx_conv_bwd_tape8")

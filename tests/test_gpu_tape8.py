@@ -374,3 +374,41 @@ def test_train_step(tape8, use_graph):
         before = len(gan._graphs)
         gan.train_step(real)
         assert len(gan._graphs) == before + 1
+
+
+@gpu
+def test_two_captured_graphs_share_nothing():
+    """Two backward calls captured into graphs of their own and replayed on two streams at once: each call's scratch memory is
+    its own, also after later calls asked for more."""
+    sets = []
+    for seed, (n, h, w) in enumerate(((2, 16, 700), (1, 24, 900))):
+        d, x, g, wt = conv_case(n, h, w, 32, 3, seed + 30)
+        t, g, wt = ops.tape8_pack(x.cuda()), g.cuda(), wt.cuda()
+        dx, dw, db = torch.empty_like(g), torch.zeros_like(wt), torch.zeros((32,)).cuda()
+
+        def step(d=d, t=t, g=g, wt=wt, dx=dx, dw=dw, db=db):
+            dw.zero_()
+            db.zero_()
+            ops.conv_bwd_tape8(d, t, g, wt, dw, db, dx, ALPHA)
+
+        step()
+        torch.cuda.synchronize()
+        want = [v.clone() for v in (dx, dw, db)]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        sets.append((graph, (dx, dw, db), want, torch.cuda.Stream(), (t, g, wt)))      # a replay reads the captured tensors
+    d, x, g, wt = conv_case(2, 64, 3000, 32, 3, 40)
+    ops.conv_bwd_tape8(d, ops.tape8_pack(x.cuda()), g.cuda(), wt.cuda(), torch.zeros_like(wt).cuda(), torch.zeros((32,)).cuda(),
+                       torch.empty_like(g).cuda(), ALPHA)
+    for _ in range(3):
+        for graph, outs, _, st, _ in sets:
+            for v in outs:
+                v.fill_(7.0)
+        torch.cuda.synchronize()
+        for graph, _, _, st, _ in sets:
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, outs, want, _, _ in sets:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
