@@ -137,9 +137,12 @@ def labels_to_device(y) -> torch.Tensor:
     return t.to(device=K.device(), dtype=torch.float32).contiguous()
 
 
-def _class_numbers(y) -> bool:
-    """Labels are class numbers (an integer type: sparse categorical cross-entropy) rather than one-hot rows."""
-    return not (y.is_floating_point() if isinstance(y, torch.Tensor) else np.issubdtype(np.asarray(y).dtype, np.floating))
+def _class_numbers(y, model=None) -> bool:
+    """Labels are class numbers (sparse categorical cross-entropy) rather than one-hot rows: an integer type, and not the
+    shape of the model's output, which one-hot rows of any type have."""
+    y = y if isinstance(y, torch.Tensor) else np.asarray(y)
+    whole = not (y.is_floating_point() if isinstance(y, torch.Tensor) else np.issubdtype(y.dtype, np.floating))
+    return whole and (model is None or tuple(y.shape[1:]) != tuple(model.output.shape[1:]))
 
 
 def class_numbers_to_device(y) -> torch.Tensor:
@@ -161,7 +164,7 @@ def evaluate(model, x, y, batch_size: int = 32) -> Dict[str, float]:
     """Mean categorical cross-entropy and accuracy over (x, y) - keras' evaluate / validation pass.  y: one-hot rows, or
     class numbers (one per sample or per position, negative: none), then the mean is over the labelled rows."""
     n = x.shape[0]
-    if _class_numbers(y):
+    if _class_numbers(y, model):
         trunk, head = _split_head(model)
         sums = torch.zeros((3,), dtype=torch.float64, device=K.device())
         for i in range(0, n, batch_size):
@@ -188,7 +191,7 @@ def fit_evaluator(model, x, y, epochs: int, batch_size: int, optimizer=None, val
     model.fit(X, y, epochs, batch_size, validation_data) of evaluacion.py:160-161.  Returns the
     history: per epoch the sample-weighted mean of the batch losses / accuracies (and val_*).
 
-    y as an integer array holds class numbers instead of one-hot rows (keras' sparse categorical cross-entropy): one per
+    y as an integer array that has not the shape of one-hot rows holds class numbers (keras' sparse categorical cross-entropy): one per
     sample, or one per position for a head without a Flatten in front; negative numbers are positions without a label, and
     a batch's loss is the mean over its labelled ones.  The logits of that form are never stored, so that it is the one for
     many classes or many positions; backend.TAPE8 keeps the rest of the tape in 8 bits."""
@@ -197,7 +200,7 @@ def fit_evaluator(model, x, y, epochs: int, batch_size: int, optimizer=None, val
     n = x.shape[0]
     rng = np.random.default_rng(shuffle_seed)
     hist: Dict[str, List[float]] = {"loss": [], "accuracy": []}
-    numbers = _class_numbers(y)
+    numbers = _class_numbers(y, model)
     if numbers:
         trunk, head = _split_head(model)
         y = np.ascontiguousarray(y.cpu().numpy() if isinstance(y, torch.Tensor) else y)

@@ -527,3 +527,87 @@ def test_blocks_of_rows(n, e, v, dtype, accumulate):
         check(run(x, w, b, labels, dloss, accumulate=True, dw=dw, db=db), want, dtype, largest)
     else:
         check(run(x, w, b, labels, dloss), want, dtype, largest)
+
+
+@gpu
+def test_integer_one_hot_rows_are_one_hot_rows():
+    """One-hot labels of an integer type, which have the shape of the model's output, are what they were with float rows."""
+    from music_generator_amd import evaluacion
+    from music_generator_amd.graph import Input, Model
+    from music_generator_amd.layers import Flatten
+
+    gen = np.random.default_rng(5)
+    x = gen.uniform(-1, 1, (6, 2, 8, 4)).astype(np.float32)
+    hot = np.eye(5, dtype=np.int64)[gen.integers(0, 5, 6)]
+    M.clear_session()
+    t = Input(shape=(2, 8, 4))
+    model = Model(t, evaluacion.SoftmaxDense(5)(Flatten()(t)))
+    a = evaluacion.evaluate(model, x, hot.astype(np.float32), 4)
+    assert evaluacion.evaluate(model, x, hot, 4) == a == evaluacion.evaluate(model, x, torch.from_numpy(hot), 4)
+    b = evaluacion.evaluate(model, x, hot.argmax(axis=1), 4)
+    assert b["accuracy"] == a["accuracy"] and b["loss"] == pytest.approx(a["loss"], rel=1e-5)
+    start = [v.numpy().copy() for v in model.trainable_variables]
+    runs = []
+    for y in (hot.astype(np.float32), hot, hot.argmax(axis=1)):
+        for v, value in zip(model.trainable_variables, start):
+            v.assign(value)
+        runs.append(evaluacion.fit_evaluator(model, x, y, 2, 4))
+    assert runs[0] == runs[1]
+    assert runs[2]["loss"] == pytest.approx(runs[0]["loss"], rel=1e-4)
+
+
+@gpu
+@pytest.mark.parametrize("n,e,v,dtype", [(3, 300, 7500000, torch.float32), (100, 300, 7500001, torch.float32), (200, 300, 7500000, torch.float32),
+                                         (150, 128, 8000000, torch.bfloat16), (8000000, 128, 300, torch.bfloat16),
+                                         (8000000, 290, 140, torch.bfloat16)])
+def test_offsets_beyond_32_bits(n, e, v, dtype):
+    """Operands of more than 2^32 bytes: loss, lse and gradients of some rows and classes, the last ones among them, against
+    float64 on the device.  Tolerances of check(), per row and class."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn((n, e), generator=gen, device="cuda").to(dtype)
+    w = torch.randn((e, v), generator=gen, device="cuda") / e ** 0.5
+    b = torch.randn((v,), generator=gen, device="cuda") * 0.3
+    labels = torch.randint(0, v, (n,), generator=gen, device="cuda", dtype=torch.int32)
+    labels[-1] = v - 1
+    dloss = torch.rand((n,), generator=gen, device="cuda") + 0.5
+    loss, lse = torch.empty((n,), device="cuda"), torch.empty((n,), device="cuda")
+    ops.dense_xent_fwd(x, w, b, labels, loss, lse)
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+    ops.dense_xent_bwd(x, w, b, labels, lse, dloss, dx, dw, db)
+    rows = torch.unique(torch.cat([torch.randint(0, n, (20,), generator=gen, device="cuda"), torch.tensor([0, n - 1], device="cuda")]))
+    cols = torch.unique(torch.cat([torch.randint(0, v, (20,), generator=gen, device="cuda"), torch.tensor([0, v - 1], device="cuda")]))
+    xr, lr = x[rows].double(), labels[rows].long()
+    z = torch.empty((len(rows), v), dtype=torch.float64, device="cuda")
+    for c in range(0, v, 500000):
+        z[:, c:c + 500000] = xr @ w[:, c:c + 500000].double() + b[c:c + 500000].double()
+    unit = 2.0 ** -23 * (8 + 2 * float(z.abs().max()))
+    want = torch.logsumexp(z, dim=1)
+    at = z.gather(1, lr[:, None])[:, 0]
+    assert float((lse[rows].double() - want).abs().max()) <= unit + 2.0 ** -23 * float(want.abs().max())
+    assert float((loss[rows].double() - (want - at)).abs().max()) <= unit + 2.0 ** -23 * float(want.abs().max())
+    z = torch.exp(z - want[:, None])
+    z[torch.arange(len(rows), device="cuda"), lr] -= 1.0
+    z *= dloss[rows].double()[:, None]
+    dxr = torch.zeros((len(rows), e), dtype=torch.float64, device="cuda")
+    for c in range(0, v, 500000):
+        dxr += z[:, c:c + 500000] @ w[:, c:c + 500000].double().t().contiguous()
+    del z
+    slack = unit * dloss[rows].double() * w[:, lr].double().norm(dim=0)
+    tol = 4 * unit + (2.0 ** -8 + 2.0 ** -10 if dtype == torch.bfloat16 else 0.0)
+    assert bool(((dx[rows].double() - dxr).norm(dim=1) <= tol * dxr.norm(dim=1) + slack).all())
+    # classes: every row's probability of them, from the kernel's lse (checked above on the rows)
+    dwc, dbc = torch.zeros((e, len(cols)), dtype=torch.float64, device="cuda"), torch.zeros((len(cols),), dtype=torch.float64, device="cuda")
+    size = torch.zeros((len(cols),), dtype=torch.float64, device="cuda")
+    wc, bc = w[:, cols].double(), b[cols].double()
+    for i in range(0, n, 500000):
+        xi = x[i:i + 500000].double()
+        hot = (labels[i:i + 500000, None].long() == cols[None]).double()
+        d = (torch.exp(xi @ wc + bc - lse[i:i + 500000].double()[:, None]) - hot) * dloss[i:i + 500000].double()[:, None]
+        dwc += xi.t().contiguous() @ d
+        dbc += d.sum(dim=0)
+        size += d.abs().sum(dim=0)          # terms of both signs: a float32 sum and 2^-24 of the scale are relative to these
+    most = float(x[:500000].abs().max())
+    assert bool(((db[cols].double() - dbc).abs() <= 4 * unit * size + 2.0 ** -24 * 1.5).all())
+    assert bool(((dw[:, cols].double() - dwc).abs().amax(dim=0) <= (4 * unit * size + 2.0 ** -24 * 1.5) * most).all())
+    del x, w, dx, dw
+    torch.cuda.empty_cache()

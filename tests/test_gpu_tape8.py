@@ -412,3 +412,45 @@ def test_two_captured_graphs_share_nothing():
         torch.cuda.synchronize()
         for _, outs, want, _, _ in sets:
             assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """Six clips of the full resolution (2.36e9 values): packing, unpacking and the derivative's product at both ends and
+    where the 32-bit offsets end, and the convolution's data gradient of the last clip against a call with that clip alone."""
+    n, h, w = 6, 256, 48000
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.empty((n, h, w, 32), dtype=torch.bfloat16, device="cuda")
+    g = torch.empty_like(x)
+    for i in range(n):
+        x[i] = torch.tanh(torch.randn((h, w, 32), generator=gen, device="cuda"))
+        g[i] = torch.randn((h, w, 32), generator=gen, device="cuda")
+    t = ops.tape8_pack(x)
+    y = ops.tape8_unpack(t)
+    flat, back = x.view(-1), y.view(-1)
+    for at in (0, 2 ** 30 - 4096, 2 ** 31 - 4096, flat.numel() - 8192):
+        part = ops.tape8_pack(flat[at:at + 8192].contiguous())
+        assert torch.equal(part.codes, t.codes[at:at + 8192]) and torch.equal(part.exps, t.exps[at // 32:at // 32 + 256])
+        assert torch.equal(back[at:at + 8192], ops.tape8_unpack(part))
+        product = ops.mul_dact_tape8(g.view(-1)[at:at + 8192].contiguous(), part, ALPHA)
+    del y, back
+    whole = ops.mul_dact_tape8(g, t, ALPHA)
+    assert torch.equal(whole.view(-1)[-8192:], product)
+    del whole
+    wt = (torch.randn((3, 3, 32, 32), generator=gen, device="cuda") / 17.0)
+    dw, db, dx = torch.zeros_like(wt), torch.zeros((32,), device="cuda"), torch.empty_like(x)
+
+    def desc(images):
+        return ops.make_conv_desc(nimg=images, hin=h, win=w, cin=32, hout=h, wout=w, kh=3, kw=3, pt=1, pl=1, ngemm=32, cout=32, wsk=32, wsn=1,
+                                  wtap=32 * 32, nbias=32)
+
+    ops.conv_bwd_tape8(desc(n), t, g, wt, dw, db, dx, ALPHA)
+    one = torch.empty_like(x[:1])
+    sums = torch.zeros_like(wt)
+    for i in range(n):
+        ops.conv_bwd_tape8(desc(1), ops.tape8_pack(x[i:i + 1]), g[i:i + 1], wt, sums, torch.zeros_like(db), one, ALPHA)
+        assert torch.equal(dx[i:i + 1], one), i
+    # the same terms added in another order: sums over 7.4e7 positions whose float32 partial sums are off by 2^-24 a level
+    assert float((dw - sums).norm()) <= 2.0 ** -16 * float(sums.norm())
+    del x, g, dx, t
+    torch.cuda.empty_cache()
