@@ -548,7 +548,7 @@ int mgx_tape8_unpack(const void* codes, const void* exps, void* y, int y_is_f32,
  * 1/act_alpha) recovered from it (mgx_mul_dact_bf16 reads a bf16 y). */
 int mgx_mul_dact_tape8(const void* a, int a_is_f32, const void* codes, const void* exps, float act_alpha, void* out,
                        int64_t n, void* stream);
-/* mgx_conv_bwd_bf16 (same descriptors, workspace and results) with the layer input read from the 8-bit tape. */
+/* mgx_conv_bwd_bf16 (same descriptors and workspace) with the layer input read from the 8-bit tape. */
 int mgx_conv_bwd_tape8(const mgx_conv_desc* d, const void* codes, const void* exps, const void* g, const float* w,
                        float* dw, float* dbias, void* dx, float act_alpha, void* workspace, int64_t workspace_bytes,
                        void* stream);
