@@ -966,18 +966,26 @@ __device__ __forceinline__ float sum_parts(const float* __restrict__ p, int n, l
 
 // dx from its parts in G groups of consecutive parts, then the groups in order: one group where the outputs fill the chip, sixteen
 // where they are few and the parts many
+struct XentDxJoin {
+    const float *parts, *scales;
+    const float2* rowinfo;
+    const float* rs;
+    void* dx;
+    int dx_f32, np;
+    long part, n;
+    int e, ep;
+};
+
 template <int G>
-__global__ __launch_bounds__(G == 1 ? 256 : 1024) void xent_dx_join_kernel(const float* __restrict__ parts, const float* __restrict__ scales,
-                                                                           const float2* __restrict__ rowinfo, const float* __restrict__ rs,
-                                                                           void* __restrict__ dx,
-                                                                           int dx_f32, int np, long part, long n, int e, int ep) {
+__device__ __forceinline__ void xent_dx_join(const XentDxJoin& j, long block, long blocks) {
     constexpr int W = G == 1 ? 256 : 64;
     __shared__ float red[G][G == 1 ? 1 : 64];
+    const auto [parts, scales, rowinfo, rs, dx, dx_f32, np, part, n, e, ep] = j;
     // streamed: the parts hold 2^14 dz / dloss, the rows 2^14 dloss / scales[2]; wide: 2^14 dz / rs
     const float f = !scales ? 1.f : (rs ? 1.f : scales[2] / kDz) / kDz / scales[0];
     const int lane = threadIdx.x % W, q = threadIdx.x / W;
     const int per = (np + G - 1) / G, p0 = q * per, cnt = np - p0 < per ? np - p0 : per;
-    for (long i = (long)blockIdx.x * W + lane; i - lane < n * ep; i += (long)gridDim.x * W) {
+    for (long i = block * W + lane; i - lane < n * ep; i += blocks * W) {
         float s = i < n * ep && cnt > 0 ? sum_parts(parts + p0 * part + i, cnt, part) : 0.f;
         if constexpr (G > 1) {
             __syncthreads();
@@ -994,6 +1002,11 @@ __global__ __launch_bounds__(G == 1 ? 256 : 1024) void xent_dx_join_kernel(const
             else ((bf16_t*)dx)[row * e + c] = (bf16_t)s;
         }
     }
+}
+
+template <int G>
+__global__ __launch_bounds__(G == 1 ? 256 : 1024) void xent_dx_join_kernel(XentDxJoin j) {
+    xent_dx_join<G>(j, blockIdx.x, gridDim.x);
 }
 
 // loss and lse of 32 rows per workgroup from the partial (maximum, sum) of the parts or of every 64 classes
@@ -1034,27 +1047,40 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
     }
 }
 
-// dW and db of a piece of the classes from the slabs of the split contraction, in order
-__global__ __launch_bounds__(256) void xent_dw_reduce_kernel(const float* __restrict__ slabs, const float* __restrict__ slabs_b,
-                                                             const float* __restrict__ scales, float* __restrict__ dw,
-                                                             float* __restrict__ db, int nz, long slab, long ldo, int e,
-                                                             long v, long c0, int accumulate) {
-    const long c = (long)blockIdx.x * 256 + threadIdx.x;
-    const int k = blockIdx.y;
-    if (c >= ldo || c0 + c >= v) return;
-    float s = 0.f;
-    if (k < e) {
-        if (!dw) return;
-        s = sum_parts(slabs + k * ldo + c, nz, slab);
-        s = s * (scales[2] / kDz) / scales[1];
-        float* d = dw + k * v + c0 + c;
-        *d = accumulate ? *d + s : s;
-    } else if (db) {
-        s = sum_parts(slabs_b + c, nz, ldo);
-        s *= scales[2] / kDz;
-        float* d = db + c0 + c;
-        *d = accumulate ? *d + s : s;
+// dW and db of a piece of the classes from the slabs of the split contraction, in order: 256 classes of a feature (or of db) a block
+struct XentDwReduce {
+    const float *slabs, *slabs_b, *scales;
+    float *dw, *db;
+    int nz;
+    long slab, ldo;
+    int e;
+    long v, c0, cnt;                   // classes of W, first class, classes of the piece
+    int accumulate;
+    long blocks() const { return (cnt + 255) / 256 * (e + 1); }
+};
+
+__device__ __forceinline__ void xent_dw_reduce(const XentDwReduce& g, long block) {
+    const long cols = (g.cnt + 255) / 256, k = block / cols, c = (block - k * cols) * 256 + threadIdx.x;
+    if (c >= g.cnt || g.c0 + c >= g.v) return;
+    const float f = g.scales[2] / kDz;
+    if (k < g.e) {
+        if (!g.dw) return;
+        const float s = sum_parts(g.slabs + k * g.ldo + c, g.nz, g.slab) * f / g.scales[1];
+        float* d = g.dw + k * g.v + g.c0 + c;
+        *d = g.accumulate ? *d + s : s;
+    } else if (g.db) {
+        const float s = sum_parts(g.slabs_b + c, g.nz, g.ldo) * f;
+        float* d = g.db + g.c0 + c;
+        *d = g.accumulate ? *d + s : s;
     }
+}
+
+__global__ __launch_bounds__(256) void xent_dw_reduce_kernel(XentDwReduce g) { xent_dw_reduce(g, blockIdx.x); }
+
+// both in one launch: the first `blocks` workgroups join dx
+__global__ __launch_bounds__(256) void xent_joins_kernel(XentDxJoin j, long blocks, XentDwReduce g) {
+    if ((long)blockIdx.x < blocks) xent_dx_join<1>(j, blockIdx.x, blocks);
+    else xent_dw_reduce(g, blockIdx.x - blocks);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -1920,19 +1946,20 @@ void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const floa
     else hipLaunchKernelGGL(xent_prep_kernel<false>, grid, dim3(256), 0, st, p);
 }
 
-// dx from `nx` parts of `part` values; scales NULL: they are dx, not the streamed or the wide products' planes
-void launch_dx_join(const float* parts, const float* scales, const float2* row, const float* rs, void* dx, bool xf32, int64_t nx, int64_t part,
-                    int64_t n, int64_t e, int64_t ep, hipStream_t st) {
+// dx from its parts (scales NULL: they are dx itself, not the streamed or the wide products' planes), together with dW from its slabs
+// where both remain to be done
+void launch_joins(const XentDxJoin* j, const XentDwReduce* g, hipStream_t st) {
     // sixteen groups of parts: 200 x 128 x 65536 94.8 us a backward against 101.3 with one, 53 x 75 x 25145 56.4 against 61.3; with the
     // outputs of 3000 x 32 x 8192 one group fills the chip (75.2 against 83.3)
-    if (nx >= 16 && n * ep <= 1 << 16) {
-        hipLaunchKernelGGL(xent_dx_join_kernel<16>, dim3((unsigned)(up(n * ep, 64) / 64)), dim3(1024), 0, st, parts, scales, row, rs, dx,
-                           (int)xf32, (int)nx, (long)part, (long)n, (int)e, (int)ep);
-    } else {
-        const int64_t blocks = up(n * ep, 256) / 256;
-        hipLaunchKernelGGL(xent_dx_join_kernel<1>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, parts, scales, row, rs, dx,
-                           (int)xf32, (int)nx, (long)part, (long)n, (int)e, (int)ep);
-    }
+    const int64_t outs = j ? j->n * j->ep : 0;
+    const bool groups = j && j->np >= 16 && outs <= 1 << 16;
+    if (groups) hipLaunchKernelGGL(xent_dx_join_kernel<16>, dim3((unsigned)(up(outs, 64) / 64)), dim3(1024), 0, st, *j);
+    int64_t blocks = up(outs, 256) / 256;
+    blocks = blocks < 4096 ? blocks : 4096;
+    if (g && j && !groups)
+        hipLaunchKernelGGL(xent_joins_kernel, dim3((unsigned)(blocks + g->blocks())), dim3(256), 0, st, *j, (long)blocks, *g);
+    else if (g) hipLaunchKernelGGL(xent_dw_reduce_kernel, dim3((unsigned)g->blocks()), dim3(256), 0, st, *g);
+    else if (!groups) hipLaunchKernelGGL(xent_dx_join_kernel<1>, dim3((unsigned)blocks), dim3(256), 0, st, *j);
 }
 
 // ------------------------------------------------ a block of rows
@@ -2007,7 +2034,8 @@ void short_backward(const XentShort& g, void* dx, bool xf32, int64_t parts, hipS
     if (dx) {
         if (g.v % 4 == 0) launch_short_dx<RB, true>(g, parts, st);
         else launch_short_dx<RB, false>(g, parts, st);
-        launch_dx_join(g.dxp, nullptr, nullptr, nullptr, dx, xf32, parts, (int64_t)g.np * g.ep, g.n, g.e, g.ep, st);
+        const XentDxJoin j = {g.dxp, nullptr, nullptr, nullptr, dx, (int)xf32, (int)parts, (long)g.np * g.ep, (long)g.n, g.e, g.ep};
+        launch_joins(&j, nullptr, st);
     }
     if (g.dw) {
         const int64_t cols = up(g.v, 128) / 128, blocks = up(g.e, 32) / 32;
@@ -2167,20 +2195,23 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
             q.tiles = (int)(l.vp / ST); q.out = (float*)(ws + l.dxw); q.ld = l.np;
             if (xf) launch_stream<2, 2, 1, MODE_DX, 2>(l, q, l.np / l.rows_wg, l.nx, st);
             else launch_stream<1, 1, 2, MODE_DX, 1>(l, q, l.np / l.rows_wg, l.nx, st);
-            launch_dx_join((float*)(ws + l.dxw), q.scales, q.row, nullptr, dx, xf, l.nx, l.np * l.ep, n, e, l.ep, st);
         }
+        const XentDxJoin j = {(float*)(ws + l.dxw), q.scales, q.row, nullptr, dx, (int)xf, (int)l.nx, (long)(l.np * l.ep), (long)n, (int)e, (int)l.ep};
         if (dw || db) {
             q.r[0] = wh; q.r[1] = wl; q.s[0] = xh; q.s[1] = xl;
             q.tiles = (int)(l.np / ST); q.out = (float*)(ws + l.slabs); q.outb = (float*)(ws + l.slabs_b); q.ld = l.vp;
             q.o = {dw, db, (long)v, (long)v, (int)e, accumulate, l.nz == 1};
             if (xf) launch_stream<2, 2, 1, MODE_DW, 2>(l, q, l.vp / 128, l.nz, st);
             else launch_stream<2, 1, 1, MODE_DW, 2>(l, q, l.vp / 128, l.nz, st);
-            if (l.nz > 1) hipLaunchKernelGGL(xent_dw_reduce_kernel, dim3((unsigned)(up(l.vp, 256) / 256), (unsigned)(e + 1)), dim3(256), 0, st,
-                               q.out, q.outb, q.scales, dw, db, (int)l.nz, (long)(l.ep * l.vp), (long)l.vp, (int)e, (long)v, 0L,
-                               accumulate);
         }
+        const XentDwReduce w_ = {q.out, q.outb, q.scales, dw, db, (int)l.nz, (long)(l.ep * l.vp), (long)l.vp, (int)e, (long)v, 0L, (long)l.vp, accumulate};
+        const bool slabs = (dw || db) && l.nz > 1;
+        if (dx || slabs) launch_joins(dx ? &j : nullptr, slabs ? &w_ : nullptr, st);
         return mgx_launch_status();
     }
+    const XentDxJoin join = {(float*)(ws + l.dxw), (float*)(ws + l.scales), nullptr, (float*)(ws + l.rs), dx, (int)xf, (int)l.nx,
+                             (long)(l.np * l.ep), (long)n, (int)e, (int)l.ep};
+    bool joined = false;
     for (int64_t c0 = 0; c0 < l.vp; c0 += l.vc) {
         const int64_t cnt = l.vp - c0 < l.vc ? l.vp - c0 : l.vc;
         f16_t *wh = (f16_t*)(ws + l.wh) + c0 * l.ep, *wl = (f16_t*)(ws + l.wl) + c0 * l.ep;
@@ -2216,16 +2247,18 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
                 q.o = {dw ? dw + first : nullptr, db ? db + first : nullptr, (long)v, (long)valid, (int)e, accumulate, nz == 1};
                 if (xf) launch_gemm<2, 2, true, true, EPI_DW, 2>(q, l.ep, a1 - a0, nz, st);
                 else launch_gemm<1, 2, true, true, EPI_DW, 2>(q, l.ep, a1 - a0, nz, st);
-                if (nz > 1) hipLaunchKernelGGL(xent_dw_reduce_kernel, dim3((unsigned)(up(a1 - a0, 256) / 256), (unsigned)(e + 1)), dim3(256), 0, st,
-                                   q.out, q.outb, g.scales, dw, db, (int)nz, (long)q.np, (long)vs, (int)e, (long)v, (long)first,
-                                   accumulate);
+                if (nz == 1) return;
+                const XentDwReduce s = {q.out, q.outb, g.scales, dw, db, (int)nz, (long)q.np, (long)vs, (int)e, (long)v, (long)first, (long)(a1 - a0),
+                                        accumulate};
+                const bool last = dx && c0 + cnt == l.vp;            // dx is complete with the last piece
+                launch_joins(last ? &join : nullptr, &s, st);
+                joined = joined || last;
             };
             const int64_t vm = l.vm < cnt ? l.vm : cnt;
             weights(0, vm, 1);
             weights(vm, cnt, l.nz);
         }
     }
-    if (dx)
-        launch_dx_join((float*)(ws + l.dxw), (float*)(ws + l.scales), nullptr, (float*)(ws + l.rs), dx, xf, l.nx, l.np * l.ep, n, e, l.ep, st);
+    if (dx && !joined) launch_joins(&join, nullptr, st);
     return mgx_launch_status();
 }
