@@ -611,3 +611,37 @@ def test_offsets_beyond_32_bits(n, e, v, dtype):
     assert bool(((dw[:, cols].double() - dwc).abs().amax(dim=0) <= (4 * unit * size + 2.0 ** -24 * 1.5) * most).all())
     del x, w, dx, dw
     torch.cuda.empty_cache()
+
+
+@gpu
+@pytest.mark.parametrize("n,e,v,dtype", [(2, 40, 500, torch.float32), (13, 30, 600, torch.bfloat16), (90, 200, 33000, torch.float32),
+                                         (60, 70, 500, torch.bfloat16), (140, 60, 700, torch.float32), (140, 200, 700, torch.bfloat16)])
+def test_two_captured_graphs_of_every_form(n, e, v, dtype):
+    """Each form captured twice, into graphs of their own, replayed on two streams at once and again: every replay gives the
+    bits of an eager call on the same values."""
+    sets = []
+    for seed in (90, 91):
+        x, w, b, labels, dloss = [t.cuda() for t in case(n, e, v, dtype, seed=seed)]
+        outs = [torch.empty((n,)).cuda(), torch.empty((n,)).cuda(), torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)]
+
+        def step(x=x, w=w, b=b, labels=labels, dloss=dloss, outs=outs):
+            ops.dense_xent_fwd(x, w, b, labels, outs[0], outs[1])
+            ops.dense_xent_bwd(x, w, b, labels, outs[1], dloss, outs[2], outs[3], outs[4])
+
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        sets.append((graph, step, outs, torch.cuda.Stream()))
+    for _ in range(3):
+        torch.cuda.synchronize()
+        for graph, _, _, st in sets:
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for graph, step, outs, _ in sets:
+            got = [t.clone() for t in outs]
+            for t in outs:
+                t.fill_(5.0)
+            step()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(got, outs))
