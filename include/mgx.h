@@ -535,9 +535,10 @@ int mgx_cast_bf16_to_f32(const void* x, float* y, int64_t n, void* stream);
  * 8-bit activation tape: what a taped forward keeps of an activation (tf.GradientTape keeps float32, trainer/models.py:118)
  * at 33 bytes per 32 values.  32 consecutive values share H, the smallest power of two (2^-118 or more) that
  * their largest magnitude does not exceed by more than H / 256; a value v is kept as the byte floor(128 v / H) + 128, held in
- * 0 .. 255, and stands for (byte - 127.5) H / 128, exact in bf16 and half a step (H / 256) off at most (above H: a step).  The block's exponent byte is log2(H) + 126; 0: a block of zeros, which
- * stands for zeros; 255: a block with an infinity or a NaN, which stands for NaN throughout.  The last block of a tensor
- * may be shorter; its codes are stored as a whole block.
+ * 0 .. 255, and stands for (byte - 127.5) H / 128, exact in bf16 and half a step (H / 256) off at most (above H: a step).
+ * The block's exponent byte is log2(H) + 126; 0: a block of zeros, which stands for zeros; 255: a block with an
+ * infinity or a NaN, which stands for NaN throughout.  The last block of a tensor may be shorter; its codes are
+ * stored as a whole block.
  *   codes: 32 * mgx_tape8_blocks(n) bytes, exps: mgx_tape8_blocks(n) bytes.  Tensor pointers and `codes` are 16-byte
  *   aligned (MGX_ERR_ARG otherwise); n = 0 does nothing.
  * ---------------------------------------------------------------------------------------- */
@@ -563,10 +564,11 @@ int mgx_conv_bwd_tape8(const mgx_conv_desc* d, const void* codes, const void* ex
  * x (n, e) float32 or bf16, w (e, v) and b (v, may be NULL) float32, labels (n).  A label outside [0, v) marks a row without
  * a loss: loss, lse, hits and its gradients are 0 and its features are not used.  A bias of -inf (or the lowest float)
  * masks a class: its probability is 0 and its column of w is not used (one class at least is not masked; a row whose label is
- * masked has the loss of that bias).  Any of dx, dw, db may be NULL.  n <= 8 000 000, v <= 8 000 000, e <= 65 000; x, w and the workspace
- * 16-byte aligned; the workspace (mgx_dense_xent_workspace bytes, -1: sizes out of range) is the call's alone while it
+ * masked has the loss of that bias).  Any of dx, dw, db may be NULL.  n <= 8 000 000, v <= 8 000 000, e <= 65 000; x, w
+ * and the workspace 16-byte aligned; the workspace (mgx_dense_xent_workspace bytes, -1: sizes out of range) is the call's alone while it
  * runs.  float32 quality throughout: the products are sums of products of fp16 halves of the operands (22 bits, counted from an
- * operand's largest magnitude down to 2^-14 of it), or in float32 where rows are few.
+ * operand's largest magnitude down to 2^-14 of it), or in float32 where rows are few; a bf16 dx is within 2^-10 of its 2-norm
+ * before it is rounded.
  * ---------------------------------------------------------------------------------------- */
 int64_t mgx_dense_xent_workspace(int64_t n, int64_t e, int64_t v, int x_is_f32, int backward);
 int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, const float* b, const int32_t* labels, float* loss,

@@ -2,11 +2,12 @@
 // takes them as a tensor: the reference's Dense(9, softmax) + categorical_crossentropy, trainer/evaluacion.py:97, 160).
 //     z = x W + b (n x v)     lse_i = log sum_j exp(z_ij)     loss_i = lse_i - z_i,label(i)
 //     dz_ij = dloss_i (exp(z_ij - lse_i) - [j = label(i)])    dx = dz W^T    dW = x^T dz    db_j = sum_i dz_ij
-// x is n x e (float32 or bf16), W e x v and b v (float32, the Keras layout).  The logits exist as 32 x 32 accumulator
-// tiles only: the forward reduces each to a maximum and a sum per row, the backward computes them again, turns them into
-// dz and feeds dz to the two gradient products, a piece of the classes at a time.
+// x is n x e (float32 or bf16), W e x v and b v (float32, the Keras layout).  The logits exist in registers (accumulator
+// tiles) only: the forward reduces each tile to a maximum and a sum per row, the backward computes them again, turns them into
+// dz and feeds dz to the two gradient products.
 //
-// Arithmetic: all products run on v_mfma_f32_32x32x16_f16 with float32 accumulation, at float32 quality.  A float32
+// Arithmetic: few rows in float32.  The products of many rows run on v_mfma_f32_32x32x16_f16 with float32 accumulation, at
+// float32 quality.  A float32
 // operand is the sum of two fp16 planes, hi = fp16(s a) and lo = fp16(s a - hi) with s a power of two that brings the
 // operand's largest magnitude below 2^14: 22 significant bits, and 2^-25 of 2^14 absolute where a value is small.  The
 // product keeps hi hi + hi lo + lo hi (the dropped lo lo is 2^-24 of it).  A bf16 operand is exact in one plane.  This is
@@ -627,8 +628,9 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
     const int t0 = blockIdx.y * per, t1 = t0 + per < g.tiles ? t0 + per : g.tiles;
 
     // LDS-DMA of tile t: a wave fills 1 KB pieces (4 rows of 256 B or 8 of 128 B), lane l the 16-byte place l of the piece with
-    // the chunk that belongs there: the swizzle of the lane's row in the first piece, and a bit that is uniform in later ones.  In assembly: in front of a transposed LDS read the compiler waits for every LDS-DMA it knows of, the
-    // one just issued for a later tile included.
+    // the chunk that belongs there: the swizzle of the lane's row in the first piece, and a bit that is uniform in later ones.
+    // In assembly: in front of a transposed LDS read the compiler waits for every LDS-DMA it knows of, the one just issued
+    // for a later tile included.
     // beside the planes: FWD and DX the biases, DW (lse, dloss) and the labels of the tile's items
     const void* ip = MODE != MODE_DW ? (const void*)g.bias : wv == 0 ? (const void*)g.row : (const void*)g.lab;
     const int lrow = EP == 128 ? lane >> 4 : lane >> 3;
@@ -1800,13 +1802,16 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
     l.vp = up(v, l.narrow ? 128 : 256);
     l.ep = e <= 64 ? 64 : up(e, 128);
     // Parts of a contraction of `tiles` steps by `wgs` workgroups, `slots` of which run at once: a step takes step_us, and each part
-    // costs a start of half a step's latency (1 us) and `bytes` written and read once more for the join at 4 TB/s (one part of dW goes to the gradient itself).
+    // costs a start of half a step's latency (1 us) and `bytes` written and read once more for the join at 4 TB/s (one part
+    // of dW goes to the gradient itself).  Swept over the parts, the choice was within 5 % of the best from 300 x 64 x 3001
+    // to 700 x 128 x 65536 and 8000 x 100 x 1500.
     auto split = [](int64_t wgs, int64_t tiles, int64_t slots, double step_us, double bytes, bool direct = false, double* time = nullptr) {
         int64_t best = 1;
         double least = 1e30;
         for (int64_t p = 1; p <= 128 && (p == 1 || tiles / p >= 4); ++p) {
             const double rounds = (double)((wgs * p + slots - 1) / slots);
-            const double t = rounds * ((double)((tiles + p - 1) / p) * step_us + 1.0) + (direct && p == 1 ? 0.0 : 4.0 + (double)p * (bytes * 2.0 / 4e6 + 0.05));
+            const double join = direct && p == 1 ? 0.0 : 4.0 + (double)p * (bytes * 2.0 / 4e6 + 0.05);
+            const double t = rounds * ((double)((tiles + p - 1) / p) * step_us + 1.0) + join;
             if (t < least) {
                 least = t;
                 best = p;
@@ -2196,7 +2201,8 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
             if (xf) launch_stream<2, 2, 1, MODE_DX, 2>(l, q, l.np / l.rows_wg, l.nx, st);
             else launch_stream<1, 1, 2, MODE_DX, 1>(l, q, l.np / l.rows_wg, l.nx, st);
         }
-        const XentDxJoin j = {(float*)(ws + l.dxw), q.scales, q.row, nullptr, dx, (int)xf, (int)l.nx, (long)(l.np * l.ep), (long)n, (int)e, (int)l.ep};
+        const XentDxJoin j = {(float*)(ws + l.dxw), q.scales, q.row, nullptr, dx, (int)xf, (int)l.nx, (long)(l.np * l.ep), (long)n, (int)e,
+                              (int)l.ep};
         if (dw || db) {
             q.r[0] = wh; q.r[1] = wl; q.s[0] = xh; q.s[1] = xl;
             q.tiles = (int)(l.np / ST); q.out = (float*)(ws + l.slabs); q.outb = (float*)(ws + l.slabs_b); q.ld = l.vp;
@@ -2204,9 +2210,10 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
             if (xf) launch_stream<2, 2, 1, MODE_DW, 2>(l, q, l.vp / 128, l.nz, st);
             else launch_stream<2, 1, 1, MODE_DW, 2>(l, q, l.vp / 128, l.nz, st);
         }
-        const XentDwReduce w_ = {q.out, q.outb, q.scales, dw, db, (int)l.nz, (long)(l.ep * l.vp), (long)l.vp, (int)e, (long)v, 0L, (long)l.vp, accumulate};
+        const XentDwReduce s = {q.out, q.outb, q.scales, dw, db, (int)l.nz, (long)(l.ep * l.vp), (long)l.vp, (int)e, (long)v, 0L, (long)l.vp,
+                                accumulate};
         const bool slabs = (dw || db) && l.nz > 1;
-        if (dx || slabs) launch_joins(dx ? &j : nullptr, slabs ? &w_ : nullptr, st);
+        if (dx || slabs) launch_joins(dx ? &j : nullptr, slabs ? &s : nullptr, st);
         return mgx_launch_status();
     }
     const XentDxJoin join = {(float*)(ws + l.dxw), (float*)(ws + l.scales), nullptr, (float*)(ws + l.rs), dx, (int)xf, (int)l.nx,
