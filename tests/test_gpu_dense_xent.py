@@ -645,3 +645,17 @@ def test_two_captured_graphs_of_every_form(n, e, v, dtype):
             step()
             torch.cuda.synchronize()
             assert all(torch.equal(p, q) for p, q in zip(got, outs))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,e,v", [(1, 30, 400), (4, 30, 400), (16, 30, 400), (60, 30, 400), (100, 140, 33000), (200, 140, 400)])
+def test_hits_of_every_form(n, e, v, dtype):
+    x, w, b, labels, dloss = case(n, e, v, dtype, seed=95, unlabelled=0)
+    z = x.double() @ w.double() + b.double()
+    top = z.topk(2, dim=1)
+    clear = top.values[:, 0] - top.values[:, 1] > 1e-3          # no tie within the logits' accuracy
+    labels[::2] = top.indices[::2, 0].int()
+    labels[n // 2] = -1
+    got, want = run(x, w, b, labels, dloss)["hits"], reference(x, w, b, labels, dloss)["hits"]
+    assert torch.equal(got[clear], want[clear]) and int(got[n // 2]) == 0
