@@ -195,10 +195,11 @@ __global__ __launch_bounds__(256, 1) void bwgrad_kernel(mgx_conv_desc d, const b
 // dW[tap*wtap + k*wsk + n*wsn] += sum over slots of the slab element; block = 64 elements x 16 slot
 // groups (group q adds slots q, q+16, ... in order), then a fixed tree over the groups.  Elements past
 // the weights are the bias gradient (row 0 of the bias tile of chunk 0, or of every chunk when the
-// chunks split the output channels).
+// chunks split the output channels).  A slab holds a tile's 16 registers as [register][lane], or (quads) four at a time as
+// [register / 4][lane][4].
 __global__ __launch_bounds__(1024) void bwgrad_reduce_kernel(mgx_conv_desc d, const float* __restrict__ partial,
                                                              float* __restrict__ dw, float* __restrict__ db,
-                                                             int nslots, int chunks, int taps) {
+                                                             int nslots, int chunks, int taps, int quads) {
     __shared__ float red[16][64];
     const int e = threadIdx.x & 63, q = threadIdx.x >> 6;
     const long idx = (long)blockIdx.x * 64 + e;
@@ -216,6 +217,11 @@ __global__ __launch_bounds__(1024) void bwgrad_reduce_kernel(mgx_conv_desc d, co
             tile = rem >> 10;
             i = (rem >> 5) & 31;
             j = rem & 31;
+            if (quads) {                                 // elements in the order of the slab, so that reads are consecutive
+                const int lane = (rem >> 2) & 63;
+                i = (rem & 3) + 8 * ((rem >> 8) & 3) + 4 * (lane >> 5);
+                j = lane & 31;
+            }
             const int k = (d.cin > 32 ? chunk * 32 : 0) + i, n = (d.ngemm > 32 ? chunk * 32 : 0) + j;
             dst = (long)tile * d.wtap + (long)k * d.wsk + (long)n * d.wsn;
         } else {
@@ -228,7 +234,7 @@ __global__ __launch_bounds__(1024) void bwgrad_reduce_kernel(mgx_conv_desc d, co
             is_bias = true;
         }
         const int lane = j + 32 * ((i >> 2) & 1), reg = (i & 3) + 4 * (i >> 3);
-        const float* src = partial + ((long)chunk * (taps + 1) + tile) * 1024 + reg * 64 + lane;
+        const float* src = partial + ((long)chunk * (taps + 1) + tile) * 1024 + (quads ? (reg >> 2) * 256 + lane * 4 + (reg & 3) : reg * 64 + lane);
         const long stride = (long)chunks * (taps + 1) * 1024;
         for (int sp = q; sp < nslots; sp += 16) s += src[sp * stride];
     }
@@ -587,43 +593,56 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const voi
 
     if constexpr (CIN == 128) {
         // every wave holds the tiles of its own input-channel chunk: slab (slot, chunk) of the workspace
-        float* dst = partial + ((long)(slot * NCH + cch) * (TAPS + 1)) * 1024;
+        float* dst = partial + ((long)(slot * NCH + cch) * (TAPS + 1)) * 1024 + lane * 4;
 #pragma unroll
         for (int a = 0; a <= TAPS; ++a)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dst[(a * 16 + i) * 64 + lane] = acc[a][i];
+            for (int q = 0; q < 4; ++q)
+                *(f32x4*)(dst + (a * 4 + q) * 256) = (f32x4){acc[a][4 * q], acc[a][4 * q + 1], acc[a][4 * q + 2], acc[a][4 * q + 3]};
         return;
     }
-    // ---- add the four waves in fixed order: (w0 + w2) + (w1 + w3), through LDS ----
-    float* red = (float*)lds;                           // [2][TAPS+1][16][64] floats <= 80 KB
+    // ---- add the four waves in fixed order: (w0 + w2) + (w1 + w3), through LDS, four registers an access (this code runs once,
+    // so its time is that of fetching it: one register an access took 6 us of the 18 of a launch of one tile, this 4) ----
+    f32x4* const red = (f32x4*)lds + lane;              // [2][TAPS+1][4][64] pieces of 16 B <= 80 KB
     __syncthreads();
     if (wvs >= 2) {
 #pragma unroll
         for (int a = 0; a <= TAPS; ++a)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) red[(((wvs - 2) * (TAPS + 1) + a) * 16 + i) * 64 + lane] = acc[a][i];
+            for (int q = 0; q < 4; ++q)
+                red[(((wvs - 2) * (TAPS + 1) + a) * 4 + q) * 64] = (f32x4){acc[a][4 * q], acc[a][4 * q + 1], acc[a][4 * q + 2], acc[a][4 * q + 3]};
     }
     __syncthreads();
     if (wvs < 2) {
 #pragma unroll
         for (int a = 0; a <= TAPS; ++a)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[a][i] += red[((wvs * (TAPS + 1) + a) * 16 + i) * 64 + lane];
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 v = red[((wvs * (TAPS + 1) + a) * 4 + q) * 64];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[a][4 * q + i] += v[i];
+            }
     }
     __syncthreads();
     if (wvs == 1) {
 #pragma unroll
         for (int a = 0; a <= TAPS; ++a)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) red[(a * 16 + i) * 64 + lane] = acc[a][i];
+            for (int q = 0; q < 4; ++q)
+                red[(a * 4 + q) * 64] = (f32x4){acc[a][4 * q], acc[a][4 * q + 1], acc[a][4 * q + 2], acc[a][4 * q + 3]};
     }
     __syncthreads();
     if (wvs == 0) {
-        float* dst = partial + ((long)slot * (TAPS + 1)) * 1024;
+        float* const dst = partial + (long)slot * (TAPS + 1) * 1024 + lane * 4;
 #pragma unroll
         for (int a = 0; a <= TAPS; ++a)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dst[(a * 16 + i) * 64 + lane] = acc[a][i] + red[(a * 16 + i) * 64 + lane];
+            for (int q = 0; q < 4; ++q) {
+                f32x4 v = red[(a * 4 + q) * 64];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] += acc[a][4 * q + i];
+                *(f32x4*)(dst + (a * 4 + q) * 256) = v;
+            }
     }
 }
 
@@ -645,7 +664,7 @@ int launch_w(const mgx_conv_desc& d, const bf16_t* x, const bf16_t* g, float* dw
     const int nslots = WGRID / chunks;
     const long total = (long)chunks * G::TAPS * 1024 + (db ? d.ngemm : 0);
     hipLaunchKernelGGL(bwgrad_reduce_kernel, dim3((unsigned)((total + 63) / 64)), dim3(1024), 0, st, d, partial, dw, db,
-                       nslots, chunks, G::TAPS);
+                       nslots, chunks, G::TAPS, 0);
     return mgx_launch_status();
 }
 
@@ -670,7 +689,7 @@ int launch_f(const mgx_conv_desc& d, const void* x, const bf16_t* g, const float
                            ntiles, tiles_h, tiles_w, act_alpha);
     const long total = (long)G::NCH * G::TAPS * 1024 + (db ? d.ngemm : 0);
     hipLaunchKernelGGL(bwgrad_reduce_kernel, dim3((unsigned)((total + 63) / 64)), dim3(1024), 0, st, d, partial, dw, db,
-                       grid, G::NCH, G::TAPS);
+                       grid, G::NCH, G::TAPS, 1);
     return mgx_launch_status();
 }
 
