@@ -677,16 +677,19 @@ int launch_f(const mgx_conv_desc& d, const void* x, const bf16_t* g, const float
     const int tiles_h = (d.hout + G::TH - 1) / G::TH, tiles_w = (d.wout + G::TW - 1) / G::TW;
     const long ntiles = (long)d.nimg * tiles_h * tiles_w;
     if (ntiles <= 0 || ntiles >= (1L << 31)) return MGX_ERR_ARG;
-    // workgroups without a tile would only leave slabs of zeros to be added (8 x 1500: 29 -> 21 us with the reduction)
+    // workgroups without a tile would only leave slabs of zeros to be added (8 x 1500: 29 -> 21 us with the reduction); further
+    // tiles are dealt as in the bf16 form, whose sums these equal bit for bit
     const int grid = X8 && ntiles < WGRID ? (int)ntiles : WGRID;
-    const void* fn = act_alpha > 0.f ? (const void*)bbwd_kernel<KH, KW, true, CIN, X8> : (const void*)bbwd_kernel<KH, KW, false, CIN, X8>;
-    if (hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS) != hipSuccess) return MGX_ERR_LAUNCH;
-    if (act_alpha > 0.f)
+    static std::atomic<uint64_t> allowed[2];
+    if (act_alpha > 0.f) {
+        mgx_allow_dynamic_lds(bbwd_kernel<KH, KW, true, CIN, X8>, G::LDS, allowed[0]);
         hipLaunchKernelGGL((bbwd_kernel<KH, KW, true, CIN, X8>), dim3(grid), dim3(256), G::LDS, st, d, x, xe, g, w, dx, partial,
                            ntiles, tiles_h, tiles_w, act_alpha);
-    else
+    } else {
+        mgx_allow_dynamic_lds(bbwd_kernel<KH, KW, false, CIN, X8>, G::LDS, allowed[1]);
         hipLaunchKernelGGL((bbwd_kernel<KH, KW, false, CIN, X8>), dim3(grid), dim3(256), G::LDS, st, d, x, xe, g, w, dx, partial,
                            ntiles, tiles_h, tiles_w, act_alpha);
+    }
     const long total = (long)G::NCH * G::TAPS * 1024 + (db ? d.ngemm : 0);
     hipLaunchKernelGGL(bwgrad_reduce_kernel, dim3((unsigned)((total + 63) / 64)), dim3(1024), 0, st, d, partial, dw, db,
                        grid, G::NCH, G::TAPS, 1);

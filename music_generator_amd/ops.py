@@ -1003,10 +1003,19 @@ def cast_to_f32(x: torch.Tensor) -> torch.Tensor:
 class Tape8:
     """A tensor as the 8-bit tape keeps it: `codes` (uint8, whole blocks of 32 values), `exps` (uint8, one exponent byte
     a block), and the shape and type it was packed from.  The values it stands for are exact in bfloat16."""
-    __slots__ = ("shape", "dtype", "codes", "exps")
+    __slots__ = ("shape", "dtype", "_codes", "_exps", "_both")
 
-    def __init__(self, shape, dtype, codes, exps):
-        self.shape, self.dtype, self.codes, self.exps = torch.Size(shape), dtype, codes, exps
+    def __init__(self, shape, dtype, codes=None, exps=None, both=None):
+        """`both` instead of codes and exps: one uint8 tensor with the codes and the exponent bytes behind them."""
+        self.shape, self.dtype, self._codes, self._exps, self._both = torch.Size(shape), dtype, codes, exps, both
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._codes if self._both is None else self._both[:self._both.numel() // 33 * 32]
+
+    @property
+    def exps(self) -> torch.Tensor:
+        return self._exps if self._both is None else self._both[self._both.numel() // 33 * 32:]
 
     def numel(self) -> int:
         return self.shape.numel()
@@ -1018,15 +1027,15 @@ class Tape8:
         """The same bytes as a tensor of another shape (same number of values in the same order)."""
         if torch.Size(shape).numel() != self.numel():
             raise MgxError("Tape8.view: another number of values")
-        return self if tuple(shape) == tuple(self.shape) else Tape8(shape, self.dtype, self.codes, self.exps)
+        return self if tuple(shape) == tuple(self.shape) else Tape8(shape, self.dtype, self._codes, self._exps, self._both)
 
     def nbytes(self) -> int:
-        return self.codes.numel() + self.exps.numel()
+        return self._both.numel() if self._both is not None else self._codes.numel() + self._exps.numel()
 
 
 def _on_current(*ts):
     """Kernels run on the current device's stream: a tensor of another device would be read through a foreign address."""
-    dev = torch.cuda.current_device()
+    dev = torch._C._cuda_getDevice()
     for t in ts:
         if t is not None and t.get_device() != dev:
             raise MgxError("operand on %s, the current device is cuda:%d" % (t.device, dev))
@@ -1039,9 +1048,16 @@ def _p_act(t):
 def _p8(t: Tape8):
     n = t.numel()
     blocks = (n + 31) // 32
+    b = t._both
+    if b is not None:
+        if b.dtype != torch.uint8 or not b.is_cuda or not b.is_contiguous() or b.numel() != 33 * blocks:
+            raise MgxError("tape8: codes / exponent bytes do not match a tensor of %d values" % n)
+        _on_current(b)
+        return b.data_ptr(), b.data_ptr() + 32 * blocks
     for b, size in ((t.codes, 32 * blocks), (t.exps, blocks)):
         if b.dtype != torch.uint8 or not b.is_cuda or not b.is_contiguous() or b.numel() != size:
             raise MgxError("tape8: codes / exponent bytes do not match a tensor of %d values" % n)
+    _on_current(t.codes, t.exps)
     return t.codes.data_ptr(), t.exps.data_ptr()
 
 
@@ -1051,11 +1067,11 @@ def tape8_pack(x: torch.Tensor) -> Tape8:
     _on_current(x)
     n = x.numel()
     blocks = (n + 31) // 32
-    t = Tape8(x.shape, x.dtype, torch.empty((32 * blocks,), dtype=torch.uint8, device=x.device),
-              torch.empty((blocks,), dtype=torch.uint8, device=x.device))
+    t = Tape8(x.shape, x.dtype, both=torch.empty((33 * blocks,), dtype=torch.uint8, device=x.device))
+    pc = t._both.data_ptr()
     e0 = PROFILER.start() if PROFILER is not None else None
-    check(_lib().mgx_tape8_pack(px, int(x.dtype == torch.float32), t.codes.data_ptr(), t.exps.data_ptr(), n,
-                                K.stream_ptr()), "mgx_tape8_pack")
+    check(_lib().mgx_tape8_pack(px, int(x.dtype == torch.float32), pc, pc + 32 * blocks, n, K.stream_ptr()),
+          "mgx_tape8_pack")
     if e0 is not None:
         PROFILER.stop("tape8_pack", 0.0, e0, n * x.element_size() + t.nbytes())
     return t
@@ -1067,8 +1083,7 @@ def tape8_unpack(t: Tape8, dtype=None) -> torch.Tensor:
     if dtype not in (torch.float32, torch.bfloat16):
         raise MgxError("tape8_unpack: float32 or bfloat16")
     pc, pe = _p8(t)
-    _on_current(t.codes, t.exps)
-    y = torch.empty(t.shape, dtype=dtype, device=t.codes.device)
+    y = torch.empty(t.shape, dtype=dtype, device=(t._codes if t._both is None else t._both).device)
     e0 = PROFILER.start() if PROFILER is not None else None
     check(_lib().mgx_tape8_unpack(pc, pe, y.data_ptr(), int(dtype == torch.float32), t.numel(), K.stream_ptr()),
           "mgx_tape8_unpack")
@@ -1084,7 +1099,7 @@ def mul_dact_tape8(a: torch.Tensor, t: Tape8, act_alpha) -> torch.Tensor:
     if not act_alpha > 0.0:
         raise MgxError("mul_dact_tape8: act_alpha must be positive")
     pa, (pc, pe) = _p_act(a), _p8(t)
-    _on_current(a, t.codes, t.exps)
+    _on_current(a)
     out = torch.empty(t.shape, dtype=torch.bfloat16, device=a.device)
     e0 = PROFILER.start() if PROFILER is not None else None
     check(_lib().mgx_mul_dact_tape8(pa, int(a.dtype == torch.float32), pc, pe, float(act_alpha), out.data_ptr(), a.numel(),
@@ -1102,7 +1117,7 @@ def conv_bwd_tape8(d: ConvDesc, t: Tape8, g, w, dw, dbias, dx, act_alpha=0.0):
     if dbias is not None and dbias.numel() != d.nbias:
         raise MgxError("conv_bwd_tape8: bias gradient size mismatch")
     pc, pe = _p8(t)
-    _on_current(t.codes, t.exps, g, w, dw, dbias, dx)
+    _on_current(g, w, dw, dbias, dx)
     lib = _lib()
     nbytes = lib.mgx_conv_bwd_bf16_workspace(C.byref(d))
     if nbytes <= 0:
