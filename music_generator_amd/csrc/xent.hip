@@ -472,7 +472,7 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
                 for (int q = 0; q < 4; ++q) {
                     const f32x4 bv = *(const f32x4*)(g.bias + mw + i * 32 + 8 * q + 4 * h);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[i][j][4 * q + k] = (acc[i][j][4 * q + k] + bv[k]) * unit;
+                    for (int k = 0; k < 4; ++k) acc[i][j][4 * q + k] += bv[k];
                 }
             const long rel = lab - g.class0 - mw;           // the label's place among the wave's 64 classes
             if constexpr (EPI == EPI_FWD) {
@@ -485,15 +485,15 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) s += __builtin_amdgcn_exp2f(acc[i][j][k] - m);
+                    for (int k = 0; k < 16; ++k) s += __builtin_amdgcn_exp2f((acc[i][j][k] - m) * unit);     // the difference first, as in the streamed form
                 s += __shfl_xor(s, 32, 64);
-                if (h == 0) g.part[(mw / 64) * g.np + row] = make_float2(m, s);
+                if (h == 0) g.part[(mw / 64) * g.np + row] = make_float2(m * unit, s);
                 if (lab >= 0 && rel >= 0 && rel < 64) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int k = 0; k < 16; ++k)
-                            if (i * 32 + (k & 3) + 8 * (k >> 2) + 4 * h == (int)rel) g.zlab[row] = acc[i][j][k];
+                            if (i * 32 + (k & 3) + 8 * (k >> 2) + 4 * h == (int)rel) g.zlab[row] = acc[i][j][k] * unit;
                 }
             } else {
                 const float lse = g.row[row].x, dl = g.row[row].y;
@@ -501,7 +501,7 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
                 for (int i = 0; i < 2; ++i) {
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        float p = __builtin_amdgcn_exp2f(acc[i][j][k] - lse);
+                        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][k], unit, -lse));
                         if (i * 32 + (k & 3) + 8 * (k >> 2) + 4 * h == rel) p -= 1.f;           // no label: rel < 0
                         acc[i][j][k] = p * dl;
                     }
@@ -799,9 +799,9 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                 ssum[b] *= __builtin_amdgcn_exp2f((m[b] - mm) * unit);
                 m[b] = mm;
             } else if constexpr (MODE == MODE_FWD) {
-                const float off = -m[b] * unit;
+                // the difference first: beside a large mask the rounding of m unit alone would be any number
 #pragma unroll
-                for (int k = 2 * j; k < 2 * j + 2; ++k) ssum[b] += __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k], unit, off));
+                for (int k = 2 * j; k < 2 * j + 2; ++k) ssum[b] += __builtin_amdgcn_exp2f((cur[b][k] - m[b]) * unit);
             } else if constexpr (MODE == MODE_DX) {
                 put(P_, __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j], unit, rinfo[b])),
                     __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j + 1], unit, rinfo[b])));
