@@ -12,9 +12,9 @@
 // operand's largest magnitude below 2^14: 22 significant bits, and 2^-25 of 2^14 absolute where a value is small.  The
 // product keeps hi hi + hi lo + lo hi (the dropped lo lo is 2^-24 of it).  A bf16 operand is exact in one plane.  This is
 // three (two) of 2.5 PFLOP/s instead of one of the 157 TFLOP/s of the float32 matrix instructions.
-// Logits, maxima, sums, lse and all gradient sums are float32.  An accumulator starts at the class's bias times both scales
-// (exact, they are powers of two), and log2(e) is in the factor that takes the scales out again: an exponential is one fma
-// and one v_exp_f32.
+// Logits, maxima, sums, lse and all gradient sums are float32.  Biases are in units of log 2 and log2(e) is in the factor that
+// takes the scales out: an exponential is one fma, one difference and one v_exp_f32.  (Accumulators that start at the bias
+// times both scales save the difference, but that product leaves float32 where the operands are small or the bias is a mask.)
 //
 // Four forms.  What each is bound by, and forward + backward times (us; n x e x v):
 //   few rows (up to 4, up to 16 of a small W): launches and HBM (W read twice, dW written), float32 on the vector ALU.
@@ -169,6 +169,16 @@ __device__ __forceinline__ float scale_of(unsigned maxbits) {
     return __builtin_bit_cast(float, (unsigned)(e + 127) << 23);
 }
 
+// A bias in units of log 2; a finite one stays finite.
+__device__ __forceinline__ float log2_units(float b) {
+    const float q = b * kLog2e;
+    return __builtin_isfinite(b) ? fminf(fmaxf(q, kLowest), -kLowest) : q;
+}
+
+// What takes the scales out of a product and brings it into units of log 2: at most the largest float, so that a product of zero
+// stays one; 0 where both operands are too small for any logit to differ from its bias.
+__device__ __forceinline__ float logit_unit(const float* scales) { return fminf(kLog2e / scales[0] / scales[1], -kLowest); }
+
 // {s_w, s_x, largest |dloss| rounded up to a power of two} into scales[0..2]; part has `parts` partials per tensor.
 __device__ __forceinline__ float scale_from_parts(const unsigned* __restrict__ part, int which, int parts) {
     unsigned m = 0u, o[kMaxParts / 64];
@@ -307,8 +317,7 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
             p.scales[2] = sd;
         }
         for (long i = first * 256 + tid; i < p.vp; i += nb * 256) {
-            const float b = i < p.v ? (p.b ? p.b[i] : 0.f) : -__builtin_inff(), q = b * sw * sx;
-            p.bias[i] = b >= kLowest ? fmaxf(q, kLowest) : q;       // a finite mask stays finite
+            p.bias[i] = log2_units(i < p.v ? (p.b ? p.b[i] : 0.f) : -__builtin_inff());
         }
         for (long i = first * 256 + tid; i < p.np; i += nb * 256) {
             int lab = i < p.n ? p.labels[i] : -1;
@@ -461,7 +470,7 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
     const long mw = m0 + wm * 64, nw = n0 + wn * 64;
     if constexpr (EPI == EPI_FWD || EPI == EPI_DZ) {
         // A: classes, B: rows of x
-        const float unit = kLog2e / g.scales[0] / g.scales[1];
+        const float unit = logit_unit(g.scales);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const long row = nw + j * 32 + r;
@@ -472,7 +481,7 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
                 for (int q = 0; q < 4; ++q) {
                     const f32x4 bv = *(const f32x4*)(g.bias + mw + i * 32 + 8 * q + 4 * h);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[i][j][4 * q + k] += bv[k];
+                    for (int k = 0; k < 4; ++k) acc[i][j][4 * q + k] = __builtin_fmaf(acc[i][j][4 * q + k], unit, bv[k]);
                 }
             const long rel = lab - g.class0 - mw;           // the label's place among the wave's 64 classes
             if constexpr (EPI == EPI_FWD) {
@@ -485,15 +494,15 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) s += __builtin_amdgcn_exp2f((acc[i][j][k] - m) * unit);     // the difference first, as in the streamed form
+                    for (int k = 0; k < 16; ++k) s += __builtin_amdgcn_exp2f(acc[i][j][k] - m);
                 s += __shfl_xor(s, 32, 64);
-                if (h == 0) g.part[(mw / 64) * g.np + row] = make_float2(m * unit, s);
+                if (h == 0) g.part[(mw / 64) * g.np + row] = make_float2(m, s);
                 if (lab >= 0 && rel >= 0 && rel < 64) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int k = 0; k < 16; ++k)
-                            if (i * 32 + (k & 3) + 8 * (k >> 2) + 4 * h == (int)rel) g.zlab[row] = acc[i][j][k] * unit;
+                            if (i * 32 + (k & 3) + 8 * (k >> 2) + 4 * h == (int)rel) g.zlab[row] = acc[i][j][k];
                 }
             } else {
                 const float lse = g.row[row].x, dl = g.row[row].y;
@@ -501,7 +510,7 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
                 for (int i = 0; i < 2; ++i) {
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][k], unit, -lse));
+                        float p = __builtin_amdgcn_exp2f(acc[i][j][k] - lse);
                         if (i * 32 + (k & 3) + 8 * (k >> 2) + 4 * h == rel) p -= 1.f;           // no label: rel < 0
                         acc[i][j][k] = p * dl;
                     }
@@ -535,7 +544,7 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
     } else {
         // A: features, B: classes; the gradients, or slab z of the piece
         if (g.o.direct) {
-            const float fb = g.scales[2] / kDz, fw = fb / g.scales[1];
+            const float fb = g.scales[2] / kDz, fx = 1.f / g.scales[1];      // one after the other: their product may be too small
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const long c = nw + j * 32 + r;
@@ -548,7 +557,7 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
                             const long f = mw + i * 32 + acc_row(k, lane);
                             if (f < g.o.e) {
                                 float* d = g.o.dw + f * g.o.v + c;
-                                const float q = acc[i][j][k] * fw;
+                                const float q = acc[i][j][k] * fb * fx;
                                 *d = g.o.accumulate ? *d + q : q;
                             }
                         }
@@ -575,7 +584,7 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
 // Up to EP features (EP = 64 or 128) the two products around the exponential run in one kernel and no dz is stored.  One operand is
 // resident: a wave keeps 32 RB of its items (rows of x, or classes) as B fragments in registers.  The other is streamed: tiles of
 // 32 of its items in LDS, a ring of four filled by LDS-DMA and shared by the four waves.  Per streamed tile:
-//     S (32 streamed x 32 RB resident) = bias + sum over plane products                  first product
+//     S (32 streamed x 32 RB resident) = sum over plane products                         first product; logits: S unit + bias
 //     forward: the lane's running maximum and sum over the streamed classes
 //     backward: P = exp(S - lse) (times dloss where rows are streamed) - label, as fp16 planes: the accumulator registers
 //               8 t .. 8 t + 7 of a lane are the streamed items 16 t + 4 h + {0..3} and 16 t + 8 + 4 h + {0..3}, which is the
@@ -663,7 +672,7 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
                 fb[pl][b][ks] = *(const u32x4*)(g.r[pl] + ((long)item0 + 32 * b + r) * EP + 16 * ks + 8 * h);
-    const float unit = kLog2e / g.scales[0] / g.scales[1];
+    const float unit = logit_unit(g.scales);
     float rinfo[RB];                                // DX: -(lse - 14); DW: bias
     float plab[RB];                                 // DX, NR = 1: 2^14 (p - 1) of the label
     int rlab[RB];
@@ -683,7 +692,7 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                 for (int k = 0; k < 8; ++k) z = __builtin_fmaf((float)xv[k], (float)wl[k], __builtin_fmaf((float)xv[k], (float)wh[k], z));
             }
             z += __shfl_xor(z, 32, 64);
-            plab[b] = (__builtin_amdgcn_exp2f(__builtin_fmaf(z + g.bias[c], unit, rinfo[b] - 14.f)) - 1.f) * kDz;
+            plab[b] = (__builtin_amdgcn_exp2f(__builtin_fmaf(z, unit, g.bias[c]) + (rinfo[b] - 14.f)) - 1.f) * kDz;
         }
     }
     // LDS offsets of the lane: the first fragment of its row, and the first transposed reads.  A row starts at a multiple of
@@ -740,7 +749,9 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
         asm volatile("" : "+v"(ao), "+v"(to[0]), "+v"(to[1]));      // keeps the 16 addresses derived from them out of registers
         const int s0 = i * ST;
         u32x4 fr[3];
-        f32x4 ri2[2];
+        f32x4 ri2[2];                                // DW
+        f32x2 bi2[2];                                // DX: biases of the next pairs
+        f32x4 bv[4];                                 // FWD: biases of the tile
         float tsum[RB];                              // DW: the tile's sum of P, added to the running one once a tile
 #pragma unroll
         for (int b = 0; b < RB; ++b) tsum[b] = 0.f;
@@ -790,25 +801,32 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
         };
         // (lse, dloss) of the two streamed rows of pair j
         auto row2 = [&](int j) { return *(const f32x4*)(te + (8 * (j >> 1) + 4 * h + 2 * (j & 1)) * 8); };
+        // biases of the two streamed classes of pair j
+        auto bias2 = [&](int j) { return *(const f32x2*)(te + (8 * (j >> 1) + 4 * h + 2 * (j & 1)) * 4); };
         auto piece = [&](auto P_) {
             constexpr int p = decltype(P_)::value, b = p / PB, j = p % PB - (PB - 8);
             if constexpr (MODE == MODE_FWD && j < 0) {
                 float mm = m[b];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) mm = fmaxf(mm, cur[b][k]);
-                ssum[b] *= __builtin_amdgcn_exp2f((m[b] - mm) * unit);
+                for (int k = 0; k < 16; ++k) {
+                    cur[b][k] = __builtin_fmaf(cur[b][k], unit, bv[k >> 2][k & 3]);
+                    mm = fmaxf(mm, cur[b][k]);
+                }
+                ssum[b] *= __builtin_amdgcn_exp2f(m[b] - mm);
                 m[b] = mm;
             } else if constexpr (MODE == MODE_FWD) {
-                // the difference first: beside a large mask the rounding of m unit alone would be any number
 #pragma unroll
-                for (int k = 2 * j; k < 2 * j + 2; ++k) ssum[b] += __builtin_amdgcn_exp2f((cur[b][k] - m[b]) * unit);
+                for (int k = 2 * j; k < 2 * j + 2; ++k) ssum[b] += __builtin_amdgcn_exp2f(cur[b][k] - m[b]);
             } else if constexpr (MODE == MODE_DX) {
-                put(P_, __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j], unit, rinfo[b])),
-                    __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j + 1], unit, rinfo[b])));
+                const f32x2 q = bi2[j & 1];
+                const float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j], unit, q[0]) + rinfo[b]);
+                const float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j + 1], unit, q[1]) + rinfo[b]);
+                if constexpr (b < RB - 1 || j + 2 < 8) bi2[j & 1] = bias2((j + 2) & 7);
+                put(P_, v0, v1);
             } else {
                 const f32x4 q = ri2[j & 1];
-                const float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j], unit, -q[0])) * q[1];
-                const float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j + 1], unit, -q[2])) * q[3];
+                const float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j], unit, rinfo[b]) - q[0]) * q[1];
+                const float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j + 1], unit, rinfo[b]) - q[2]) * q[3];
                 tsum[b] += v0 + v1;
                 if constexpr (b == RB - 1 && j + 2 < 8) ri2[j & 1] = row2(j + 2);
                 put(P_, v0, v1);
@@ -819,12 +837,13 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
             constexpr int p = decltype(P_)::value, b = p / 8, j = p % 8, k = 2 * j, c0 = (k & 3) + 8 * (k >> 2);
             if constexpr (MODE == MODE_FWD) {
                 const int rel = rlab[b] - s0 - 4 * h;
-                if (rel == c0) g.zlab[item0 + 32 * b + r] = cur[b][k] * unit;
-                if (rel == c0 + 1) g.zlab[item0 + 32 * b + r] = cur[b][k + 1] * unit;
+                if (rel == c0) g.zlab[item0 + 32 * b + r] = cur[b][k];
+                if (rel == c0 + 1) g.zlab[item0 + 32 * b + r] = cur[b][k + 1];
             } else if constexpr (MODE == MODE_DX) {
                 const int rel = rlab[b] - s0 - 4 * h;
-                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k], unit, rinfo[b]));
-                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k + 1], unit, rinfo[b]));
+                const f32x2 q = bias2(j);
+                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k], unit, q[0]) + rinfo[b]);
+                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k + 1], unit, q[1]) + rinfo[b]);
                 put(P_, rel == c0 ? (NR == 1 ? plab[b] : e0 - kDz) : e0, rel == c0 + 1 ? (NR == 1 ? plab[b] : e1 - kDz) : e1);
             } else {
                 const f32x4 q = row2(j);
@@ -832,25 +851,24 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                 const float d0 = (int)lb[0] - item0 - 32 * b == r ? q[1] : 0.f, d1 = (int)lb[1] - item0 - 32 * b == r ? q[3] : 0.f;
                 tsum[b] -= d0 + d1;
                 // (p - 1) dloss, as one fma each: p dloss would have lost the digits of a p next to 1
-                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k], unit, -q[0]));
-                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k + 1], unit, -q[2]));
+                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k], unit, rinfo[b]) - q[0]);
+                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k + 1], unit, rinfo[b]) - q[2]);
                 put(P_, __builtin_fmaf(e0, q[1], -d0), __builtin_fmaf(e1, q[3], -d1));
             }
         };
-        if constexpr (DO_S) {                        // S starts at the biases
-            if constexpr (MODE == MODE_DW) {         // or the compiler keeps 16 copies of the lane's
+        if constexpr (DO_S) {
 #pragma unroll
-                for (int b = 0; b < RB; ++b) asm volatile("" : "+v"(rinfo[b]));
-            }
+            for (int b = 0; b < RB; ++b)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                f32x4 bv;
-                if constexpr (MODE != MODE_DW) bv = *(const f32x4*)(ts + NS * SPLANE + (8 * q + 4 * h) * 4);
+                for (int k = 0; k < 16; ++k) nxt[b][k] = 0.f;
+        }
+        if constexpr (DO_E && MODE == MODE_FWD) {
 #pragma unroll
-                for (int b = 0; b < RB; ++b)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) nxt[b][4 * q + k] = MODE == MODE_DW ? rinfo[b] : bv[k];
-            }
+            for (int q = 0; q < 4; ++q) bv[q] = *(const f32x4*)(te + (8 * q + 4 * h) * 4);
+        }
+        if constexpr (DO_E && MODE == MODE_DX) {
+            bi2[0] = bias2(0);
+            bi2[1] = bias2(1);
         }
         if constexpr (DO_E && MODE == MODE_DW) {
             ri2[0] = row2(0);
@@ -909,8 +927,8 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
         if constexpr (MODE == MODE_FWD) {
             const float mo = __shfl_xor(m[b], 32, 64), so = __shfl_xor(ssum[b], 32, 64);
             const float mm = fmaxf(m[b], mo);
-            const float s = ssum[b] * __builtin_amdgcn_exp2f((m[b] - mm) * unit) + so * __builtin_amdgcn_exp2f((mo - mm) * unit);
-            if (h == 0) g.part[(long)blockIdx.y * g.ld + it] = make_float2(mm * unit, s);
+            const float s = ssum[b] * __builtin_amdgcn_exp2f(m[b] - mm) + so * __builtin_amdgcn_exp2f(mo - mm);
+            if (h == 0) g.part[(long)blockIdx.y * g.ld + it] = make_float2(mm, s);
         } else if constexpr (MODE == MODE_DX) {
             float* o = g.out + ((long)blockIdx.y * g.ld + it) * EP;
 #pragma unroll
@@ -923,7 +941,7 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
             const float so = __shfl_xor(ssum[b], 32, 64);
             if (g.o.direct) {
                 if (it >= g.o.cnt) continue;
-                const float fb_ = g.scales[2] / kDz, fw = fb_ / g.scales[1];
+                const float fb_ = g.scales[2] / kDz, fx = 1.f / g.scales[1];
                 if (g.o.dw) {
 #pragma unroll
                     for (int eb = 0; eb < EB; ++eb)
@@ -932,7 +950,7 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                             const int f = 32 * eb + acc_row(i, lane);
                             if (f < g.o.e) {
                                 float* d = g.o.dw + f * g.o.v + it;
-                                const float q = dacc[eb][b][i] * fw;
+                                const float q = dacc[eb][b][i] * fb_ * fx;
                                 *d = g.o.accumulate ? *d + q : q;
                             }
                         }
@@ -984,7 +1002,7 @@ __device__ __forceinline__ void xent_dx_join(const XentDxJoin& j, long block, lo
     __shared__ float red[G][G == 1 ? 1 : 64];
     const auto [parts, scales, rowinfo, rs, dx, dx_f32, np, part, n, e, ep] = j;
     // streamed: the parts hold 2^14 dz / dloss, the rows 2^14 dloss / scales[2]; wide: 2^14 dz / rs
-    const float f = !scales ? 1.f : (rs ? 1.f : scales[2] / kDz) / kDz / scales[0];
+    const float f = !scales ? 1.f : (rs ? 1.f : scales[2] / kDz) / kDz, fw = scales ? 1.f / scales[0] : 1.f;
     const int lane = threadIdx.x % W, q = threadIdx.x / W;
     const int per = (np + G - 1) / G, p0 = q * per, cnt = np - p0 < per ? np - p0 : per;
     for (long i = block * W + lane; i - lane < n * ep; i += blocks * W) {
@@ -999,7 +1017,7 @@ __device__ __forceinline__ void xent_dx_join(const XentDxJoin& j, long block, lo
         const long row = i / ep;
         const int c = (int)(i - row * ep);
         if (q == 0 && row < n && c < e) {
-            if (scales) s *= f * (rs ? rs[row] : rowinfo[row].y);
+            if (scales) s = s * fw * (f * (rs ? rs[row] : rowinfo[row].y));
             if (dx_f32) ((float*)dx)[row * e + c] = s;
             else ((bf16_t*)dx)[row * e + c] = (bf16_t)s;
         }

@@ -28,3 +28,27 @@ def test_finite_masks(mask, n, e, v, dtype):
     got = run(x, w, b, labels, dloss)
     check(got, want, dtype, float((x.double() @ w.double()).abs().max()))
     assert bool((got["dw"][:, b == mask] == 0).all()) and bool((got["db"][b == mask] == 0).all())
+
+
+def gradients_close(got, want, unit, dtype):
+    """dw, db and dx in the 2-norm as in check(), with nothing absolute: the operands may be of any size."""
+    for k in ("dw", "db", "dx"):
+        norm = float(want[k].norm())
+        tol = 4 * unit + (2.0 ** -8 + 2.0 ** -10 if k == "dx" and dtype == torch.bfloat16 else 0.0)
+        off = float((got[k].double() - want[k]).norm())
+        assert off <= tol * norm + unit * want["slack"][k], (k, off / max(norm, 1e-300), tol)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,e,v", FORMS)
+@pytest.mark.parametrize("scale_x,scale_w", [(1e-16, 1e-15), (1e-30, 1e-2), (1e-2, 1e-30), (1e-25, 1e3), (1e-32, 1e-32)])
+def test_small_operands_beside_a_bias(scale_x, scale_w, n, e, v, dtype):
+    """max |x| max |W| far below the bias: the logits are the biases, the gradients as exact as at any other size."""
+    x, w, b, labels, dloss = case(n, e, v, torch.float32, seed=110 + e)
+    args = ((x * scale_x).to(dtype), w * scale_w, b, labels, dloss * n)
+    want, got = reference(*args), run(*args)
+    unit = 2.0 ** -23 * (8 + 2 * 2.0)          # logits: the biases, up to 1.5
+    for k in ("loss", "lse"):
+        assert float((got[k].double() - want[k]).abs().max()) <= unit + 2.0 ** -23 * float(want[k].abs().max())
+    gradients_close(got, want, unit, dtype)
