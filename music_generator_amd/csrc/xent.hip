@@ -175,6 +175,13 @@ __device__ __forceinline__ float log2_units(float b) {
     return __builtin_isfinite(b) ? fminf(fmaxf(q, kLowest), -kLowest) : q;
 }
 
+// loss of a row from its maximum, log of the sum and its label's logit, all in units of log 2, and the label's bias.  (m - z) first:
+// the loss of a row whose label has nearly all the probability is far below an ulp of lse.  Units of log 2 end at a logit
+// of -2.36e38: a bias below that is the label's logit.
+__device__ __forceinline__ float row_loss(float m, float ls, float z, float bias) {
+    return bias < kLowest * kLn2 ? (m + ls) * kLn2 - bias : ((m - z) + ls) * kLn2;
+}
+
 // What takes the scales out of a product and brings it into units of log 2: at most the largest float, so that a product of zero
 // stays one; 0 where both operands are too small for any logit to differ from its bias.
 __device__ __forceinline__ float logit_unit(const float* scales) { return fminf(kLog2e / scales[0] / scales[1], -kLowest); }
@@ -1031,7 +1038,7 @@ __global__ __launch_bounds__(G == 1 ? 256 : 1024) void xent_dx_join_kernel(XentD
 
 // loss and lse of 32 rows per workgroup from the partial (maximum, sum) of the parts or of every 64 classes
 __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict__ part, const float* __restrict__ zlab,
-                                                        const int* __restrict__ lab, float* __restrict__ loss,
+                                                        const float* __restrict__ b, const int* __restrict__ lab, float* __restrict__ loss,
                                                         float* __restrict__ lse, int* __restrict__ hits, long n, long np,
                                                         long slices) {
     __shared__ float2 red[8][32];
@@ -1059,9 +1066,8 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
             m = mm;
         }
         const bool ok = lab[row] >= 0;
-        // (m - z) first: the loss of a row whose label has nearly all the probability is far below an ulp of lse
         const float ls = __builtin_amdgcn_logf(s);
-        loss[row] = ok ? ((m - zlab[row]) + ls) * kLn2 : 0.f;
+        loss[row] = ok ? row_loss(m, ls, zlab[row], b ? b[lab[row]] : 0.f) : 0.f;
         lse[row] = ok ? (m + ls) * kLn2 : 0.f;
         if (hits) hits[row] = ok && zlab[row] >= m ? 1 : 0;
     }
@@ -1215,7 +1221,7 @@ __global__ __launch_bounds__(64) void xent_rows_join_kernel(XentRows g, float* _
         const int lab = g.labels[i];
         const bool ok = lab >= 0 && lab < g.v;
         const float z = ok ? g.zlab[i] : 0.f, ls = __builtin_amdgcn_logf(s);
-        loss[i] = ok ? ((m - z) + ls) * kLn2 : 0.f;
+        loss[i] = ok ? row_loss(m, ls, z, g.b ? g.b[lab] : 0.f) : 0.f;
         lse[i] = ok ? (m + ls) * kLn2 : 0.f;
         if (hits) hits[i] = ok && z >= m ? 1 : 0;
     }
@@ -1636,7 +1642,7 @@ __global__ __launch_bounds__(256) void xent_short_join_kernel(XentShort g, float
         for (int k = 1; k < 4; ++k) join(red[k].x, red[k].y);
         const int lab = g.lab[row];
         const float z = lab >= 0 ? g.zlab[row] : 0.f, ls = __builtin_amdgcn_logf(s);
-        loss[row] = lab >= 0 ? ((m - z) + ls) * kLn2 : 0.f;
+        loss[row] = lab >= 0 ? row_loss(m, ls, z, g.b ? g.b[lab] : 0.f) : 0.f;
         lse[row] = lab >= 0 ? (m + ls) * kLn2 : 0.f;
         if (hits) hits[row] = lab >= 0 && z >= m ? 1 : 0;
     }
@@ -2168,7 +2174,7 @@ extern "C" int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, c
     } else {
         launch_gemm<2, 1, false, false, EPI_FWD, 4>(g, l.vp, l.np, 1, st);
     }
-    hipLaunchKernelGGL(xent_join_kernel, dim3((unsigned)(l.np / 32)), dim3(256), 0, st, g.part, g.zlab, g.lab, loss, lse, hits,
+    hipLaunchKernelGGL(xent_join_kernel, dim3((unsigned)(l.np / 32)), dim3(256), 0, st, g.part, g.zlab, b, g.lab, loss, lse, hits,
                        (long)n, (long)l.np, (long)l.nf);
     return mgx_launch_status();
 }

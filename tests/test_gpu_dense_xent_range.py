@@ -52,3 +52,31 @@ def test_small_operands_beside_a_bias(scale_x, scale_w, n, e, v, dtype):
     for k in ("loss", "lse"):
         assert float((got[k].double() - want[k]).abs().max()) <= unit + 2.0 ** -23 * float(want[k].abs().max())
     gradients_close(got, want, unit, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,e,v", FORMS)
+@pytest.mark.parametrize("mask", [-1e25, -1e32, -3e38, LOWEST, float("-inf")])
+def test_masked_labels(mask, n, e, v, dtype):
+    """A row whose label is masked has the loss of that bias, and p - 1 = -1 at it; a mask of the lowest float or -inf leaves
+    the class's column of W out of dx."""
+    x, w, b, labels, dloss = case(n, e, v, dtype, seed=120 + e, unlabelled=0)
+    b[7] = mask
+    labels[labels == 7] = 8
+    hidden = torch.arange(n) % 3 == 1
+    labels[hidden] = 7
+    w_used = w.clone()
+    if mask <= LOWEST:
+        w_used[:, 7] = 0.0
+    want, got = reference(x, w_used, b, labels, dloss), run(x, w, b, labels, dloss)
+    if mask == float("-inf"):
+        assert bool(torch.isposinf(got["loss"][hidden]).all())
+    else:
+        # the bias into units of log 2 and back, the difference from lse: four roundings at most
+        assert bool(((got["loss"].double() - want["loss"]).abs()[hidden] <= 2.0 ** -22 * want["loss"][hidden]).all()), float(got["loss"][1])
+    unit = 2.0 ** -23 * (8 + 2 * float((x.double() @ w.double()).abs().max()))
+    assert float((got["loss"].double() - want["loss"])[~hidden].abs().max()) <= unit + 2.0 ** -23 * float(want["loss"][~hidden].max())
+    assert float((got["lse"].double() - want["lse"]).abs().max()) <= unit + 2.0 ** -23 * float(want["lse"].abs().max())
+    gradients_close(got, want, unit, dtype)
+    assert bool((got["hits"][hidden] == 0).all())
