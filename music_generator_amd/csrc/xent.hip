@@ -186,6 +186,10 @@ __device__ __forceinline__ float row_loss(float m, float ls, float z, float bias
 // stays one; 0 where both operands are too small for any logit to differ from its bias.
 __device__ __forceinline__ float logit_unit(const float* scales) { return fminf(kLog2e / scales[0] / scales[1], -kLowest); }
 
+// The power of two above a magnitude, 2^-105 at least: the one of a row of dloss is never above that of the largest, and reciprocals
+// and ratios stay normal.
+__device__ __forceinline__ float row_scale(float d) { return 16384.f / scale_of(__builtin_bit_cast(unsigned, fmaxf(fabsf(d), 0x1p-106f))); }
+
 // {s_w, s_x, largest |dloss| rounded up to a power of two} into scales[0..2]; part has `parts` partials per tensor.
 __device__ __forceinline__ float scale_from_parts(const unsigned* __restrict__ part, int which, int parts) {
     unsigned m = 0u, o[kMaxParts / 64];
@@ -201,13 +205,8 @@ __device__ __forceinline__ float scale_from_parts(const unsigned* __restrict__ p
         const unsigned q = (unsigned)__shfl_xor((int)m, off, 64);
         m = m > q ? m : q;
     }
-    if (which == 2) return 16384.f / scale_of(m);
+    if (which == 2) return row_scale(__builtin_bit_cast(float, m));
     return scale_of(m);
-}
-
-// The power of two above a magnitude (2^-100 at least, so that reciprocals and ratios stay normal).
-__device__ __forceinline__ float row_scale(float d) {
-    return 16384.f / scale_of(__builtin_bit_cast(unsigned, fmaxf(fabsf(d), 7.9e-31f)));
 }
 
 // ---------------------------------------------------------------- planes

@@ -80,3 +80,13 @@ def test_masked_labels(mask, n, e, v, dtype):
     assert float((got["lse"].double() - want["lse"]).abs().max()) <= unit + 2.0 ** -23 * float(want["lse"].abs().max())
     gradients_close(got, want, unit, dtype)
     assert bool((got["hits"][hidden] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,e,v", FORMS)
+@pytest.mark.parametrize("size", [1e-33, 1e30])
+def test_weights_of_any_size(size, n, e, v, dtype):
+    x, w, b, labels, dloss = case(n, e, v, dtype, seed=140 + e)
+    args = (x, w, b, labels, dloss * n * size)
+    gradients_close(run(*args), reference(*args), 2.0 ** -23 * (8 + 2 * float((x.double() @ w.double()).abs().max())), dtype)
