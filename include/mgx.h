@@ -567,8 +567,8 @@ int mgx_conv_bwd_tape8(const mgx_conv_desc* d, const void* codes, const void* ex
  * masked has the loss of that bias).  Any of dx, dw, db may be NULL.  n <= 8 000 000, v <= 8 000 000, e <= 65 000; x, w
  * and the workspace 16-byte aligned; the workspace (mgx_dense_xent_workspace bytes, -1: sizes out of range) is the call's alone while it
  * runs.  float32 quality throughout: the products are sums of products of fp16 halves of the operands (22 bits, counted from an
- * operand's largest magnitude down to 2^-14 of it), or in float32 where rows are few; a bf16 dx is within 2^-10 of its 2-norm
- * before it is rounded.
+ * operand's largest magnitude down to 2^-14 of it), or in float32 where rows are few; a bf16 dx is within 2^-10 of
+ * sum_j |dz_ij w_kj| before it is rounded.
  * ---------------------------------------------------------------------------------------- */
 int64_t mgx_dense_xent_workspace(int64_t n, int64_t e, int64_t v, int x_is_f32, int backward);
 int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, const float* b, const int32_t* labels, float* loss,

@@ -603,9 +603,9 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
 // again with the comparisons (a branch around two whole copies of the step costs 100 registers of copies where they meet).
 // MODE FWD and DX: rows resident, classes streamed; DW: classes resident, rows streamed.  gridDim.y parts of the streamed
 // operand leave partial results that are joined in order.
-// DX of a bf16 x (NR = 1), whose result is rounded to 8 bits, takes one plane of W in both products and one of P: a logit is then
-// 2^-12 of its terms off and a probability that much of itself.  Only the label's p - 1 could be smaller than that; it is
-// formed from the whole logit, a dot product of a lane with the two planes of its label's class in front of the loop.
+// DX of a bf16 x (NR = 1), whose result is rounded to 8 bits, takes one plane of W and one of P in the second product, 2^-11 of a
+// term each.  The logits take both planes of W: an exponential turns a logit's absolute error into a relative one, and
+// one plane, 2^-11 of the logit's terms, would be off by more than the result's rounding for logits of a few units.
 enum { MODE_FWD = 0, MODE_DX = 1, MODE_DW = 2 };
 constexpr int ST = 32;                              // streamed items of a tile
 
@@ -680,26 +680,12 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                 fb[pl][b][ks] = *(const u32x4*)(g.r[pl] + ((long)item0 + 32 * b + r) * EP + 16 * ks + 8 * h);
     const float unit = logit_unit(g.scales);
     float rinfo[RB];                                // DX: -(lse - 14); DW: bias
-    float plab[RB];                                 // DX, NR = 1: 2^14 (p - 1) of the label
     int rlab[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
         const long it = item0 + 32 * b + r;
         rinfo[b] = MODE == MODE_DW ? g.bias[it] : MODE == MODE_DX ? 14.f - g.row[it].x : 0.f;
         rlab[b] = MODE == MODE_DW ? 0 : g.lab[it];
-        if constexpr (MODE == MODE_DX && NR == 1) {
-            const long c = rlab[b] < 0 ? 0 : rlab[b];
-            float z = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const f16x8 xv = __builtin_bit_cast(f16x8, fb[0][b][ks]);
-                const f16x8 wh = *(const f16x8*)(g.s[0] + c * EP + 16 * ks + 8 * h), wl = *(const f16x8*)(g.s[1] + c * EP + 16 * ks + 8 * h);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) z = __builtin_fmaf((float)xv[k], (float)wl[k], __builtin_fmaf((float)xv[k], (float)wh[k], z));
-            }
-            z += __shfl_xor(z, 32, 64);
-            plab[b] = (__builtin_amdgcn_exp2f(__builtin_fmaf(z, unit, g.bias[c]) + (rinfo[b] - 14.f)) - 1.f) * kDz;
-        }
     }
     // LDS offsets of the lane: the first fragment of its row, and the first transposed reads.  A row starts at a multiple of
     // its size and the swizzle is an XOR, so further fragments (feature blocks) are an XOR of 32 ks (64 eb) away.
@@ -798,9 +784,9 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                 }
             }
         };
-        // pair j of P as fp16 planes
+        // a pair of P as fp16 planes (piece p: pair p / RB of resident item block p % RB)
         auto put = [&](auto P_, float v0, float v1) {
-            constexpr int p = decltype(P_)::value, b = p / 8, j = p % 8;
+            constexpr int p = decltype(P_)::value, b = p % RB, j = p / RB;
             const f16x2 h2 = __builtin_convertvector((f32x2){v0, v1}, f16x2);
             fcur[0][b][j >> 2][j & 3] = __builtin_bit_cast(unsigned, h2);
             if constexpr (NP > 1) fcur[NP - 1][b][j >> 2][j & 3] = f16_pack(v0 - (float)h2[0], v1 - (float)h2[1]);
@@ -810,7 +796,7 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
         // biases of the two streamed classes of pair j
         auto bias2 = [&](int j) { return *(const f32x2*)(te + (8 * (j >> 1) + 4 * h + 2 * (j & 1)) * 4); };
         auto piece = [&](auto P_) {
-            constexpr int p = decltype(P_)::value, b = p / PB, j = p % PB - (PB - 8);
+            constexpr int p = decltype(P_)::value, b = MODE == MODE_FWD ? p / PB : p % RB, j = MODE == MODE_FWD ? p % PB - 1 : p / RB;
             if constexpr (MODE == MODE_FWD && j < 0) {
                 float mm = m[b];
 #pragma unroll
@@ -827,7 +813,7 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                 const f32x2 q = bi2[j & 1];
                 const float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j], unit, q[0]) + rinfo[b]);
                 const float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j + 1], unit, q[1]) + rinfo[b]);
-                if constexpr (b < RB - 1 || j + 2 < 8) bi2[j & 1] = bias2((j + 2) & 7);
+                if constexpr (b == RB - 1 && j + 2 < 8) bi2[j & 1] = bias2(j + 2);
                 put(P_, v0, v1);
             } else {
                 const f32x4 q = ri2[j & 1];
@@ -840,7 +826,7 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
         };
         // the labels of tile i: FWD keeps their logits, DX and DW form P again
         auto label_piece = [&](auto P_) {
-            constexpr int p = decltype(P_)::value, b = p / 8, j = p % 8, k = 2 * j, c0 = (k & 3) + 8 * (k >> 2);
+            constexpr int p = decltype(P_)::value, b = MODE == MODE_FWD ? p / 8 : p % RB, j = MODE == MODE_FWD ? p % 8 : p / RB, k = 2 * j, c0 = (k & 3) + 8 * (k >> 2);
             if constexpr (MODE == MODE_FWD) {
                 const int rel = rlab[b] - s0 - 4 * h;
                 if (rel == c0) g.zlab[item0 + 32 * b + r] = cur[b][k];
@@ -850,7 +836,7 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                 const f32x2 q = bias2(j);
                 const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k], unit, q[0]) + rinfo[b]);
                 const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k + 1], unit, q[1]) + rinfo[b]);
-                put(P_, rel == c0 ? (NR == 1 ? plab[b] : e0 - kDz) : e0, rel == c0 + 1 ? (NR == 1 ? plab[b] : e1 - kDz) : e1);
+                put(P_, rel == c0 ? e0 - kDz : e0, rel == c0 + 1 ? e1 - kDz : e1);
             } else {
                 const f32x4 q = row2(j);
                 const u32x2 lb = *(const u32x2*)(te + 256 + (c0 + 4 * h) * 4);
@@ -1846,7 +1832,7 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
     if (l.narrow) {      // step times: 128 (256) resident items x 32 streamed x 128 (64) features at 1 PFLOP/s over the slots
         const double f = l.ep == 64 ? 0.6 : 1.0;
         l.nf = split(l.np / l.rows_wg, l.vp / ST, 512, f * (xf32 ? 1.6 : 2.1), 8.0 * (double)l.np);
-        l.nx = split(l.np / l.rows_wg, l.vp / ST, xf32 || l.ep == 64 ? 512 : 256, f * (xf32 ? 3.2 : l.ep == 64 ? 2.2 : 1.1),
+        l.nx = split(l.np / l.rows_wg, l.vp / ST, xf32 || l.ep == 64 ? 512 : 256, f * (xf32 ? 3.2 : l.ep == 64 ? 3.3 : 1.65),
                      4.0 * (double)(l.np * l.ep));
         l.nz = split(l.vp / 128, l.np / ST, 512, f * (xf32 ? 3.2 : 2.1), 4.0 * (double)(l.ep * l.vp), true);
     }
@@ -2222,7 +2208,7 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
             q.r[0] = xh; q.r[1] = xl; q.s[0] = wh; q.s[1] = wl;
             q.tiles = (int)(l.vp / ST); q.out = (float*)(ws + l.dxw); q.ld = l.np;
             if (xf) launch_stream<2, 2, 1, MODE_DX, 2>(l, q, l.np / l.rows_wg, l.nx, st);
-            else launch_stream<1, 1, 2, MODE_DX, 1>(l, q, l.np / l.rows_wg, l.nx, st);
+            else launch_stream<1, 2, 2, MODE_DX, 1>(l, q, l.np / l.rows_wg, l.nx, st);
         }
         const XentDxJoin j = {(float*)(ws + l.dxw), q.scales, q.row, nullptr, dx, (int)xf, (int)l.nx, (long)(l.np * l.ep), (long)n, (int)e,
                               (int)l.ep};

@@ -12,6 +12,31 @@ LOWEST = -3.4028234663852886e38
 FORMS = [(3, 40, 300), (60, 70, 500), (40, 30, 33000), (100, 40, 777), (200, 128, 900), (2000, 100, 9000), (150, 300, 1000)]
 
 
+def row_bounds(x, w, b, labels, dloss, dtype):
+    """Per row: how far a loss or lse (beside 2^-23 of its own size) and the 2-norm of a dx may be off.  Logits are
+    sums of float32 quality: 22 bits of each operand and one dropped product, 3 2^-22 of a term |x_k w_kj| at most, and 3 e / 16
+    additions, half a unit of the sum so far each.  Both are of either sign, so that over the e terms of a logit they stay
+    below 2^-22 of sum_k |x_k w_kj| (0.8 of it in emulation with up to 300 terms and 18 million logits; one float32 sum in the
+    order of k comes to 1.5).  lse adds its own to the label's: `unit` is twice that of the row's largest sum, beside a few
+    2^-23 for bias, exponential and logarithm.  A probability is off by unit relative to itself, and the label's p - 1 by
+    unit however small it is.  A bf16 dx is rounded once (2^-8 of it at most), and its second product takes both
+    operands to 11 bits: 2^-11 of a term each, terms |dz_ij| |w_kj|."""
+    x64, w64 = x.double(), w.double()
+    z = x64 @ w64
+    unit = 2.0 ** -23 * 8 + 2.0 ** -21 * (x64.abs() @ w64.abs()).amax(dim=1)
+    z = z + (b.double() if b is not None else 0.0)
+    d = torch.softmax(z, dim=1)
+    at = torch.arange(len(labels)), labels.long()
+    d[at] -= 1.0
+    d *= dloss.double()[:, None]
+    dx = d @ w64.t()
+    size = d.abs() @ w64.abs().t()
+    off = 4 * unit * size.norm(dim=1) + unit * dloss.double().abs() * w64.norm(dim=0)[labels.long()]
+    if dtype == torch.bfloat16:
+        off = off + 2.0 ** -8 * dx.norm(dim=1) + 2.0 ** -10 * size.norm(dim=1)
+    return unit, off
+
+
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("n,e,v", FORMS)
@@ -80,6 +105,22 @@ def test_masked_labels(mask, n, e, v, dtype):
     assert float((got["lse"].double() - want["lse"]).abs().max()) <= unit + 2.0 ** -23 * float(want["lse"].abs().max())
     gradients_close(got, want, unit, dtype)
     assert bool((got["hits"][hidden] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("spread", [2.0, 8.0, 16.0, 32.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,e,v", FORMS)
+def test_sharp_logits(n, e, v, dtype, spread):
+    """Logits of standard deviation up to 32: each row's dx within its own bound."""
+    x, w, b, labels, dloss = case(n, e, v, dtype, seed=130 + e, unlabelled=0, spread=spread)
+    want, got = reference(x, w, b, labels, dloss), run(x, w, b, labels, dloss)
+    unit, off = row_bounds(x, w, b, labels, dloss, dtype)
+    for k in ("loss", "lse"):
+        assert bool(((got[k].double() - want[k]).abs() <= unit + 2.0 ** -23 * want[k].abs()).all()), k
+    short = (got["dx"].double() - want["dx"]).norm(dim=1) / off
+    assert float(short.max()) <= 1.0, float(short.max())
+    gradients_close({**got, "dx": want["dx"]}, want, float(unit.max()), dtype)
 
 
 @gpu
