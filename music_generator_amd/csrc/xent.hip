@@ -182,6 +182,14 @@ __device__ __forceinline__ float row_loss(float m, float ls, float z, float bias
     return bias < kLowest * kLn2 ? (m + ls) * kLn2 - bias : ((m - z) + ls) * kLn2;
 }
 
+// lse in units of log 2 for the backward, which takes exp2(z - lse).  From 2^21 on lse's and z's roundings are worth a unit and more:
+// lse is raised by what they may come to, so that no probability is above 1 (one that overflows the fp16 planes would make
+// the gradient of W infinite for every row).
+__device__ __forceinline__ float lse_units(float lse) {
+    const float l = lse * kLog2e;
+    return fabsf(l) >= 0x1p21f ? __builtin_fmaf(fabsf(l), 0x1p-20f, l) : l;
+}
+
 // What takes the scales out of a product and brings it into units of log 2: at most the largest float, so that a product of zero
 // stays one; 0 where both operands are too small for any logit to differ from its bias.
 __device__ __forceinline__ float logit_unit(const float* scales) { return fminf(kLog2e / scales[0] / scales[1], -kLowest); }
@@ -331,7 +339,7 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
             p.lab[i] = lab < 0 ? -1 : lab;
             if (p.row) {                                     // no label: every exponential of the row is 0
                 const float rs = p.rs && lab >= 0 ? row_scale(p.dloss[i]) : sd;
-                p.row[i] = lab < 0 ? make_float2(__builtin_inff(), 0.f) : make_float2(p.lse[i] * kLog2e, p.dloss[i] / rs * kDz);
+                p.row[i] = lab < 0 ? make_float2(__builtin_inff(), 0.f) : make_float2(lse_units(p.lse[i]), p.dloss[i] / rs * kDz);
                 if (p.rs) {
                     p.rs[i] = lab < 0 ? 0.f : rs;
                     p.ones[i] = (f16_t)(lab < 0 ? 0.f : rs / sd);
@@ -1225,7 +1233,7 @@ __global__ __launch_bounds__(256) void xent_rows_bwd_kernel(XentRows g) {
         const int lab = i < g.n ? g.labels[i] : -1;
         float d = 0.f;
         if (lab >= 0 && lab < g.v) {
-            const float p = __builtin_amdgcn_exp2f(zs[k] - g.lse[i] * kLog2e);
+            const float p = __builtin_amdgcn_exp2f(zs[k] - lse_units(g.lse[i]));
             d = ((long)blockIdx.x * 64 + (k & 63) == lab ? p - 1.f : p) * g.dloss[i];
         }
         zs[k] = d;
@@ -1372,7 +1380,7 @@ __global__ __launch_bounds__(256) void xent_short_prep_kernel(XentShort g, int t
             int lab = i < g.n ? g.labels[i] : -1;
             if (lab < 0 || lab >= g.v) lab = -1;
             g.lab[i] = lab;
-            if (g.row) g.row[i] = lab < 0 ? make_float2(__builtin_inff(), 0.f) : make_float2(g.lse[i] * kLog2e, g.dloss[i]);
+            if (g.row) g.row[i] = lab < 0 ? make_float2(__builtin_inff(), 0.f) : make_float2(lse_units(g.lse[i]), g.dloss[i]);
         }
     }
 }

@@ -131,3 +131,18 @@ def test_weights_of_any_size(size, n, e, v, dtype):
     x, w, b, labels, dloss = case(n, e, v, dtype, seed=140 + e)
     args = (x, w, b, labels, dloss * n * size)
     gradients_close(run(*args), reference(*args), 2.0 ** -23 * (8 + 2 * float((x.double() @ w.double()).abs().max())), dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,e,v", FORMS)
+def test_logits_beyond_the_digits_of_lse(n, e, v, dtype):
+    """Logits around 1e8, where lse, a float32, is known to a few units only: no probability comes out above 1, and
+    gradients stay finite."""
+    x, w, b, labels, dloss = case(n, e, v, dtype, seed=160 + e, unlabelled=0)
+    large = torch.arange(n) % 3 == 2
+    x[large] *= 1e8
+    got = run(x, w, b, labels, dloss)
+    assert all(bool(got[name].isfinite().all()) for name in ("loss", "lse", "dx", "dw", "db"))
+    # |dz| of a row sums to 2 at most
+    assert float(got["db"].abs().sum()) <= 2.001 * float(dloss.sum())
