@@ -566,9 +566,13 @@ int mgx_conv_bwd_tape8(const mgx_conv_desc* d, const void* codes, const void* ex
  * masks a class: its probability is 0 and its column of w is not used (one class at least is not masked; a row whose label is
  * masked has the loss of that bias).  Any of dx, dw, db may be NULL.  n <= 8 000 000, v <= 8 000 000, e <= 65 000; x, w
  * and the workspace 16-byte aligned; the workspace (mgx_dense_xent_workspace bytes, -1: sizes out of range) is the call's alone while it
- * runs.  float32 quality throughout: the products are sums of products of fp16 halves of the operands (22 bits, counted from an
- * operand's largest magnitude down to 2^-14 of it), or in float32 where rows are few; a bf16 dx is within 2^-10 of
- * sum_j |dz_ij w_kj| before it is rounded.
+ * runs.  float32 quality: the products are sums of products of fp16 halves of the operands, or in float32 where rows are few.  The
+ * halves hold 22 bits of what is above 2^-17 of the largest magnitude in the row of x, or in the unmasked classes of w, and
+ * the rest to 2^-39 of it: rows do not depend on each other's size; a class whose column of w is far smaller than another's
+ * has its logits to 2^-39 of the larger one's terms.  In dw, terms are counted from the largest |dloss_i| max_k |x_ik| in the same
+ * way.  The backward's probabilities are relative to lse, a float32: 2^-23 |lse| of themselves off, and from
+ * |lse| = 1.4e6 on known to a factor only, but never above 1.  A bf16 dx is within 2^-10 of sum_j |dz_ij w_kj| before it
+ * is rounded.
  * ---------------------------------------------------------------------------------------- */
 int64_t mgx_dense_xent_workspace(int64_t n, int64_t e, int64_t v, int x_is_f32, int backward);
 int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, const float* b, const int32_t* labels, float* loss,

@@ -8,13 +8,14 @@
 //
 // Arithmetic: few rows in float32.  The products of many rows run on v_mfma_f32_32x32x16_f16 with float32 accumulation, at
 // float32 quality.  A float32
-// operand is the sum of two fp16 planes, hi = fp16(s a) and lo = fp16(s a - hi) with s a power of two that brings the
-// operand's largest magnitude below 2^14: 22 significant bits, and 2^-25 of 2^14 absolute where a value is small.  The
+// operand is the sum of two fp16 planes, hi = fp16(s a) and lo = fp16(s a - hi) with s a power of two that brings a row of x (each
+// its own, so that no row's digits depend on another's), or all of W, below 2^14 in magnitude: 22 significant bits, and 2^-25 of
+// 2^14 absolute where a value is small.  The
 // product keeps hi hi + hi lo + lo hi (the dropped lo lo is 2^-24 of it).  A bf16 operand is exact in one plane.  This is
 // three (two) of 2.5 PFLOP/s instead of one of the 157 TFLOP/s of the float32 matrix instructions.
 // Logits, maxima, sums, lse and all gradient sums are float32.  Biases are in units of log 2 and log2(e) is in the factor that
-// takes the scales out: an exponential is one fma, one difference and one v_exp_f32.  (Accumulators that start at the bias
-// times both scales save the difference, but that product leaves float32 where the operands are small or the bias is a mask.)
+// takes the powers of two out: an exponential is one fma, one difference and one v_exp_f32.  (Accumulators that start at the bias
+// times both powers save the difference, but that product leaves float32 where the operands are small or the bias is a mask.)
 //
 // Four forms.  What each is bound by, and forward + backward times (us; n x e x v):
 //   few rows (up to 4, up to 16 of a small W): launches and HBM (W read twice, dW written), float32 on the vector ALU.
@@ -69,21 +70,23 @@ struct XentOut {
     int e, accumulate, direct;
 };
 
-constexpr float kDz = 16384.f;                     // dz planes hold 2^14 dz / (largest |dloss|, rounded up to a power of two)
+constexpr float kDz = 16384.f;                     // planes of probabilities hold 2^14 p
 constexpr int kMaxParts = 512;
 
 inline int64_t up(int64_t a, int64_t m) { return (a + m - 1) / m * m; }
 
-// ---------------------------------------------------------------- scales
-// Largest finite magnitudes of the unmasked classes of W and of the labelled rows of x and dloss (the others may hold anything) as
-// float32 bits: one partial per workgroup and tensor.  A thread takes 4 features of 4 classes of W (WVEC, rows of whole 16-byte
+// ---------------------------------------------------------------- powers of two
+// Largest finite magnitudes as float32 bits: of every labelled row of x (rmax), and one partial per workgroup of the unmasked classes of
+// W, of the labelled rows' dloss, and of their product with the row's largest (as the sum of both exponents, 1 more: 0 is
+// none); what is unlabelled or masked may hold anything.  A thread takes 4 features of 4 classes of W (WVEC, rows of whole 16-byte
 // pieces) or 16 features of one; 2^lsh lanes walk a row of x, in pieces of 16 bytes where rows consist of them (VEC).
 __device__ __forceinline__ bool masked(float b) { return b <= kLowest; }
 
 template <bool XF32, bool VEC, bool WVEC>
 __global__ __launch_bounds__(256) void xent_max_kernel(const float* __restrict__ w, const float* __restrict__ b,
                                                        const void* __restrict__ x, long n, int e, const int* __restrict__ labels,
-                                                       long v, int lsh, const float* __restrict__ dl, unsigned* __restrict__ part) {
+                                                       long v, int lsh, const float* __restrict__ dl, unsigned* __restrict__ part,
+                                                       unsigned* __restrict__ rmax) {
     __shared__ unsigned red[3][4];
     const long t = (long)blockIdx.x * 256 + threadIdx.x, stride = (long)gridDim.x * 256;
     unsigned m[3] = {0u, 0u, 0u};
@@ -117,7 +120,7 @@ __global__ __launch_bounds__(256) void xent_max_kernel(const float* __restrict__
     for (long row = t >> lsh; row < n; row += stride >> lsh) {
         const int lab = labels[row];
         if (lab < 0 || lab >= v) continue;
-        if (dl && (threadIdx.x & (lanes - 1)) == 0) take(m[2], __builtin_bit_cast(unsigned, dl[row]));
+        unsigned rm = 0u;
         for (int c = threadIdx.x & (lanes - 1); c < cols; c += 4 * lanes) {
             if constexpr (VEC) {
                 u32x4 q[4];
@@ -128,8 +131,8 @@ __global__ __launch_bounds__(256) void xent_max_kernel(const float* __restrict__
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        take(m[1], XF32 ? q[j][k] : q[j][k] & 0xffff0000u);
-                        if (!XF32) take(m[1], q[j][k] << 16);
+                        take(rm, XF32 ? q[j][k] : q[j][k] & 0xffff0000u);
+                        if (!XF32) take(rm, q[j][k] << 16);
                     }
             } else {
                 unsigned q[4];
@@ -139,7 +142,21 @@ __global__ __launch_bounds__(256) void xent_max_kernel(const float* __restrict__
                     q[j] = c + j * lanes >= cols ? 0u : XF32 ? ((const unsigned*)x)[at] : (unsigned)((const unsigned short*)x)[at] << 16;
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) take(m[1], q[j]);
+                for (int j = 0; j < 4; ++j) take(rm, q[j]);
+            }
+        }
+        for (int off = lanes >> 1; off > 0; off >>= 1) {
+            const unsigned o = (unsigned)__shfl_xor((int)rm, off, 64);
+            rm = rm > o ? rm : o;
+        }
+        if ((threadIdx.x & (lanes - 1)) == 0) {
+            rmax[row] = rm;
+            if (dl) {
+                unsigned d = 0u;
+                take(d, __builtin_bit_cast(unsigned, dl[row]));
+                m[2] = m[2] > d ? m[2] : d;
+                const unsigned both = d && rm ? (d >> 23) + (rm >> 23) + 1u : 0u;
+                m[1] = m[1] > both ? m[1] : both;
             }
         }
     }
@@ -161,13 +178,8 @@ __global__ __launch_bounds__(256) void xent_max_kernel(const float* __restrict__
     }
 }
 
-// Power of two that brings magnitudes up to the float32 with these bits below 2^14 (its reciprocal stays normal too).
-__device__ __forceinline__ float scale_of(unsigned maxbits) {
-    int e = 14 + 126 - (int)(maxbits >> 23);                  // max < 2^(field - 126)
-    if (maxbits == 0u) e = 0;
-    e = e < -120 ? -120 : (e > 120 ? 120 : e);
-    return __builtin_bit_cast(float, (unsigned)(e + 127) << 23);
-}
+// Exponent that brings magnitudes up to the float32 with these bits below 2^14 (max < 2^(field - 126)).
+__device__ __forceinline__ int exponent_of(unsigned maxbits) { return maxbits == 0u ? 0 : 140 - (int)(maxbits >> 23); }
 
 // A bias in units of log 2; a finite one stays finite.
 __device__ __forceinline__ float log2_units(float b) {
@@ -190,16 +202,12 @@ __device__ __forceinline__ float lse_units(float lse) {
     return fabsf(l) >= 0x1p21f ? __builtin_fmaf(fabsf(l), 0x1p-20f, l) : l;
 }
 
-// What takes the scales out of a product and brings it into units of log 2: at most the largest float, so that a product of zero
-// stays one; 0 where both operands are too small for any logit to differ from its bias.
-__device__ __forceinline__ float logit_unit(const float* scales) { return fminf(kLog2e / scales[0] / scales[1], -kLowest); }
+// What takes the powers of two out of a row's products and brings them into units of log 2: at most the largest float, so that a
+// product of zero stays one; 0 where the operands are too small for any logit to differ from its bias.
+__device__ __forceinline__ float logit_unit(int ew, int ex) { return fminf(ldexpf(kLog2e, -ew - ex), -kLowest); }
 
-// The power of two above a magnitude, 2^-105 at least: the one of a row of dloss is never above that of the largest, and reciprocals
-// and ratios stay normal.
-__device__ __forceinline__ float row_scale(float d) { return 16384.f / scale_of(__builtin_bit_cast(unsigned, fmaxf(fabsf(d), 0x1p-106f))); }
-
-// {s_w, s_x, largest |dloss| rounded up to a power of two} into scales[0..2]; part has `parts` partials per tensor.
-__device__ __forceinline__ float scale_from_parts(const unsigned* __restrict__ part, int which, int parts) {
+// The largest of the `parts` partials of quantity `which`.
+__device__ __forceinline__ unsigned max_of_parts(const unsigned* __restrict__ part, int which, int parts) {
     unsigned m = 0u, o[kMaxParts / 64];
 #pragma unroll
     for (int k = 0; k < kMaxParts / 64; ++k) {                   // all loads in flight at once
@@ -213,9 +221,11 @@ __device__ __forceinline__ float scale_from_parts(const unsigned* __restrict__ p
         const unsigned q = (unsigned)__shfl_xor((int)m, off, 64);
         m = m > q ? m : q;
     }
-    if (which == 2) return row_scale(__builtin_bit_cast(float, m));
-    return scale_of(m);
+    return m;
 }
+
+// Exponent field of a float: |d| < 2^(field - 126).
+__device__ __forceinline__ int field_of(float d) { return (int)(__builtin_bit_cast(unsigned, d) >> 23 & 0xffu); }
 
 // ---------------------------------------------------------------- planes
 __device__ __forceinline__ void split8(const float* v, u32x4& hi, u32x4& lo) {
@@ -236,19 +246,23 @@ struct XentPrep {
     long n, v, np, vp;            // rows, classes, and both padded to 128
     int e, ep;                    // features, padded to 128
     f16_t *xh, *xl, *wh, *wl;     // planes: rows x ep, classes x ep
-    float *bias, *scales;
-    // per row: lse (log 2 units) and the factor of its dz.  Streamed: 2^14 dloss / scales[2].  Wide features, where dz is stored:
-    // 2^14 dloss / rs, rs the power of two above |dloss|, so that the dz of a row of small weight keeps its digits; rs goes into
-    // dx, and rs / scales[2] into the planes of x that dW is made of (xsh, xsl) and into the weights of db (ones).
-    float2* row;
-    float* rs;
+    const unsigned* rmax;         // per labelled row: its largest magnitude
+    float* bias;
+    // {exponent of W's planes, the largest exponent sum of a row's dloss and x, that of dloss (fields)}
+    int* exps;
+    // per row: lse (units of log 2), the factor of its dz, the unit of its logits, dloss; (inf, 0, 0, 0) without a label.  A row of x is held
+    // under its own power of two 2^ex, so no row's digits depend on another's.  The factor of dz, streamed: dloss 2^-ex, counted
+    // from its largest, so that the planes of x times dz sum to dW.  Wide features, where dz is stored and serves dx too:
+    // dloss 2^14 over its own power of two, which goes into dx; both powers, counted from the largest, go into
+    // the planes of x that dW is made of (xsh, xsl), and dloss's into the weights of db (ones).
+    f32x4* row;
     f16_t *xsh, *xsl, *ones;
     int* lab;
     long wtiles, xblocks;
 };
 
 // Workgroups 0 .. wtiles-1: a 64 classes x 64 features tile of W, transposed through LDS into the class-major planes;
-// the next xblocks: the planes of x; the rest: padded bias, labels and per-row scalars, and the scales.
+// the next xblocks: the planes of x; the rest: padded bias, labels and per-row scalars, and the exponents.
 template <bool XF32>
 __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
     const int tid = threadIdx.x;
@@ -258,15 +272,15 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
         const long c0 = ct * 64, e0 = et * 64;
         const int cc = tid & 63, k0 = tid >> 6;
         const float bc = p.b && c0 + cc < p.v ? p.b[c0 + cc] : 0.f;
-        float in[16];                                          // in flight while the scale is found
+        float in[16];                                          // in flight while the exponent is found
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             const int k = k0 + 4 * j;
             in[j] = c0 + cc < p.v && e0 + k < p.e ? p.w[(e0 + k) * p.v + c0 + cc] : 0.f;
         }
-        const float s = scale_from_parts(p.part, 0, p.parts);
+        const int ew = exponent_of(max_of_parts(p.part, 0, p.parts));
 #pragma unroll
-        for (int j = 0; j < 16; ++j) t[k0 + 4 * j][cc] = masked(bc) ? 0.f : in[j] * s;
+        for (int j = 0; j < 16; ++j) t[k0 + 4 * j][cc] = masked(bc) ? 0.f : ldexpf(in[j], ew);
         __syncthreads();
         const int e8 = tid & 7;
         for (int c = tid >> 3; c < 64; c += 32) {
@@ -280,7 +294,7 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
             *(u32x4*)(p.wl + at) = lo;
         }
     } else if ((long)blockIdx.x < p.wtiles + p.xblocks) {
-        const float s = scale_from_parts(p.part, 1, p.parts), sd = p.xsh ? scale_from_parts(p.part, 2, p.parts) : 1.f;
+        const int most = p.xsh ? (int)max_of_parts(p.part, 1, p.parts) - 1 : 0;
         const int q = p.ep / 8;
         for (long i = ((long)blockIdx.x - p.wtiles) * 256 + tid; i < p.np * q; i += p.xblocks * 256) {
             const long row = i / q;
@@ -288,6 +302,8 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
             const int lab = row < p.n ? p.labels[row] : -1;
             const bool ok = lab >= 0 && lab < p.v;
             const long at = row * p.e + c;
+            const unsigned rm = ok ? p.rmax[row] : 0u;
+            const int ex = exponent_of(rm);
             float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
             if (ok && (p.e & 7) == 0) {                        // rows of whole 16-byte pieces
                 if (c < p.e) {
@@ -307,44 +323,52 @@ __global__ __launch_bounds__(256) void xent_prep_kernel(XentPrep p) {
                     if (c + k < p.e) v[k] = XF32 ? ((const float*)p.x)[at + k] : (float)((const bf16_t*)p.x)[at + k];
             }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] *= s;
+            for (int k = 0; k < 8; ++k) v[k] = ldexpf(v[k], ex);
             u32x4 hi, lo;
             split8(v, hi, lo);
             *(u32x4*)(p.xh + row * p.ep + c) = hi;
             if (XF32) *(u32x4*)(p.xl + row * p.ep + c) = lo;
             if (p.xsh) {
-                const float rel = ok ? row_scale(p.dloss[row]) / sd : 0.f;
+                const int rel = ok ? field_of(p.dloss[row]) + (int)(rm >> 23) - most : 0;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] *= rel;
+                for (int k = 0; k < 8; ++k) v[k] = ldexpf(v[k], rel < 0 ? rel : 0);
                 split8(v, hi, lo);
                 *(u32x4*)(p.xsh + row * p.ep + c) = hi;
                 if (XF32) *(u32x4*)(p.xsl + row * p.ep + c) = lo;
             }
         }
     } else {
-        const float sw = scale_from_parts(p.part, 0, p.parts), sx = scale_from_parts(p.part, 1, p.parts),
-                    sd = scale_from_parts(p.part, 2, p.parts);
+        const int ew = exponent_of(max_of_parts(p.part, 0, p.parts)), most = (int)max_of_parts(p.part, 1, p.parts) - 1,
+                  fd = (int)(max_of_parts(p.part, 2, p.parts) >> 23);
         const long first = (long)blockIdx.x - p.wtiles - p.xblocks, nb = gridDim.x - p.wtiles - p.xblocks;
         if (first == 0 && tid == 0) {
-            p.scales[0] = sw;
-            p.scales[1] = sx;
-            p.scales[2] = sd;
+            p.exps[0] = ew;
+            p.exps[1] = most;
+            p.exps[2] = fd;
         }
-        for (long i = first * 256 + tid; i < p.vp; i += nb * 256) {
+        for (long i = first * 256 + tid; i < p.vp; i += nb * 256)
             p.bias[i] = log2_units(i < p.v ? (p.b ? p.b[i] : 0.f) : -__builtin_inff());
-        }
         for (long i = first * 256 + tid; i < p.np; i += nb * 256) {
             int lab = i < p.n ? p.labels[i] : -1;
-            if (lab >= p.v) lab = -1;
-            p.lab[i] = lab < 0 ? -1 : lab;
-            if (p.row) {                                     // no label: every exponential of the row is 0
-                const float rs = p.rs && lab >= 0 ? row_scale(p.dloss[i]) : sd;
-                p.row[i] = lab < 0 ? make_float2(__builtin_inff(), 0.f) : make_float2(lse_units(p.lse[i]), p.dloss[i] / rs * kDz);
-                if (p.rs) {
-                    p.rs[i] = lab < 0 ? 0.f : rs;
-                    p.ones[i] = (f16_t)(lab < 0 ? 0.f : rs / sd);
+            if (lab < 0 || lab >= p.v) lab = -1;
+            p.lab[i] = lab;
+            f32x4 info = {__builtin_inff(), 0.f, 0.f, 0.f};       // no label: every exponential of the row is 0
+            float weight = 0.f;
+            if (lab >= 0) {
+                const unsigned rm = p.rmax[i];
+                const int ex = exponent_of(rm);
+                info[2] = logit_unit(ew, ex);
+                if (p.dloss) {
+                    const float d = p.dloss[i];
+                    const int f = field_of(d);
+                    info[0] = lse_units(p.lse[i]);
+                    info[1] = p.xsh ? ldexpf(d, 140 - f) : rm ? ldexpf(d, 280 - ex - most) : 0.f;      // a row of zeros adds none to dW
+                    info[3] = d;
+                    weight = ldexpf(1.f, f < fd ? f - fd : 0);
                 }
             }
+            p.row[i] = info;
+            if (p.ones) p.ones[i] = (f16_t)weight;
         }
     }
 }
@@ -362,8 +386,9 @@ struct XentGemm {
     long lda, ldb;
     int kiters;
     // epilogues
-    const float *bias, *scales;
-    const float2* row;
+    const float* bias;
+    const int* exps;
+    const f32x4* row;
     const int* lab;
     float2* part;
     float *zlab, *out, *outb;
@@ -484,11 +509,12 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
     const long mw = m0 + wm * 64, nw = n0 + wn * 64;
     if constexpr (EPI == EPI_FWD || EPI == EPI_DZ) {
         // A: classes, B: rows of x
-        const float unit = logit_unit(g.scales);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const long row = nw + j * 32 + r;
             const int lab = g.lab[row];
+            const f32x4 info = g.row[row];
+            const float unit = info[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -519,7 +545,7 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
                             if (i * 32 + (k & 3) + 8 * (k >> 2) + 4 * h == (int)rel) g.zlab[row] = acc[i][j][k];
                 }
             } else {
-                const float lse = g.row[row].x, dl = g.row[row].y;
+                const float lse = info[0], dl = info[1];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -558,7 +584,7 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
     } else {
         // A: features, B: classes; the gradients, or slab z of the piece
         if (g.o.direct) {
-            const float fb = g.scales[2] / kDz, fx = 1.f / g.scales[1];      // one after the other: their product may be too small
+            const int ed = g.exps[1] - 280, eb = g.exps[2] - 140;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const long c = nw + j * 32 + r;
@@ -571,12 +597,15 @@ __global__ __launch_bounds__(512, 2) void xent_gemm_kernel(XentGemm g) {
                             const long f = mw + i * 32 + acc_row(k, lane);
                             if (f < g.o.e) {
                                 float* d = g.o.dw + f * g.o.v + c;
-                                const float q = acc[i][j][k] * fb * fx;
+                                const float q = ldexpf(acc[i][j][k], ed);
                                 *d = g.o.accumulate ? *d + q : q;
                             }
                         }
                 }
-                if (bias_wave && h == 0 && g.o.db) g.o.db[c] = g.o.accumulate ? g.o.db[c] + accb[j][0] * fb : accb[j][0] * fb;
+                if (bias_wave && h == 0 && g.o.db) {
+                    const float q = ldexpf(accb[j][0], eb);
+                    g.o.db[c] = g.o.accumulate ? g.o.db[c] + q : q;
+                }
             }
             return;
         }
@@ -619,9 +648,9 @@ constexpr int ST = 32;                              // streamed items of a tile
 
 struct XentStream {
     const f16_t *r[2], *s[2];
-    const float *scales;
-    const float *bias;                              // classes
-    const float2* row;                              // rows: lse, scaled dloss
+    const int* exps;
+    const float* bias;                              // classes
+    const f32x4* row;                               // rows: lse, factor of dz, unit, dloss
     const int* lab;                                 // rows
     int tiles;                                      // streamed tiles
     float2* part;                                   // FWD: (maximum, sum) per part and row
@@ -654,8 +683,8 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
     // the chunk that belongs there: the swizzle of the lane's row in the first piece, and a bit that is uniform in later ones.
     // In assembly: in front of a transposed LDS read the compiler waits for every LDS-DMA it knows of, the one just issued
     // for a later tile included.
-    // beside the planes: FWD and DX the biases, DW (lse, dloss) and the labels of the tile's items
-    const void* ip = MODE != MODE_DW ? (const void*)g.bias : wv == 0 ? (const void*)g.row : (const void*)g.lab;
+    // beside the planes: FWD and DX the biases (128 B, twice), DW what the rows have (512 B) and their labels
+    const float* ip = MODE != MODE_DW ? g.bias : wv < 2 ? (const float*)g.row + 64 * wv : (const float*)g.lab;
     const int lrow = EP == 128 ? lane >> 4 : lane >> 3;
     const int lo0 = lrow * ROWB + (((lane & (EP / 8 - 1)) ^ swz_item<EP>(lrow)) << 4);
     auto stage = [&](int t) {
@@ -668,9 +697,9 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                 const int piece = wv * (PIECES / 4) + i, flip = EP == 128 ? (piece & 3) << 4 : (piece & 1) << 5;
                 lds_dma16(g.s[pl] + ((long)t * SPLANE + piece * 1024) / 2, lo0 ^ flip, dst + pl * SPLANE + piece * 1024);
             }
-        if (wv < (MODE == MODE_DW ? 2 : 1)) {        // 64 floats, or 32 twice
-            const bool two = MODE == MODE_DW && wv == 0;
-            lds_dma4((const float*)ip + (long)t * (two ? 2 * ST : ST), two ? lane * 4 : r * 4, dst + NS * SPLANE + wv * 256);
+        if (wv < (MODE == MODE_DW ? 3 : 1)) {        // 64 floats, or 32 twice
+            const bool half = MODE == MODE_DW && wv < 2;
+            lds_dma4(ip + (long)t * (half ? 4 * ST : ST), half ? lane * 4 : r * 4, dst + NS * SPLANE + wv * 256);
         }
     };
 
@@ -686,13 +715,14 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
                 fb[pl][b][ks] = *(const u32x4*)(g.r[pl] + ((long)item0 + 32 * b + r) * EP + 16 * ks + 8 * h);
-    const float unit = logit_unit(g.scales);
+    float unit[RB];                                 // FWD, DX
     float rinfo[RB];                                // DX: -(lse - 14); DW: bias
     int rlab[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
         const long it = item0 + 32 * b + r;
-        rinfo[b] = MODE == MODE_DW ? g.bias[it] : MODE == MODE_DX ? 14.f - g.row[it].x : 0.f;
+        rinfo[b] = MODE == MODE_DW ? g.bias[it] : MODE == MODE_DX ? 14.f - g.row[it][0] : 0.f;
+        unit[b] = MODE == MODE_DW ? 0.f : g.row[it][2];
         rlab[b] = MODE == MODE_DW ? 0 : g.lab[it];
     }
     // LDS offsets of the lane: the first fragment of its row, and the first transposed reads.  A row starts at a multiple of
@@ -722,7 +752,7 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
     auto labels_in = [&](int t) -> bool {
         bool in = false;
         if constexpr (MODE == MODE_DW) {
-            const int lb = *(const int*)(lds + (t & 3) * BUF + NS * SPLANE + 256 + r * 4);
+            const int lb = *(const int*)(lds + (t & 3) * BUF + NS * SPLANE + 512 + r * 4);
             in = lb >= item0 && lb < item0 + 32 * RB;
         } else {
 #pragma unroll
@@ -749,8 +779,8 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
         asm volatile("" : "+v"(ao), "+v"(to[0]), "+v"(to[1]));      // keeps the 16 addresses derived from them out of registers
         const int s0 = i * ST;
         u32x4 fr[3];
-        f32x4 ri2[2];                                // DW
-        f32x2 bi2[2];                                // DX: biases of the next pairs
+        f32x4 ri2[2];                                // DW: what the two rows of the next pair have
+        f32x2 bi2;                                   // DX: biases of the next pair
         f32x4 bv[4];                                 // FWD: biases of the tile
         float tsum[RB];                              // DW: the tile's sum of P, added to the running one once a tile
 #pragma unroll
@@ -799,8 +829,8 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
             fcur[0][b][j >> 2][j & 3] = __builtin_bit_cast(unsigned, h2);
             if constexpr (NP > 1) fcur[NP - 1][b][j >> 2][j & 3] = f16_pack(v0 - (float)h2[0], v1 - (float)h2[1]);
         };
-        // (lse, dloss) of the two streamed rows of pair j
-        auto row2 = [&](int j) { return *(const f32x4*)(te + (8 * (j >> 1) + 4 * h + 2 * (j & 1)) * 8); };
+        // what streamed row k of pair j has
+        auto row2 = [&](int j, int k) { return *(const f32x4*)(te + (8 * (j >> 1) + 4 * h + 2 * (j & 1) + k) * 16); };
         // biases of the two streamed classes of pair j
         auto bias2 = [&](int j) { return *(const f32x2*)(te + (8 * (j >> 1) + 4 * h + 2 * (j & 1)) * 4); };
         auto piece = [&](auto P_) {
@@ -809,7 +839,7 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                 float mm = m[b];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    cur[b][k] = __builtin_fmaf(cur[b][k], unit, bv[k >> 2][k & 3]);
+                    cur[b][k] = __builtin_fmaf(cur[b][k], unit[b], bv[k >> 2][k & 3]);
                     mm = fmaxf(mm, cur[b][k]);
                 }
                 ssum[b] *= __builtin_amdgcn_exp2f(m[b] - mm);
@@ -818,17 +848,20 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
 #pragma unroll
                 for (int k = 2 * j; k < 2 * j + 2; ++k) ssum[b] += __builtin_amdgcn_exp2f(cur[b][k] - m[b]);
             } else if constexpr (MODE == MODE_DX) {
-                const f32x2 q = bi2[j & 1];
-                const float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j], unit, q[0]) + rinfo[b]);
-                const float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j + 1], unit, q[1]) + rinfo[b]);
-                if constexpr (b == RB - 1 && j + 2 < 8) bi2[j & 1] = bias2(j + 2);
+                const f32x2 q = bi2;
+                const float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j], unit[b], q[0]) + rinfo[b]);
+                const float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j + 1], unit[b], q[1]) + rinfo[b]);
+                if constexpr (b == RB - 1 && j < 7) bi2 = bias2(j + 1);
                 put(P_, v0, v1);
             } else {
-                const f32x4 q = ri2[j & 1];
-                const float v0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j], unit, rinfo[b]) - q[0]) * q[1];
-                const float v1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j + 1], unit, rinfo[b]) - q[2]) * q[3];
-                tsum[b] += v0 + v1;
-                if constexpr (b == RB - 1 && j + 2 < 8) ri2[j & 1] = row2(j + 2);
+                const f32x4 q0 = ri2[0], q1 = ri2[1];
+                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j], q0[2], rinfo[b]) - q0[0]), v0 = e0 * q0[1];
+                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][2 * j + 1], q1[2], rinfo[b]) - q1[0]), v1 = e1 * q1[1];
+                tsum[b] = __builtin_fmaf(e1, q1[3], __builtin_fmaf(e0, q0[3], tsum[b]));
+                if constexpr (b == RB - 1 && j < 7) {
+                    ri2[0] = row2(j + 1, 0);
+                    ri2[1] = row2(j + 1, 1);
+                }
                 put(P_, v0, v1);
             }
         };
@@ -842,18 +875,19 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
             } else if constexpr (MODE == MODE_DX) {
                 const int rel = rlab[b] - s0 - 4 * h;
                 const f32x2 q = bias2(j);
-                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k], unit, q[0]) + rinfo[b]);
-                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k + 1], unit, q[1]) + rinfo[b]);
+                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k], unit[b], q[0]) + rinfo[b]);
+                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k + 1], unit[b], q[1]) + rinfo[b]);
                 put(P_, rel == c0 ? e0 - kDz : e0, rel == c0 + 1 ? e1 - kDz : e1);
             } else {
-                const f32x4 q = row2(j);
-                const u32x2 lb = *(const u32x2*)(te + 256 + (c0 + 4 * h) * 4);
-                const float d0 = (int)lb[0] - item0 - 32 * b == r ? q[1] : 0.f, d1 = (int)lb[1] - item0 - 32 * b == r ? q[3] : 0.f;
-                tsum[b] -= d0 + d1;
-                // (p - 1) dloss, as one fma each: p dloss would have lost the digits of a p next to 1
-                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k], unit, rinfo[b]) - q[0]);
-                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k + 1], unit, rinfo[b]) - q[2]);
-                put(P_, __builtin_fmaf(e0, q[1], -d0), __builtin_fmaf(e1, q[3], -d1));
+                const f32x4 q0 = row2(j, 0), q1 = row2(j, 1);
+                const u32x2 lb = *(const u32x2*)(te + 512 + (c0 + 4 * h) * 4);
+                const bool is0 = (int)lb[0] - item0 - 32 * b == r, is1 = (int)lb[1] - item0 - 32 * b == r;
+                const float d0 = is0 ? q0[1] : 0.f, d1 = is1 ? q1[1] : 0.f;
+                tsum[b] -= (is0 ? q0[3] : 0.f) + (is1 ? q1[3] : 0.f);
+                // (p - 1) times the factor, as one fma each: p times it would have lost the digits of a p next to 1
+                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k], q0[2], rinfo[b]) - q0[0]);
+                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[b][k + 1], q1[2], rinfo[b]) - q1[0]);
+                put(P_, __builtin_fmaf(e0, q0[1], -d0), __builtin_fmaf(e1, q1[1], -d1));
             }
         };
         if constexpr (DO_S) {
@@ -867,12 +901,11 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
             for (int q = 0; q < 4; ++q) bv[q] = *(const f32x4*)(te + (8 * q + 4 * h) * 4);
         }
         if constexpr (DO_E && MODE == MODE_DX) {
-            bi2[0] = bias2(0);
-            bi2[1] = bias2(1);
+            bi2 = bias2(0);
         }
         if constexpr (DO_E && MODE == MODE_DW) {
-            ri2[0] = row2(0);
-            ri2[1] = row2(1);
+            ri2[0] = row2(0, 0);
+            ri2[1] = row2(0, 1);
         }
         load(std::integral_constant<int, 0>{});
         load(std::integral_constant<int, 1>{});
@@ -941,7 +974,7 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
             const float so = __shfl_xor(ssum[b], 32, 64);
             if (g.o.direct) {
                 if (it >= g.o.cnt) continue;
-                const float fb_ = g.scales[2] / kDz, fx = 1.f / g.scales[1];
+                const int ed = g.exps[1] - 280;
                 if (g.o.dw) {
 #pragma unroll
                     for (int eb = 0; eb < EB; ++eb)
@@ -950,13 +983,13 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                             const int f = 32 * eb + acc_row(i, lane);
                             if (f < g.o.e) {
                                 float* d = g.o.dw + f * g.o.v + it;
-                                const float q = dacc[eb][b][i] * fb_ * fx;
+                                const float q = ldexpf(dacc[eb][b][i], ed);
                                 *d = g.o.accumulate ? *d + q : q;
                             }
                         }
                 }
                 if (h == 0 && g.o.db) {
-                    const float q = (ssum[b] + so) * fb_;
+                    const float q = ssum[b] + so;
                     g.o.db[it] = g.o.accumulate ? g.o.db[it] + q : q;
                 }
                 continue;
@@ -987,9 +1020,10 @@ __device__ __forceinline__ float sum_parts(const float* __restrict__ p, int n, l
 // dx from its parts in G groups of consecutive parts, then the groups in order: one group where the outputs fill the chip, sixteen
 // where they are few and the parts many
 struct XentDxJoin {
-    const float *parts, *scales;
-    const float2* rowinfo;
-    const float* rs;
+    const float* parts;
+    const int* exps;               // NULL: the parts are those of dx itself
+    const f32x4* row;
+    bool wide;
     void* dx;
     int dx_f32, np;
     long part, n;
@@ -1000,9 +1034,9 @@ template <int G>
 __device__ __forceinline__ void xent_dx_join(const XentDxJoin& j, long block, long blocks) {
     constexpr int W = G == 1 ? 256 : 64;
     __shared__ float red[G][G == 1 ? 1 : 64];
-    const auto [parts, scales, rowinfo, rs, dx, dx_f32, np, part, n, e, ep] = j;
-    // streamed: the parts hold 2^14 dz / dloss, the rows 2^14 dloss / scales[2]; wide: 2^14 dz / rs
-    const float f = !scales ? 1.f : (rs ? 1.f : scales[2] / kDz) / kDz, fw = scales ? 1.f / scales[0] : 1.f;
+    const auto [parts, exps, rowinfo, wide, dx, dx_f32, np, part, n, e, ep] = j;
+    // streamed: the parts are of 2^14 dz / dloss; wide: of 2^14 dz over the power of two of dloss
+    const int ew = exps ? exps[0] : 0;
     const int lane = threadIdx.x % W, q = threadIdx.x / W;
     const int per = (np + G - 1) / G, p0 = q * per, cnt = np - p0 < per ? np - p0 : per;
     for (long i = block * W + lane; i - lane < n * ep; i += blocks * W) {
@@ -1017,7 +1051,11 @@ __device__ __forceinline__ void xent_dx_join(const XentDxJoin& j, long block, lo
         const long row = i / ep;
         const int c = (int)(i - row * ep);
         if (q == 0 && row < n && c < e) {
-            if (scales) s = s * fw * (f * (rs ? rs[row] : rowinfo[row].y));
+            if (exps) {
+                const float d = rowinfo[row][3];
+                const int f = field_of(d);
+                s = ldexpf(wide ? s : s * ldexpf(d, 126 - f), f - 140 - ew);
+            }
             if (dx_f32) ((float*)dx)[row * e + c] = s;
             else ((bf16_t*)dx)[row * e + c] = (bf16_t)s;
         }
@@ -1068,7 +1106,9 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
 
 // dW and db of a piece of the classes from the slabs of the split contraction, in order: 256 classes of a feature (or of db) a block
 struct XentDwReduce {
-    const float *slabs, *slabs_b, *scales;
+    const float *slabs, *slabs_b;
+    const int* exps;
+    bool wide;                         // slabs_b under the largest dloss's power of two
     float *dw, *db;
     int nz;
     long slab, ldo;
@@ -1081,14 +1121,13 @@ struct XentDwReduce {
 __device__ __forceinline__ void xent_dw_reduce(const XentDwReduce& g, long block) {
     const long cols = (g.cnt + 255) / 256, k = block / cols, c = (block - k * cols) * 256 + threadIdx.x;
     if (c >= g.cnt || g.c0 + c >= g.v) return;
-    const float f = g.scales[2] / kDz;
     if (k < g.e) {
         if (!g.dw) return;
-        const float s = sum_parts(g.slabs + k * g.ldo + c, g.nz, g.slab) * f / g.scales[1];
+        const float s = ldexpf(sum_parts(g.slabs + k * g.ldo + c, g.nz, g.slab), g.exps[1] - 280);
         float* d = g.dw + k * g.v + g.c0 + c;
         *d = g.accumulate ? *d + s : s;
     } else if (g.db) {
-        const float s = sum_parts(g.slabs_b + c, g.nz, g.ldo) * f;
+        const float all = sum_parts(g.slabs_b + c, g.nz, g.ldo), s = g.wide ? ldexpf(all, g.exps[2] - 140) : all;
         float* d = g.db + g.c0 + c;
         *d = g.accumulate ? *d + s : s;
     }
@@ -1329,7 +1368,7 @@ __global__ __launch_bounds__(1024) void xent_rows_dx_kernel(const float* __restr
 
 // ---------------------------------------------------------------- a block of rows
 // Up to 128 rows (RB blocks of 32) W and dW are still what a call moves, but the products belong on the matrix pipe: float32
-// instructions on W as it lies in memory, no scales and no planes.  A block of rows needs 64 cycles of a SIMD for every 64 values
+// instructions on W as it lies in memory, no powers of two and no planes.  A block of rows needs 64 cycles of a SIMD for every 64 values
 // of W and product: with one block the four SIMDs of a CU would take 16 bytes of W a cycle, 8 TB/s over the chip.
 //   logits: a workgroup takes 32 classes, its waves a quarter of the features each; W goes from memory to the A fragments (a lane a
 //       class), x comes transposed from the cache.  Forward: (maximum, sum) per row; backward: dz (rows x classes) and db.
@@ -1808,7 +1847,7 @@ struct Layout {
     int rows_wg;                   // resident rows of a workgroup (FWD, DX)
     int64_t np, vp, ep, vc, nz, nf, nx;      // nf, nx, nz: parts of the streamed operand in FWD, DX, DW (nz: of the rows in general)
     int64_t vm;                    // classes of a piece whose dW is not split, before the ones whose dW has nz parts
-    int64_t part, bias, scales, lab, zlab, row, rs, ones, xh, xl, xsh, xsl, wh, wl, slices, dzh, dzl, dxw, slabs, slabs_b, total;
+    int64_t part, bias, exps, rmax, lab, zlab, row, ones, xh, xl, xsh, xsl, wh, wl, slices, dzh, dzl, dxw, slabs, slabs_b, total;
 };
 
 Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
@@ -1851,7 +1890,9 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
         return o;
     };
     l.part = take(3 * kMaxParts * 4);
-    l.scales = take(16);
+    l.exps = take(16);
+    l.rmax = take(l.np * 4);
+    l.row = take(l.np * 16);
     l.bias = take(l.vp * 4);
     l.lab = take(l.np * 4);
     l.xh = take(l.np * l.ep * 2);
@@ -1863,14 +1904,11 @@ Layout layout(int64_t n, int64_t e, int64_t v, bool xf32, bool backward) {
         if (!l.narrow) l.nf = l.vp / 64;
         l.slices = take(l.np * l.nf * 8);
     } else if (l.narrow) {
-        l.row = take(l.np * 8);
         l.vc = l.vp;
         l.dxw = take(l.nx * l.np * l.ep * 4);
         l.slabs = l.nz > 1 ? take(l.nz * l.ep * l.vp * 4) : 0;
         l.slabs_b = l.nz > 1 ? take(l.nz * l.vp * 4) : 0;
     } else {
-        l.row = take(l.np * 8);
-        l.rs = take(l.np * 4);
         l.ones = take(l.np * 2);
         l.xsh = take(l.np * l.ep * 2);
         l.xsl = xf32 ? take(l.np * l.ep * 2) : 0;
@@ -1944,7 +1982,7 @@ void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const floa
     while (lsh < 6 && (4 << lsh) < cols) ++lsh;
     auto largest = [&](auto f32_, auto vec_, auto wvec_) {
         hipLaunchKernelGGL((xent_max_kernel<decltype(f32_)::value, decltype(vec_)::value, decltype(wvec_)::value>), dim3((unsigned)parts),
-                           dim3(256), 0, st, w, b, x, (long)n, (int)e, labels, (long)v, lsh, dloss, part);
+                           dim3(256), 0, st, w, b, x, (long)n, (int)e, labels, (long)v, lsh, dloss, part, (unsigned*)(ws + l.rmax));
     };
     const std::true_type yes;
     const std::false_type no;
@@ -1955,10 +1993,10 @@ void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const floa
     p.x = x; p.w = w; p.b = b; p.lse = lse; p.dloss = dloss; p.labels = labels; p.part = part; p.parts = (int)parts;
     p.n = n; p.v = v; p.np = l.np; p.vp = l.vp; p.e = (int)e; p.ep = (int)l.ep;
     p.xh = (f16_t*)(ws + l.xh); p.xl = (f16_t*)(ws + l.xl); p.wh = (f16_t*)(ws + l.wh); p.wl = (f16_t*)(ws + l.wl);
-    p.bias = (float*)(ws + l.bias); p.scales = (float*)(ws + l.scales); p.lab = (int*)(ws + l.lab);
-    p.row = dloss ? (float2*)(ws + l.row) : nullptr;
+    p.bias = (float*)(ws + l.bias); p.exps = (int*)(ws + l.exps); p.rmax = (unsigned*)(ws + l.rmax); p.lab = (int*)(ws + l.lab);
+    p.row = (f32x4*)(ws + l.row);
     if (dloss && !l.narrow) {
-        p.rs = (float*)(ws + l.rs); p.ones = (f16_t*)(ws + l.ones); p.xsh = (f16_t*)(ws + l.xsh); p.xsl = (f16_t*)(ws + l.xsl);
+        p.ones = (f16_t*)(ws + l.ones); p.xsh = (f16_t*)(ws + l.xsh); p.xsl = (f16_t*)(ws + l.xsl);
     }
     p.wtiles = (l.vp / 64) * (l.ep / 64);
     p.xblocks = up(l.np * l.ep / 8, 256) / 256;
@@ -1968,7 +2006,7 @@ void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const floa
     else hipLaunchKernelGGL(xent_prep_kernel<false>, grid, dim3(256), 0, st, p);
 }
 
-// dx from its parts (scales NULL: they are dx itself, not the streamed or the wide products' planes), together with dW from its slabs
+// dx from its parts (exps NULL: they are dx itself, not of the streamed or the wide products' planes), together with dW from its slabs
 // where both remain to be done
 void launch_joins(const XentDxJoin* j, const XentDwReduce* g, hipStream_t st) {
     // sixteen groups of parts: 200 x 128 x 65536 94.8 us a backward against 101.3 with one, 53 x 75 x 25145 56.4 against 61.3; with the
@@ -2056,7 +2094,7 @@ void short_backward(const XentShort& g, void* dx, bool xf32, int64_t parts, hipS
     if (dx) {
         if (g.v % 4 == 0) launch_short_dx<RB, true>(g, parts, st);
         else launch_short_dx<RB, false>(g, parts, st);
-        const XentDxJoin j = {g.dxp, nullptr, nullptr, nullptr, dx, (int)xf32, (int)parts, (long)g.np * g.ep, (long)g.n, g.e, g.ep};
+        const XentDxJoin j = {g.dxp, nullptr, nullptr, false, dx, (int)xf32, (int)parts, (long)g.np * g.ep, (long)g.n, g.e, g.ep};
         launch_joins(&j, nullptr, st);
     }
     if (g.dw) {
@@ -2153,12 +2191,12 @@ extern "C" int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, c
     XentGemm g = {};
     g.a[0] = (f16_t*)(ws + l.wh); g.a[1] = (f16_t*)(ws + l.wl); g.b[0] = (f16_t*)(ws + l.xh); g.b[1] = (f16_t*)(ws + l.xl);
     g.lda = g.ldb = l.ep; g.kiters = (int)(l.ep / BK);
-    g.bias = (float*)(ws + l.bias); g.scales = (float*)(ws + l.scales); g.lab = (int*)(ws + l.lab);
+    g.bias = (float*)(ws + l.bias); g.row = (f32x4*)(ws + l.row); g.lab = (int*)(ws + l.lab);
     g.part = (float2*)(ws + l.slices); g.zlab = (float*)(ws + l.zlab); g.np = l.np;
     if (l.narrow) {
         XentStream q = {};
         q.r[0] = g.b[0]; q.r[1] = g.b[1]; q.s[0] = g.a[0]; q.s[1] = g.a[1];
-        q.scales = g.scales; q.bias = g.bias; q.lab = g.lab; q.tiles = (int)(l.vp / ST);
+        q.row = g.row; q.bias = g.bias; q.lab = g.lab; q.tiles = (int)(l.vp / ST);
         q.part = g.part; q.zlab = g.zlab; q.ld = l.np;
         if (xf) launch_stream<2, 2, 1, MODE_FWD, 2>(l, q, l.np / l.rows_wg, l.nf, st);
         else launch_stream<1, 2, 2, MODE_FWD, 2>(l, q, l.np / l.rows_wg, l.nf, st);
@@ -2209,8 +2247,8 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
     f16_t *xh = (f16_t*)(ws + l.xh), *xl = (f16_t*)(ws + l.xl), *dzh = (f16_t*)(ws + l.dzh), *dzl = (f16_t*)(ws + l.dzl);
     if (l.narrow) {
         XentStream q = {};
-        q.scales = (float*)(ws + l.scales); q.bias = (float*)(ws + l.bias); q.lab = (int*)(ws + l.lab);
-        q.row = (float2*)(ws + l.row);
+        q.exps = (int*)(ws + l.exps); q.bias = (float*)(ws + l.bias); q.lab = (int*)(ws + l.lab);
+        q.row = (f32x4*)(ws + l.row);
         f16_t *wh = (f16_t*)(ws + l.wh), *wl = (f16_t*)(ws + l.wl);
         if (dx) {
             q.r[0] = xh; q.r[1] = xl; q.s[0] = wh; q.s[1] = wl;
@@ -2218,7 +2256,7 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
             if (xf) launch_stream<2, 2, 1, MODE_DX, 2>(l, q, l.np / l.rows_wg, l.nx, st);
             else launch_stream<1, 2, 2, MODE_DX, 1>(l, q, l.np / l.rows_wg, l.nx, st);
         }
-        const XentDxJoin j = {(float*)(ws + l.dxw), q.scales, q.row, nullptr, dx, (int)xf, (int)l.nx, (long)(l.np * l.ep), (long)n, (int)e,
+        const XentDxJoin j = {(float*)(ws + l.dxw), q.exps, q.row, false, dx, (int)xf, (int)l.nx, (long)(l.np * l.ep), (long)n, (int)e,
                               (int)l.ep};
         if (dw || db) {
             q.r[0] = wh; q.r[1] = wl; q.s[0] = xh; q.s[1] = xl;
@@ -2227,29 +2265,28 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
             if (xf) launch_stream<2, 2, 1, MODE_DW, 2>(l, q, l.vp / 128, l.nz, st);
             else launch_stream<2, 1, 1, MODE_DW, 2>(l, q, l.vp / 128, l.nz, st);
         }
-        const XentDwReduce s = {q.out, q.outb, q.scales, dw, db, (int)l.nz, (long)(l.ep * l.vp), (long)l.vp, (int)e, (long)v, 0L, (long)l.vp,
+        const XentDwReduce s = {q.out, q.outb, q.exps, false, dw, db, (int)l.nz, (long)(l.ep * l.vp), (long)l.vp, (int)e, (long)v, 0L, (long)l.vp,
                                 accumulate};
         const bool slabs = (dw || db) && l.nz > 1;
         if (dx || slabs) launch_joins(dx ? &j : nullptr, slabs ? &s : nullptr, st);
         return mgx_launch_status();
     }
-    const XentDxJoin join = {(float*)(ws + l.dxw), (float*)(ws + l.scales), nullptr, (float*)(ws + l.rs), dx, (int)xf, (int)l.nx,
+    const XentDxJoin join = {(float*)(ws + l.dxw), (int*)(ws + l.exps), (f32x4*)(ws + l.row), true, dx, (int)xf, (int)l.nx,
                              (long)(l.np * l.ep), (long)n, (int)e, (int)l.ep};
     bool joined = false;
     for (int64_t c0 = 0; c0 < l.vp; c0 += l.vc) {
         const int64_t cnt = l.vp - c0 < l.vc ? l.vp - c0 : l.vc;
         f16_t *wh = (f16_t*)(ws + l.wh) + c0 * l.ep, *wl = (f16_t*)(ws + l.wl) + c0 * l.ep;
         XentGemm g = {};
-        g.scales = (float*)(ws + l.scales);
+        g.exps = (int*)(ws + l.exps);
         g.a[0] = wh; g.a[1] = wl; g.b[0] = xh; g.b[1] = xl;
         g.lda = g.ldb = l.ep; g.kiters = (int)(l.ep / BK);
-        g.bias = (float*)(ws + l.bias) + c0; g.lab = (int*)(ws + l.lab); g.row = (float2*)(ws + l.row);
+        g.bias = (float*)(ws + l.bias) + c0; g.lab = (int*)(ws + l.lab); g.row = (f32x4*)(ws + l.row);
         g.dzh = dzh; g.dzl = dzl; g.ldo = l.vc; g.np = l.np; g.class0 = c0;
         if (xf) launch_gemm<2, 2, false, false, EPI_DZ, 4>(g, cnt, l.np, 1, st);
         else launch_gemm<2, 1, false, false, EPI_DZ, 4>(g, cnt, l.np, 1, st);
         if (dx) {
             XentGemm q = {};
-            q.scales = g.scales;
             q.a[0] = dzh; q.a[1] = dzl; q.b[0] = wh; q.b[1] = wl;
             q.lda = l.vc; q.ldb = l.ep; q.kiters = (int)(cnt / BK);
             q.out = (float*)(ws + l.dxw); q.ldo = l.ep; q.np = l.np; q.class0 = c0;
@@ -2262,7 +2299,7 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
                 if (a0 >= a1) return;
                 const int64_t vs = l.vc - l.vm, first = c0 + a0;
                 XentGemm q = {};
-                q.scales = g.scales;
+                q.exps = g.exps;
                 q.a[0] = (f16_t*)(ws + l.xsh); q.a[1] = (f16_t*)(ws + l.xsl); q.b[0] = dzh + a0; q.b[1] = dzl + a0;
                 q.ones = (f16_t*)(ws + l.ones);
                 q.lda = l.ep; q.ldb = l.vc; q.kiters = (int)(l.np / BK);
@@ -2272,7 +2309,7 @@ extern "C" int mgx_dense_xent_bwd(const void* x, int x_is_f32, const float* w, c
                 if (xf) launch_gemm<2, 2, true, true, EPI_DW, 2>(q, l.ep, a1 - a0, nz, st);
                 else launch_gemm<1, 2, true, true, EPI_DW, 2>(q, l.ep, a1 - a0, nz, st);
                 if (nz == 1) return;
-                const XentDwReduce s = {q.out, q.outb, g.scales, dw, db, (int)nz, (long)q.np, (long)vs, (int)e, (long)v, (long)first, (long)(a1 - a0),
+                const XentDwReduce s = {q.out, q.outb, g.exps, true, dw, db, (int)nz, (long)q.np, (long)vs, (int)e, (long)v, (long)first, (long)(a1 - a0),
                                         accumulate};
                 const bool last = dx && c0 + cnt == l.vp;            // dx is complete with the last piece
                 launch_joins(last ? &join : nullptr, &s, st);

@@ -135,6 +135,31 @@ def test_weights_of_any_size(size, n, e, v, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,e,v", [f for f in FORMS if f[0] > 16])
+@pytest.mark.parametrize("large", [1e6, 1e8])
+def test_rows_of_very_different_size(large, n, e, v, dtype):
+    """One labelled row has features `large` times the others', one as much smaller ones: no other row's loss or dx loses digits.
+    With a weight of zero at the large row, neither do dw and db."""
+    x, w, b, labels, dloss = case(n, e, v, dtype, seed=150 + e, unlabelled=0)
+    k = n // 2
+    x[k] *= large
+    x[3] /= large
+    rest = torch.arange(n) != k
+    unit, off = row_bounds(x, w, b, labels, dloss, dtype)
+    want, got = reference(x, w, b, labels, dloss), run(x, w, b, labels, dloss)
+    for name in ("loss", "lse"):
+        short = (got[name].double() - want[name]).abs() / (unit + 2.0 ** -23 * want[name].abs())
+        assert float(short.max()) <= 1.0, (name, float(short.max()))
+    short = ((got["dx"].double() - want["dx"]).norm(dim=1) / off)[rest]
+    assert float(short.max()) <= 1.0, float(short.max())
+    assert all(bool(got[name].isfinite().all()) for name in ("dx", "dw", "db"))
+    dloss[k] = 0.0
+    want, got = reference(x, w, b, labels, dloss), run(x, w, b, labels, dloss)
+    gradients_close(got, want, float(unit[rest].max()), dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("n,e,v", FORMS)
 def test_logits_beyond_the_digits_of_lse(n, e, v, dtype):
     """Logits around 1e8, where lse, a float32, is known to a few units only: no probability comes out above 1, and
