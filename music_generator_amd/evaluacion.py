@@ -44,6 +44,8 @@ class SoftmaxDense(Dense):
         features beside them (the 9 classes of define_evaluator on 384 000 features): then storing them costs nothing."""
         x = features.reshape(-1, self.cin)
         n = x.shape[0]
+        if labels.numel() != n:
+            raise ops.MgxError("%s: %d class numbers for %d rows of features" % (self.name, labels.numel(), n))
         labelled = (labels >= 0) & (labels < self.units)
         count = labelled.sum().float()
         if self.units <= self.cin and features.dim() == 2:

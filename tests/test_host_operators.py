@@ -84,3 +84,19 @@ def test_dense_xent(lib, n, e, v):
         refuse(lib.mgx_dense_xent_bwd, bwd, [{k: None} for k in ("x", "w", "labels", "lse", "dloss", "ws")]
                + [dict(x=P + 8), dict(w=P + 4), dict(ws=P + 4)], _cabi.MGX_ERR_ARG)
         refuse(lib.mgx_dense_xent_bwd, bwd, [dict(bytes=bwd["bytes"] - 1), dict(bytes=0)], _cabi.MGX_ERR_WORKSPACE)
+
+
+@pytest.mark.parametrize("rows,numbers", [(1, 10), (1, 0), (4, 1), (4, 40), (4, 5)])
+@pytest.mark.parametrize("units,cin", [(9, 64), (80, 64)])
+def test_class_numbers_of_another_count(rows, numbers, units, cin):
+    """One class number for each row of features, for heads that store their logits and heads that do not: integer rows that are
+    no one-hot rows of the model's classes must not be read as class numbers of other rows."""
+    import torch
+
+    from music_generator_amd.evaluacion import SoftmaxDense
+    head = SoftmaxDense(units)
+    head.cin = cin
+    for features in (torch.zeros((rows, cin)), torch.zeros((rows, 1, 1, cin))):
+        for backward in (False, True):
+            with pytest.raises(_cabi.MgxError, match="class numbers"):
+                head.loss(features, torch.zeros((numbers,), dtype=torch.int32), backward)
