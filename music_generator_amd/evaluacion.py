@@ -55,11 +55,13 @@ class SoftmaxDense(Dense):
         ops.dense_xent_fwd(x, w, b, labels, loss, lse, hits)
         dx = None
         if backward:
-            if self.kernel.grad is None or self.bias.grad is None:
-                raise RuntimeError("gradient buffers of %s are not bound" % self.name)
+            dw = db = None                               # a frozen head passes the gradient on
+            if self.trainable:
+                if self.kernel.grad is None or self.bias.grad is None:
+                    raise RuntimeError("gradient buffers of %s are not bound" % self.name)
+                dw, db = self.kernel.grad.view(self.cin, self.units), self.bias.grad
             dx = torch.empty_like(x)
-            ops.dense_xent_bwd(x, w, b, labels, lse, labelled.float() / count.clamp(min=1.0), dx,
-                               self.kernel.grad.view(self.cin, self.units), self.bias.grad, accumulate=True)
+            ops.dense_xent_bwd(x, w, b, labels, lse, labelled.float() / count.clamp(min=1.0), dx, dw, db, accumulate=True)
             dx = dx.view(features.shape)
         return loss.sum(), hits.sum(), count, dx
 
