@@ -363,7 +363,8 @@ class Model:
             half = bf and conv and shape[1] >= K.BF16_MIN_ROWS and shape[-1] in (32, 128)
             copies = 2 if (op.act_node is not None and (not half or K.BF16_SAVE_DERIVATIVE)) else 1
             if conv and K.TAPE8 and shape[-1] % 32 == 0:
-                total += -(-elems // 32) * 33 * copies
+                kept = -(-elems // 32) * 33
+                total += kept + (copies - 1) * (elems * 2 if half else kept)      # a saved bf16 derivative stays what it is
                 continue
             total += elems * (2 if half else 4) * copies
         return int(total) * int(n)

@@ -100,3 +100,24 @@ def test_class_numbers_of_another_count(rows, numbers, units, cin):
         for backward in (False, True):
             with pytest.raises(_cabi.MgxError, match="class numbers"):
                 head.loss(features, torch.zeros((numbers,), dtype=torch.int32), backward)
+
+
+@pytest.mark.parametrize("precision", ["float32", "bfloat16"])
+def test_tape_estimate_of_saved_derivatives(precision):
+    """The 8-bit tape leaves saved bf16 derivatives in bf16: they cost the same with it and without."""
+    import music_generator_amd as M
+    model = M.define_discriminator(3)[2][0]
+    M.backend.set_precision(precision)
+    try:
+        cost = []
+        for tape8 in (False, True):
+            M.backend.TAPE8 = tape8
+            each = []
+            for derivative in (False, True):
+                M.backend.BF16_SAVE_DERIVATIVE = derivative
+                each.append(model.tape_bytes_estimate(2))
+            cost.append(each[1] - each[0])
+        assert cost[0] == cost[1] and (cost[0] > 0) == (precision == "bfloat16")
+    finally:
+        M.backend.TAPE8 = M.backend.BF16_SAVE_DERIVATIVE = False
+        M.backend.set_precision("float32")
