@@ -282,6 +282,9 @@ struct FGeo {
     static constexpr int LDS = 2 * (GPIX + NCH * XPIX) * 64;
 };
 
+// Four floats of a slab: the caller's workspace is aligned as its floats are.
+typedef float f32x4_slab __attribute__((ext_vector_type(4), aligned(4)));
+
 __device__ __forceinline__ int sw_off(int p, int c16) { return p * 64 + ((c16 ^ ((p >> 2) & 3)) << 4); }
 
 // X8: X is the 8-bit tape of the layer input (tape8.h), x its codes and xe its exponent bytes: 33 instead of 64 bytes
@@ -598,7 +601,7 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const voi
         for (int a = 0; a <= TAPS; ++a)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                *(f32x4*)(dst + (a * 4 + q) * 256) = (f32x4){acc[a][4 * q], acc[a][4 * q + 1], acc[a][4 * q + 2], acc[a][4 * q + 3]};
+                *(f32x4_slab*)(dst + (a * 4 + q) * 256) = (f32x4){acc[a][4 * q], acc[a][4 * q + 1], acc[a][4 * q + 2], acc[a][4 * q + 3]};
         return;
     }
     // ---- add the four waves in fixed order: (w0 + w2) + (w1 + w3), through LDS, four registers an access (this code runs once,
@@ -641,7 +644,7 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const voi
                 f32x4 v = red[(a * 4 + q) * 64];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] += acc[a][4 * q + i];
-                *(f32x4*)(dst + (a * 4 + q) * 256) = v;
+                *(f32x4_slab*)(dst + (a * 4 + q) * 256) = v;
             }
     }
 }
