@@ -194,9 +194,10 @@ __device__ __forceinline__ float row_loss(float m, float ls, float z, float bias
     return bias < kLowest * kLn2 ? (m + ls) * kLn2 - bias : ((m - z) + ls) * kLn2;
 }
 
-// lse in units of log 2 for the backward, which takes exp2(z - lse).  From 2^21 on lse's and z's roundings are worth a unit and more:
-// lse is raised by what they may come to, so that no probability is above 1 (one that overflows the fp16 planes would make
-// the gradient of W infinite for every row).
+// lse in units of log 2 for the backward, which takes exp2(z - lse) of the forward's z, bit for bit.  Between the two lse has been
+// rounded a few times, 2^-22 of it: from 2^21 on that is worth a good part of a unit and more, and lse is raised by 2^-20, so
+// that no probability is above 1 (one that overflows the fp16 planes would make the gradient of W infinite for every
+// row).
 __device__ __forceinline__ float lse_units(float lse) {
     const float l = lse * kLog2e;
     return fabsf(l) >= 0x1p21f ? __builtin_fmaf(fabsf(l), 0x1p-20f, l) : l;
@@ -671,6 +672,9 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     constexpr int KS = EP / 16, EB = EP / 32, ROWB = EP * 2, SPLANE = ST * ROWB;
     constexpr int BUF = NS * SPLANE + 1024;
+    // Plane of unit si of S.  The products of a logit are added in one order in every mode (x lo W hi, x hi W hi, x hi W lo): the backward
+    // meets the bits of the forward's logits, so that exp(z - lse) is above 1 by the rounding of lse only, whatever the terms cancel.
+    constexpr auto s_plane = [](int si) constexpr { return MODE == MODE_DW ? NS - 1 - si % NS : si % NS; };
     constexpr int NP = MODE == MODE_DW ? 2 : NR;    // planes of P: DX of a bf16 x needs one (its result is rounded to 8 bits)
     constexpr int NA = MODE == MODE_DW ? NS : NR;   // planes of the streamed operand in the second product
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -797,7 +801,7 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                         fr[u % 3] = (u32x4){a0[0], a0[1], a1[0], a1[1]};
                     }
                 } else if constexpr (DO_S) {
-                    constexpr int si = u - gc, ks = si / NS, pl = NS - 1 - si % NS;
+                    constexpr int si = u - gc, ks = si / NS, pl = s_plane(si);
                     fr[u % 3] = *(const u32x4*)(ts + pl * SPLANE + (ao ^ (ks << 5)));
                 }
             }
@@ -814,11 +818,12 @@ __global__ __launch_bounds__(256, OCC) void xent_stream_kernel(XentStream g) {
                     }
                 }
             } else if constexpr (DO_S) {
-                constexpr int si = u - gc, ks = si / NS, pl = NS - 1 - si % NS;
+                constexpr int si = u - gc, ks = si / NS, pl = s_plane(si);
 #pragma unroll
                 for (int b = 0; b < RB; ++b) {
-                    if constexpr (NR > 1 && pl == 0) nxt[b] = mfma_f16(fr[u % 3], fb[NR - 1][b][ks], nxt[b]);
+                    if constexpr (MODE != MODE_DW && NR > 1 && pl == 0) nxt[b] = mfma_f16(fr[u % 3], fb[NR - 1][b][ks], nxt[b]);
                     nxt[b] = mfma_f16(fr[u % 3], fb[0][b][ks], nxt[b]);
+                    if constexpr (MODE == MODE_DW && NR > 1 && pl == 0) nxt[b] = mfma_f16(fr[u % 3], fb[NR - 1][b][ks], nxt[b]);
                 }
             }
         };

@@ -171,3 +171,21 @@ def test_logits_beyond_the_digits_of_lse(n, e, v, dtype):
     assert all(bool(got[name].isfinite().all()) for name in ("loss", "lse", "dx", "dw", "db"))
     # |dz| of a row sums to 2 at most
     assert float(got["db"].abs().sum()) <= 2.001 * float(dloss.sum())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,e,v", FORMS)
+def test_logits_that_are_all_cancellation(n, e, v, dtype):
+    """Features of 1e9 against columns of W whose halves cancel to the last digits: what is left of the logits are the roundings
+    of terms a billion times larger.  The backward meets the forward's logits again: its probabilities sum to 1 and stay finite."""
+    x, w, b, labels, dloss = case(n, e, v, dtype, seed=170 + e, unlabelled=0)
+    half = e // 2
+    x[:, :half] = (x[:, :half].float() * 1e9).to(dtype)
+    x[:, half:] = -x[:, :half]
+    w[half:] = w[:half] * (1.0 + 2.0 ** -22 * torch.randint(-1, 2, w[:half].shape, generator=torch.Generator().manual_seed(2)))
+    got = run(x, w, b, labels, dloss)
+    assert all(bool(got[name].isfinite().all()) for name in ("loss", "lse", "dx", "dw", "db"))
+    # a row's dz sums to 0 but for the rounding of lse, 2^-22 of it, and the 11 and 22 bits of the planes in front of a float32 sum
+    assert abs(float(got["db"].double().sum())) <= (2.0 ** -20 * float(got["lse"].abs().max()) + 2.0 ** -18) * float(dloss.sum())
+    assert float(got["db"].abs().sum()) <= 2.001 * float(dloss.sum())
