@@ -546,10 +546,12 @@ int64_t mgx_tape8_blocks(int64_t n);
 int mgx_tape8_pack(const void* x, int x_is_f32, void* codes, void* exps, int64_t n, void* stream);
 int mgx_tape8_unpack(const void* codes, const void* exps, void* y, int y_is_f32, int64_t n, void* stream);
 /* out (bf16) = a (bf16 or float32) * f'(y): y the kept output of tanh(v) + v / act_alpha, f' = max(1 + 1/act_alpha - y^2,
- * 1/act_alpha) recovered from it (mgx_mul_dact_bf16 reads a bf16 y). */
+ * 1/act_alpha) recovered from it (mgx_mul_dact_bf16 reads a bf16 y).  Off by up to 2 H^2 / 256 with the kept value: a saturated y = +-1
+ * stands for +-255/256, whose f' is 0.0078 where the unit's own is 1/act_alpha. */
 int mgx_mul_dact_tape8(const void* a, int a_is_f32, const void* codes, const void* exps, float act_alpha, void* out,
                        int64_t n, void* stream);
-/* mgx_conv_bwd_bf16 (same descriptors and workspace) with the layer input read from the 8-bit tape. */
+/* mgx_conv_bwd_bf16 (same descriptors and workspace) with the layer input read from the 8-bit tape.  As there, the data gradient
+ * takes w rounded to bf16 (2^-8 of a weight at most); codes, g, w and dx are 16-byte aligned. */
 int mgx_conv_bwd_tape8(const mgx_conv_desc* d, const void* codes, const void* exps, const void* g, const float* w,
                        float* dw, float* dbias, void* dx, float act_alpha, void* workspace, int64_t workspace_bytes,
                        void* stream);
@@ -566,13 +568,14 @@ int mgx_conv_bwd_tape8(const mgx_conv_desc* d, const void* codes, const void* ex
  * masks a class: its probability is 0 and its column of w is not used (one class at least is not masked; a row whose label is
  * masked has the loss of that bias).  Any of dx, dw, db may be NULL.  n <= 8 000 000, v <= 8 000 000, e <= 65 000; x, w
  * and the workspace 16-byte aligned; the workspace (mgx_dense_xent_workspace bytes, -1: sizes out of range) is the call's alone while it
- * runs.  float32 quality: the products are sums of products of fp16 halves of the operands, or in float32 where rows are few.  The
- * halves hold 22 bits of what is above 2^-17 of the largest magnitude in the row of x, or in the unmasked classes of w, and
- * the rest to 2^-39 of it: rows do not depend on each other's size; a class whose column of w is far smaller than another's
- * has its logits to 2^-39 of the larger one's terms.  In dw, terms are counted from the largest |dloss_i| max_k |x_ik| in the same
- * way.  The backward's probabilities are relative to lse, a float32: 2^-23 |lse| of themselves off, and from
- * |lse| = 1.4e6 on known to a factor only, but never above 1.  A bf16 dx is within 2^-10 of sum_j |dz_ij w_kj| before it
- * is rounded.
+ * runs.  lse is the forward's for the same x, w, b and labels.
+ * float32 quality: the products are sums of products of fp16 halves of the operands, or in float32 where rows are few.  The halves
+ * hold 22 bits of what is above 2^-16 of the largest magnitude in its row of x, or in the unmasked classes of w, and the rest
+ * to 2^-38 of that.  So rows do not depend on each other's size, but a class whose column of w is 2^16 times smaller than
+ * another's has fewer digits.  The terms of dw are held in the same way, counted from the largest |dloss_i| max_k |x_ik|.
+ * The backward's probabilities are exp(z - lse) of the forward's logits and carry the rounding of lse, a float32: 2^-22 |lse| of
+ * themselves, so that with logits beyond 10^6 they are known to a factor only (never above 1).  A bf16 dx is within 2^-10 of
+ * sum_j |dz_ij w_kj| before it is rounded.
  * ---------------------------------------------------------------------------------------- */
 int64_t mgx_dense_xent_workspace(int64_t n, int64_t e, int64_t v, int x_is_f32, int backward);
 int mgx_dense_xent_fwd(const void* x, int x_is_f32, const float* w, const float* b, const int32_t* labels, float* loss,

@@ -139,8 +139,9 @@ BF16_SAVE_DERIVATIVE = False
 BF16_FUSED_CONV_BACKWARD = os.environ.get("MGX_FUSED_CONV_BWD", "1") != "0"
 # Taped forwards of a layer-by-layer plan keep the inputs of contractions and of the fade-in blend (tensors of whole blocks of
 # 32 channels) in 8 bits (ops.tape8_pack: 33 bytes per 32 values instead of 64 in bf16, 128 in float32); the backward
-# reads the bytes.  Forward results do not change; gradients are those of activations rounded to 8 bits.  The fused
-# generator blocks keep their own tape (GBLOCK_LEAN_TAPE).
+# reads the bytes.  Forward results do not change; gradients are those of activations rounded to 8 bits: the derivative of
+# a saturated unit (1/alpha) is taken for 0.0078 (0.0039 in float32 layers), so gradients through layers that are
+# mostly saturated are too large, always to the same side.  The fused generator blocks keep their own tape (GBLOCK_LEAN_TAPE).
 TAPE8 = os.environ.get("MGX_TAPE8", "0") != "0"
 # bf16 generator grow blocks: leave the outputs of the Conv2DTranspose(64) / Dense(256) layers and the gradients
 # arriving at them off the tape (5120 of its 8138 rows per 32 positions); the weight-gradient kernels recompute

@@ -289,7 +289,7 @@ __device__ __forceinline__ int sw_off(int p, int c16) { return p * 64 + ((c16 ^ 
 
 // X8: X is the 8-bit tape of the layer input (tape8.h), x its codes and xe its exponent bytes: 33 instead of 64 bytes
 // are read per 32 channels.  A thread loads the eight codes of a 16-byte piece and turns them into the piece between the
-// MFMAs of the tile before; everything behind the staging is the same.  3x3, 256 x 48000: 632 us (0.72 PFLOP/s, 3.1 TB/s), 629 from
+// MFMAs of the tile before; everything behind the staging is the same.  3x3, 256 x 48000: 645 us (0.70 PFLOP/s, 3.0 TB/s), 629 from
 // bf16: at one wave a SIMD the kernel is bound by its own instruction order, so the bytes saved are memory, not time; with the
 // conversion in front of the MFMAs it took 70 us more.
 template <int KH, int KW, bool ACT, int CIN, bool X8>
@@ -416,6 +416,9 @@ __global__ __launch_bounds__(256, 1) void bbwd_kernel(mgx_conv_desc d, const voi
     };
 
     // weights W[tap][ci][co] (Keras layout, co fastest) as A fragments of the data gradient: lane (ci, h), k = co
+    // Rounded to bf16 (2^-8 of a weight at most) as in the forward's kernels: both operands of a bf16 matrix instruction are bf16, and
+    // a second plane of weights would double the data gradient's.  dX against float32 weights is off by 2.4e-3 of its
+    // norm, of which the rounding of the result alone is 1.7e-3.
     u32x4 wf[TAPS][2];
 #pragma unroll
     for (int tap = 0; tap < TAPS; ++tap)

@@ -12,7 +12,10 @@
 //     within half a step (H / 256; bf16 itself is H / 512 off in the upper half of the range), one above H within a
 //     whole one.  With a code point on zero
 //     the 256 codes would reach -1 but only 127 / 128 on the other side, and the derivative 1 - y^2 recovered from the
-//     two ends would differ.  The price: a zero in a block that is not all zeros comes back as half a step.
+//     two ends would differ.  The price: a zero in a block that is not all zeros comes back as half a step, and a saturated
+//     unit's +-1 as +-255/256, so that no derivative recovered in a block that reaches 1 is under 1 - (255/256)^2 = 0.0078
+//     where the unit's own is 1/alpha (0.00005): gradients through saturated units come out too large, by 0.0078 of the
+//     arriving gradient.  A float32 layer keeps its derivative itself in this form: 0.0039 there.
 //   - e = 0 is a block of zeros, which comes back as zeros; e = 255 a block that held an infinity or a NaN, which comes
 //     back as NaN throughout (nothing non-finite is hidden from the gradients).
 #pragma once

@@ -21,13 +21,14 @@
 //   few rows (up to 4, up to 16 of a small W): launches and HBM (W read twice, dW written), float32 on the vector ALU.
 //     1 x 128 x 4097 15 + 17, 4 x 128 x 65536 15 + 42.
 //   a block of rows (up to 64, 128 of a large W): HBM up to 32 rows (a kernel each for the logits, dx and dW, 4.4 to 4.9 TB/s at 32 x
-//     1000 x 65536; a large copy reaches 4.75), the float32 matrix instructions beyond (64 x 1000 x 65536 96 + 265).
-//   e <= 128: the matrix pipe, streamed, dz never stored.  24000 x 128 x 65536 bf16: 725 + 2090 (the three products 0.78, 0.92
-//     and 1.45 ms, 1.0 to 1.1 PFLOP/s of fp16 products; a large library product reaches 1.22).  The form below takes 1400 + 6116 for
-//     it, and 1720 + 7494 against 1049 + 3722 for float32 features; at 3000 x 128 x 8192 bf16 40 + 103 against 41 + 89.
-//   e > 128: the matrix pipe, tiled products with dz in planes of 128 MB a piece.  1501 x 1000 x 10001 float32: 470 in all, of which
-//     the four products (0.97 PFLOP/s) take 415.
-// Up to 64 features the streamed kernels have a form of 64 (24000 x 32 x 65536 bf16: 420 + 1135 against 622 + 1770 us).
+//     1000 x 65536; a large copy reaches 4.75), the float32 matrix instructions beyond (64 x 1000 x 65536 94 + 260).
+//   e <= 128: the matrix pipe, streamed, dz never stored.  24000 x 128 x 65536 bf16: 780 + 2490 (the three products 0.72, 1.11
+//     and 1.35 ms, 1.1 to 1.2 PFLOP/s of fp16 products; a library product of 8192^3 reaches 1.22).  The form below takes 1450 +
+//     5920 for it, and 1725 + 7320 against 1090 + 3910 for float32 features (products at 1.1 to 1.23); at 3000 x 128 x 8192 bf16
+//     41 + 100 against 42 + 92.
+//   e > 128: the matrix pipe, tiled products with dz in planes of 128 MB a piece.  1501 x 1000 x 10001 float32: 132 + 346, of which
+//     the four products (0.93 PFLOP/s) take 390; bf16 106 + 254.
+// Up to 64 features the streamed kernels have a form of 64 (24000 x 32 x 65536 bf16: 440 + 1340 against 680 + 2110 us).
 //
 // A row whose label lies outside [0, v) has no loss: loss 0, lse 0, gradient 0 and nothing of its features is read into
 // a product (they may hold anything).  A class masked with a bias of -inf or the lowest float has a probability of 0, and its column
@@ -2014,8 +2015,8 @@ void launch_prep(const Layout& l, char* ws, const void* x, bool xf32, const floa
 // dx from its parts (exps NULL: they are dx itself, not of the streamed or the wide products' planes), together with dW from its slabs
 // where both remain to be done
 void launch_joins(const XentDxJoin* j, const XentDwReduce* g, hipStream_t st) {
-    // sixteen groups of parts: 200 x 128 x 65536 94.8 us a backward against 101.3 with one, 53 x 75 x 25145 56.4 against 61.3; with the
-    // outputs of 3000 x 32 x 8192 one group fills the chip (75.2 against 83.3)
+    // sixteen groups of parts: 200 x 128 x 65536 94.0 us a backward against 99.2 with one, 53 x 75 x 25145 52.5 against 57.8; with the
+    // outputs of 3000 x 32 x 8192 one group fills the chip (67.9 against 77.7)
     const int64_t outs = j ? j->n * j->ep : 0;
     const bool groups = j && j->np >= 16 && outs <= 1 << 16;
     if (groups) hipLaunchKernelGGL(xent_dx_join_kernel<16>, dim3((unsigned)(up(outs, 64) / 64)), dim3(1024), 0, st, *j);
@@ -2143,9 +2144,9 @@ int short_call(XentShort g, bool xf32, const ShortLayout& l, char* ws, float* lo
 //   few rows | a block of rows   1 x 128 x 4097 15 + 17 | 18 + 30; 4 x 128 x 65536 15 + 42 | 19 + 45; 4 x 1000 x 10001 32 + 97 | 27 + 64;
 //                                16 x 128 x 4097 16 + 24 | 18 + 31; 8 x 32 x 65536 16 + 44 | 18 + 35; 8 x 300 x 1000 19 + 46 | 18 + 31;
 //                                16 x 1000 x 65536 80 + 486 | 62 + 200
-//   a block of rows | matrix     17 x 1000 x 65536 62 + 201 | 300 + 603; 64 x 1000 x 10001 43 + 98 | 72 + 138; 64 x 128 x 4097 18 + 37 | 22 + 37;
-//                                64 x 32 x 65536 18 + 47 | 35 + 52; 128 x 1000 x 65536 172 + 495 | 328 + 648;
-//                                128 x 128 x 65536 38 + 109 | 51 + 80; 128 x 1000 x 10001 74 + 174 | 73 + 146
+//   a block of rows | matrix     17 x 1000 x 65536 62 + 196 | 300 + 606; 64 x 1000 x 10001 42 + 96 | 74 + 136; 64 x 128 x 4097 16 + 37 | 23 + 38;
+//                                64 x 32 x 65536 17 + 47 | 35 + 53; 128 x 1000 x 65536 171 + 492 | 300 + 611;
+//                                128 x 128 x 65536 38 + 109 | 52 + 85; 128 x 1000 x 10001 74 + 174 | 73 + 135
 enum { FORM_FEW, FORM_SHORT, FORM_MATRIX };
 int form_of(int64_t n, int64_t e, int64_t v) {
     if (n <= 4 && e * v <= 1 << 23) return FORM_FEW;
